@@ -10,11 +10,13 @@ _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libcatccos_hip.so")
 
 OK, EINVAL, EHIP, ENODEV, ENOSUP = 0, -1, -2, -3, -4
-FMT_E4M3, FMT_E5M2, FMT_E2M1, FMT_E1M2 = 0, 1, 2, 3
+FMT_E4M3, FMT_E5M2, FMT_E2M1, FMT_E1M2, FMT_INT4 = 0, 1, 2, 3, 4
 ROUND_RNE, ROUND_LUT = 0, 1
+DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2
+SCORING_SOFTMAX, SCORING_SIGMOID = 0, 1
 
 c = ctypes
-_P, _I64, _I, _SZ = c.c_void_p, c.c_int64, c.c_int, c.c_size_t
+_P, _I64, _I, _SZ, _F = c.c_void_p, c.c_int64, c.c_int, c.c_size_t, c.c_float
 
 # name -> argument types; every entry returns int unless listed in _RESTYPE
 PROTOTYPES = {
@@ -58,11 +60,21 @@ PROTOTYPES = {
     "cch_mx_gmm_mapped": [_P, _P, _P, _P, _P, _P, _P, _I64, _I, _I64, _I64, _I64, _I64, _I, _I, _P],
     "cch_moe_ffn_mxfp8_workspace_bytes": [_I64, _I64, _I, _I64, _I64],
     "cch_moe_ffn_mxfp8": [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I, _I64, _I64, _I, _P, _I64, _P],
+    "cch_moe_router": [_P, _I, _I64, _I64, _I, _I, _I, _F, _P, _P, _P, _P, _P],
+    "cch_moe_router_backward": [_P, _P, _I, _P, _I64, _I64, _I, _I, _I, _F, _P, _P],
+    "cch_moe_balance_loss_workspace_bytes": [_I64, _I64, _I64],
+    "cch_moe_balance_loss": [_P, _I, _P, _P, _P, _I64, _I64, _I, _I64, _I, _F, _F, _P, _P, _P, _P, _I64, _P],
+    "cch_moe_balance_loss_backward": [_P, _P, _I, _P, _P, _P, _P, _I64, _I64, _I, _I64, _I, _F, _F, _P, _P],
+    "cch_w4a16_matmul_workspace_bytes": [_I64, _I64, _I64],
+    "cch_w4a16_matmul": [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I, _I, _I, _P, _I64, _P],
+    "cch_moe_ffn_w4a16_workspace_bytes": [_I64, _I64, _I, _I64, _I64],
+    "cch_moe_ffn_w4a16": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I, _I64, _I64, _I, _I, _I, _P, _I64, _P],
     "cch_set_option": [c.c_char_p, _I],
     "cch_gemm_tail_rows": [_P, _I64, _I64, _I64, _I, _I, _P, _P],
     "cch_gemm_kernel_for": [_I, _I, _I64, _I64, _I64, _I64, _I, _I],
 }
-_RESTYPE = {"cch_last_error": c.c_char_p, "cch_moe_init_routing_workspace_bytes": _I64, "cch_moe_ffn_mxfp8_workspace_bytes": _I64}
+_RESTYPE = {"cch_last_error": c.c_char_p, "cch_moe_init_routing_workspace_bytes": _I64, "cch_moe_ffn_mxfp8_workspace_bytes": _I64,
+            "cch_moe_balance_loss_workspace_bytes": _I64, "cch_w4a16_matmul_workspace_bytes": _I64, "cch_moe_ffn_w4a16_workspace_bytes": _I64}
 
 _lib = None
 

@@ -1,0 +1,222 @@
+// The gate of a mixture of experts: what makes the expert_idx and probs that the routing sort, the grouped products and the combine take.
+//
+// Of a token's logits l over E experts: scores s = softmax(l), or sigmoid(l) of each; the top_k experts by score, or by score + bias where a bias steers
+// the load (it only selects); weights w_j = scale s_j, or scale s_j / sum of the selected s ("renormalised").  Scores grow with the logits, so
+// without a bias the logits themselves are compared: what is selected then depends on no rounding.  Equal keys go to the lower index.  An expert
+// whose logit is -inf or NaN is not there; where fewer than top_k are, or the token is masked, the remaining routes are -1 with weight 0, which
+// the routing sort drops.
+//
+// Backward, g the weights' gradient, p = softmax(l):
+//   softmax                  dl_e = p_e (scale g_e [e selected] - sum_j g_j w_j)
+//   softmax, renormalised    dl_j = w_j (g_j - sum_i g_i w_i / scale), the selected experts only
+//   sigmoid                  dl_j = w_j (1 - s_j) g_j
+//   sigmoid, renormalised    dl_j = w_j (1 - s_j) (g_j - sum_i g_i w_i / scale)
+// Everything is fp32 in registers; a row of logits is read once, and in the backward pass of three of the four forms not at all but for the selected ones.
+#include <algorithm>
+
+#include "router_lanes.h"
+
+namespace cch {
+
+constexpr int ROUTER_THREADS = 256;
+
+// This lane's selected logit l (lane `at` < top_k of its token; `there`: it is one) to its weight.  `top`: the largest selected logit, or, for
+// softmax over all experts, of all of them with `denominator` their sum.
+template <int L, bool SIGMOID, bool RENORM>
+__device__ __forceinline__ float route_weight(float l, bool there, float top, float denominator, float scale)
+{
+    if (SIGMOID && !RENORM) return there ? scale * sigmoid(l) : 0.0f;
+    if (!RENORM) return there ? scale * (__expf(l - top) / denominator) : 0.0f;
+    const float c = SIGMOID ? fminf(top, 0.0f) : top;
+    const float s = !there ? 0.0f : SIGMOID ? scaled_sigmoid(l, c, __expf(c)) : __expf(l - c);
+    const float sum = lanes_sum<L>(s);
+    return there ? scale * (s / sum) : 0.0f;
+}
+
+template <class T, int V, int L, bool SIGMOID, bool RENORM>
+__global__ __launch_bounds__(ROUTER_THREADS) void moe_router_kernel(const T *__restrict__ logits, const float *__restrict__ bias, const uint8_t *__restrict__ token_mask,
+                                                                   float *__restrict__ probs, int32_t *__restrict__ expert_idx, int tokens, int experts, int top_k,
+                                                                   float scale, bool vec)
+{
+    const int lane = threadIdx.x & 63, at = lane & (L - 1), base = lane & ~(L - 1);
+    const int64_t t = ((int64_t)blockIdx.x * ROUTER_THREADS + threadIdx.x) / L;
+    const bool inside = t < tokens;
+    float l[V], key[V];
+    LaneRow<T, V>::load(logits + (inside ? t : 0) * experts, at * V, experts, vec, l);
+    const bool counted = inside && (token_mask == nullptr || token_mask[t] != 0);
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        key[i] = l[i] == l[i] && counted ? l[i] : -INFINITY;
+        top = fmaxf(top, key[i]);
+    }
+    float denominator = 1.0f;
+    if ((!SIGMOID && !RENORM) || (!SIGMOID && bias)) {
+        top = lanes_max<L>(top);
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; i++) sum += at * V + i < experts ? __expf(l[i] - top) : 0.0f;
+        denominator = lanes_sum<L>(sum);
+    }
+    if (bias) {
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const int e = at * V + i;
+            if (e >= experts || key[i] == -INFINITY) continue;
+            key[i] = (SIGMOID ? sigmoid(l[i]) : __expf(l[i] - top) / denominator) + bias[e];
+            if (!(key[i] == key[i])) key[i] = -INFINITY;
+        }
+    }
+    int mine_idx = -1;
+    float mine_l = -INFINITY;
+    for (int j = 0; j < top_k; j++) {
+        float best = key[0];
+#pragma unroll
+        for (int i = 1; i < V; i++) best = fmaxf(best, key[i]);
+        const float all = lanes_max<L>(best);
+        int which = 0;
+        float its_l = l[0];
+#pragma unroll
+        for (int i = V - 1; i >= 0; i--)
+            if (key[i] == all) {
+                which = i;
+                its_l = l[i];
+            }
+        const uint64_t holders = (__ballot(best == all) >> base) & (L == 64 ? ~0ull : (1ull << (L & 63)) - 1);
+        const int owner = __ffsll((unsigned long long)holders) - 1;   // (at least one lane holds the maximum)
+        const bool found = all > -INFINITY;
+        const int idx = __shfl(at * V + which, base + owner, 64);
+        const float sel = bias ? __shfl(its_l, base + owner, 64) : all;
+        if (at == j && found) {
+            mine_idx = idx;
+            mine_l = sel;
+        }
+        const int taken = found && at == owner ? which : V;
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            if (i == taken) key[i] = -INFINITY;
+    }
+    const bool there = mine_idx >= 0;
+    if (RENORM) top = lanes_max<L>(mine_l);
+    const float w = route_weight<L, SIGMOID, RENORM>(mine_l, there, top, denominator, scale);
+    if (inside && at < top_k) {
+        probs[t * top_k + at] = w;
+        expert_idx[t * top_k + at] = mine_idx;
+    }
+}
+
+template <class T, int V, int L, bool SIGMOID, bool RENORM>
+__global__ __launch_bounds__(ROUTER_THREADS) void moe_router_backward_kernel(const float *__restrict__ grad_probs, const T *__restrict__ logits,
+                                                                            const int32_t *__restrict__ expert_idx, T *__restrict__ grad_logits, int tokens, int experts,
+                                                                            int top_k, float scale, bool vec)
+{
+    const int lane = threadIdx.x & 63, at = lane & (L - 1), base = lane & ~(L - 1);
+    const int64_t t = ((int64_t)blockIdx.x * ROUTER_THREADS + threadIdx.x) / L;
+    const bool inside = t < tokens;
+    const T *row = logits + (inside ? t : 0) * experts;
+    int idx = -1;
+    float g = 0.0f, sel = -INFINITY;
+    if (inside && at < top_k) {
+        idx = expert_idx[t * top_k + at];
+        if (idx < 0 || idx >= experts) idx = -1;
+        if (idx >= 0) {
+            g = grad_probs[t * top_k + at];
+            sel = to_f32(row[idx]);
+        }
+    }
+    const bool there = idx >= 0;
+    float d[V], top, denominator = 1.0f;
+    if (!SIGMOID && !RENORM) {
+        LaneRow<T, V>::load(row, at * V, experts, vec, d);
+        top = d[0];
+#pragma unroll
+        for (int i = 1; i < V; i++) top = fmaxf(top, d[i]);
+        top = lanes_max<L>(top);
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            d[i] = at * V + i < experts ? __expf(d[i] - top) : 0.0f;
+            sum += d[i];
+        }
+        denominator = lanes_sum<L>(sum);
+    } else {
+        top = RENORM ? lanes_max<L>(sel) : 0.0f;
+    }
+    const float w = route_weight<L, SIGMOID, RENORM>(sel, there, top, denominator, 1.0f);   // of scale 1
+    const float dot = lanes_sum<L>(there ? g * w : 0.0f);
+    float own = RENORM ? w * (g - dot) : w * g;
+    if (SIGMOID) own *= 1.0f / (1.0f + __expf(sel));   // 1 - sigmoid
+    own = there ? own * scale : 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; i++) d[i] = !SIGMOID && !RENORM && dot != 0.0f ? -scale * dot * (d[i] / denominator) : 0.0f;
+    for (int j = 0; j < top_k; j++) {
+        const int e = __shfl(idx, base + j, 64) - at * V;
+        const float x = __shfl(own, base + j, 64);
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            if (e == i) d[i] += x;
+    }
+    if (inside) LaneRow<T, V>::store(grad_logits + t * experts, at * V, experts, vec, d);
+}
+
+static int router_shape(const char *what, int dtype, int64_t tokens, int64_t experts, int top_k, int scoring)
+{
+    CCH_REQUIRE(logits_type_ok(dtype), "%s: logits of type %d", what, dtype);
+    CCH_REQUIRE(tokens >= 0 && tokens < (int64_t)1 << 31, "%s: %lld tokens", what, (long long)tokens);
+    CCH_REQUIRE(experts >= 1 && experts <= ROUTER_MAX_EXPERTS, "%s: num_experts=%lld outside 1..%d", what, (long long)experts, ROUTER_MAX_EXPERTS);
+    CCH_REQUIRE(top_k >= 1 && top_k <= ROUTER_MAX_TOPK && top_k <= experts, "%s: top_k=%d outside 1..min(%d, num_experts)", what, top_k, ROUTER_MAX_TOPK);
+    CCH_REQUIRE(scoring == CCH_SCORING_SOFTMAX || scoring == CCH_SCORING_SIGMOID, "%s: scoring %d", what, scoring);
+    return CCH_OK;
+}
+
+template <int L>
+static unsigned router_grid(int64_t tokens)
+{
+    return (unsigned)((tokens + ROUTER_THREADS / L - 1) / (ROUTER_THREADS / L));
+}
+
+}  // namespace cch
+
+extern "C" int cch_moe_router(const void *logits, int dtype, int64_t tokens, int64_t num_experts, int top_k, int scoring, int renormalize, float scale, const float *bias,
+                              const uint8_t *token_mask, float *probs, int32_t *expert_idx, void *stream)
+{
+    using namespace cch;
+    if (const int rc = router_shape("cch_moe_router", dtype, tokens, num_experts, top_k, scoring)) return rc;
+    CCH_REQUIRE(renormalize == 0 || renormalize == 1, "cch_moe_router: renormalize %d", renormalize);
+    if (tokens == 0) return CCH_OK;
+    CCH_REQUIRE(logits && probs && expert_idx, "cch_moe_router: null pointer");
+    return with_logits_type(dtype, [&](auto *type) {
+        return with_lanes((int)num_experts, [&](auto v, auto lanes) {
+            typedef std::remove_pointer_t<decltype(type)> T;
+            constexpr int V = decltype(v)::value, L = decltype(lanes)::value;
+            auto kern = scoring == CCH_SCORING_SIGMOID ? (renormalize ? moe_router_kernel<T, V, L, true, true> : moe_router_kernel<T, V, L, true, false>)
+                                                       : (renormalize ? moe_router_kernel<T, V, L, false, true> : moe_router_kernel<T, V, L, false, false>);
+            hipLaunchKernelGGL(kern, dim3(router_grid<L>(tokens)), dim3(ROUTER_THREADS), 0, static_cast<hipStream_t>(stream), static_cast<const T *>(logits), bias,
+                               token_mask, probs, expert_idx, (int)tokens, (int)num_experts, top_k, scale, LaneRow<T, V>::vec(logits, num_experts));
+            return launch_status("moe_router_kernel");
+        });
+    });
+}
+
+extern "C" int cch_moe_router_backward(const float *grad_probs, const void *logits, int dtype, const int32_t *expert_idx, int64_t tokens, int64_t num_experts, int top_k,
+                                       int scoring, int renormalize, float scale, void *grad_logits, void *stream)
+{
+    using namespace cch;
+    if (const int rc = router_shape("cch_moe_router_backward", dtype, tokens, num_experts, top_k, scoring)) return rc;
+    CCH_REQUIRE(renormalize == 0 || renormalize == 1, "cch_moe_router_backward: renormalize %d", renormalize);
+    if (tokens == 0) return CCH_OK;
+    CCH_REQUIRE(grad_probs && logits && expert_idx && grad_logits, "cch_moe_router_backward: null pointer");
+    return with_logits_type(dtype, [&](auto *type) {
+        return with_lanes((int)num_experts, [&](auto v, auto lanes) {
+            typedef std::remove_pointer_t<decltype(type)> T;
+            constexpr int V = decltype(v)::value, L = decltype(lanes)::value;
+            auto kern = scoring == CCH_SCORING_SIGMOID
+                            ? (renormalize ? moe_router_backward_kernel<T, V, L, true, true> : moe_router_backward_kernel<T, V, L, true, false>)
+                            : (renormalize ? moe_router_backward_kernel<T, V, L, false, true> : moe_router_backward_kernel<T, V, L, false, false>);
+            hipLaunchKernelGGL(kern, dim3(router_grid<L>(tokens)), dim3(ROUTER_THREADS), 0, static_cast<hipStream_t>(stream), grad_probs, static_cast<const T *>(logits),
+                               expert_idx, static_cast<T *>(grad_logits), (int)tokens, (int)num_experts, top_k, scale,
+                               LaneRow<T, V>::vec(logits, num_experts) && aligned(grad_logits, 16));
+            return launch_status("moe_router_backward_kernel");
+        });
+    });
+}

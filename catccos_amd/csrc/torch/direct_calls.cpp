@@ -10,6 +10,7 @@
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/GradMode.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
@@ -107,6 +108,17 @@ PyObject *Pair(const at::Tensor &a, const at::Tensor &b)
     return t;
 }
 
+PyObject *Three(const at::Tensor &a, const at::Tensor &b, const at::Tensor &c)
+{
+    PyObject *o[3] = {THPVariable_Wrap(a), THPVariable_Wrap(b), THPVariable_Wrap(c)};
+    PyObject *t = o[0] && o[1] && o[2] ? PyTuple_New(3) : nullptr;
+    for (int i = 0; i < 3; i++) {
+        if (t) PyTuple_SET_ITEM(t, i, o[i]);
+        else Py_XDECREF(o[i]);
+    }
+    return t;
+}
+
 // mx_quant(x, fmt, rounding)
 PyObject *MxQuant(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
@@ -172,14 +184,7 @@ PyObject *MoeInitRouting(PyObject *, PyObject *const *a, Py_ssize_t n)
                                   static_cast<int32_t *>(s2d.data_ptr()), static_cast<int32_t *>(tokens.data_ptr()), a[2] == Py_True ? 1 : 0, ws.data_ptr(), bytes,
                                   Stream());
     }
-    if (rc != CCH_OK) return Decline();
-    PyObject *o[3] = {THPVariable_Wrap(d2s), THPVariable_Wrap(s2d), THPVariable_Wrap(tokens)};
-    PyObject *t = o[0] && o[1] && o[2] ? PyTuple_New(3) : nullptr;
-    for (int i = 0; i < 3; i++) {
-        if (t) PyTuple_SET_ITEM(t, i, o[i]);
-        else Py_XDECREF(o[i]);
-    }
-    return t;
+    return rc == CCH_OK ? Three(d2s, s2d, tokens) : Decline();
     END_HANDLE_TH_ERRORS
 }
 
@@ -301,6 +306,235 @@ PyObject *MoeFfnMxfp8(PyObject *, PyObject *const *v, Py_ssize_t nv)
     END_HANDLE_TH_ERRORS
 }
 
+// Options and tensors of the router, the balance loss and the 4-bit products.
+bool Real(PyObject *o, float &v)   // a Python float or int
+{
+    if (PyFloat_Check(o)) {
+        v = (float)PyFloat_AS_DOUBLE(o);
+        return true;
+    }
+    int64_t i;
+    if (!Int(o, i)) return false;
+    v = (float)i;
+    return true;
+}
+bool Scoring(PyObject *o, int &v)
+{
+    if (!PyUnicode_Check(o)) return false;
+    const bool softmax = PyUnicode_CompareWithASCIIString(o, "softmax") == 0;
+    v = softmax ? CCH_SCORING_SOFTMAX : CCH_SCORING_SIGMOID;
+    return softmax || PyUnicode_CompareWithASCIIString(o, "sigmoid") == 0;
+}
+bool W4Format(PyObject *o, int &v)
+{
+    if (!PyUnicode_Check(o)) return false;
+    const bool ints = PyUnicode_CompareWithASCIIString(o, "int4") == 0;
+    v = ints ? CCH_FMT_INT4 : CCH_FMT_E2M1;
+    return ints || PyUnicode_CompareWithASCIIString(o, "e2m1") == 0;
+}
+int DtypeCode(at::ScalarType t) { return t == at::kHalf ? CCH_DTYPE_F16 : t == at::kBFloat16 ? CCH_DTYPE_BF16 : CCH_DTYPE_F32; }
+// forward: and the call has no gradient to record, which is the general path's.
+bool Logits(PyObject *o, bool forward)
+{
+    return (Plain(o, at::kFloat, 2) || Plain(o, at::kBFloat16, 2) || Plain(o, at::kHalf, 2)) && !(forward && c10::GradMode::is_enabled() && T(o).requires_grad());
+}
+bool Mask(PyObject *o, int64_t tokens, const uint8_t *&p)
+{
+    p = nullptr;
+    if (o == Py_None) return true;
+    if ((!Plain(o, at::kBool, 1) && !Plain(o, at::kByte, 1)) || T(o).size(0) != tokens) return false;
+    p = static_cast<const uint8_t *>(T(o).data_ptr());
+    return true;
+}
+template <class E>
+E *P(const at::Tensor &t)
+{
+    return static_cast<E *>(t.data_ptr());
+}
+
+// moe_router(logits, top_k, scoring, renormalize, scale, bias, token_mask)
+PyObject *MoeRouter(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    int scoring, renorm;
+    int64_t top_k;
+    float scale;
+    const uint8_t *mask;
+    if (n != 7 || !PlainThread() || !Logits(a[0], true) || !Int(a[1], top_k) || top_k < 1 || top_k > 8 || !Scoring(a[2], scoring) || !Flag(a[3], renorm) ||
+        !Real(a[4], scale) || (a[5] != Py_None && !Plain(a[5], at::kFloat, 1)) || !Mask(a[6], T(a[0]).size(0), mask))
+        return Decline();
+    const at::Tensor &l = T(a[0]);
+    const int64_t tokens = l.size(0), e = l.size(1);
+    if (top_k > e || (a[5] != Py_None && T(a[5]).size(0) != e)) return Decline();
+    const float *bias = a[5] != Py_None ? P<const float>(T(a[5])) : nullptr;
+    at::Tensor probs, idx;
+    int rc;
+    {
+        pybind11::gil_scoped_release nogil;
+        probs = New(l, {tokens, top_k}, at::kFloat);
+        idx = New(l, {tokens, top_k}, at::kInt);
+        rc = cch_moe_router(l.data_ptr(), DtypeCode(l.scalar_type()), tokens, e, (int)top_k, scoring, renorm, scale, bias, mask, P<float>(probs), P<int32_t>(idx), Stream());
+    }
+    return rc == CCH_OK ? Pair(probs, idx) : Decline();
+    END_HANDLE_TH_ERRORS
+}
+
+// moe_router_backward(grad_probs, logits, expert_idx, scoring, renormalize, scale)
+PyObject *MoeRouterBackward(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    int scoring, renorm;
+    float scale;
+    if (n != 6 || !PlainThread() || !Plain(a[0], at::kFloat, 2) || !Logits(a[1], false) || !Plain(a[2], at::kInt, 2) || !Scoring(a[3], scoring) || !Flag(a[4], renorm) ||
+        !Real(a[5], scale))
+        return Decline();
+    const at::Tensor &g = T(a[0]), &l = T(a[1]), &idx = T(a[2]);
+    if (idx.size(0) != l.size(0) || g.sizes() != idx.sizes()) return Decline();
+    at::Tensor grad;
+    int rc;
+    {
+        pybind11::gil_scoped_release nogil;
+        grad = New(l, l.sizes(), l.scalar_type());
+        rc = cch_moe_router_backward(P<const float>(g), l.data_ptr(), DtypeCode(l.scalar_type()), P<const int32_t>(idx), l.size(0), l.size(1), (int)idx.size(1), scoring,
+                                     renorm, scale, grad.data_ptr(), Stream());
+    }
+    return rc == CCH_OK ? THPVariable_Wrap(grad) : Decline();
+    END_HANDLE_TH_ERRORS
+}
+
+bool Offsets(PyObject *o, const int32_t *&p, int64_t &sequences)
+{
+    p = nullptr;
+    sequences = 1;
+    if (o == Py_None) return true;
+    if (!Plain(o, at::kInt, 1) || T(o).size(0) < 2) return false;
+    p = P<const int32_t>(T(o));
+    sequences = T(o).size(0) - 1;
+    return true;
+}
+
+// moe_balance_loss(logits, expert_idx, coef, z_coef, scoring, token_mask, seq_offsets)
+PyObject *MoeBalanceLoss(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    int scoring;
+    float coef, z_coef;
+    const uint8_t *mask;
+    const int32_t *offsets;
+    int64_t s;
+    if (n != 7 || !PlainThread() || !Logits(a[0], true) || !Plain(a[1], at::kInt, 2) || !Real(a[2], coef) || !Real(a[3], z_coef) || !Scoring(a[4], scoring) ||
+        !Mask(a[5], T(a[0]).size(0), mask) || !Offsets(a[6], offsets, s) || T(a[1]).size(0) != T(a[0]).size(0))
+        return Decline();
+    const at::Tensor &l = T(a[0]), &idx = T(a[1]);
+    const int64_t tokens = l.size(0), e = l.size(1);
+    at::Tensor loss, counts, counted;
+    int rc;
+    {
+        pybind11::gil_scoped_release nogil;
+        loss = New(l, {}, at::kFloat);
+        counts = offsets ? New(l, {s, e}, at::kInt) : New(l, {e}, at::kInt);
+        counted = New(l, {s}, at::kInt);
+        const int64_t bytes = std::max<int64_t>(cch_moe_balance_loss_workspace_bytes(tokens, e, s), 4);
+        const at::Tensor ws = New(l, {bytes}, at::kByte);
+        rc = cch_moe_balance_loss(l.data_ptr(), DtypeCode(l.scalar_type()), P<const int32_t>(idx), mask, offsets, tokens, e, (int)idx.size(1), s, scoring, coef, z_coef,
+                                  P<float>(loss), P<int32_t>(counts), P<int32_t>(counted), ws.data_ptr(), bytes, Stream());
+    }
+    return rc == CCH_OK ? Three(loss, counts, counted) : Decline();
+    END_HANDLE_TH_ERRORS
+}
+
+// moe_balance_loss_backward(grad_loss, logits, counts, tokens, top_k, coef, z_coef, scoring, token_mask, seq_offsets)
+PyObject *MoeBalanceLossBackward(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    int scoring;
+    float coef, z_coef;
+    const uint8_t *mask;
+    const int32_t *offsets;
+    int64_t s, top_k;
+    if (n != 10 || !PlainThread() || !Plain(a[0], at::kFloat, -1) || !Logits(a[1], false) || !Plain(a[2], at::kInt, -1) || !Plain(a[3], at::kInt, -1) ||
+        !Int(a[4], top_k) || !Real(a[5], coef) || !Real(a[6], z_coef) || !Scoring(a[7], scoring) || !Mask(a[8], T(a[1]).size(0), mask) || !Offsets(a[9], offsets, s))
+        return Decline();
+    const at::Tensor &l = T(a[1]), &counts = T(a[2]), &counted = T(a[3]);
+    if (T(a[0]).numel() != 1 || counts.numel() != s * l.size(1) || counted.numel() != s) return Decline();
+    at::Tensor grad;
+    int rc;
+    {
+        pybind11::gil_scoped_release nogil;
+        grad = New(l, l.sizes(), l.scalar_type());
+        rc = cch_moe_balance_loss_backward(P<const float>(T(a[0])), l.data_ptr(), DtypeCode(l.scalar_type()), mask, offsets, P<const int32_t>(counts),
+                                           P<const int32_t>(counted), l.size(0), l.size(1), (int)top_k, s, scoring, coef, z_coef, grad.data_ptr(), Stream());
+    }
+    return rc == CCH_OK ? THPVariable_Wrap(grad) : Decline();
+    END_HANDLE_TH_ERRORS
+}
+
+// Codes, scales and zero points (or None) of weights of k columns; rank: of the codes.
+bool W4Weights(PyObject *w, PyObject *s, PyObject *z, int64_t rank, int64_t k, int fmt, int64_t group, at::ScalarType type)
+{
+    if (!Plain(w, at::kByte, rank) || !Plain(s, fmt == CCH_FMT_INT4 ? type : at::kByte, rank) || (fmt == CCH_FMT_INT4 && group != 32 && group != 64 && group != 128))
+        return false;
+    const at::Tensor &codes = T(w), &scales = T(s);
+    if (codes.size(rank - 1) != (k + 1) / 2 || scales.size(rank - 1) != (fmt == CCH_FMT_INT4 ? (k + group - 1) / group : ScaleCols(k))) return false;
+    for (int64_t i = 0; i < rank - 1; i++)
+        if (codes.size(i) != scales.size(i)) return false;
+    return z == Py_None || (fmt == CCH_FMT_INT4 && Plain(z, at::kByte, rank) && T(z).sizes() == scales.sizes());
+}
+const void *Data(PyObject *o) { return o == Py_None ? nullptr : T(o).data_ptr(); }
+
+// w4a16_matmul(x, w, scales, zeros, fmt, group_size)
+PyObject *W4A16(PyObject *, PyObject *const *v, Py_ssize_t nv)
+{
+    HANDLE_TH_ERRORS
+    int fmt;
+    int64_t group;
+    if (nv != 6 || !PlainThread() || !(Plain(v[0], at::kBFloat16, 2) || Plain(v[0], at::kHalf, 2)) || !W4Format(v[4], fmt) || !Int(v[5], group) ||
+        !W4Weights(v[1], v[2], v[3], 2, T(v[0]).size(1), fmt, group, T(v[0]).scalar_type()))
+        return Decline();
+    const at::Tensor &x = T(v[0]), &w = T(v[1]);
+    const int64_t m = x.size(0), k = x.size(1), n = w.size(0);
+    at::Tensor out, ws;
+    int rc;
+    {
+        pybind11::gil_scoped_release nogil;
+        out = New(x, {m, n}, x.scalar_type());
+        const int64_t bytes = cch_w4a16_matmul_workspace_bytes(m, n, k);
+        if (bytes > 0) ws = New(x, {bytes}, at::kByte);
+        rc = cch_w4a16_matmul(x.data_ptr(), w.data_ptr(), Data(v[2]), Data(v[3]), out.data_ptr(), m, n, k, fmt, (int)group, DtypeCode(x.scalar_type()),
+                              bytes > 0 ? ws.data_ptr() : nullptr, bytes, Stream());
+    }
+    return rc == CCH_OK ? THPVariable_Wrap(out) : Decline();
+    END_HANDLE_TH_ERRORS
+}
+
+// moe_ffn_w4a16(x, expert_idx, probs, w1, scales1, zeros1, w2, scales2, zeros2, fmt, group_size)
+PyObject *MoeFfnW4A16(PyObject *, PyObject *const *v, Py_ssize_t nv)
+{
+    HANDLE_TH_ERRORS
+    int fmt;
+    int64_t group;
+    if (nv != 11 || !PlainThread() || !(Plain(v[0], at::kBFloat16, 2) || Plain(v[0], at::kHalf, 2)) || !Plain(v[1], at::kInt, 2) || !Plain(v[2], at::kFloat, 2) ||
+        !Plain(v[3], at::kByte, 3) || !W4Format(v[9], fmt) || !Int(v[10], group))
+        return Decline();
+    const at::Tensor &x = T(v[0]), &idx = T(v[1]), &probs = T(v[2]), &w1 = T(v[3]);
+    const int64_t m = x.size(0), k = x.size(1), top_k = idx.size(1), e = w1.size(0), n = w1.size(1);
+    if (idx.size(0) != m || probs.sizes() != idx.sizes() || top_k > 8 || n % 2 || !W4Weights(v[3], v[4], v[5], 3, k, fmt, group, x.scalar_type()) ||
+        !W4Weights(v[6], v[7], v[8], 3, n / 2, fmt, group, x.scalar_type()) || T(v[6]).size(0) != e || T(v[6]).size(1) != k)
+        return Decline();
+    at::Tensor out;
+    int rc;
+    {
+        pybind11::gil_scoped_release nogil;
+        const int64_t bytes = cch_moe_ffn_w4a16_workspace_bytes(m, k, (int)top_k, e, n);
+        const at::Tensor ws = New(x, {bytes}, at::kByte);
+        out = New(x, {m, k}, x.scalar_type());
+        rc = cch_moe_ffn_w4a16(x.data_ptr(), P<const int32_t>(idx), P<const float>(probs), w1.data_ptr(), Data(v[4]), Data(v[5]), Data(v[6]), Data(v[7]), Data(v[8]),
+                               out.data_ptr(), m, k, (int)top_k, e, n, fmt, (int)group, DtypeCode(x.scalar_type()), ws.data_ptr(), bytes, Stream());
+    }
+    return rc == CCH_OK ? THPVariable_Wrap(out) : Decline();
+    END_HANDLE_TH_ERRORS
+}
+
 #define CCH_FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr
 PyMethodDef methods[] = {
     {"mx_quant", CCH_FAST(MxQuant)},
@@ -311,6 +545,12 @@ PyMethodDef methods[] = {
     {"mx_matmul", CCH_FAST(MxMatmul)},
     {"mx_grouped_matmul", CCH_FAST(MxGroupedMatmul)},
     {"moe_ffn_mxfp8", CCH_FAST(MoeFfnMxfp8)},
+    {"moe_router", CCH_FAST(MoeRouter)},
+    {"moe_router_backward", CCH_FAST(MoeRouterBackward)},
+    {"moe_balance_loss", CCH_FAST(MoeBalanceLoss)},
+    {"moe_balance_loss_backward", CCH_FAST(MoeBalanceLossBackward)},
+    {"w4a16_matmul", CCH_FAST(W4A16)},
+    {"moe_ffn_w4a16", CCH_FAST(MoeFfnW4A16)},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_direct", "native form of the tensor-level entry points", -1, methods, nullptr, nullptr, nullptr, nullptr};

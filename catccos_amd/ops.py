@@ -13,7 +13,8 @@ import warnings as _warnings
 import torch
 
 from . import _abi
-from ._abi import FMT_E1M2, FMT_E2M1, FMT_E4M3, FMT_E5M2, ROUND_LUT, ROUND_RNE, check
+from ._abi import (DTYPE_BF16, DTYPE_F16, DTYPE_F32, FMT_E1M2, FMT_E2M1, FMT_E4M3, FMT_E5M2, FMT_INT4, ROUND_LUT, ROUND_RNE, SCORING_SIGMOID,
+                   SCORING_SOFTMAX, check)
 
 _FMT_NAMES = {"e4m3": FMT_E4M3, "e5m2": FMT_E5M2, "e2m1": FMT_E2M1, "e1m2": FMT_E1M2, "fp8": FMT_E4M3, "fp4": FMT_E2M1}
 _FP4 = (FMT_E2M1, FMT_E1M2)   # two codes per byte; E1M2 exists for the quantiser only
@@ -50,7 +51,8 @@ class _Direct:
     or does not load, a warning says so once and every call takes the general path, which needs the HIP library alone."""
 
     def __getattr__(self, name):
-        names = ("mx_quant", "dynamic_quant_i8", "moe_init_routing", "w8a8_matmul_dequant", "gmm_i8", "mx_matmul", "mx_grouped_matmul", "moe_ffn_mxfp8")
+        names = ("mx_quant", "dynamic_quant_i8", "moe_init_routing", "w8a8_matmul_dequant", "gmm_i8", "mx_matmul", "mx_grouped_matmul", "moe_ffn_mxfp8",
+                 "moe_router", "moe_router_backward", "moe_balance_loss", "moe_balance_loss_backward", "w4a16_matmul", "moe_ffn_w4a16")
         if name not in names:
             raise AttributeError(name)
         try:
@@ -530,4 +532,258 @@ def moe_ffn_mxfp8(x, expert_idx, probs, w1, sw1, w2, sw2, trans_b=1):
     ws = torch.empty(max(int(nbytes), 1), dtype=torch.uint8, device=x.device)
     check(_abi.lib().cch_moe_ffn_mxfp8(_ptr(x), _ptr(expert_idx), _ptr(probs), _ptr(w1), _ptr(sw1), _ptr(w2), _ptr(sw2), _ptr(out), m, k, top_k, e, n,
                                        int(trans_b), _ptr(ws), ws.numel(), _stream()))
+    return out
+
+
+_DTYPES = {torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16, torch.float32: DTYPE_F32}
+_SCORINGS = {"softmax": SCORING_SOFTMAX, "sigmoid": SCORING_SIGMOID}
+
+
+def _scoring(scoring):
+    if scoring not in _SCORINGS:
+        raise ValueError("unknown scoring %r (softmax or sigmoid)" % (scoring,))
+    return _SCORINGS[scoring]
+
+
+def _check_logits(logits):
+    if logits.dim() != 2 or logits.dtype not in _DTYPES:
+        raise ValueError("logits must be a 2-D bfloat16, float16 or float32 tensor")
+
+
+def _check_mask(token_mask, tokens):
+    if token_mask is None:
+        return None
+    if token_mask.dtype not in (torch.bool, torch.uint8) or tuple(token_mask.shape) != (tokens,):
+        raise ValueError("token_mask must be a bool (or uint8) tensor [tokens]")
+    return token_mask.contiguous()
+
+
+def _recorded(t):
+    return torch.is_grad_enabled() and t.requires_grad
+
+
+def moe_router(logits, top_k, scoring="softmax", renormalize=True, scale=1.0, bias=None, token_mask=None):
+    """The gate: every token's top_k experts and their weights, ready for moe_init_routing, the grouped products and the FFN entry points.
+
+    logits bf16, half or float32 [tokens, E], E <= 1024, top_k <= 8.  Scores are the logits' softmax over the experts or each one's sigmoid; the
+    top_k largest are taken, by score + bias[e] where a bias (float32 [E]) steers the load, ties to the lower index.  Returns (probs float32
+    [tokens, top_k], expert_idx int32 [tokens, top_k]): probs = scale * score, with renormalize divided by the token's sum of selected
+    scores.  A logit of -inf or NaN is no candidate, a token whose token_mask is False has none: entries without an expert are -1
+    with weight 0, which the routing sort drops.  Differentiable in the logits."""
+    r = _direct.moe_router(logits, top_k, scoring, renormalize, scale, bias, token_mask)
+    if r is not NotImplemented:
+        return r
+    _require_gpu(logits, bias, token_mask)
+    _check_logits(logits)
+    if _recorded(logits):
+        return _Router.apply(logits, top_k, scoring, renormalize, scale, bias, token_mask)   # (comes back here without the record)
+    tokens, e = logits.shape
+    if not 1 <= top_k <= min(8, e):
+        raise ValueError("top_k must be 1..8 and no more than the experts")
+    if bias is not None:
+        if bias.dtype != torch.float32 or tuple(bias.shape) != (e,):
+            raise ValueError("bias must be a float32 tensor [experts]")
+        bias = bias.contiguous()
+    token_mask = _check_mask(token_mask, tokens)
+    logits = logits.contiguous()
+    probs = torch.empty((tokens, top_k), dtype=torch.float32, device=logits.device)
+    idx = torch.empty((tokens, top_k), dtype=torch.int32, device=logits.device)
+    check(_abi.lib().cch_moe_router(_ptr(logits), _DTYPES[logits.dtype], tokens, e, int(top_k), _scoring(scoring), int(bool(renormalize)), float(scale), _ptr(bias),
+                                    _ptr(token_mask), _ptr(probs), _ptr(idx), _stream()))
+    return probs, idx
+
+
+def moe_router_backward(grad_probs, logits, expert_idx, scoring="softmax", renormalize=True, scale=1.0):
+    """The logits' gradient (their type) of moe_router's probs: grad_probs float32 [tokens, top_k], expert_idx as moe_router returned it,
+    the options as they were given to it.  What autograd calls; for programs that do without it."""
+    r = _direct.moe_router_backward(grad_probs, logits, expert_idx, scoring, renormalize, scale)
+    if r is not NotImplemented:
+        return r
+    _require_gpu(grad_probs, logits, expert_idx)
+    _check_logits(logits)
+    tokens, e = logits.shape
+    if expert_idx.dtype != torch.int32 or expert_idx.dim() != 2 or expert_idx.shape[0] != tokens or grad_probs.shape != expert_idx.shape:
+        raise ValueError("expert_idx must be int32 [tokens, top_k] and grad_probs of its shape")
+    if grad_probs.dtype != torch.float32:
+        raise ValueError("grad_probs must be float32")
+    grad_probs, logits, expert_idx = grad_probs.contiguous(), logits.contiguous(), expert_idx.contiguous()
+    grad = torch.empty((tokens, e), dtype=logits.dtype, device=logits.device)
+    check(_abi.lib().cch_moe_router_backward(_ptr(grad_probs), _ptr(logits), _DTYPES[logits.dtype], _ptr(expert_idx), tokens, e, expert_idx.shape[1],
+                                             _scoring(scoring), int(bool(renormalize)), float(scale), _ptr(grad), _stream()))
+    return grad
+
+
+class _Router(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, top_k, scoring, renormalize, scale, bias, token_mask):
+        probs, idx = moe_router(logits.detach(), top_k, scoring, renormalize, scale, bias, token_mask)
+        ctx.save_for_backward(logits, idx)
+        ctx.options = (scoring, renormalize, scale)
+        ctx.mark_non_differentiable(idx)
+        return probs, idx
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_probs, _):
+        logits, idx = ctx.saved_tensors
+        return (moe_router_backward(grad_probs, logits, idx, *ctx.options),) + (None,) * 6
+
+
+def _check_balance(logits, expert_shape, token_mask, seq_offsets):
+    _check_logits(logits)
+    tokens, e = logits.shape
+    if expert_shape is not None and (len(expert_shape) != 2 or expert_shape[0] != tokens):
+        raise ValueError("expert_idx must be int32 [tokens, top_k]")
+    if seq_offsets is not None:
+        if seq_offsets.dtype != torch.int32 or seq_offsets.dim() != 1 or seq_offsets.numel() < 2:
+            raise ValueError("seq_offsets must be an int32 tensor [sequences + 1]")
+        seq_offsets = seq_offsets.contiguous()
+    return tokens, e, _check_mask(token_mask, tokens), seq_offsets, 1 if seq_offsets is None else seq_offsets.numel() - 1
+
+
+def moe_balance_loss(logits, expert_idx, coef=1.0, z_coef=0.0, scoring="softmax", token_mask=None, seq_offsets=None):
+    """The balance loss of a gate's logits and its choice of experts, the z loss and the routes per expert.
+
+    Over a sequence's N counted tokens: f_e = E * routes to e / (top_k * N), P_e = mean of p_te with p the softmax of the logits, or their sigmoids
+    divided by the token's sum of them; loss = coef * mean over sequences of sum_e f_e P_e + z_coef * mean over tokens of
+    logsumexp(logits)^2.  The batch is one sequence, or seq_offsets (int32 [S + 1], rising) says where the sequences
+    begin; tokens in none of them, masked ones (token_mask False) and those without a logit above -inf do not count.
+    expert_idx int32 [tokens, top_k], entries outside the experts are no routes.  Returns (loss float32 [], counts int32 [E], or [S, E] with
+    seq_offsets, tokens int32 [1] or [S]: those that counted).  Differentiable in the logits; the same inputs give the same bits."""
+    r = _direct.moe_balance_loss(logits, expert_idx, coef, z_coef, scoring, token_mask, seq_offsets)
+    if r is not NotImplemented:
+        return r
+    _require_gpu(logits, expert_idx, token_mask, seq_offsets)
+    if expert_idx.dtype != torch.int32:
+        raise ValueError("expert_idx must be int32 [tokens, top_k]")
+    tokens, e, token_mask, offsets, s = _check_balance(logits, expert_idx.shape, token_mask, seq_offsets)
+    if _recorded(logits):
+        return _BalanceLoss.apply(logits, expert_idx, coef, z_coef, scoring, token_mask, seq_offsets)
+    logits, idx = logits.contiguous(), expert_idx.contiguous()
+    loss = torch.empty((), dtype=torch.float32, device=logits.device)
+    counts = torch.empty((s, e) if seq_offsets is not None else (e,), dtype=torch.int32, device=logits.device)
+    counted = torch.empty((s,), dtype=torch.int32, device=logits.device)
+    nbytes = _abi.lib().cch_moe_balance_loss_workspace_bytes(tokens, e, s)
+    ws = torch.empty(max(int(nbytes), 4), dtype=torch.uint8, device=logits.device)
+    check(_abi.lib().cch_moe_balance_loss(_ptr(logits), _DTYPES[logits.dtype], _ptr(idx), _ptr(token_mask), _ptr(offsets), tokens, e, idx.shape[1], s, _scoring(scoring),
+                                          float(coef), float(z_coef), _ptr(loss), _ptr(counts), _ptr(counted), _ptr(ws), ws.numel(), _stream()))
+    return loss, counts, counted
+
+
+def moe_balance_loss_backward(grad_loss, logits, counts, tokens, top_k, coef=1.0, z_coef=0.0, scoring="softmax", token_mask=None, seq_offsets=None):
+    """The logits' gradient (their type) of moe_balance_loss: grad_loss float32 [] on the GPU, counts and tokens as moe_balance_loss
+    returned them, the options as they were given to it.  What autograd calls; for programs that do without it."""
+    r = _direct.moe_balance_loss_backward(grad_loss, logits, counts, tokens, top_k, coef, z_coef, scoring, token_mask, seq_offsets)
+    if r is not NotImplemented:
+        return r
+    _require_gpu(grad_loss, logits, counts, tokens, token_mask, seq_offsets)
+    if grad_loss.dtype != torch.float32 or grad_loss.numel() != 1:
+        raise ValueError("grad_loss must be one float32 value")
+    rows, e, token_mask, offsets, s = _check_balance(logits, None, token_mask, seq_offsets)
+    if counts.dtype != torch.int32 or counts.numel() != s * e or tokens.dtype != torch.int32 or tokens.numel() != s:
+        raise ValueError("counts must be int32 [sequences, experts] and tokens int32 [sequences]")
+    logits, counts, tokens = logits.contiguous(), counts.contiguous(), tokens.contiguous()
+    grad = torch.empty((rows, e), dtype=logits.dtype, device=logits.device)
+    check(_abi.lib().cch_moe_balance_loss_backward(_ptr(grad_loss), _ptr(logits), _DTYPES[logits.dtype], _ptr(token_mask), _ptr(offsets), _ptr(counts), _ptr(tokens),
+                                                   rows, e, int(top_k), s, _scoring(scoring), float(coef), float(z_coef), _ptr(grad), _stream()))
+    return grad
+
+
+class _BalanceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, expert_idx, coef, z_coef, scoring, token_mask, seq_offsets):
+        loss, counts, tokens = moe_balance_loss(logits.detach(), expert_idx, coef, z_coef, scoring, token_mask, seq_offsets)
+        ctx.save_for_backward(logits, counts, tokens, token_mask, seq_offsets)
+        ctx.options = (expert_idx.shape[1], coef, z_coef, scoring)
+        ctx.mark_non_differentiable(counts, tokens)
+        return loss, counts, tokens
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_loss, _counts, _tokens):
+        logits, counts, tokens, token_mask, seq_offsets = ctx.saved_tensors
+        return (moe_balance_loss_backward(grad_loss.float(), logits, counts, tokens, *ctx.options, token_mask, seq_offsets),) + (None,) * 6
+
+
+def _w4_fmt(fmt):
+    if fmt in ("int4", FMT_INT4):
+        return FMT_INT4
+    if fmt in ("e2m1", "fp4", FMT_E2M1):
+        return FMT_E2M1
+    raise ValueError("unknown 4-bit weight format %r (int4 or e2m1)" % (fmt,))
+
+
+def _check_w4(name, w, scales, zeros, lead, k, fmt, group_size, dtype):
+    """Codes, scales and zero points of [*lead, k] weights; returns them contiguous."""
+    if fmt == FMT_INT4 and group_size not in (32, 64, 128):
+        raise ValueError("group_size must be 32, 64 or 128")
+    if w.dtype != torch.uint8 or tuple(w.shape) != tuple(lead) + ((k + 1) // 2,):
+        raise ValueError("%s must be a uint8 tensor %s" % (name, list(lead) + [(k + 1) // 2]))
+    groups = (k + group_size - 1) // group_size if fmt == FMT_INT4 else scale_cols(k)
+    if scales.dtype != (dtype if fmt == FMT_INT4 else torch.uint8) or tuple(scales.shape) != tuple(lead) + (groups,):
+        raise ValueError("scales of %s must be a tensor %s of %s" % (name, list(lead) + [groups], "the activations' type" if fmt == FMT_INT4 else "E8M0 bytes"))
+    if zeros is not None and (fmt != FMT_INT4 or zeros.dtype != torch.uint8 or zeros.shape != scales.shape):
+        raise ValueError("zeros of %s must be uint8 of the scales' shape, with int4 weights only" % name)
+    return w.contiguous(), scales.contiguous(), None if zeros is None else zeros.contiguous()
+
+
+def _check_w4_x(x):
+    if x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("x must be a 2-D bfloat16 or float16 tensor")
+
+
+def w4a16_matmul(x, w, scales, zeros=None, fmt="int4", group_size=128):
+    """x [M, K] (bf16 or half) times 4-bit weights of N rows: the linear layer of a decode step.  Returns [M, N] in x's type; sums in fp32.
+
+    w uint8 [N, ceil(K/2)], element 2j in the low nibble.  fmt "int4": an element stands for (code - zero) * scale with scales [N, ceil(K/group_size)]
+    of x's type and zeros uint8 of that shape, or None for 8 everywhere; group_size 32, 64 or 128.  fmt "e2m1": MXFP4, scales E8M0 uint8
+    [N, scale_cols(K)], payload and scales as mx_quant(weights [N, K], "e2m1") returns them.  Inference only."""
+    r = _direct.w4a16_matmul(x, w, scales, zeros, fmt, group_size)
+    if r is not NotImplemented:
+        return r
+    fmt = _w4_fmt(fmt)
+    _require_gpu(x, w, scales, zeros)
+    _check_w4_x(x)
+    if w.dim() != 2:
+        raise ValueError("w must be a 2-D uint8 tensor")
+    x = x.contiguous()
+    (m, k), n = x.shape, w.shape[0]
+    w, scales, zeros = _check_w4("w", w, scales, zeros, (n,), k, fmt, group_size, x.dtype)
+    out = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    ws = torch.empty(int(_abi.lib().cch_w4a16_matmul_workspace_bytes(m, n, k)), dtype=torch.uint8, device=x.device)
+    check(_abi.lib().cch_w4a16_matmul(_ptr(x), _ptr(w), _ptr(scales), _ptr(zeros), _ptr(out), m, n, k, fmt, int(group_size), _DTYPES[x.dtype], _ptr(ws), ws.numel(),
+                                      _stream()))
+    return out
+
+
+def moe_ffn_w4a16(x, expert_idx, probs, w1, scales1, zeros1, w2, scales2, zeros2, fmt="int4", group_size=128):
+    """The mixture-of-experts feed-forward of few tokens with 4-bit weights, one rank that holds every expert: what moe_ffn_mxfp8 computes, with bf16 or
+    half activations throughout.  x [m, k]; expert_idx int32 and probs float32 [m, top_k] (moe_router's; entries outside the experts are
+    dropped); w1 [E, n, ceil(k/2)] up projections, gate rows first, w2 [E, k, ceil(n/2/2)] down projections, each with scales and zeros (or
+    None) as in w4a16_matmul.  Returns [m, k] in x's type.  Inference only."""
+    r = _direct.moe_ffn_w4a16(x, expert_idx, probs, w1, scales1, zeros1, w2, scales2, zeros2, fmt, group_size)
+    if r is not NotImplemented:
+        return r
+    fmt = _w4_fmt(fmt)
+    _require_gpu(x, expert_idx, probs, w1, scales1, zeros1, w2, scales2, zeros2)
+    _check_w4_x(x)
+    if expert_idx.dim() != 2 or expert_idx.shape[0] != x.shape[0] or probs.shape != expert_idx.shape:
+        raise ValueError("expert_idx and probs must be [m, top_k]")
+    if expert_idx.dtype != torch.int32 or probs.dtype != torch.float32:
+        raise ValueError("expert_idx must be int32 and probs float32")
+    m, k = x.shape
+    top_k = expert_idx.shape[1]
+    if not 1 <= top_k <= 8:
+        raise ValueError("top_k must be 1..8")
+    if w1.dim() != 3 or w1.shape[1] % 2:
+        raise ValueError("w1 must be a 3-D uint8 tensor of gate and up halves")
+    e, n = w1.shape[:2]
+    x, expert_idx, probs = x.contiguous(), expert_idx.contiguous(), probs.contiguous()
+    w1, scales1, zeros1 = _check_w4("w1", w1, scales1, zeros1, (e, n), k, fmt, group_size, x.dtype)
+    w2, scales2, zeros2 = _check_w4("w2", w2, scales2, zeros2, (e, k), n // 2, fmt, group_size, x.dtype)
+    out = torch.empty((m, k), dtype=x.dtype, device=x.device)
+    nbytes = _abi.lib().cch_moe_ffn_w4a16_workspace_bytes(m, k, top_k, e, n)
+    ws = torch.empty(max(int(nbytes), 1), dtype=torch.uint8, device=x.device)
+    check(_abi.lib().cch_moe_ffn_w4a16(_ptr(x), _ptr(expert_idx), _ptr(probs), _ptr(w1), _ptr(scales1), _ptr(zeros1), _ptr(w2), _ptr(scales2), _ptr(zeros2), _ptr(out),
+                                       m, k, top_k, e, n, fmt, int(group_size), _DTYPES[x.dtype], _ptr(ws), ws.numel(), _stream()))
     return out

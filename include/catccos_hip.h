@@ -33,6 +33,7 @@ extern "C" {
 #define CCH_FMT_E5M2 1
 #define CCH_FMT_E2M1 2
 #define CCH_FMT_E1M2 3 /* FP4 with one exponent and two mantissa bits (0, .25 ... 1.75): quantiser only */
+#define CCH_FMT_INT4 4 /* weights of the w4a16 entry points only: unsigned integers with a scale and a zero point per group */
 
 /* payload rounding: 0 = round to nearest even, sign of zero kept (the device
  * cast, include/catccos/comm/block/comm_block_mx_quant.hpp:596-642);
@@ -348,6 +349,70 @@ int cch_dyn_quant_i8_rows(const void *x, const int32_t *src_rows, void *q, float
 int cch_dyn_quant_i8_rows_smooth(const void *x, const int32_t *src_rows, const float *smooth, const int32_t *smooth_rows,
                                  int64_t num_smooth, void *q, float *scale, int64_t rows_in, int64_t t, int64_t k, int topk,
                                  int mode, void *stream);
+
+/* ---- The gate of a mixture of experts: expert_idx and probs from its logits ----
+ * What the reference's examples take from files (examples/utils/gen_data_moe.py:48-57 draws them at random).
+ *   logits       [tokens, num_experts] of type `dtype`; num_experts 1..1024, top_k 1..min(8, num_experts)
+ *   scoring      scores s = softmax over the experts, or sigmoid of each logit (fp32)
+ *   bias         fp32 [num_experts] or NULL: added to the scores for the selection only
+ *   token_mask   bytes [tokens] or NULL: a token whose byte is 0 gets no expert
+ *   expert_idx   int32 [tokens, top_k], by falling score (+ bias), ties by rising index.  A logit of -inf or NaN is no candidate;
+ *                where fewer than top_k are, the remaining entries are -1 (which cch_moe_init_routing drops)
+ *   probs        fp32 [tokens, top_k]: scale * s, or, with renormalize = 1, scale * s / (sum of the token's selected s); 0 for entries of -1
+ * The backward call takes the gradient of probs and expert_idx as the forward call wrote it, and writes the logits' gradient in
+ * their type (zeros for tokens without experts; the bias has none). */
+#define CCH_DTYPE_BF16 0
+#define CCH_DTYPE_F16 1
+#define CCH_DTYPE_F32 2
+#define CCH_SCORING_SOFTMAX 0
+#define CCH_SCORING_SIGMOID 1
+int cch_moe_router(const void *logits, int dtype, int64_t tokens, int64_t num_experts, int top_k, int scoring, int renormalize, float scale,
+                   const float *bias, const uint8_t *token_mask, float *probs, int32_t *expert_idx, void *stream);
+int cch_moe_router_backward(const float *grad_probs, const void *logits, int dtype, const int32_t *expert_idx, int64_t tokens,
+                            int64_t num_experts, int top_k, int scoring, int renormalize, float scale, void *grad_logits, void *stream);
+
+/* ---- Balance loss, z loss and routes per expert ----
+ * Of a sequence with N tokens that count (mask byte not 0, some logit above -inf), c_e routes to expert e, k = top_k and E experts:
+ * f_e = E c_e / (k N), P_e = mean over its tokens of p_te, p = softmax(l), or sigmoid(l) / sum over the experts of sigmoid(l);
+ *   loss = coef * mean over sequences with N > 0 of sum_e f_e P_e + z_coef * mean over all counted tokens of (log sum_e exp l_te)^2
+ *   expert_idx   int32 [tokens, top_k]; entries outside [0, num_experts) are no routes; tokens * top_k < 2^31
+ *   token_mask   bytes [tokens] or NULL
+ *   seq_offsets  int32 [num_sequences + 1], rising: sequence s is tokens seq_offsets[s] .. seq_offsets[s+1] - 1 (read up to `tokens`;
+ *                tokens in none do not count); NULL: one sequence.  num_sequences 1..65535
+ *   loss         fp32;  counts  int32 [num_sequences, num_experts] = c;  seq_tokens  int32 [num_sequences] = N
+ *   workspace    device memory of at least cch_moe_balance_loss_workspace_bytes(...)
+ * Two calls with the same inputs give the same bits.  The backward call takes counts and seq_tokens as the forward call wrote
+ * them, the gradient of the loss (fp32, device memory), and writes the logits' gradient in their type, zeros where tokens do not count. */
+int64_t cch_moe_balance_loss_workspace_bytes(int64_t tokens, int64_t num_experts, int64_t num_sequences);
+int cch_moe_balance_loss(const void *logits, int dtype, const int32_t *expert_idx, const uint8_t *token_mask, const int32_t *seq_offsets,
+                         int64_t tokens, int64_t num_experts, int top_k, int64_t num_sequences, int scoring, float coef, float z_coef,
+                         float *loss, int32_t *counts, int32_t *seq_tokens, void *workspace, int64_t workspace_bytes, void *stream);
+int cch_moe_balance_loss_backward(const float *grad_loss, const void *logits, int dtype, const uint8_t *token_mask, const int32_t *seq_offsets,
+                                  const int32_t *counts, const int32_t *seq_tokens, int64_t tokens, int64_t num_experts, int top_k,
+                                  int64_t num_sequences, int scoring, float coef, float z_coef, void *grad_logits, void *stream);
+
+/* ---- Products of a few 16-bit rows with 4-bit weights (decode steps) ----
+ *   x        [m, k] of type dtype (CCH_DTYPE_BF16 or CCH_DTYPE_F16), out [m, n] in the same type; sums in fp32
+ *   w        [n, ceil(k/2)] bytes, element 2j in the low nibble
+ *   scales   CCH_FMT_INT4: [n, ceil(k/group_size)] of x's type, group_size 32, 64 or 128;
+ *            CCH_FMT_E2M1: E8M0 [n, 2*ceil(k/64)], groups of 32 (what cch_mx_quant_rows writes for rows of weights)
+ *   zeros    CCH_FMT_INT4: bytes of scales' shape or NULL (8 everywhere): an element stands for (code - zero) * scale
+ *   workspace  device memory on a 16-byte boundary of at least cch_w4a16_matmul_workspace_bytes(...) bytes (none for 0); nothing in it has to be
+ *            kept or cleared between calls, calls that overlap need one each
+ * Any k; k a multiple of 32 and pointers on 16-byte boundaries take the fast kernels. */
+int64_t cch_w4a16_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int cch_w4a16_matmul(const void *x, const void *w, const void *scales, const void *zeros, void *out, int64_t m, int64_t n, int64_t k, int fmt,
+                     int group_size, int dtype, void *workspace, int64_t workspace_bytes, void *stream);
+/* The MoE FFN of one rank that holds every expert with such weights, routing to combine: cch_moe_ffn_mxfp8's block for few tokens.
+ *   x, out      [m, k] of type dtype; expert_idx int32 [m, top_k] (an entry outside [0, num_experts) is dropped)
+ *   probs       fp32 [m, top_k]; top_k 1..8; num_experts 1..1024
+ *   w1 / s1 / z1   up projections [num_experts] x [n, k], gate rows first, as above; w2 / s2 / z2 down projections [k, n/2]
+ *   The activation silu(gate) * up is rounded to dtype between the two products; sums over a token's routes are fp32, in their order.
+ *   workspace   device memory on a 512-byte boundary, at least cch_moe_ffn_w4a16_workspace_bytes(...); as above */
+int64_t cch_moe_ffn_w4a16_workspace_bytes(int64_t m, int64_t k, int top_k, int64_t num_experts, int64_t n);
+int cch_moe_ffn_w4a16(const void *x, const int32_t *expert_idx, const float *probs, const void *w1, const void *s1, const void *z1,
+                      const void *w2, const void *s2, const void *z2, void *out, int64_t m, int64_t k, int top_k, int64_t num_experts,
+                      int64_t n, int fmt, int group_size, int dtype, void *workspace, int64_t workspace_bytes, void *stream);
 
 /* Library switches for tests and benchmarks.  They are process-wide (one atomic each, read at
  * every call): two callers that want different settings at the same time race; set them once, or
