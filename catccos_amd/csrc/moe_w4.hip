@@ -71,10 +71,10 @@ extern "C" int cch_moe_ffn_w4a16(const void *x, const int32_t *expert_idx, const
     uint8_t *p = static_cast<uint8_t *>(workspace);
     const int64_t routes = m * top_k;
     if (n > 0)
-        if (const int rc = w4_product(W4_OUT_SWIGLU, fmt, dtype, W4Rows{x, expert_idx, routes, (int)num_experts, top_k},
+        if (const int rc = w4_product(W4_OUT_SWIGLU, fmt, dtype, W4Rows{x, expert_idx, routes, (int)num_experts, top_k, top_k},
                                       w4_matrix(w1, s1, z1, n, k, fmt, group_size), p + at.h, stream))
             return rc;
-    if (const int rc = w4_product(W4_OUT_F32, fmt, dtype, W4Rows{p + at.h, expert_idx, routes, (int)num_experts, 1}, w4_matrix(w2, s2, z2, k, n / 2, fmt, group_size),
+    if (const int rc = w4_product(W4_OUT_F32, fmt, dtype, W4Rows{p + at.h, expert_idx, routes, (int)num_experts, 1, top_k}, w4_matrix(w2, s2, z2, k, n / 2, fmt, group_size),
                                   p + at.y, stream))
         return rc;
     const float *y = reinterpret_cast<const float *>(p + at.y);

@@ -41,16 +41,19 @@ inline W4Matrix w4_matrix(const void *codes, const void *scales, const void *zer
 }
 
 // Where a product's left rows and its weights are: output row r takes row r / x_div of x and, with `experts`, matrix experts[r]
-// (entries outside [0, num_experts): a dropped route, nothing is read or written).
+// (entries outside [0, num_experts): a dropped route, nothing is read or written), top_k of a token back to back.
 struct W4Rows {
     const void *x;
     const int32_t *experts;
     int64_t rows;
-    int num_experts, x_div;
+    int num_experts, x_div, top_k;
 };
 
 // What a product leaves: out[r, n] in the activations' type; silu(gate) * up of columns n and n + N/2 in that type; fp32.
 enum { W4_OUT_PLAIN = 0, W4_OUT_SWIGLU = 1, W4_OUT_F32 = 2 };
+
+constexpr int W4_LIST = 2048;   // routes that a workgroup of the tiled kernel sorts out for itself
+enum { W4_I4_G32 = 0, W4_I4_G64 = 1, W4_I4_G128 = 2, W4_MX = 3 };   // kinds of weights it knows
 
 int w4_product(int out_kind, int fmt, int dtype, const W4Rows &rows, const W4Matrix &w, void *out, void *stream);
 

@@ -70,12 +70,33 @@ static int w4_simple(int out_kind, const W4Rows &rows, const W4Matrix &w, void *
     return launch_status("w4_simple_kernel");
 }
 
+int w4_tile_int4_bf16(int kind, int out_kind, const W4Rows &rows, const W4Matrix &w, void *out, hipStream_t s);   // w4_tile_*.hip
+int w4_tile_int4_f16(int kind, int out_kind, const W4Rows &rows, const W4Matrix &w, void *out, hipStream_t s);
+int w4_tile_mx_bf16(int kind, int out_kind, const W4Rows &rows, const W4Matrix &w, void *out, hipStream_t s);
+int w4_tile_mx_f16(int kind, int out_kind, const W4Rows &rows, const W4Matrix &w, void *out, hipStream_t s);
+
 int w4_product(int out_kind, int fmt, int dtype, const W4Rows &rows, const W4Matrix &w, void *out, void *stream)
 {
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (dtype == CCH_DTYPE_F16)
-        return fmt == CCH_FMT_INT4 ? w4_simple<_Float16, true>(out_kind, rows, w, out, s) : w4_simple<_Float16, false>(out_kind, rows, w, out, s);
-    return fmt == CCH_FMT_INT4 ? w4_simple<__bf16, true>(out_kind, rows, w, out, s) : w4_simple<__bf16, false>(out_kind, rows, w, out, s);
+    const bool half = dtype == CCH_DTYPE_F16, ints = fmt == CCH_FMT_INT4;
+    if (w.k > 0 && w.k % 32 == 0 && aligned(w.codes, 16) && aligned(rows.x, 16) && (!ints || aligned(w.scales, 2))) {
+        const int kind = !ints ? W4_MX : w.group == 32 ? W4_I4_G32 : w.group == 64 ? W4_I4_G64 : W4_I4_G128;
+        const auto tile = ints ? (half ? w4_tile_int4_f16 : w4_tile_int4_bf16) : (half ? w4_tile_mx_f16 : w4_tile_mx_bf16);
+        if (!rows.experts) return tile(kind, out_kind, rows, w, out, s);
+        // routes in windows of as many whole tokens as a workgroup sorts out for itself
+        const int64_t window = W4_LIST / rows.top_k * rows.top_k, cols = out_kind == W4_OUT_SWIGLU ? w.rows / 2 : w.rows;
+        for (int64_t r = 0; r < rows.rows; r += window) {
+            W4Rows some = rows;
+            some.rows = std::min(window, rows.rows - r);
+            some.experts = rows.experts + r;
+            some.x = static_cast<const uint16_t *>(rows.x) + r / rows.x_div * w.k;
+            const int rc = tile(kind, out_kind, some, w, static_cast<uint8_t *>(out) + r * cols * (out_kind == W4_OUT_F32 ? 4 : 2), s);
+            if (rc != CCH_OK) return rc;
+        }
+        return CCH_OK;
+    }
+    if (half) return ints ? w4_simple<_Float16, true>(out_kind, rows, w, out, s) : w4_simple<_Float16, false>(out_kind, rows, w, out, s);
+    return ints ? w4_simple<__bf16, true>(out_kind, rows, w, out, s) : w4_simple<__bf16, false>(out_kind, rows, w, out, s);
 }
 
 // What every product of this kind asks of its weights.
@@ -100,5 +121,5 @@ extern "C" int cch_w4a16_matmul(const void *x, const void *w, const void *scales
     if (const int rc = w4_check("cch_w4a16_matmul", fmt, group_size, dtype)) return rc;
     if (m == 0 || n == 0) return CCH_OK;
     CCH_REQUIRE(out && (k == 0 || (x && w && scales)), "cch_w4a16_matmul: null pointer");
-    return w4_product(W4_OUT_PLAIN, fmt, dtype, W4Rows{x, nullptr, m, 1, 1}, w4_matrix(w, scales, zeros, n, k, fmt, group_size), out, stream);
+    return w4_product(W4_OUT_PLAIN, fmt, dtype, W4Rows{x, nullptr, m, 1, 1, 1}, w4_matrix(w, scales, zeros, n, k, fmt, group_size), out, stream);
 }
