@@ -79,7 +79,9 @@ int w4_product(int out_kind, int fmt, int dtype, const W4Rows &rows, const W4Mat
 {
     hipStream_t s = static_cast<hipStream_t>(stream);
     const bool half = dtype == CCH_DTYPE_F16, ints = fmt == CCH_FMT_INT4;
-    if (w.k > 0 && w.k % 32 == 0 && aligned(w.codes, 16) && aligned(rows.x, 16) && (!ints || aligned(w.scales, 2))) {
+    // (offsets of lanes are 32 bits: 64 rows of codes, and all rows of x that a workgroup can meet)
+    const int64_t x_rows = rows.experts ? std::min<int64_t>(rows.rows, W4_LIST) : 64;
+    if (w.k > 0 && w.k % 32 == 0 && w.k <= 1 << 24 && x_rows * w.k < (int64_t)1 << 30 && aligned(w.codes, 16) && aligned(rows.x, 16) && (!ints || aligned(w.scales, 2))) {
         const int kind = !ints ? W4_MX : w.group == 32 ? W4_I4_G32 : w.group == 64 ? W4_I4_G64 : W4_I4_G128;
         const auto tile = ints ? (half ? w4_tile_int4_f16 : w4_tile_int4_bf16) : (half ? w4_tile_mx_f16 : w4_tile_mx_bf16);
         if (!rows.experts) return tile(kind, out_kind, rows, w, out, s);

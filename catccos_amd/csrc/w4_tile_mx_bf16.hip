@@ -5,7 +5,7 @@ namespace cch {
 
 int w4_tile_mx_bf16(int kind, int out_kind, const W4Rows &rows, const W4Matrix &w, void *out, hipStream_t s)
 {
-    return w4_tile_choose<__bf16, W4_MX>(out_kind, rows, w, out, s);
+    return w4_tile_choose<__bf16, W4_MX, false>(out_kind, rows, w, out, s);
 }
 
 }  // namespace cch
