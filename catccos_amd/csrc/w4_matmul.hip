@@ -84,7 +84,17 @@ int w4_product(int out_kind, int fmt, int dtype, const W4Rows &rows, const W4Mat
     if (w.k > 0 && w.k % 32 == 0 && w.k <= 1 << 24 && x_rows * w.k < (int64_t)1 << 30 && aligned(w.codes, 16) && aligned(rows.x, 16) && (!ints || aligned(w.scales, 2))) {
         const int kind = !ints ? W4_MX : w.group == 32 ? W4_I4_G32 : w.group == 64 ? W4_I4_G64 : W4_I4_G128;
         const auto tile = ints ? (half ? w4_tile_int4_f16 : w4_tile_int4_bf16) : (half ? w4_tile_mx_f16 : w4_tile_mx_bf16);
-        if (!rows.experts) return tile(kind, out_kind, rows, w, out, s);
+        if (!rows.experts) {
+            // as many rows as the grid's second dimension has tiles of 16 for
+            for (int64_t r = 0; r < rows.rows; r += 65535 * 16) {
+                W4Rows some = rows;
+                some.rows = std::min<int64_t>(65535 * 16, rows.rows - r);
+                some.x = static_cast<const uint16_t *>(rows.x) + r * w.k;
+                const int rc = tile(kind, out_kind, some, w, static_cast<uint16_t *>(out) + r * w.rows, s);
+                if (rc != CCH_OK) return rc;
+            }
+            return CCH_OK;
+        }
         // routes in windows of as many whole tokens as a workgroup sorts out for itself
         const int64_t window = W4_LIST / rows.top_k * rows.top_k, cols = out_kind == W4_OUT_SWIGLU ? w.rows / 2 : w.rows;
         for (int64_t r = 0; r < rows.rows; r += window) {

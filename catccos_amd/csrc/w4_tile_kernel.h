@@ -104,7 +104,7 @@ struct W4Tile {
         return (w4_u32x4){z, z, z, z};
     }
 
-    static __device__ __forceinline__ w4_u32x4 operand(uint32_t q, float scale)
+    static __device__ __forceinline__ w4_u32x4 operand(uint32_t q, float scale, uint32_t mask, uint32_t sixteen)
     {
         w4_u32x4 r;
         if (MX) {
@@ -114,10 +114,10 @@ struct W4Tile {
             r[3] = Type::template fp4<3>(q, scale);
         } else {
             constexpr int S = Type::SHIFT;
-            r[0] = (q << S & Type::MASK) | Type::SIXTEEN;
-            r[1] = ((S >= 4 ? q << (S >= 4 ? S - 4 : 0) : q >> (S >= 4 ? 0 : 4 - S)) & Type::MASK) | Type::SIXTEEN;
-            r[2] = (q >> (8 - S) & Type::MASK) | Type::SIXTEEN;
-            r[3] = (q >> (12 - S) & Type::MASK) | Type::SIXTEEN;
+            r[0] = (q << S & mask) | sixteen;
+            r[1] = ((S >= 4 ? q << (S >= 4 ? S - 4 : 0) : q >> (S >= 4 ? 0 : 4 - S)) & mask) | sixteen;
+            r[2] = (q >> (8 - S) & mask) | sixteen;
+            r[3] = (q >> (12 - S) & mask) | sixteen;
         }
         return r;
     }
@@ -143,7 +143,7 @@ __host__ __device__ inline int w4_param_pitch(int groups, int param) { return ((
 
 // Scales and zero points of groups [g0, g0 + count) of all tiles to LDS.
 template <class T, int KIND, bool ZEROS, int TILES, int HALVES, int THREADS>
-__device__ __forceinline__ void w4_stage_params(const W4Matrix &w, const W4Job &job, uint8_t *params, int pitch, int g0, int count)
+__device__ __forceinline__ void w4_stage_params(const int row_groups, const W4Job &job, uint8_t *params, int pitch, int g0, int count)
 {
     typedef W4Tile<T, KIND, ZEROS> Tile;
     typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
@@ -152,7 +152,7 @@ __device__ __forceinline__ void w4_stage_params(const W4Matrix &w, const W4Job &
 #pragma unroll
     for (int h = 0; h < HALVES; h++) {
         uint8_t *to = params + h * ROWS * pitch;
-        if (count == w.row_groups && aligned16(job.scales[h]) && (!ZEROS || aligned16(job.zeros[h]))) {
+        if (count == row_groups && aligned16(job.scales[h]) && (!ZEROS || aligned16(job.zeros[h]))) {
             // the rows lie back to back: runs of eight (a last one may end behind the last row, in the next one's)
             const int total = job.rows * count;
             for (int i = threadIdx.x * 8; i < total; i += THREADS * 8) {
@@ -192,7 +192,7 @@ __device__ __forceinline__ void w4_stage_params(const W4Matrix &w, const W4Job &
         } else {
             for (int i = threadIdx.x; i < job.rows * count; i += THREADS) {
                 const int row = i / count, g = i - row * count;
-                const int64_t at = (int64_t)row * w.row_groups + g0 + g;
+                const int64_t at = (int64_t)row * row_groups + g0 + g;
                 const uint32_t s = SIZE == 1 ? job.scales[h][at] : reinterpret_cast<const uint16_t *>(job.scales[h])[at];
                 Tile::put_param(to + row * pitch + g * P, s, ZEROS ? job.zeros[h][at] : 0);
             }
@@ -217,8 +217,9 @@ __device__ __forceinline__ void w4_sums(const W4Matrix &w, const W4Job &job, con
 {
     typedef W4Tile<T, KIND, ZEROS> Tile;
     constexpr int NT = S::NT, MT = S::MT, XU = S::XU, COLS = NT / HALVES, COUNT = NT + XU, D = S::D;
-    // x's order: by the wave that loaded it, in LDS, a block ahead; or, where no wave shares it and all its rows are there, with the operands
-    constexpr bool ORDER_IN_LDS = !Tile::MX && (S::WN > 1 || S::XR < 4), ORDER_LATE = !Tile::MX && !ORDER_IN_LDS;
+    // x's order: by the wave that loaded it, in LDS, a block ahead; or, where no wave shares it, with the operands
+    constexpr bool ORDER_IN_LDS = !Tile::MX && S::WN > 1, ORDER_LATE = !Tile::MX && !ORDER_IN_LDS;
+    constexpr bool TWO = Tile::PER > 1 && NT * MT <= 2;
     constexpr int LANDED = ORDER_IN_LDS ? D - 3 : D - 2;                     // blocks behind the one awaited that are still on their way
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int wn = wave % S::WN, wk = wave / S::WN, n = lane & 15, g = lane >> 4, last = (w.k - 1) / 128, f = n >> 2;
@@ -247,6 +248,9 @@ __device__ __forceinline__ void w4_sums(const W4Matrix &w, const W4Job &job, con
 #pragma unroll
         for (int mt = 0; mt < MT; mt++) acc[j][mt] = (w4_f32x4){0, 0, 0, 0};
 
+    uint32_t mask = Tile::Type::MASK, sixteen = Tile::Type::SIXTEEN;
+    asm volatile("" : "+s"(mask), "+v"(sixteen));               // (in registers: one instruction takes both, none takes two literals)
+
     auto request = [&](int block, int end, int slot) {
         const bool none = block >= end, part = block == last;
         const uint32_t at = none ? 0 : block;
@@ -271,13 +275,13 @@ __device__ __forceinline__ void w4_sums(const W4Matrix &w, const W4Job &job, con
         if (b0 > 0) __syncthreads();
 #pragma unroll
         for (int d = 0; d < D - 1; d++) request(begin + d, end, d);
-        const int g0 = b0 * Tile::GROUPS, count = min(here * Tile::GROUPS, w.row_groups - g0);
-        w4_stage_params<T, KIND, ZEROS, S::TILES, HALVES, S::THREADS>(w, job, params, pitch, g0, count);
-        if (ORDER_IN_LDS) {
-            CCH_WAIT_VM((D - 2) * COUNT);
-            asm volatile("" ::: "memory");
-            order(0);
-        }
+        int row_groups = w.row_groups;
+        asm volatile("" : "+s"(row_groups));   // (nothing of what follows is worked out in front of the requests)
+        const int g0 = b0 * Tile::GROUPS, count = min(here * Tile::GROUPS, row_groups - g0);
+        w4_stage_params<T, KIND, ZEROS, S::TILES, HALVES, S::THREADS>(row_groups, job, params, pitch, g0, count);
+        CCH_WAIT_VM(0);                // (the compiler knows of the loads above, not of the requests: with some of its own open it would wait for all in the loop)
+        asm volatile("" ::: "memory");
+        if (ORDER_IN_LDS) order(0);
         CCH_WAIT_LGKM0();
         CCH_BARRIER();
         int slot = 0;
@@ -309,7 +313,7 @@ __device__ __forceinline__ void w4_sums(const W4Matrix &w, const W4Job &job, con
                     for (int i = 0; i < Tile::GROUPS; i++) p[j][i] = first + i < count ? Tile::get_param(params + row * pitch + (first + i) * Tile::PARAM) : 0;
                 }
             }
-            w4_f32x4 part[NT][MT];
+            w4_f32x4 part[NT][MT], less[NT][MT];   // of the codes and of the constant: two chains of instructions, not one of twice the length
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 w4_u32x4 x[MT];
@@ -321,20 +325,20 @@ __device__ __forceinline__ void w4_sums(const W4Matrix &w, const W4Job &job, con
 #pragma unroll
                 for (int j = 0; j < NT; j++) {
                     if constexpr (Tile::IN_WEIGHT) {
-                        const w4_u32x4 b = Tile::operand(q[j][i], Tile::scale_of(p[j][0]));
+                        const w4_u32x4 b = Tile::operand(q[j][i], Tile::scale_of(p[j][0]), 0, 0);
 #pragma unroll
                         for (int mt = 0; mt < MT; mt++) acc[j][mt] = Tile::Type::mfma(x[mt], b, acc[j][mt]);
                     } else {
-                        const w4_u32x4 b = Tile::operand(q[j][i], 1.0f);
+                        const w4_u32x4 b = Tile::operand(q[j][i], 1.0f, mask, sixteen);
                         const uint32_t pj = p[j][i / Tile::PER];
 #pragma unroll
                         for (int mt = 0; mt < MT; mt++) {
-                            if (i % Tile::PER == 0) part[j][mt] = (w4_f32x4){0, 0, 0, 0};
-                            if (!Tile::MX) part[j][mt] = Tile::Type::mfma(x[mt], Tile::zero_of(pj), part[j][mt]);
+                            if (i % Tile::PER == 0) part[j][mt] = less[j][mt] = (w4_f32x4){0, 0, 0, 0};
+                            if (!Tile::MX) (TWO ? less : part)[j][mt] = Tile::Type::mfma(x[mt], Tile::zero_of(pj), (TWO ? less : part)[j][mt]);
                             part[j][mt] = Tile::Type::mfma(x[mt], b, part[j][mt]);
                             if (i % Tile::PER == Tile::PER - 1) {
 #pragma unroll
-                                for (int r = 0; r < 4; r++) acc[j][mt][r] += Tile::scale_of(pj) * part[j][mt][r];
+                                for (int r = 0; r < 4; r++) acc[j][mt][r] += Tile::scale_of(pj) * (TWO && !Tile::MX ? part[j][mt][r] + less[j][mt][r] : part[j][mt][r]);
                             }
                         }
                     }
@@ -350,7 +354,7 @@ __device__ __forceinline__ void w4_sums(const W4Matrix &w, const W4Job &job, con
 // Which matrix, and which rows of x: workgroup column `slot` of the grid takes the slot-th expert that some route names (up to 64 routes: the expert of route
 // `slot`, if no earlier one names it).  Returns the number of its routes, their numbers in `list`; 0: nothing to do.
 template <int W>
-__device__ __forceinline__ int w4_routes(const W4Rows &rows, int slot, int (&list)[W4_LIST], int (&scratch)[1024 + 2], int &expert)
+__device__ __forceinline__ int w4_routes(const W4Rows &rows, int slot, int *list, int *scratch, int &expert)
 {
     const int lane = threadIdx.x & 63, routes = (int)rows.rows;
     if (routes <= 64) {
@@ -456,18 +460,15 @@ __device__ __forceinline__ void w4_pass(const W4Rows &rows, const W4Matrix &w, i
 }
 
 template <class T, int KIND, bool ZEROS, class S, int OUT, bool GROUPED>
-__global__ __launch_bounds__(S::THREADS, S::MT * S::NT <= 4 ? 4 : 2) void w4_tile_kernel(W4Rows rows, W4Matrix w, int pitch, int chunk, void *__restrict__ out)
+__global__ __launch_bounds__(S::THREADS, S::MT * S::NT <= 4 ? 4 : 2) void w4_tile_kernel(W4Rows rows, W4Matrix w, int pitch, int chunk, int list_at, void *__restrict__ out)
 {
     if constexpr (!GROUPED) {
-        const int total = (int)rows.rows;
-        for (int m0 = (int)blockIdx.y * (16 * S::MT); m0 < total; m0 += (int)gridDim.y * (16 * S::MT)) {
-            w4_pass<T, KIND, ZEROS, S, OUT, false>(rows, w, 0, nullptr, m0, total, pitch, chunk, out);
-            __syncthreads();
-        }
+        w4_pass<T, KIND, ZEROS, S, OUT, false>(rows, w, 0, nullptr, (int)blockIdx.y * (16 * S::MT), (int)rows.rows, pitch, chunk, out);
     } else {
-        __shared__ int list[W4_LIST], scratch[1024 + 2];
+        int *const scratch = reinterpret_cast<int *>(smem), *const list = reinterpret_cast<int *>(smem + list_at);   // (the rings come later)
         int expert = 0;
         const int total = w4_routes<S::W>(rows, blockIdx.y, list, scratch, expert);
+        __syncthreads();
         for (int m0 = 0; m0 < total; m0 += S::MT == 1 ? 4 * S::XR : 16 * S::MT) {
             w4_pass<T, KIND, ZEROS, S, OUT, true>(rows, w, expert, list, m0, total, pitch, chunk, out);
             __syncthreads();
@@ -483,25 +484,28 @@ int w4_tile_launch(const W4Rows &rows, const W4Matrix &w, void *out, hipStream_t
     auto kern = w4_tile_kernel<T, KIND, ZEROS, S, OUT, GROUPED>;
     constexpr int HALVES = OUT == W4_OUT_SWIGLU ? 2 : 1, COLS = S::NT / HALVES;
     // blocks whose scales are in LDS at a time, evenly
-    constexpr int ROOM = 160 * 1024 - S::FIXED - (GROUPED ? 4 * (W4_LIST + 1024 + 2) : 0), PARAMS = ROOM < 32 * 1024 ? ROOM : 32 * 1024;
+    constexpr int ROOM = 160 * 1024 - S::FIXED - (GROUPED ? 4 * W4_LIST : 0), PARAMS = ROOM < 32 * 1024 ? ROOM : 32 * 1024;
     static_assert(PARAMS >= 16 * S::TILES * 4 * 8);
     const int blocks = (w.k + 127) / 128, most = ((PARAMS / (16 * S::TILES) - 4) / 4 * 4) / (Tile::GROUPS * Tile::PARAM), chunks = (blocks + most - 1) / most;
-    const int chunk = (blocks + chunks - 1) / chunks, pitch = w4_param_pitch(chunk * Tile::GROUPS, Tile::PARAM), lds = S::FIXED + 16 * S::TILES * pitch;
-    if (S::FIXED + PARAMS > 48 * 1024) {
+    const int chunk = (blocks + chunks - 1) / chunks, pitch = w4_param_pitch(chunk * Tile::GROUPS, Tile::PARAM), list_at = S::FIXED + 16 * S::TILES * pitch;
+    const int lds = list_at + (GROUPED ? 4 * (int)rows.rows : 0);
+    static_assert(S::FIXED >= 4 * (1024 + 2));
+    if (S::FIXED + PARAMS + (GROUPED ? 4 * W4_LIST : 0) > 48 * 1024) {
         // set once per device and kernel; setting it twice from two threads is harmless
         static std::atomic<uint64_t> attr_set{0};
         int dev = 0;
         CCH_HIP(hipGetDevice(&dev));
         const uint64_t dev_bit = (uint64_t)1 << (dev & 63);
         if (dev >= 64 || !(attr_set.load(std::memory_order_acquire) & dev_bit)) {
-            CCH_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, S::FIXED + PARAMS));
+            CCH_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                        S::FIXED + PARAMS + (GROUPED ? 4 * W4_LIST : 0)));
             attr_set.fetch_or(dev_bit, std::memory_order_release);
         }
     }
     const int64_t cols = w.rows / HALVES, per = 16 * S::WN * COLS;
     const int64_t y = GROUPED ? (rows.rows <= 64 ? rows.rows : std::min<int64_t>(rows.num_experts, rows.rows))
-                              : std::min<int64_t>((rows.rows + 16 * S::MT - 1) / (16 * S::MT), 65535);
-    hipLaunchKernelGGL(kern, dim3((unsigned)((cols + per - 1) / per), (unsigned)y), dim3(S::THREADS), lds, s, rows, w, pitch, chunk, out);
+                              : (rows.rows + 16 * S::MT - 1) / (16 * S::MT);
+    hipLaunchKernelGGL(kern, dim3((unsigned)((cols + per - 1) / per), (unsigned)y), dim3(S::THREADS), lds, s, rows, w, pitch, chunk, list_at, out);
     return launch_status("w4_tile_kernel");
 }
 
@@ -511,24 +515,31 @@ int w4_tile_choose(int out_kind, const W4Rows &rows, const W4Matrix &w, void *ou
 {
 #define W4_GO(S, OUT, GROUPED) w4_tile_launch<T, KIND, ZEROS, S, OUT, GROUPED>(rows, w, out, s)
     if (out_kind == W4_OUT_PLAIN) {
-        typedef W4Shape<1, 1, 1, 1, 8, 4> One;
-        typedef W4Shape<2, 1, 1, 1, 4, 4> OneWide;
-        typedef W4Shape<1, 1, 4, 2, 4, 4> Few;
-        typedef W4Shape<2, 1, 4, 4, 2, 4> FewWide;
-        typedef W4Shape<1, 2, 8, 4, 2, 3> Some;
-        typedef W4Shape<2, 4, 16, 4, 2, 3> Many;
+        typedef W4Shape<1, 1, 1, 1, 8, 3> One;
+        typedef W4Shape<2, 1, 1, 1, 4, 3> OneWide;
+        typedef std::conditional_t<KIND == W4_MX, W4Shape<1, 1, 4, 2, 4, 3>, W4Shape<1, 1, 4, 1, 8, 3>> Few;
+        typedef W4Shape<1, 1, 4, 4, 2, 3> FewWide;
+        typedef W4Shape<1, 2, 8, 2, 4, 3> Some;
+        typedef W4Shape<1, 4, 16, 2, 2, 3> Many;
+        typedef W4Shape<1, 4, 16, 8, 1, 3> ManyWide;
         const bool wide = w.rows >= 16 * 2 * 256;
         if (rows.rows <= 4) return wide ? W4_GO(OneWide, W4_OUT_PLAIN, false) : W4_GO(One, W4_OUT_PLAIN, false);
         if (rows.rows <= 16) return wide ? W4_GO(FewWide, W4_OUT_PLAIN, false) : W4_GO(Few, W4_OUT_PLAIN, false);
         if (rows.rows <= 32) return W4_GO(Some, W4_OUT_PLAIN, false);
-        return W4_GO(Many, W4_OUT_PLAIN, false);
+        return wide ? W4_GO(ManyWide, W4_OUT_PLAIN, false) : W4_GO(Many, W4_OUT_PLAIN, false);
     }
-    typedef W4Shape<2, 1, 1, 1, 4, 4> One;
-    typedef W4Shape<2, 1, 4, 2, 2, 4> Few;
-    typedef W4Shape<2, 2, 8, 4, 1, 4> Some;
     const int64_t tokens = rows.rows / rows.top_k;   // no expert has more of them
-    if (out_kind == W4_OUT_SWIGLU) return tokens <= 4 ? W4_GO(One, W4_OUT_SWIGLU, true) : tokens <= 16 ? W4_GO(Few, W4_OUT_SWIGLU, true) : W4_GO(Some, W4_OUT_SWIGLU, true);
-    return tokens <= 4 ? W4_GO(One, W4_OUT_F32, true) : tokens <= 16 ? W4_GO(Few, W4_OUT_F32, true) : W4_GO(Some, W4_OUT_F32, true);
+    const bool few = rows.rows <= 8 * rows.num_experts;
+    if (out_kind == W4_OUT_SWIGLU) {
+        typedef W4Shape<2, 1, 1, 1, 4, 3> One;
+        typedef W4Shape<2, 1, 4, 4, 1, 3> Few;
+        typedef W4Shape<2, 4, 16, 8, 1, 3> Some;
+        return tokens <= 4 ? W4_GO(One, W4_OUT_SWIGLU, true) : tokens <= 16 || few ? W4_GO(Few, W4_OUT_SWIGLU, true) : W4_GO(Some, W4_OUT_SWIGLU, true);
+    }
+    typedef W4Shape<2, 1, 1, 1, 4, 3> One;
+    typedef W4Shape<1, 1, 4, 4, 1, 3> Few;
+    typedef W4Shape<1, 2, 8, 8, 1, 3> Some;
+    return tokens <= 4 ? W4_GO(One, W4_OUT_F32, true) : tokens <= 16 || few ? W4_GO(Few, W4_OUT_F32, true) : W4_GO(Some, W4_OUT_F32, true);
 #undef W4_GO
 }
 
