@@ -2,7 +2,7 @@
 //
 // A workgroup has WN * NT tiles of 16 rows of weights and MT tiles of 16 rows of x, and walks K in blocks of 128.  Its waves are WN columns, NT tiles each, times
 // WK parts of K, whose sums meet in LDS at the end.  A block's codes (64 bytes of each row, a wave's own) and x (256 bytes of each row, shared by a part's WN
-// waves) come from memory straight into rings of D blocks in LDS, in runs that the memory system takes whole: four lanes to a row of codes, sixteen to a row of x.
+// waves) come from memory straight into rings of two blocks in LDS, in runs that the memory system takes whole: four lanes to a row of codes, sixteen to a row of x.
 // (Loaded by the lanes that need them, every lane of 16 another row, a block of codes costs the vector cache 64 accesses instead of 16, and x as many per instruction;
 // through registers the loop needs its blocks unrolled, and its code is what a small launch waits for.)  One barrier a block, none where WN is 1.
 //
@@ -141,6 +141,11 @@ struct W4Job {
 constexpr int W4_CODES = 1024, W4_X4 = 1024;   // of a tile, of four rows of x
 __host__ __device__ inline int w4_param_pitch(int groups, int param) { return ((groups * param + 3) / 4 | 1) * 4; }
 
+// What is exchanged: piece p of a row of codes lies at p ^ turn(row / 4), of x at p ^ x_turn(row).  A 16-byte read serves 16 lanes at a time, and
+// these are lanes 0-3, 12-15, 20-23, 24-27 and so on: rows of fours from two neighbouring lane groups, which have to differ.
+__device__ __forceinline__ int w4_turn(int fours) { return -fours & 3; }
+__device__ __forceinline__ int w4_x_turn(int row) { return (row & 3) | w4_turn(row >> 2) << 2; }
+
 // Scales and zero points of groups [g0, g0 + count) of all tiles to LDS.
 template <class T, int KIND, bool ZEROS, int TILES, int HALVES, int THREADS>
 __device__ __forceinline__ void w4_stage_params(const int row_groups, const W4Job &job, uint8_t *params, int pitch, int g0, int count)
@@ -200,15 +205,15 @@ __device__ __forceinline__ void w4_stage_params(const int row_groups, const W4Jo
     }
 }
 
-// The shape of a workgroup.  XR: four rows of x each are loaded (MT = 1: as few as there are).  D: blocks in a ring.
-template <int NT_, int MT_, int XR_, int WN_, int WK_, int D_>
+// The shape of a workgroup.  XR: four rows of x each are loaded (MT = 1: as few as there are).
+template <int NT_, int MT_, int XR_, int WN_, int WK_>
 struct W4Shape {
-    static constexpr int NT = NT_, MT = MT_, XR = XR_, WN = WN_, WK = WK_, D = D_, W = WN * WK, THREADS = 64 * W, TILES = WN * NT;
+    static constexpr int NT = NT_, MT = MT_, XR = XR_, WN = WN_, WK = WK_, W = WN * WK, THREADS = 64 * W, TILES = WN * NT;
     static constexpr int XU = XR / WN;                                       // x loads of a wave and block
-    static constexpr int X_RING = D * XR * W4_X4, CODE_RING = D * NT * W4_CODES;
+    static constexpr int X_RING = 2 * XR * W4_X4, CODE_RING = 2 * NT * W4_CODES;
     static constexpr int RINGS = WK * X_RING + W * CODE_RING, SUMS = W * NT * MT * 1024;
     static constexpr int FIXED = RINGS > SUMS ? RINGS : SUMS;                // LDS in front of the scales
-    static_assert(XR % WN == 0 && XR <= 4 * MT && (MT == 1 || XR == 4 * MT) && D >= 3);
+    static_assert(XR % WN == 0 && XR <= 4 * MT && (MT == 1 || XR == 4 * MT));
 };
 
 // The wave's sums of its tiles over its part of K.
@@ -216,18 +221,16 @@ template <class T, int KIND, bool ZEROS, class S, int HALVES>
 __device__ __forceinline__ void w4_sums(const W4Matrix &w, const W4Job &job, const uint32_t (&x_row)[S::XU], int pitch, int chunk, w4_f32x4 (&acc)[S::NT][S::MT])
 {
     typedef W4Tile<T, KIND, ZEROS> Tile;
-    constexpr int NT = S::NT, MT = S::MT, XU = S::XU, COLS = NT / HALVES, COUNT = NT + XU, D = S::D;
-    // x's order: by the wave that loaded it, in LDS, a block ahead; or, where no wave shares it, with the operands
+    constexpr int NT = S::NT, MT = S::MT, XU = S::XU, COLS = NT / HALVES;
+    // x's order: by the wave that loaded it, in LDS; or, where no wave shares it, with the operands
     constexpr bool ORDER_IN_LDS = !Tile::MX && S::WN > 1, ORDER_LATE = !Tile::MX && !ORDER_IN_LDS;
-    constexpr bool TWO = Tile::PER > 1 && NT * MT <= 2;
-    constexpr int LANDED = ORDER_IN_LDS ? D - 3 : D - 2;                     // blocks behind the one awaited that are still on their way
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int wn = wave % S::WN, wk = wave / S::WN, n = lane & 15, g = lane >> 4, last = (w.k - 1) / 128, f = n >> 2;
+    const int wn = wave % S::WN, wk = wave / S::WN, n = lane & 15, g = lane >> 4, last = (w.k - 1) / 128, f = w4_turn(n >> 2);
     uint8_t *const params = smem + S::FIXED, *const x_ring = smem + wk * S::X_RING, *const code_ring = smem + S::WK * S::X_RING + wave * S::CODE_RING;
     const uint32_t x_lds = w4_lds_address(x_ring) + wn * XU * W4_X4, code_lds = w4_lds_address(code_ring);
     // this lane's loads of a block: 16 bytes of codes of row lane / 4, of x of row lane / 16, pieces of a row exchanged so that an operand's lanes, of different
     // rows, meet different banks; of the last block perhaps none
-    const int code_piece = (lane & 3) ^ (lane >> 4), tile0 = wn * COLS;
+    const int code_piece = (lane & 3) ^ w4_turn(lane >> 4), tile0 = wn * COLS;
     const uint32_t code_at = (lane >> 2) * w.row_bytes + 16 * code_piece;
     const bool code_in_last = last * 128 + 32 * code_piece < w.k;
     bool code_row[COLS], x_in_last[XU];
@@ -236,12 +239,12 @@ __device__ __forceinline__ void w4_sums(const W4Matrix &w, const W4Job &job, con
     for (int j = 0; j < COLS; j++) code_row[j] = 16 * (tile0 + j) + (lane >> 2) < job.rows;
 #pragma unroll
     for (int u = 0; u < XU; u++) {
-        const int piece = (lane & 15) ^ ((4 * (wn * XU + u) + g) & 15);
+        const int piece = (lane & 15) ^ w4_x_turn(4 * (wn * XU + u) + g);
         x_at[u] = x_row[u] + 16 * piece;
         x_in_last[u] = last * 128 + 8 * piece < w.k;
     }
     const int x_n = MT == 1 ? n & (4 * S::XR - 1) : n;
-    const uint32_t code_from = n * 64 + (Tile::BY_DWORD ? f * 16 + 4 * g : (g ^ f) * 16), x_from = x_n * 256 + ((Tile::BY_DWORD ? g : 4 * g) ^ x_n) * 16;
+    const uint32_t code_from = n * 64 + (Tile::BY_DWORD ? f * 16 + 4 * g : (g ^ f) * 16), x_from = x_n * 256 + ((Tile::BY_DWORD ? g : 4 * g) ^ w4_x_turn(x_n)) * 16;
     const Rsrc codes[2] = {make_rsrc(job.codes[0], W4_REACH), make_rsrc(job.codes[HALVES - 1], W4_REACH)}, xs = make_rsrc(job.x, W4_REACH);
 #pragma unroll
     for (int j = 0; j < NT; j++)
@@ -269,12 +272,72 @@ __device__ __forceinline__ void w4_sums(const W4Matrix &w, const W4Job &job, con
             *p = Tile::x_order(*p);
         }
     };
+    // What a block's products take from LDS; read while the block before is multiplied.
+    struct Operands {
+        w4_u32x4 q[NT], x[MT][4];
+        uint32_t p[NT][Tile::IN_WEIGHT ? 1 : Tile::GROUPS];
+    };
+    auto read = [&](Operands &o, int slot, int first, int count) {     // first: group of the block in the scales there are
+        const uint8_t *const c = code_ring + slot * NT * W4_CODES, *const xb = x_ring + slot * S::XR * W4_X4;
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            if constexpr (Tile::BY_DWORD) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) o.q[j][i] = *reinterpret_cast<const uint32_t *>(c + j * W4_CODES + (code_from ^ (16 * i)));
+            } else {
+                o.q[j] = *reinterpret_cast<const w4_u32x4 *>(c + j * W4_CODES + code_from);
+            }
+            // of groups behind K's last one there is no scale: none is needed, but it must be a number
+            const int row = (j / COLS) * (16 * S::WN * COLS) + 16 * (tile0 + j % COLS) + n;
+            if constexpr (Tile::IN_WEIGHT) {
+                o.p[j][0] = first + g < count ? Tile::get_param(params + row * pitch + (first + g) * Tile::PARAM) : 0;
+            } else {
+#pragma unroll
+                for (int i = 0; i < Tile::GROUPS; i++) o.p[j][i] = first + i < count ? Tile::get_param(params + row * pitch + (first + i) * Tile::PARAM) : 0;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) o.x[mt][i] = *reinterpret_cast<const w4_u32x4 *>(xb + mt * 4 * W4_X4 + (x_from ^ ((Tile::BY_DWORD ? 64 : 16) * i)));
+    };
+    auto multiply = [&](Operands &o) {
+        w4_f32x4 part[NT][MT];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (ORDER_LATE) {
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++) o.x[mt][i] = Tile::x_order(o.x[mt][i]);
+            }
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+                if constexpr (Tile::IN_WEIGHT) {
+                    const w4_u32x4 b = Tile::operand(o.q[j][i], Tile::scale_of(o.p[j][0]), 0, 0);
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) acc[j][mt] = Tile::Type::mfma(o.x[mt][i], b, acc[j][mt]);
+                } else {
+                    const w4_u32x4 b = Tile::operand(o.q[j][i], 1.0f, mask, sixteen);
+                    const uint32_t pj = o.p[j][i / Tile::PER];
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) {
+                        if (i % Tile::PER == 0) part[j][mt] = (w4_f32x4){0, 0, 0, 0};
+                        if (!Tile::MX) part[j][mt] = Tile::Type::mfma(o.x[mt][i], Tile::zero_of(pj), part[j][mt]);
+                        part[j][mt] = Tile::Type::mfma(o.x[mt][i], b, part[j][mt]);
+                        if (i % Tile::PER == Tile::PER - 1) {
+#pragma unroll
+                            for (int r = 0; r < 4; r++) acc[j][mt][r] += Tile::scale_of(pj) * part[j][mt][r];
+                        }
+                    }
+                }
+            }
+        }
+    };
     const int blocks = last + 1;
     for (int b0 = 0; b0 < blocks; b0 += chunk) {
         const int here = min(chunk, blocks - b0), begin = b0 + here * wk / S::WK, end = b0 + here * (wk + 1) / S::WK, steps = (here + S::WK - 1) / S::WK;
         if (b0 > 0) __syncthreads();
 #pragma unroll
-        for (int d = 0; d < D - 1; d++) request(begin + d, end, d);
+        for (int d = 0; d < 2; d++) request(begin + d, end, d);
         int row_groups = w.row_groups;
         asm volatile("" : "+s"(row_groups));   // (nothing of what follows is worked out in front of the requests)
         const int g0 = b0 * Tile::GROUPS, count = min(here * Tile::GROUPS, row_groups - g0);
@@ -284,67 +347,26 @@ __device__ __forceinline__ void w4_sums(const W4Matrix &w, const W4Job &job, con
         if (ORDER_IN_LDS) order(0);
         CCH_WAIT_LGKM0();
         CCH_BARRIER();
-        int slot = 0;
-        for (int step = 0; step < steps; step++) {
-            const int block = begin + step, next = slot + 1 == D ? 0 : slot + 1, free = slot == 0 ? D - 1 : slot - 1;
-            CCH_WAIT_VM(LANDED * COUNT);
+        Operands a, b;
+        const int group0 = (begin - b0) * Tile::GROUPS;
+        read(a, 0, group0, count);
+        // ring slot `SLOT` holds block `step`, whose operands are read or on their way; the other one the next
+        auto advance = [&](auto which, Operands &o, int step) {
+            constexpr int SLOT = decltype(which)::value;
+            CCH_WAIT_VM(0);
             asm volatile("" ::: "memory");
-            if (ORDER_IN_LDS) order(next);
-            CCH_WAIT_LGKM0();          // (and this wave has read what it wanted of the block before)
+            if (ORDER_IN_LDS) order(1 - SLOT);
+            CCH_WAIT_LGKM0();          // (and this wave has the operands of block `step`)
             if (S::WN > 1) CCH_BARRIER();
-            request(block + D - 1, end, free);
-            const uint8_t *const c = code_ring + slot * NT * W4_CODES, *const xb = x_ring + slot * S::XR * W4_X4;
-            w4_u32x4 q[NT];
-            uint32_t p[NT][Tile::IN_WEIGHT ? 1 : Tile::GROUPS];
-#pragma unroll
-            for (int j = 0; j < NT; j++) {
-                if constexpr (Tile::BY_DWORD) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) q[j][i] = *reinterpret_cast<const uint32_t *>(c + j * W4_CODES + (code_from ^ (16 * i)));
-                } else {
-                    q[j] = *reinterpret_cast<const w4_u32x4 *>(c + j * W4_CODES + code_from);
-                }
-                // of groups behind K's last one there is no scale: none is needed, but it must be a number
-                const int row = (j / COLS) * (16 * S::WN * COLS) + 16 * (tile0 + j % COLS) + n, first = (block - b0) * Tile::GROUPS;
-                if constexpr (Tile::IN_WEIGHT) {
-                    p[j][0] = first + g < count ? Tile::get_param(params + row * pitch + (first + g) * Tile::PARAM) : 0;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < Tile::GROUPS; i++) p[j][i] = first + i < count ? Tile::get_param(params + row * pitch + (first + i) * Tile::PARAM) : 0;
-                }
-            }
-            w4_f32x4 part[NT][MT], less[NT][MT];   // of the codes and of the constant: two chains of instructions, not one of twice the length
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                w4_u32x4 x[MT];
-#pragma unroll
-                for (int mt = 0; mt < MT; mt++) {
-                    x[mt] = *reinterpret_cast<const w4_u32x4 *>(xb + mt * 4 * W4_X4 + (x_from ^ ((Tile::BY_DWORD ? 64 : 16) * i)));
-                    if (ORDER_LATE) x[mt] = Tile::x_order(x[mt]);
-                }
-#pragma unroll
-                for (int j = 0; j < NT; j++) {
-                    if constexpr (Tile::IN_WEIGHT) {
-                        const w4_u32x4 b = Tile::operand(q[j][i], Tile::scale_of(p[j][0]), 0, 0);
-#pragma unroll
-                        for (int mt = 0; mt < MT; mt++) acc[j][mt] = Tile::Type::mfma(x[mt], b, acc[j][mt]);
-                    } else {
-                        const w4_u32x4 b = Tile::operand(q[j][i], 1.0f, mask, sixteen);
-                        const uint32_t pj = p[j][i / Tile::PER];
-#pragma unroll
-                        for (int mt = 0; mt < MT; mt++) {
-                            if (i % Tile::PER == 0) part[j][mt] = less[j][mt] = (w4_f32x4){0, 0, 0, 0};
-                            if (!Tile::MX) (TWO ? less : part)[j][mt] = Tile::Type::mfma(x[mt], Tile::zero_of(pj), (TWO ? less : part)[j][mt]);
-                            part[j][mt] = Tile::Type::mfma(x[mt], b, part[j][mt]);
-                            if (i % Tile::PER == Tile::PER - 1) {
-#pragma unroll
-                                for (int r = 0; r < 4; r++) acc[j][mt][r] += Tile::scale_of(pj) * (TWO && !Tile::MX ? part[j][mt][r] + less[j][mt][r] : part[j][mt][r]);
-                            }
-                        }
-                    }
-                }
-            }
-            slot = next;
+            request(begin + step + 2, end, SLOT);
+            read(o, 1 - SLOT, group0 + (step + 1) * Tile::GROUPS, count);
+        };
+        for (int step = 0; step < steps; step += 2) {
+            advance(IC<0>{}, b, step);
+            multiply(a);
+            if (step + 1 == steps) break;
+            advance(IC<1>{}, a, step + 1);
+            multiply(b);
         }
         CCH_WAIT_VM(0);                // (requests of no block write zeros)
         CCH_WAIT_LGKM0();
@@ -460,7 +482,7 @@ __device__ __forceinline__ void w4_pass(const W4Rows &rows, const W4Matrix &w, i
 }
 
 template <class T, int KIND, bool ZEROS, class S, int OUT, bool GROUPED>
-__global__ __launch_bounds__(S::THREADS, S::MT * S::NT <= 4 ? 4 : 2) void w4_tile_kernel(W4Rows rows, W4Matrix w, int pitch, int chunk, int list_at, void *__restrict__ out)
+__global__ __launch_bounds__(S::THREADS, S::MT <= 2 ? 4 : 2) void w4_tile_kernel(W4Rows rows, W4Matrix w, int pitch, int chunk, int list_at, void *__restrict__ out)
 {
     if constexpr (!GROUPED) {
         w4_pass<T, KIND, ZEROS, S, OUT, false>(rows, w, 0, nullptr, (int)blockIdx.y * (16 * S::MT), (int)rows.rows, pitch, chunk, out);
@@ -515,13 +537,13 @@ int w4_tile_choose(int out_kind, const W4Rows &rows, const W4Matrix &w, void *ou
 {
 #define W4_GO(S, OUT, GROUPED) w4_tile_launch<T, KIND, ZEROS, S, OUT, GROUPED>(rows, w, out, s)
     if (out_kind == W4_OUT_PLAIN) {
-        typedef W4Shape<1, 1, 1, 1, 8, 3> One;
-        typedef W4Shape<2, 1, 1, 1, 4, 3> OneWide;
-        typedef std::conditional_t<KIND == W4_MX, W4Shape<1, 1, 4, 2, 4, 3>, W4Shape<1, 1, 4, 1, 8, 3>> Few;
-        typedef W4Shape<1, 1, 4, 4, 2, 3> FewWide;
-        typedef W4Shape<1, 2, 8, 2, 4, 3> Some;
-        typedef W4Shape<1, 4, 16, 2, 2, 3> Many;
-        typedef W4Shape<1, 4, 16, 8, 1, 3> ManyWide;
+        typedef W4Shape<1, 1, 1, 1, 8> One;
+        typedef W4Shape<2, 1, 1, 1, 4> OneWide;
+        typedef std::conditional_t<KIND == W4_MX, W4Shape<1, 1, 4, 2, 4>, W4Shape<1, 1, 4, 1, 8>> Few;
+        typedef W4Shape<1, 1, 4, 4, 2> FewWide;
+        typedef W4Shape<1, 2, 8, 2, 4> Some;
+        typedef W4Shape<1, 4, 16, 2, 2> Many;
+        typedef W4Shape<2, 4, 16, 4, 2> ManyWide;
         const bool wide = w.rows >= 16 * 2 * 256;
         if (rows.rows <= 4) return wide ? W4_GO(OneWide, W4_OUT_PLAIN, false) : W4_GO(One, W4_OUT_PLAIN, false);
         if (rows.rows <= 16) return wide ? W4_GO(FewWide, W4_OUT_PLAIN, false) : W4_GO(Few, W4_OUT_PLAIN, false);
@@ -530,15 +552,14 @@ int w4_tile_choose(int out_kind, const W4Rows &rows, const W4Matrix &w, void *ou
     }
     const int64_t tokens = rows.rows / rows.top_k;   // no expert has more of them
     const bool few = rows.rows <= 8 * rows.num_experts;
+    typedef W4Shape<2, 1, 1, 1, 4> One;
     if (out_kind == W4_OUT_SWIGLU) {
-        typedef W4Shape<2, 1, 1, 1, 4, 3> One;
-        typedef W4Shape<2, 1, 4, 4, 1, 3> Few;
-        typedef W4Shape<2, 4, 16, 8, 1, 3> Some;
+        typedef W4Shape<2, 1, 4, 4, 2> Few;
+        typedef W4Shape<2, 4, 16, 4, 1> Some;
         return tokens <= 4 ? W4_GO(One, W4_OUT_SWIGLU, true) : tokens <= 16 || few ? W4_GO(Few, W4_OUT_SWIGLU, true) : W4_GO(Some, W4_OUT_SWIGLU, true);
     }
-    typedef W4Shape<2, 1, 1, 1, 4, 3> One;
-    typedef W4Shape<1, 1, 4, 4, 1, 3> Few;
-    typedef W4Shape<1, 2, 8, 8, 1, 3> Some;
+    typedef W4Shape<2, 1, 4, 4, 1> Few;
+    typedef W4Shape<1, 2, 8, 4, 1> Some;
     return tokens <= 4 ? W4_GO(One, W4_OUT_F32, true) : tokens <= 16 || few ? W4_GO(Few, W4_OUT_F32, true) : W4_GO(Some, W4_OUT_F32, true);
 #undef W4_GO
 }
