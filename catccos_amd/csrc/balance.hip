@@ -7,8 +7,11 @@
 //   dl_te = coef / (S' N_s) p_te (f_se - sum_i p_ti f_si) [(1 - sigmoid(l_te)) for sigmoid scores] + z_coef 2 lse_t softmax(l)_te / N
 // times the loss's own gradient.
 //
-// Forward: workgroups take tokens of one sequence each, keep P in registers (fp32) and the routes in LDS, and leave their sums in the workspace;
-// the sequences' workgroups add those up in a fixed order, so that the same inputs give the same bits.  Backward: one pass, logits in, gradient out.
+// Forward: a workgroup takes a run of tokens, whatever sequences they belong to; of each of those it leaves the sums of p (fp32 in registers) and the routes
+// (LDS) in the workspace, and a second launch adds a sequence's sums up, in their order, so that the same inputs give the same bits.  The last workgroup of that
+// launch has the loss.  Backward: one pass, logits in, gradient out.
+//
+// Bound by the logits' bytes on paper, by exponentials and the latency of few tokens per wave in fact.
 #include <algorithm>
 
 #include "router_lanes.h"
@@ -28,120 +31,101 @@ __device__ __forceinline__ Span span_of(const int32_t *offsets, int s, int token
     return {b, min(max(offsets[s + 1], b), tokens)};
 }
 
-// A token's p (in place of l), and with Z softmax(l) in `q` and the log of the sum of exponentials.  False: no logit is above -inf (NaN is not).
-template <int V, int L, bool SIGMOID, bool Z>
-__device__ __forceinline__ bool token_shares(float (&l)[V], float (&q)[V], float &lse)
+// Where a workgroup of token `first` on stands among the sequences, from one look at all of them: the sequence that holds `first`, or the one before it where none
+// does (as many sequences begin at or before it, less one; -1: none), the number of sequences with tokens, and the tokens of all.  `staged` (the workgroup's, in
+// LDS) then holds the offsets of up to THREADS - 1 sequences.
+struct Place {
+    int s, alive, all;
+};
+template <int THREADS, bool COUNTS, bool ALL>
+__device__ __forceinline__ Place place_of(const int32_t *offsets, const int32_t *seq_tokens, int sequences, int first, int32_t *staged, int (&scratch)[3][THREADS / 64])
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int before = 0, alive = 0, all = 0;
+    for (int i0 = 0; i0 <= sequences; i0 += THREADS) {
+        const int i = i0 + (int)threadIdx.x;
+        int offset = 0, n = 0;
+        if (offsets && i <= sequences) offset = offsets[i];
+        if (COUNTS && i < sequences) n = seq_tokens[i];
+        if (i0 == 0) staged[threadIdx.x] = offset;
+        before += __builtin_popcountll(__ballot(i < sequences && offset <= first));
+        if (COUNTS) alive += __builtin_popcountll(__ballot(n > 0));
+        if (ALL) all += n;
+    }
+    if (ALL) {
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) all += __shfl_xor(all, off, 64);
+    }
+    if (lane == 0) {
+        scratch[0][wave] = before;
+        scratch[1][wave] = alive;
+        scratch[2][wave] = all;
+    }
+    __syncthreads();
+    Place p = {-1, 0, 0};
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; w++) {
+        p.s += scratch[0][w];
+        p.alive += scratch[1][w];
+        p.all += scratch[2][w];
+    }
+    if (offsets == nullptr) p.s = 0;
+    p.s = __builtin_amdgcn_readfirstlane(p.s);
+    return p;
+}
+
+// A token's p (in place of l) and for sigmoid scores `rest` = 1 - sigmoid(l); with z also softmax(l) in `q` and the log of the sum of exponentials.  False: no logit
+// is above -inf (NaN is not).
+template <int V, int L, bool SIGMOID>
+__device__ __forceinline__ bool token_shares(float (&l)[V], float (&rest)[V], float (&q)[V], float &lse, bool z)
 {
     float top = l[0];
 #pragma unroll
     for (int i = 1; i < V; i++) top = fmaxf(top, l[i]);
     top = lanes_max<L>(top);
-    if (SIGMOID && Z) {
-        float sum = 0.0f;
+    float sum = 0.0f;
+    if (!SIGMOID || z) {
 #pragma unroll
         for (int i = 0; i < V; i++) {
-            q[i] = __expf(l[i] - top);
+            q[i] = exp_of(l[i] - top);
             sum += q[i];
         }
         sum = lanes_sum<L>(sum);
-        lse = __logf(sum) + top;
+        if (z) lse = __logf(sum) + top;
+        const float over = reciprocal(sum);
 #pragma unroll
-        for (int i = 0; i < V; i++) q[i] /= sum;
+        for (int i = 0; i < V; i++) q[i] *= over;
     }
-    float sum = 0.0f;
-    const float c = fminf(top, 0.0f), ec = __expf(c);
+    if (!SIGMOID) {
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-        l[i] = SIGMOID ? scaled_sigmoid(l[i], c, ec) : __expf(l[i] - top);
-        sum += l[i];
+        for (int i = 0; i < V; i++) l[i] = q[i];
+        return top > -INFINITY;
     }
-    sum = lanes_sum<L>(sum);
-    if (!SIGMOID && Z) lse = __logf(sum) + top;
+    sum = 0.0f;
+    if (__ballot(!(top >= SIGMOID_IN_RANGE)) == 0) {
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-        l[i] /= sum;
-        if (!SIGMOID && Z) q[i] = l[i];
+        for (int i = 0; i < V; i++) {
+            sigmoid_pair(l[i], l[i], rest[i]);
+            sum += l[i];
+        }
+    } else {
+        const float c = fminf(top, 0.0f), ec = exp_of(c);
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            rest[i] = reciprocal(1.0f + exp_of(l[i]));
+            l[i] = scaled_sigmoid(l[i], c, ec);
+            sum += l[i];
+        }
     }
+    const float over = reciprocal(lanes_sum<L>(sum));
+#pragma unroll
+    for (int i = 0; i < V; i++) l[i] *= over;
     return top > -INFINITY;
 }
 
-// Sums of workgroup (c, s) in part[(s * gridDim.x + c) * (2 experts + 2)]: P per expert, routes per expert, sum of lse^2, tokens.
-template <class T, int V, int L, bool SIGMOID, bool Z>
-__global__ __launch_bounds__(BAL_THREADS) void moe_balance_sums_kernel(const T *__restrict__ logits, const int32_t *__restrict__ expert_idx,
-                                                                      const uint8_t *__restrict__ token_mask, const int32_t *__restrict__ seq_offsets, int tokens,
-                                                                      int experts, int top_k, float *__restrict__ part, bool vec)
-{
-    constexpr int TPW = 64 / L;   // tokens of a wave at a time
-    __shared__ float shares[BAL_WAVES][V * L], rest[BAL_WAVES];
-    __shared__ int32_t routes[V * L], counted[BAL_WAVES];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at = lane & (L - 1);
-    for (int e = threadIdx.x; e < V * L; e += BAL_THREADS) routes[e] = 0;
-    __syncthreads();
-    const Span span = span_of(seq_offsets, blockIdx.y, tokens);
-    float acc[V], zsum = 0.0f;
-    int n = 0;
-#pragma unroll
-    for (int i = 0; i < V; i++) acc[i] = 0.0f;
-    const int64_t step = (int64_t)gridDim.x * BAL_WAVES * TPW;
-    for (int64_t t0 = span.begin + ((int64_t)blockIdx.x * BAL_WAVES + wave) * TPW; t0 < span.end; t0 += step) {
-        const int64_t t = t0 + lane / L;
-        const bool inside = t < span.end && (token_mask == nullptr || token_mask[t] != 0);
-        float l[V], q[V], lse = 0.0f;
-        LaneRow<T, V>::load(logits + (inside ? t : t0) * experts, at * V, experts, vec, l);
-        const bool valid = token_shares<V, L, SIGMOID, Z>(l, q, lse) && inside;
-        if (valid) {
-#pragma unroll
-            for (int i = 0; i < V; i++) acc[i] += l[i];
-            if (at == 0) {
-                n++;
-                if (Z) zsum += lse * lse;
-            }
-            if (at < top_k) {
-                const int e = expert_idx[t * top_k + at];
-                if (e >= 0 && e < experts) atomicAdd(&routes[e], 1);
-            }
-        }
-    }
-#pragma unroll
-    for (int off = L; off < 64; off <<= 1) {
-#pragma unroll
-        for (int i = 0; i < V; i++) acc[i] += __shfl_xor(acc[i], off, 64);
-        zsum += __shfl_xor(zsum, off, 64);
-        n += __shfl_xor(n, off, 64);
-    }
-    if (lane < L) {
-#pragma unroll
-        for (int i = 0; i < V; i++) shares[wave][at * V + i] = acc[i];
-    }
-    if (lane == 0) {
-        rest[wave] = zsum;
-        counted[wave] = n;
-    }
-    __syncthreads();
-    float *out = part + ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * (2 * experts + 2);
-    for (int e = threadIdx.x; e < experts; e += BAL_THREADS) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int w = 0; w < BAL_WAVES; w++) sum += shares[w][e];
-        out[e] = sum;
-        out[experts + e] = __int_as_float(routes[e]);
-    }
-    if (threadIdx.x == 0) {
-        float sum = 0.0f;
-        int all = 0;
-#pragma unroll
-        for (int w = 0; w < BAL_WAVES; w++) {
-            sum += rest[w];
-            all += counted[w];
-        }
-        out[2 * experts] = sum;
-        out[2 * experts + 1] = __int_as_float(all);
-    }
-}
-
-// The sum over the workgroup, in thread 0.
-template <class N>
-__device__ __forceinline__ N block_sum(N x, N (&scratch)[BAL_WAVES])
+// The sum over the workgroup, in every thread.
+template <int WAVES, class N>
+__device__ __forceinline__ N block_sum(N x, N (&scratch)[WAVES])
 {
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) x += __shfl_xor(x, off, 64);
@@ -150,125 +134,244 @@ __device__ __forceinline__ N block_sum(N x, N (&scratch)[BAL_WAVES])
     __syncthreads();
     N sum = 0;
 #pragma unroll
-    for (int w = 0; w < BAL_WAVES; w++) sum += scratch[w];
+    for (int w = 0; w < WAVES; w++) sum += scratch[w];
     return sum;
 }
 
-// Workgroup s: the sequence's sums, counts and tokens; its loss to of_seq[2 s] and its sum of lse^2 behind it, or, of one sequence, the whole loss.
-__global__ __launch_bounds__(BAL_THREADS) void moe_balance_sequence_kernel(const float *__restrict__ part, int chunks, int experts, int top_k, float coef, float z_coef,
-                                                                          int32_t *__restrict__ counts, int32_t *__restrict__ seq_tokens, float *__restrict__ of_seq,
-                                                                          float *__restrict__ loss)
+// Tokens [run * blockIdx.x, ...) of `run`; what they add to sequence s goes to part[(blockIdx.x + s) * (2 experts + 2)]: p per expert, routes per expert, sum of
+// lse^2, tokens.  (Workgroups in order and sequences in order: no two meet.)
+template <class T, int V, int L, bool SIGMOID, bool VEC>
+__global__ __launch_bounds__(BAL_THREADS) void moe_balance_sums_kernel(const T *__restrict__ logits, const int32_t *__restrict__ expert_idx,
+                                                                      const uint8_t *__restrict__ token_mask, const int32_t *__restrict__ seq_offsets, int tokens,
+                                                                      int experts, int top_k, int sequences, int run, float *__restrict__ part, bool z)
 {
-    __shared__ float fs[BAL_WAVES];
-    __shared__ int is[BAL_WAVES];
-    const int pitch = 2 * experts + 2;
-    const float *mine = part + (size_t)blockIdx.x * chunks * pitch;
-    float zsum = 0.0f;
-    int n = 0;
-    for (int c = threadIdx.x; c < chunks; c += BAL_THREADS) {
+    constexpr int TPW = 64 / L, STEP = BAL_WAVES * TPW;   // tokens of a wave and of the workgroup at a time
+    __shared__ float shares[BAL_WAVES][V * L], zsums[BAL_WAVES];
+    __shared__ int32_t routes[V * L], counted[BAL_WAVES], staged[BAL_THREADS], scratch[3][BAL_WAVES];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), at = lane & (L - 1);
+    const int first = (int)blockIdx.x * run, end = min(first + run, tokens);
+    const int mine = wave * TPW + lane / L;
+    if (first >= end) return;
+    // the first rows are on their way while the sequences are looked at
+    LaneRow<T, V, VEC> row;
+    row.load(logits + (int64_t)min(first + mine, end - 1) * experts, at * V, experts);
+    int s = max(place_of<BAL_THREADS, false, false>(seq_offsets, nullptr, sequences, first, staged, scratch).s, 0);
+    const int32_t *const offsets = seq_offsets && sequences < BAL_THREADS ? staged : seq_offsets;
+    for (; s < sequences; s++) {
+        const Span span = span_of(offsets, s, tokens);
+        if (span.begin >= end) break;
+        const int from = max(span.begin, first), to = min(span.end, end);
+        if (from >= to) continue;
+        if (from > first) row.load(logits + (int64_t)min(from + mine, to - 1) * experts, at * V, experts);
+        for (int e = threadIdx.x; e < V * L; e += BAL_THREADS) routes[e] = 0;
+        __syncthreads();
+        float acc[V], zsum = 0.0f;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < V; i++) acc[i] = 0.0f;
+        for (int t1 = from; t1 < to; t1 += STEP) {
+            const int t = t1 + mine;
+            LaneRow<T, V, VEC> next;
+            next.load(logits + (int64_t)min(t + STEP, to - 1) * experts, at * V, experts);
+            const bool inside = t < to && (token_mask == nullptr || token_mask[t] != 0);
+            int e = -1;
+            if (inside && at < top_k) e = expert_idx[(int64_t)t * top_k + at];
+            float l[V], rest[V], q[V], lse = 0.0f;
+            row.values(at * V, experts, l);
+            const bool valid = token_shares<V, L, SIGMOID>(l, rest, q, lse, z) && inside;
+            if (valid) {
+#pragma unroll
+                for (int i = 0; i < V; i++) acc[i] += l[i];
+                if (at == 0) {
+                    n++;
+                    if (z) zsum += lse * lse;
+                }
+                if (e >= 0 && e < experts) atomicAdd(&routes[e], 1);
+            }
+            row = next;
+        }
+#pragma unroll
+        for (int off = L; off < 64; off <<= 1) {
+#pragma unroll
+            for (int i = 0; i < V; i++) acc[i] += __shfl_xor(acc[i], off, 64);
+            zsum += __shfl_xor(zsum, off, 64);
+            n += __shfl_xor(n, off, 64);
+        }
+        if (lane < L) {
+#pragma unroll
+            for (int i = 0; i < V; i++) shares[wave][at * V + i] = acc[i];
+        }
+        if (lane == 0) {
+            zsums[wave] = zsum;
+            counted[wave] = n;
+        }
+        __syncthreads();
+        float *out = part + ((size_t)blockIdx.x + s) * (2 * experts + 2);
+        for (int e = threadIdx.x; e < experts; e += BAL_THREADS) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < BAL_WAVES; w++) sum += shares[w][e];
+            out[e] = sum;
+            out[experts + e] = __int_as_float(routes[e]);
+        }
+        if (threadIdx.x == 0) {
+            float sum = 0.0f;
+            int all = 0;
+#pragma unroll
+            for (int w = 0; w < BAL_WAVES; w++) {
+                sum += zsums[w];
+                all += counted[w];
+            }
+            out[2 * experts] = sum;
+            out[2 * experts + 1] = __int_as_float(all);
+        }
+        __syncthreads();
+    }
+}
+
+// Workgroup (b, s): experts 64 b ... of sequence s, a wave to every sixteenth workgroup's sums.  One workgroup alone has the loss; of several each leaves its
+// share, the sum of lse^2 and the tokens in of_seq, for the launch below.  (The last of them to come could add these up instead, but publishing them to one
+// another takes longer than a launch: 9.5 us against 3.0 for 16 experts, the caches of the card's parts being written back.)
+constexpr int FIN_THREADS = 1024, FIN_WAVES = FIN_THREADS / 64;
+__global__ __launch_bounds__(FIN_THREADS) void moe_balance_finish_kernel(const float *__restrict__ part, const int32_t *__restrict__ seq_offsets, int tokens, int experts,
+                                                                        int top_k, int run, float coef, float z_coef, int32_t *__restrict__ counts,
+                                                                        int32_t *__restrict__ seq_tokens, float *__restrict__ of_seq, float *__restrict__ loss)
+{
+    __shared__ float fs[FIN_WAVES], shares[FIN_WAVES][64];
+    __shared__ int is[FIN_WAVES], routes[FIN_WAVES][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, s = blockIdx.y, sequences = gridDim.y, blocks = gridDim.x;
+    const int e = (int)blockIdx.x * 64 + lane, pitch = 2 * experts + 2;
+    const Span span = span_of(seq_offsets, s, tokens);
+    const int c0 = span.begin / run, c1 = span.end > span.begin ? (span.end - 1) / run + 1 : c0;
+    const float *mine = part + (size_t)s * pitch;
+    float p = 0.0f, zsum = 0.0f;
+    int r = 0, n = 0;
+    if (e < experts) {
+#pragma unroll 4
+        for (int c = c0 + wave; c < c1; c += FIN_WAVES) {
+            p += mine[(size_t)c * pitch + e];
+            r += __float_as_int(mine[(size_t)c * pitch + experts + e]);
+        }
+    }
+    for (int c = c0 + (int)threadIdx.x; c < c1; c += FIN_THREADS) {
         zsum += mine[(size_t)c * pitch + 2 * experts];
         n += __float_as_int(mine[(size_t)c * pitch + 2 * experts + 1]);
     }
+    shares[wave][lane] = p;
+    routes[wave][lane] = r;
     zsum = block_sum(zsum, fs);
     n = block_sum(n, is);
-    float sum = 0.0f;
-    for (int e = threadIdx.x; e < experts; e += BAL_THREADS) {
-        float p = 0.0f;
-        int routes = 0;
-#pragma unroll 8
-        for (int c = 0; c < chunks; c++) {
-            p += mine[(size_t)c * pitch + e];
-            routes += __float_as_int(mine[(size_t)c * pitch + experts + e]);
+    const float counted = (float)max(n, 1);
+    if (wave == 0) {
+        p = 0.0f;
+        r = 0;
+#pragma unroll
+        for (int w = 0; w < FIN_WAVES; w++) {
+            p += shares[w][lane];
+            r += routes[w][lane];
         }
-        counts[(size_t)blockIdx.x * experts + e] = routes;
-        sum += p * (float)routes;
-    }
-    sum = block_sum(sum, fs);
-    if (threadIdx.x == 0) {
-        seq_tokens[blockIdx.x] = n;
-        const float tokens = (float)max(n, 1), r = sum / tokens * ((float)experts / ((float)top_k * tokens));
-        if (gridDim.x == 1) {
-            *loss = coef * r + z_coef * (zsum / tokens);
-        } else {
-            of_seq[2 * blockIdx.x] = r;
-            of_seq[2 * blockIdx.x + 1] = zsum;
+        if (e < experts) counts[(size_t)s * experts + e] = r;
+        float sum = p * (float)r;
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
+        if (lane == 0) {
+            sum = sum / counted * ((float)experts / ((float)top_k * counted));
+            if (blockIdx.x == 0) seq_tokens[s] = n;
+            if (blocks * sequences == 1) {
+                *loss = coef * sum + z_coef * (zsum / counted);
+            } else {
+                float *to = of_seq + ((size_t)s * blocks + blockIdx.x) * 3;
+                to[0] = sum;
+                to[1] = zsum;
+                to[2] = __int_as_float(n);
+            }
         }
     }
 }
 
-__global__ __launch_bounds__(BAL_THREADS) void moe_balance_loss_kernel(const float *__restrict__ of_seq, const int32_t *__restrict__ seq_tokens, int sequences, float coef,
-                                                                      float z_coef, float *__restrict__ loss)
+__global__ __launch_bounds__(BAL_THREADS) void moe_balance_loss_kernel(const float *__restrict__ of_seq, int blocks, int sequences, float coef, float z_coef,
+                                                                      float *__restrict__ loss)
 {
     __shared__ float fs[BAL_WAVES];
     __shared__ int is[BAL_WAVES];
-    float r = 0.0f, z = 0.0f;
-    int alive = 0, n = 0;
-    for (int s = threadIdx.x; s < sequences; s += BAL_THREADS) {
-        r += of_seq[2 * s];
-        z += of_seq[2 * s + 1];
-        n += seq_tokens[s];
-        alive += seq_tokens[s] > 0;
+    float total = 0.0f, z = 0.0f;
+    int alive = 0, all = 0;
+    for (int i = threadIdx.x; i < sequences; i += BAL_THREADS) {
+        const float *from = of_seq + (size_t)i * blocks * 3;
+        for (int b = 0; b < blocks; b++) total += from[3 * b];
+        z += from[1];
+        const int m = __float_as_int(from[2]);
+        all += m;
+        alive += m > 0;
     }
-    r = block_sum(r, fs);
+    total = block_sum(total, fs);
     z = block_sum(z, fs);
-    n = block_sum(n, is);
+    all = block_sum(all, is);
     alive = block_sum(alive, is);
-    if (threadIdx.x == 0) *loss = coef * (r / (float)max(alive, 1)) + z_coef * (z / (float)max(n, 1));
+    if (threadIdx.x == 0) *loss = coef * (total / (float)max(alive, 1)) + z_coef * (z / (float)max(all, 1));
 }
 
-// Workgroup (c, s): tokens of sequence s; the first and the last sequence's also write the zeros of tokens before and behind all sequences.
-template <class T, int V, int L, bool SIGMOID, bool Z>
+// Tokens [run * blockIdx.x, ...) of `run`, sequence by sequence; those before and behind all sequences get zeros.
+template <class T, int V, int L, bool SIGMOID, bool VEC>
 __global__ __launch_bounds__(BAL_THREADS) void moe_balance_backward_kernel(const float *__restrict__ grad_loss, const T *__restrict__ logits,
                                                                           const uint8_t *__restrict__ token_mask, const int32_t *__restrict__ seq_offsets,
                                                                           const int32_t *__restrict__ counts, const int32_t *__restrict__ seq_tokens, int tokens, int experts,
-                                                                          int top_k, float coef, float z_coef, T *__restrict__ grad_logits, bool vec)
+                                                                          int top_k, int sequences, int run, float coef, float z_coef, T *__restrict__ grad_logits)
 {
-    constexpr int TPW = 64 / L;
-    __shared__ int is[BAL_WAVES];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at = lane & (L - 1);
-    const int sequences = gridDim.y, s = blockIdx.y;
-    int alive = 0, all = 0;
-    if (sequences > 1) {
-        for (int i = threadIdx.x; i < sequences; i += BAL_THREADS) {
-            all += seq_tokens[i];
-            alive += seq_tokens[i] > 0;
+    constexpr int TPW = 64 / L, STEP = BAL_WAVES * TPW;
+    __shared__ int32_t staged[BAL_THREADS];
+    __shared__ int scratch[3][BAL_WAVES];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), at = lane & (L - 1);
+    const int first = (int)blockIdx.x * run, end = min(first + run, tokens), mine = wave * TPW + lane / L;
+    LaneRow<T, V, VEC> row;
+    row.load(logits + (int64_t)min(first + mine, end - 1) * experts, at * V, experts);
+    const float g = *grad_loss;
+    const bool z = z_coef != 0;
+    const Place place = place_of<BAL_THREADS, true, true>(seq_offsets, seq_tokens, sequences, first, staged, scratch);
+    const int32_t *const offsets = seq_offsets && sequences < BAL_THREADS ? staged : seq_offsets;
+    const float zunit = 2.0f * g * z_coef / (float)max(place.all, 1);
+    for (int s = place.s; s <= sequences; s++) {
+        const bool real = s >= 0 && s < sequences;
+        Span span = {0, 0};
+        if (real) span = span_of(offsets, s, tokens);
+        else if (offsets) span = s < 0 ? Span{0, min(max(offsets[0], 0), tokens)} : Span{min(max(offsets[sequences], 0), tokens), tokens};
+        if (span.begin >= end) break;
+        const int from = max(span.begin, first), to = min(span.end, end);
+        if (from >= to) continue;
+        if (from > first) row.load(logits + (int64_t)min(from + mine, to - 1) * experts, at * V, experts);
+        float v[V];
+        const float n = real ? (float)max(seq_tokens[s], 1) : 1.0f, unit = g * coef / ((float)max(place.alive, 1) * n) * ((float)experts / ((float)top_k * n));
+        constexpr int FEW = VEC && V >= 4 ? 4 : VEC ? 2 : 1;   // counts of one access
+        typedef int32_t Counts __attribute__((ext_vector_type(FEW)));
+#pragma unroll
+        for (int i = 0; i < V; i += FEW) {
+            Counts c = {};
+            if (real && at * V + i < experts) c = *reinterpret_cast<const Counts *>(counts + (size_t)s * experts + at * V + i);
+#pragma unroll
+            for (int u = 0; u < FEW; u++) v[i + u] = unit * (float)c[u];
         }
-        all = block_sum(all, is);
-        alive = block_sum(alive, is);
-    } else {
-        all = seq_tokens[0];
-        alive = 1;
-    }
-    const float g = *grad_loss, n = (float)max(seq_tokens[s], 1);
-    const float unit = g * coef / ((float)max(alive, 1) * n) * ((float)experts / ((float)top_k * n)), zunit = 2.0f * g * z_coef / (float)max(all, 1);
-    float v[V];
+        for (int t1 = from; t1 < to; t1 += STEP) {
+            const int t = t1 + mine;
+            LaneRow<T, V, VEC> next;
+            next.load(logits + (int64_t)min(t + STEP, to - 1) * experts, at * V, experts);
+            const bool inside = real && t < to && (token_mask == nullptr || token_mask[t] != 0);
+            float l[V], rest[V], q[V], d[V], lse = 0.0f;
+            row.values(at * V, experts, l);
+            const bool valid = token_shares<V, L, SIGMOID>(l, rest, q, lse, z) && inside;
+            float dot = 0.0f;
 #pragma unroll
-    for (int i = 0; i < V; i++) v[i] = at * V + i < experts ? unit * (float)counts[(size_t)s * experts + at * V + i] : 0.0f;
-    const Span span = span_of(seq_offsets, s, tokens);
-    const int begin = s == 0 ? 0 : span.begin, end = s == sequences - 1 ? tokens : span.end;
-    const int64_t step = (int64_t)gridDim.x * BAL_WAVES * TPW;
-    for (int64_t t0 = begin + ((int64_t)blockIdx.x * BAL_WAVES + wave) * TPW; t0 < end; t0 += step) {
-        const int64_t t = t0 + lane / L;
-        const bool inside = t >= span.begin && t < span.end && (token_mask == nullptr || token_mask[t] != 0);
-        float l[V], q[V], d[V], keep[V], lse = 0.0f;
-        LaneRow<T, V>::load(logits + (t < end ? t : t0) * experts, at * V, experts, vec, l);
-        if (SIGMOID) {
+            for (int i = 0; i < V; i++) dot += l[i] * v[i];
+            dot = lanes_sum<L>(dot);
 #pragma unroll
-            for (int i = 0; i < V; i++) keep[i] = 1.0f / (1.0f + __expf(l[i]));   // 1 - sigmoid
+            for (int i = 0; i < V; i++) {
+                d[i] = l[i] * (v[i] - dot);
+                if (SIGMOID) d[i] *= rest[i];
+                if (z) d[i] += zunit * lse * q[i];
+                if (!valid) d[i] = 0.0f;
+            }
+            if (t < to) LaneRow<T, V, VEC>::store(grad_logits + (int64_t)t * experts, at * V, experts, d);
+            row = next;
         }
-        const bool valid = token_shares<V, L, SIGMOID, Z>(l, q, lse) && inside;
-        float dot = 0.0f;
-#pragma unroll
-        for (int i = 0; i < V; i++) dot += l[i] * v[i];
-        dot = lanes_sum<L>(dot);
-#pragma unroll
-        for (int i = 0; i < V; i++) {
-            d[i] = l[i] * (v[i] - dot);
-            if (SIGMOID) d[i] *= keep[i];
-            if (Z) d[i] += zunit * lse * q[i];
-            if (!valid) d[i] = 0.0f;
-        }
-        if (t < end) LaneRow<T, V>::store(grad_logits + t * experts, at * V, experts, vec, d);
     }
 }
 
@@ -285,20 +388,40 @@ static int balance_shape(const char *what, int dtype, int64_t tokens, int64_t ex
     return CCH_OK;
 }
 
-// Workgroups per sequence.
-static int64_t balance_chunks(int64_t tokens, int64_t experts, int64_t sequences)
+// Tokens of a workgroup: several steps of it, so that the sums left in the workspace stay fewer than the logits, but two workgroups to a CU where there are
+// tokens for them.
+template <int L>
+static int balance_run(int64_t tokens, int most)
 {
-    const int64_t per = BAL_WAVES * (experts <= 64 ? 8 : experts <= 256 ? 4 : experts <= 512 ? 2 : 1);   // tokens of a workgroup at a time
-    const int64_t fill = (256 + sequences - 1) / sequences, need = (tokens + per - 1) / per;
-    return std::max<int64_t>(1, std::min(fill, need));
+    constexpr int STEP = BAL_WAVES * (64 / L);
+    return STEP * (int)std::max<int64_t>(1, std::min<int64_t>(most, tokens / (512 * STEP)));
+}
+constexpr int BAL_STEPS = 16, BAL_BACKWARD_STEPS = 4;   // at most
+
+static int64_t balance_runs(int64_t tokens, int64_t experts)
+{
+    return with_lanes((int)experts, [&](auto, auto lanes) {
+        const int run = balance_run<decltype(lanes)::value>(tokens, BAL_STEPS);
+        return (int)((tokens + run - 1) / run);
+    });
+}
+struct BalanceWorkspace {
+    int64_t part, end;
+};
+static BalanceWorkspace balance_workspace(int64_t tokens, int64_t experts, int64_t sequences)
+{
+    BalanceWorkspace w{};
+    w.part = sequences * ((experts + 63) / 64) * 3 * 4;
+    w.end = w.part + (balance_runs(tokens, experts) + sequences) * (2 * experts + 2) * 4;
+    return w;
 }
 
 }  // namespace cch
 
 extern "C" int64_t cch_moe_balance_loss_workspace_bytes(int64_t tokens, int64_t num_experts, int64_t num_sequences)
 {
-    if (tokens < 0 || num_experts < 1 || num_experts > cch::ROUTER_MAX_EXPERTS || num_sequences < 1 || num_sequences > cch::BAL_MAX_SEQUENCES) return 0;
-    return 4 * (2 * num_sequences + num_sequences * cch::balance_chunks(tokens, num_experts, num_sequences) * (2 * num_experts + 2));
+    if (tokens < 0 || tokens >> 31 || num_experts < 1 || num_experts > cch::ROUTER_MAX_EXPERTS || num_sequences < 1 || num_sequences > cch::BAL_MAX_SEQUENCES) return 0;
+    return cch::balance_workspace(tokens, num_experts, num_sequences).end;
 }
 
 extern "C" int cch_moe_balance_loss(const void *logits, int dtype, const int32_t *expert_idx, const uint8_t *token_mask, const int32_t *seq_offsets, int64_t tokens,
@@ -311,26 +434,32 @@ extern "C" int cch_moe_balance_loss(const void *logits, int dtype, const int32_t
     const int64_t need = cch_moe_balance_loss_workspace_bytes(tokens, num_experts, num_sequences);
     CCH_REQUIRE(workspace && aligned(workspace, 4) && workspace_bytes >= need, "cch_moe_balance_loss: workspace of %lld bytes, need %lld", (long long)workspace_bytes,
                 (long long)need);
-    const int chunks = (int)balance_chunks(tokens, num_experts, num_sequences);
-    float *of_seq = static_cast<float *>(workspace), *part = of_seq + 2 * num_sequences;
+    const BalanceWorkspace at = balance_workspace(tokens, num_experts, num_sequences);
+    uint8_t *p = static_cast<uint8_t *>(workspace);
+    float *of_seq = reinterpret_cast<float *>(p), *part = reinterpret_cast<float *>(p + at.part);
     hipStream_t s = static_cast<hipStream_t>(stream);
+    int run = 1;
     const int rc = with_logits_type(dtype, [&](auto *type) {
         return with_lanes((int)num_experts, [&](auto v, auto lanes) {
             typedef std::remove_pointer_t<decltype(type)> T;
             constexpr int V = decltype(v)::value, L = decltype(lanes)::value;
-            auto kern = scoring == CCH_SCORING_SIGMOID ? (z_coef != 0 ? moe_balance_sums_kernel<T, V, L, true, true> : moe_balance_sums_kernel<T, V, L, true, false>)
-                                                       : (z_coef != 0 ? moe_balance_sums_kernel<T, V, L, false, true> : moe_balance_sums_kernel<T, V, L, false, false>);
-            hipLaunchKernelGGL(kern, dim3((unsigned)chunks, (unsigned)num_sequences), dim3(BAL_THREADS), 0, s, static_cast<const T *>(logits), expert_idx, token_mask,
-                               seq_offsets, (int)tokens, (int)num_experts, top_k, part, LaneRow<T, V>::vec(logits, num_experts));
+            run = balance_run<L>(tokens, BAL_STEPS);
+            const bool vec = LanePieces<T, V>::vec(logits, num_experts);
+            auto kern = scoring == CCH_SCORING_SIGMOID ? (vec ? moe_balance_sums_kernel<T, V, L, true, true> : moe_balance_sums_kernel<T, V, L, true, false>)
+                                                       : (vec ? moe_balance_sums_kernel<T, V, L, false, true> : moe_balance_sums_kernel<T, V, L, false, false>);
+            hipLaunchKernelGGL(kern, dim3((unsigned)std::max<int64_t>(1, (tokens + run - 1) / run)), dim3(BAL_THREADS), 0, s, static_cast<const T *>(logits), expert_idx,
+                               token_mask, seq_offsets, (int)tokens, (int)num_experts, top_k, (int)num_sequences, run, part,
+                               z_coef != 0);
             return launch_status("moe_balance_sums_kernel");
         });
     });
     if (rc != CCH_OK) return rc;
-    hipLaunchKernelGGL(moe_balance_sequence_kernel, dim3((unsigned)num_sequences), dim3(BAL_THREADS), 0, s, part, chunks, (int)num_experts, top_k, coef, z_coef, counts,
-                       seq_tokens, of_seq, loss);
-    if (num_sequences > 1)
-        hipLaunchKernelGGL(moe_balance_loss_kernel, dim3(1), dim3(BAL_THREADS), 0, s, of_seq, seq_tokens, (int)num_sequences, coef, z_coef, loss);
-    return launch_status("moe_balance_sequence_kernel");
+    const dim3 grid((unsigned)((num_experts + 63) / 64), (unsigned)num_sequences);
+    hipLaunchKernelGGL(moe_balance_finish_kernel, grid, dim3(FIN_THREADS), 0, s, part, seq_offsets, (int)tokens, (int)num_experts, top_k, run, coef, z_coef, counts, seq_tokens,
+                       of_seq, loss);
+    if (grid.x * grid.y > 1)
+        hipLaunchKernelGGL(moe_balance_loss_kernel, dim3(1), dim3(BAL_THREADS), 0, s, of_seq, (int)grid.x, (int)num_sequences, coef, z_coef, loss);
+    return launch_status("moe_balance_finish_kernel");
 }
 
 extern "C" int cch_moe_balance_loss_backward(const float *grad_loss, const void *logits, int dtype, const uint8_t *token_mask, const int32_t *seq_offsets,
@@ -344,15 +473,14 @@ extern "C" int cch_moe_balance_loss_backward(const float *grad_loss, const void 
     return with_logits_type(dtype, [&](auto *type) {
         return with_lanes((int)num_experts, [&](auto v, auto lanes) {
             typedef std::remove_pointer_t<decltype(type)> T;
-            constexpr int V = decltype(v)::value, L = decltype(lanes)::value, PER = BAL_WAVES * (64 / L);
-            const int64_t need = (tokens + PER - 1) / PER, fill = (2048 + num_sequences - 1) / num_sequences;
-            auto kern = scoring == CCH_SCORING_SIGMOID
-                            ? (z_coef != 0 ? moe_balance_backward_kernel<T, V, L, true, true> : moe_balance_backward_kernel<T, V, L, true, false>)
-                            : (z_coef != 0 ? moe_balance_backward_kernel<T, V, L, false, true> : moe_balance_backward_kernel<T, V, L, false, false>);
-            hipLaunchKernelGGL(kern, dim3((unsigned)std::max<int64_t>(1, std::min(need, fill)), (unsigned)num_sequences), dim3(BAL_THREADS), 0,
-                               static_cast<hipStream_t>(stream), grad_loss, static_cast<const T *>(logits), token_mask, seq_offsets, counts, seq_tokens, (int)tokens,
-                               (int)num_experts, top_k, coef, z_coef, static_cast<T *>(grad_logits),
-                               LaneRow<T, V>::vec(logits, num_experts) && aligned(grad_logits, 16));
+            constexpr int V = decltype(v)::value, L = decltype(lanes)::value;
+            const int run = balance_run<L>(tokens, BAL_BACKWARD_STEPS);
+            const bool vec = LanePieces<T, V>::vec(logits, num_experts) && aligned(grad_logits, 16) && aligned(counts, 16);
+            auto kern = scoring == CCH_SCORING_SIGMOID ? (vec ? moe_balance_backward_kernel<T, V, L, true, true> : moe_balance_backward_kernel<T, V, L, true, false>)
+                                                       : (vec ? moe_balance_backward_kernel<T, V, L, false, true> : moe_balance_backward_kernel<T, V, L, false, false>);
+            hipLaunchKernelGGL(kern, dim3((unsigned)((tokens + run - 1) / run)), dim3(BAL_THREADS), 0, static_cast<hipStream_t>(stream), grad_loss,
+                               static_cast<const T *>(logits), token_mask, seq_offsets, counts, seq_tokens, (int)tokens, (int)num_experts, top_k, (int)num_sequences, run, coef,
+                               z_coef, static_cast<T *>(grad_logits));
             return launch_status("moe_balance_backward_kernel");
         });
     });

@@ -26,9 +26,9 @@ template <int L, bool SIGMOID, bool RENORM>
 __device__ __forceinline__ float route_weight(float l, bool there, float top, float denominator, float scale)
 {
     if (SIGMOID && !RENORM) return there ? scale * sigmoid(l) : 0.0f;
-    if (!RENORM) return there ? scale * (__expf(l - top) / denominator) : 0.0f;
+    if (!RENORM) return there ? scale * (exp_of(l - top) / denominator) : 0.0f;
     const float c = SIGMOID ? fminf(top, 0.0f) : top;
-    const float s = !there ? 0.0f : SIGMOID ? scaled_sigmoid(l, c, __expf(c)) : __expf(l - c);
+    const float s = !there ? 0.0f : SIGMOID ? scaled_sigmoid(l, c, exp_of(c)) : exp_of(l - c);
     const float sum = lanes_sum<L>(s);
     return there ? scale * (s / sum) : 0.0f;
 }
@@ -42,7 +42,7 @@ __global__ __launch_bounds__(ROUTER_THREADS) void moe_router_kernel(const T *__r
     const int64_t t = ((int64_t)blockIdx.x * ROUTER_THREADS + threadIdx.x) / L;
     const bool inside = t < tokens;
     float l[V], key[V];
-    LaneRow<T, V>::load(logits + (inside ? t : 0) * experts, at * V, experts, vec, l);
+    load_row<T, V>(logits + (inside ? t : 0) * experts, at * V, experts, vec, l);
     const bool counted = inside && (token_mask == nullptr || token_mask[t] != 0);
     float top = -INFINITY;
 #pragma unroll
@@ -55,7 +55,7 @@ __global__ __launch_bounds__(ROUTER_THREADS) void moe_router_kernel(const T *__r
         top = lanes_max<L>(top);
         float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < V; i++) sum += at * V + i < experts ? __expf(l[i] - top) : 0.0f;
+        for (int i = 0; i < V; i++) sum += at * V + i < experts ? exp_of(l[i] - top) : 0.0f;
         denominator = lanes_sum<L>(sum);
     }
     if (bias) {
@@ -63,7 +63,7 @@ __global__ __launch_bounds__(ROUTER_THREADS) void moe_router_kernel(const T *__r
         for (int i = 0; i < V; i++) {
             const int e = at * V + i;
             if (e >= experts || key[i] == -INFINITY) continue;
-            key[i] = (SIGMOID ? sigmoid(l[i]) : __expf(l[i] - top) / denominator) + bias[e];
+            key[i] = (SIGMOID ? sigmoid(l[i]) : exp_of(l[i] - top) / denominator) + bias[e];
             if (!(key[i] == key[i])) key[i] = -INFINITY;
         }
     }
@@ -127,7 +127,7 @@ __global__ __launch_bounds__(ROUTER_THREADS) void moe_router_backward_kernel(con
     const bool there = idx >= 0;
     float d[V], top, denominator = 1.0f;
     if (!SIGMOID && !RENORM) {
-        LaneRow<T, V>::load(row, at * V, experts, vec, d);
+        load_row<T, V>(row, at * V, experts, vec, d);
         top = d[0];
 #pragma unroll
         for (int i = 1; i < V; i++) top = fmaxf(top, d[i]);
@@ -135,7 +135,7 @@ __global__ __launch_bounds__(ROUTER_THREADS) void moe_router_backward_kernel(con
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < V; i++) {
-            d[i] = at * V + i < experts ? __expf(d[i] - top) : 0.0f;
+            d[i] = at * V + i < experts ? exp_of(d[i] - top) : 0.0f;
             sum += d[i];
         }
         denominator = lanes_sum<L>(sum);
@@ -145,7 +145,7 @@ __global__ __launch_bounds__(ROUTER_THREADS) void moe_router_backward_kernel(con
     const float w = route_weight<L, SIGMOID, RENORM>(sel, there, top, denominator, 1.0f);   // of scale 1
     const float dot = lanes_sum<L>(there ? g * w : 0.0f);
     float own = RENORM ? w * (g - dot) : w * g;
-    if (SIGMOID) own *= 1.0f / (1.0f + __expf(sel));   // 1 - sigmoid
+    if (SIGMOID) own *= 1.0f / (1.0f + exp_of(sel));   // 1 - sigmoid
     own = there ? own * scale : 0.0f;
 #pragma unroll
     for (int i = 0; i < V; i++) d[i] = !SIGMOID && !RENORM && dot != 0.0f ? -scale * dot * (d[i] / denominator) : 0.0f;
@@ -156,7 +156,7 @@ __global__ __launch_bounds__(ROUTER_THREADS) void moe_router_backward_kernel(con
         for (int i = 0; i < V; i++)
             if (e == i) d[i] += x;
     }
-    if (inside) LaneRow<T, V>::store(grad_logits + t * experts, at * V, experts, vec, d);
+    if (inside) store_row<T, V>(grad_logits + t * experts, at * V, experts, vec, d);
 }
 
 static int router_shape(const char *what, int dtype, int64_t tokens, int64_t experts, int top_k, int scoring)
@@ -192,7 +192,7 @@ extern "C" int cch_moe_router(const void *logits, int dtype, int64_t tokens, int
             auto kern = scoring == CCH_SCORING_SIGMOID ? (renormalize ? moe_router_kernel<T, V, L, true, true> : moe_router_kernel<T, V, L, true, false>)
                                                        : (renormalize ? moe_router_kernel<T, V, L, false, true> : moe_router_kernel<T, V, L, false, false>);
             hipLaunchKernelGGL(kern, dim3(router_grid<L>(tokens)), dim3(ROUTER_THREADS), 0, static_cast<hipStream_t>(stream), static_cast<const T *>(logits), bias,
-                               token_mask, probs, expert_idx, (int)tokens, (int)num_experts, top_k, scale, LaneRow<T, V>::vec(logits, num_experts));
+                               token_mask, probs, expert_idx, (int)tokens, (int)num_experts, top_k, scale, LanePieces<T, V>::vec(logits, num_experts));
             return launch_status("moe_router_kernel");
         });
     });
@@ -215,7 +215,7 @@ extern "C" int cch_moe_router_backward(const float *grad_probs, const void *logi
                             : (renormalize ? moe_router_backward_kernel<T, V, L, false, true> : moe_router_backward_kernel<T, V, L, false, false>);
             hipLaunchKernelGGL(kern, dim3(router_grid<L>(tokens)), dim3(ROUTER_THREADS), 0, static_cast<hipStream_t>(stream), grad_probs, static_cast<const T *>(logits),
                                expert_idx, static_cast<T *>(grad_logits), (int)tokens, (int)num_experts, top_k, scale,
-                               LaneRow<T, V>::vec(logits, num_experts) && aligned(grad_logits, 16));
+                               LanePieces<T, V>::vec(logits, num_experts) && aligned(grad_logits, 16));
             return launch_status("moe_router_backward_kernel");
         });
     });

@@ -46,60 +46,89 @@ __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__bf16 x) { return (float)x; }
 __device__ __forceinline__ float to_f32(_Float16 x) { return (float)x; }
 
-// This lane's V logits of the row at `row`, `experts` long.  vec: rows start and end on boundaries of a lane's loads.
+// This lane's V logits of a row, `experts` long, as they come from memory, so that a row can be on its way while another is worked on.  VEC: rows start and end
+// on boundaries of a lane's loads.
 template <class T, int V>
-struct LaneRow {
+struct LanePieces {
     static constexpr int CHUNK = V * (int)sizeof(T) < 16 ? V : 16 / (int)sizeof(T);   // elements of one access
     typedef T Piece __attribute__((ext_vector_type(CHUNK)));
-
     static bool vec(const void *p, int64_t experts) { return (experts * (int64_t)sizeof(T)) % (CHUNK * (int)sizeof(T)) == 0 && aligned(p, CHUNK * sizeof(T)); }
+};
+template <class T, int V, bool VEC>
+struct LaneRow {
+    static constexpr int CHUNK = VEC ? LanePieces<T, V>::CHUNK : 1;
+    typedef T Piece __attribute__((ext_vector_type(CHUNK)));
+    Piece raw[V / CHUNK];
 
-    static __device__ __forceinline__ void load(const T *row, int first, int experts, bool vec, float (&l)[V])
+    __device__ __forceinline__ void load(const T *row, int first, int experts)
     {
 #pragma unroll
-        for (int i = 0; i < V; i++) l[i] = -INFINITY;
-        if (vec) {
-#pragma unroll
-            for (int c = 0; c < V; c += CHUNK)
-                if (first + c < experts) {
-                    const Piece p = *reinterpret_cast<const Piece *>(row + first + c);
-#pragma unroll
-                    for (int i = 0; i < CHUNK; i++) l[c + i] = to_f32(p[i]);
-                }
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; i++)
-                if (first + i < experts) l[i] = to_f32(row[first + i]);
+        for (int c = 0; c < V / CHUNK; c++) {
+            raw[c] = Piece{};
+            if (first + c * CHUNK < experts) raw[c] = *reinterpret_cast<const Piece *>(row + first + c * CHUNK);
         }
     }
-    static __device__ __forceinline__ void store(T *row, int first, int experts, bool vec, const float (&d)[V])
+    __device__ __forceinline__ void values(int first, int experts, float (&l)[V]) const
     {
-        if (vec) {
 #pragma unroll
-            for (int c = 0; c < V; c += CHUNK)
-                if (first + c < experts) {
-                    Piece p;
+        for (int i = 0; i < V; i++) l[i] = first + i / CHUNK * CHUNK < experts ? to_f32(raw[i / CHUNK][i % CHUNK]) : -INFINITY;
+    }
+    static __device__ __forceinline__ void store(T *row, int first, int experts, const float (&d)[V])
+    {
 #pragma unroll
-                    for (int i = 0; i < CHUNK; i++) p[i] = (T)d[c + i];
-                    *reinterpret_cast<Piece *>(row + first + c) = p;
-                }
-        } else {
+        for (int c = 0; c < V / CHUNK; c++)
+            if (first + c * CHUNK < experts) {
+                Piece p;
 #pragma unroll
-            for (int i = 0; i < V; i++)
-                if (first + i < experts) row[first + i] = (T)d[i];
-        }
+                for (int i = 0; i < CHUNK; i++) p[i] = (T)d[c * CHUNK + i];
+                *reinterpret_cast<Piece *>(row + first + c * CHUNK) = p;
+            }
     }
 };
+template <class T, int V>
+__device__ __forceinline__ void load_row(const T *row, int first, int experts, bool vec, float (&l)[V])
+{
+    if (vec) {
+        LaneRow<T, V, true> r;
+        r.load(row, first, experts);
+        r.values(first, experts, l);
+    } else {
+        LaneRow<T, V, false> r;
+        r.load(row, first, experts);
+        r.values(first, experts, l);
+    }
+}
+template <class T, int V>
+__device__ __forceinline__ void store_row(T *row, int first, int experts, bool vec, const float (&d)[V])
+{
+    if (vec) LaneRow<T, V, true>::store(row, first, experts, d);
+    else LaneRow<T, V, false>::store(row, first, experts, d);
+}
+
+// 1 / x to a unit in the last place, one instruction (an exact division is ten).
+__device__ __forceinline__ float reciprocal(float x) { return __builtin_amdgcn_rcpf(x); }
+
+// e^x: the argument is rounded once, so that the result is off by |x| 2^-24 relative and the instruction's unit.
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
 
 // sigmoid(l) / e^c for c <= 0, c no smaller than l or zero: with c the smaller of 0 and the largest of several logits, their sum is at least 1/2
 // however negative all of them are.  `ec` = e^c.
 __device__ __forceinline__ float scaled_sigmoid(float l, float c, float ec)
 {
-    if (l > 0) return 1.0f / (1.0f + __expf(-l));   // (then c is 0)
-    const float t = __expf(l - c);
-    return t / (1.0f + t * ec);
+    // (where l > 0 c is 0)
+    const float t = exp_of(l > 0 ? -l : l - c), over = reciprocal(1.0f + (l > 0 ? t : t * ec));
+    return l > 0 ? over : t * over;
 }
-__device__ __forceinline__ float sigmoid(float l) { return 1.0f / (1.0f + __expf(-l)); }
+// sigmoid(l) and 1 - sigmoid(l) from one exponential and one reciprocal.
+__device__ __forceinline__ void sigmoid_pair(float l, float &s, float &rest)
+{
+    const float u = exp_of(-fabsf(l)), r = reciprocal(1.0f + u), ur = u * r;
+    s = l > 0 ? r : ur;
+    rest = l > 0 ? ur : r;
+}
+__device__ __forceinline__ float sigmoid(float l) { return reciprocal(1.0f + exp_of(-l)); }
+// Logits so far below zero that their sigmoids leave the range are scaled; above this none are.
+constexpr float SIGMOID_IN_RANGE = -60.0f;
 
 // The instantiation for this many experts: f(integral_constant V, integral_constant L).
 template <int N>
