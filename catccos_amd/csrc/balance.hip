@@ -378,7 +378,7 @@ __global__ __launch_bounds__(BAL_THREADS) void moe_balance_backward_kernel(const
 static int balance_shape(const char *what, int dtype, int64_t tokens, int64_t experts, int top_k, int64_t sequences, const int32_t *seq_offsets, int scoring)
 {
     CCH_REQUIRE(logits_type_ok(dtype), "%s: logits of type %d", what, dtype);
-    CCH_REQUIRE(tokens >= 0 && tokens < (int64_t)1 << 31, "%s: %lld tokens", what, (long long)tokens);
+    CCH_REQUIRE(tokens >= 0 && tokens <= ROUTER_MAX_TOKENS, "%s: %lld tokens", what, (long long)tokens);
     CCH_REQUIRE(experts >= 1 && experts <= ROUTER_MAX_EXPERTS, "%s: num_experts=%lld outside 1..%d", what, (long long)experts, ROUTER_MAX_EXPERTS);
     CCH_REQUIRE(top_k >= 1 && top_k <= ROUTER_MAX_TOPK, "%s: top_k=%d outside 1..%d", what, top_k, ROUTER_MAX_TOPK);
     CCH_REQUIRE(sequences >= 1 && sequences <= BAL_MAX_SEQUENCES && (seq_offsets || sequences == 1), "%s: num_sequences=%lld (1..%d, 1 without offsets)", what,
@@ -389,12 +389,12 @@ static int balance_shape(const char *what, int dtype, int64_t tokens, int64_t ex
 }
 
 // Tokens of a workgroup: several steps of it, so that the sums left in the workspace stay fewer than the logits, but two workgroups to a CU where there are
-// tokens for them.
+// tokens for them; more steps than `most` only where the launch would have 2^32 threads.
 template <int L>
 static int balance_run(int64_t tokens, int most)
 {
     constexpr int STEP = BAL_WAVES * (64 / L);
-    return STEP * (int)std::max<int64_t>(1, std::min<int64_t>(most, tokens / (512 * STEP)));
+    return STEP * (int)std::max<int64_t>({1, std::min<int64_t>(most, tokens / (512 * STEP)), tokens / ((int64_t)STEP << 23)});
 }
 constexpr int BAL_STEPS = 16, BAL_BACKWARD_STEPS = 4;   // at most
 
@@ -420,7 +420,7 @@ static BalanceWorkspace balance_workspace(int64_t tokens, int64_t experts, int64
 
 extern "C" int64_t cch_moe_balance_loss_workspace_bytes(int64_t tokens, int64_t num_experts, int64_t num_sequences)
 {
-    if (tokens < 0 || tokens >> 31 || num_experts < 1 || num_experts > cch::ROUTER_MAX_EXPERTS || num_sequences < 1 || num_sequences > cch::BAL_MAX_SEQUENCES) return 0;
+    if (tokens < 0 || tokens > cch::ROUTER_MAX_TOKENS || num_experts < 1 || num_experts > cch::ROUTER_MAX_EXPERTS || num_sequences < 1 || num_sequences > cch::BAL_MAX_SEQUENCES) return 0;
     return cch::balance_workspace(tokens, num_experts, num_sequences).end;
 }
 

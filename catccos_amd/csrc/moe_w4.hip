@@ -12,19 +12,47 @@ int w4_check(const char *what, int fmt, int group_size, int dtype);   // w4_matm
 
 constexpr int MW4_MAX_TOPK = 8, MW4_MAX_EXPERTS = 1024, MW4_THREADS = 256;
 
-template <class T>
+// out[t] = sum over the token's routes, in their order, of probs * y: CHUNK columns to a thread, the routes' loads issued together (one after another, each behind
+// its expert's, the kernel waits for memory top_k times).  Routes that were dropped have no y: whatever lies there is loaded and not used.
+template <class T, int ROUTES, int CHUNK>
 __global__ __launch_bounds__(MW4_THREADS) void moe_w4_combine_kernel(const float *__restrict__ y, const int32_t *__restrict__ expert_idx, const float *__restrict__ probs,
-                                                                    T *__restrict__ out, int64_t total, int k, int top_k, int experts)
+                                                                    T *__restrict__ out, int k, int top_k, int experts)
 {
-    const int64_t i = (int64_t)blockIdx.x * MW4_THREADS + threadIdx.x;
-    if (i >= total) return;
-    const int64_t t = i / k, c = i - t * k;
-    float sum = 0.0f;
-    for (int j = 0; j < top_k; j++) {
-        const int e = expert_idx[t * top_k + j];
-        if (e >= 0 && e < experts) sum += probs[t * top_k + j] * y[(t * top_k + j) * k + c];
+    typedef float In __attribute__((ext_vector_type(CHUNK)));
+    typedef T Out __attribute__((ext_vector_type(CHUNK)));
+    const int64_t t = blockIdx.y, first = t * top_k;
+    const int c = ((int)blockIdx.x * MW4_THREADS + (int)threadIdx.x) * CHUNK;
+    if (c >= k) return;
+    In v[ROUTES];
+#pragma unroll
+    for (int j = 0; j < ROUTES; j++) v[j] = *reinterpret_cast<const In *>(y + (first + min(j, top_k - 1)) * k + c);
+    In sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < ROUTES; j++) {
+        const int at = min(j, top_k - 1), e = expert_idx[first + at];
+        const float p = probs[first + at];
+        const bool there = j < top_k && e >= 0 && e < experts;
+#pragma unroll
+        for (int i = 0; i < CHUNK; i++) sum[i] = there ? sum[i] + p * v[j][i] : sum[i];
     }
-    out[i] = (T)sum;
+    Out o;
+#pragma unroll
+    for (int i = 0; i < CHUNK; i++) o[i] = (T)sum[i];
+    *reinterpret_cast<Out *>(out + t * k + c) = o;
+}
+
+template <class T>
+static int moe_w4_combine(const float *y, const int32_t *expert_idx, const float *probs, void *out, int64_t m, int64_t k, int top_k, int experts, hipStream_t s)
+{
+    const bool four = k % 4 == 0 && aligned(out, 8);
+    auto kern = top_k <= 2   ? (four ? moe_w4_combine_kernel<T, 2, 4> : moe_w4_combine_kernel<T, 2, 1>)
+                : top_k <= 4 ? (four ? moe_w4_combine_kernel<T, 4, 4> : moe_w4_combine_kernel<T, 4, 1>)
+                             : (four ? moe_w4_combine_kernel<T, 8, 4> : moe_w4_combine_kernel<T, 8, 1>);
+    const int per = MW4_THREADS * (four ? 4 : 1);
+    for (int64_t t = 0; t < m; t += 65535)   // tokens of the grid's second dimension
+        hipLaunchKernelGGL(kern, dim3((unsigned)((k + per - 1) / per), (unsigned)std::min<int64_t>(65535, m - t)), dim3(MW4_THREADS), 0, s, y + t * top_k * k,
+                           expert_idx + t * top_k, probs + t * top_k, static_cast<T *>(out) + t * k, (int)k, top_k, experts);
+    return launch_status("moe_w4_combine_kernel");
 }
 
 struct MoeW4Workspace {
@@ -47,7 +75,7 @@ static MoeW4Workspace moe_w4_workspace(int64_t m, int64_t k, int64_t top_k, int6
 
 extern "C" int64_t cch_moe_ffn_w4a16_workspace_bytes(int64_t m, int64_t k, int top_k, int64_t num_experts, int64_t n)
 {
-    if (m < 0 || k < 0 || top_k < 1 || num_experts < 1 || n < 0 || m >> 31 || k >> 30 || n >> 31 || num_experts >> 31) return 0;
+    if (m < 0 || k < 0 || top_k < 1 || num_experts < 1 || n < 0 || m >> 31 || k > cch::W4_MAX_ROWS || n > cch::W4_MAX_ROWS || num_experts >> 31 || top_k > 1024) return 0;
     return std::max<int64_t>(cch::moe_w4_workspace(m, k, top_k, n).end, 1);
 }
 
@@ -56,7 +84,7 @@ extern "C" int cch_moe_ffn_w4a16(const void *x, const int32_t *expert_idx, const
                                  int dtype, void *workspace, int64_t workspace_bytes, void *stream)
 {
     using namespace cch;
-    CCH_REQUIRE(m >= 0 && k >= 0 && n >= 0 && !(m >> 31) && !(k >> 30) && !(n >> 30), "cch_moe_ffn_w4a16: bad shape m=%lld k=%lld n=%lld", (long long)m, (long long)k,
+    CCH_REQUIRE(m >= 0 && k >= 0 && n >= 0 && !(m >> 31) && k <= W4_MAX_ROWS && n <= W4_MAX_ROWS, "cch_moe_ffn_w4a16: bad shape m=%lld k=%lld n=%lld", (long long)m, (long long)k,
                 (long long)n);
     CCH_REQUIRE(top_k >= 1 && top_k <= MW4_MAX_TOPK, "cch_moe_ffn_w4a16: top_k=%d outside 1..%d", top_k, MW4_MAX_TOPK);
     CCH_REQUIRE(num_experts >= 1 && num_experts <= MW4_MAX_EXPERTS, "cch_moe_ffn_w4a16: num_experts=%lld outside 1..%d", (long long)num_experts, MW4_MAX_EXPERTS);
@@ -78,12 +106,7 @@ extern "C" int cch_moe_ffn_w4a16(const void *x, const int32_t *expert_idx, const
                                   p + at.y, stream))
         return rc;
     const float *y = reinterpret_cast<const float *>(p + at.y);
-    const dim3 grid((unsigned)((m * k + MW4_THREADS - 1) / MW4_THREADS));
-    if (dtype == CCH_DTYPE_F16)
-        hipLaunchKernelGGL(moe_w4_combine_kernel<_Float16>, grid, dim3(MW4_THREADS), 0, static_cast<hipStream_t>(stream), y, expert_idx, probs,
-                           static_cast<_Float16 *>(out), m * k, (int)k, top_k, (int)num_experts);
-    else
-        hipLaunchKernelGGL(moe_w4_combine_kernel<__bf16>, grid, dim3(MW4_THREADS), 0, static_cast<hipStream_t>(stream), y, expert_idx, probs, static_cast<__bf16 *>(out),
-                           m * k, (int)k, top_k, (int)num_experts);
-    return launch_status("moe_w4_combine_kernel");
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    return dtype == CCH_DTYPE_F16 ? moe_w4_combine<_Float16>(y, expert_idx, probs, out, m, k, top_k, (int)num_experts, s)
+                                  : moe_w4_combine<__bf16>(y, expert_idx, probs, out, m, k, top_k, (int)num_experts, s);
 }

@@ -162,15 +162,25 @@ __global__ __launch_bounds__(ROUTER_THREADS) void moe_router_backward_kernel(con
 static int router_shape(const char *what, int dtype, int64_t tokens, int64_t experts, int top_k, int scoring)
 {
     CCH_REQUIRE(logits_type_ok(dtype), "%s: logits of type %d", what, dtype);
-    CCH_REQUIRE(tokens >= 0 && tokens < (int64_t)1 << 31, "%s: %lld tokens", what, (long long)tokens);
+    CCH_REQUIRE(tokens >= 0 && tokens <= ROUTER_MAX_TOKENS, "%s: %lld tokens", what, (long long)tokens);
     CCH_REQUIRE(experts >= 1 && experts <= ROUTER_MAX_EXPERTS, "%s: num_experts=%lld outside 1..%d", what, (long long)experts, ROUTER_MAX_EXPERTS);
     CCH_REQUIRE(top_k >= 1 && top_k <= ROUTER_MAX_TOPK && top_k <= experts, "%s: top_k=%d outside 1..min(%d, num_experts)", what, top_k, ROUTER_MAX_TOPK);
     CCH_REQUIRE(scoring == CCH_SCORING_SOFTMAX || scoring == CCH_SCORING_SIGMOID, "%s: scoring %d", what, scoring);
     return CCH_OK;
 }
 
+// f(first token, tokens) for launches of up to 2^25 tokens: one has below 2^32 threads.
+template <class F>
+static int router_launches(int64_t tokens, F f)
+{
+    for (int64_t t = 0; t < tokens; t += 1 << 25) {
+        const int rc = f(t, (int)std::min<int64_t>(1 << 25, tokens - t));
+        if (rc != CCH_OK) return rc;
+    }
+    return CCH_OK;
+}
 template <int L>
-static unsigned router_grid(int64_t tokens)
+static unsigned router_grid(int tokens)
 {
     return (unsigned)((tokens + ROUTER_THREADS / L - 1) / (ROUTER_THREADS / L));
 }
@@ -191,9 +201,12 @@ extern "C" int cch_moe_router(const void *logits, int dtype, int64_t tokens, int
             constexpr int V = decltype(v)::value, L = decltype(lanes)::value;
             auto kern = scoring == CCH_SCORING_SIGMOID ? (renormalize ? moe_router_kernel<T, V, L, true, true> : moe_router_kernel<T, V, L, true, false>)
                                                        : (renormalize ? moe_router_kernel<T, V, L, false, true> : moe_router_kernel<T, V, L, false, false>);
-            hipLaunchKernelGGL(kern, dim3(router_grid<L>(tokens)), dim3(ROUTER_THREADS), 0, static_cast<hipStream_t>(stream), static_cast<const T *>(logits), bias,
-                               token_mask, probs, expert_idx, (int)tokens, (int)num_experts, top_k, scale, LanePieces<T, V>::vec(logits, num_experts));
-            return launch_status("moe_router_kernel");
+            return router_launches(tokens, [&](int64_t t, int some) {
+                hipLaunchKernelGGL(kern, dim3(router_grid<L>(some)), dim3(ROUTER_THREADS), 0, static_cast<hipStream_t>(stream),
+                                   static_cast<const T *>(logits) + t * num_experts, bias, token_mask ? token_mask + t : nullptr, probs + t * top_k, expert_idx + t * top_k,
+                                   some, (int)num_experts, top_k, scale, LanePieces<T, V>::vec(logits, num_experts));
+                return launch_status("moe_router_kernel");
+            });
         });
     });
 }
@@ -213,10 +226,13 @@ extern "C" int cch_moe_router_backward(const float *grad_probs, const void *logi
             auto kern = scoring == CCH_SCORING_SIGMOID
                             ? (renormalize ? moe_router_backward_kernel<T, V, L, true, true> : moe_router_backward_kernel<T, V, L, true, false>)
                             : (renormalize ? moe_router_backward_kernel<T, V, L, false, true> : moe_router_backward_kernel<T, V, L, false, false>);
-            hipLaunchKernelGGL(kern, dim3(router_grid<L>(tokens)), dim3(ROUTER_THREADS), 0, static_cast<hipStream_t>(stream), grad_probs, static_cast<const T *>(logits),
-                               expert_idx, static_cast<T *>(grad_logits), (int)tokens, (int)num_experts, top_k, scale,
-                               LanePieces<T, V>::vec(logits, num_experts) && aligned(grad_logits, 16));
-            return launch_status("moe_router_backward_kernel");
+            const bool vec = LanePieces<T, V>::vec(logits, num_experts) && aligned(grad_logits, 16);
+            return router_launches(tokens, [&](int64_t t, int some) {
+                hipLaunchKernelGGL(kern, dim3(router_grid<L>(some)), dim3(ROUTER_THREADS), 0, static_cast<hipStream_t>(stream), grad_probs + t * top_k,
+                                   static_cast<const T *>(logits) + t * num_experts, expert_idx + t * top_k, static_cast<T *>(grad_logits) + t * num_experts, some,
+                                   (int)num_experts, top_k, scale, vec);
+                return launch_status("moe_router_backward_kernel");
+            });
         });
     });
 }

@@ -11,6 +11,7 @@
 namespace cch {
 
 constexpr int ROUTER_MAX_EXPERTS = 1024, ROUTER_MAX_TOPK = 8;
+constexpr int64_t ROUTER_MAX_TOKENS = 1 << 30;   // (a workgroup's last token and its step fit 32 bits)
 
 template <int CTRL>
 __device__ __forceinline__ float dpp_f32(float x)

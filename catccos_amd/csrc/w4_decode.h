@@ -8,6 +8,8 @@
 
 namespace cch {
 
+constexpr int64_t W4_MAX_ROWS = 1 << 25;   // of a matrix: a launch has below 2^32 threads, and the kernel for any K has 64 to a row
+
 // One matrix [rows, k] or a stack of them, `rows` apart.
 struct W4Matrix {
     const uint8_t *codes;

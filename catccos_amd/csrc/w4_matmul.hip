@@ -128,7 +128,7 @@ extern "C" int cch_w4a16_matmul(const void *x, const void *w, const void *scales
                                 int dtype, void *workspace, int64_t workspace_bytes, void *stream)
 {
     using namespace cch;
-    CCH_REQUIRE(m >= 0 && n >= 0 && k >= 0 && !(m >> 31) && !(n >> 31) && !(k >> 30), "cch_w4a16_matmul: bad shape m=%lld n=%lld k=%lld", (long long)m, (long long)n,
+    CCH_REQUIRE(m >= 0 && n >= 0 && k >= 0 && !(m >> 31) && n <= W4_MAX_ROWS && !(k >> 30), "cch_w4a16_matmul: bad shape m=%lld n=%lld k=%lld", (long long)m, (long long)n,
                 (long long)k);
     if (const int rc = w4_check("cch_w4a16_matmul", fmt, group_size, dtype)) return rc;
     if (m == 0 || n == 0) return CCH_OK;

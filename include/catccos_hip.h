@@ -352,7 +352,7 @@ int cch_dyn_quant_i8_rows_smooth(const void *x, const int32_t *src_rows, const f
 
 /* ---- The gate of a mixture of experts: expert_idx and probs from its logits ----
  * What the reference's examples take from files (examples/utils/gen_data_moe.py:48-57 draws them at random).
- *   logits       [tokens, num_experts] of type `dtype`; num_experts 1..1024, top_k 1..min(8, num_experts)
+ *   logits       [tokens, num_experts] of type `dtype`; tokens up to 2^30, num_experts 1..1024, top_k 1..min(8, num_experts)
  *   scoring      scores s = softmax over the experts, or sigmoid of each logit (fp32)
  *   bias         fp32 [num_experts] or NULL: added to the scores for the selection only
  *   token_mask   bytes [tokens] or NULL: a token whose byte is 0 gets no expert
@@ -375,7 +375,7 @@ int cch_moe_router_backward(const float *grad_probs, const void *logits, int dty
  * Of a sequence with N tokens that count (mask byte not 0, some logit above -inf), c_e routes to expert e, k = top_k and E experts:
  * f_e = E c_e / (k N), P_e = mean over its tokens of p_te, p = softmax(l), or sigmoid(l) / sum over the experts of sigmoid(l);
  *   loss = coef * mean over sequences with N > 0 of sum_e f_e P_e + z_coef * mean over all counted tokens of (log sum_e exp l_te)^2
- *   expert_idx   int32 [tokens, top_k]; entries outside [0, num_experts) are no routes; tokens * top_k < 2^31
+ *   expert_idx   int32 [tokens, top_k]; entries outside [0, num_experts) are no routes; tokens up to 2^30, tokens * top_k < 2^31
  *   token_mask   bytes [tokens] or NULL
  *   seq_offsets  int32 [num_sequences + 1], rising: sequence s is tokens seq_offsets[s] .. seq_offsets[s+1] - 1 (read up to `tokens`;
  *                tokens in none do not count); NULL: one sequence.  num_sequences 1..65535
@@ -399,7 +399,8 @@ int cch_moe_balance_loss_backward(const float *grad_loss, const void *logits, in
  *   zeros    CCH_FMT_INT4: bytes of scales' shape or NULL (8 everywhere): an element stands for (code - zero) * scale
  *   workspace  device memory on a 16-byte boundary of at least cch_w4a16_matmul_workspace_bytes(...) bytes (none for 0); nothing in it has to be
  *            kept or cleared between calls, calls that overlap need one each
- * Any k; k a multiple of 32 and pointers on 16-byte boundaries take the fast kernels. */
+ * m below 2^31, n up to 2^25, k below 2^30.  x and w on 16-byte boundaries with k a multiple of 32 below 2^24 (in the FFN below: 2^19 and up) take the
+ * tiled kernels, others one with a wave per output element.  Zero points are 0..240 (a byte of more is rounded by the tiled kernels where x is bf16). */
 int64_t cch_w4a16_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int cch_w4a16_matmul(const void *x, const void *w, const void *scales, const void *zeros, void *out, int64_t m, int64_t n, int64_t k, int fmt,
                      int group_size, int dtype, void *workspace, int64_t workspace_bytes, void *stream);
