@@ -482,7 +482,7 @@ __device__ __forceinline__ void w4_pass(const W4Rows &rows, const W4Matrix &w, i
 }
 
 template <class T, int KIND, bool ZEROS, class S, int OUT, bool GROUPED>
-__global__ __launch_bounds__(S::THREADS, S::MT <= 2 ? 4 : 2) void w4_tile_kernel(W4Rows rows, W4Matrix w, int pitch, int chunk, int list_at, void *__restrict__ out)
+__global__ __launch_bounds__(S::THREADS, S::NT * S::MT <= 2 ? 4 : 2) void w4_tile_kernel(W4Rows rows, W4Matrix w, int pitch, int chunk, int list_at, void *__restrict__ out)
 {
     if constexpr (!GROUPED) {
         w4_pass<T, KIND, ZEROS, S, OUT, false>(rows, w, 0, nullptr, (int)blockIdx.y * (16 * S::MT), (int)rows.rows, pitch, chunk, out);
@@ -531,36 +531,50 @@ int w4_tile_launch(const W4Rows &rows, const W4Matrix &w, void *out, hipStream_t
     return launch_status("w4_tile_kernel");
 }
 
-// Which shape.
+// Which shape.  A card of 256 CUs is full with one or two workgroups to a CU; as long as there are fewer, more waves share a tile (K in more parts), and with more
+// tiles a workgroup takes more of them (x from the caches less often, K in fewer parts).  Measured in us, bf16, int4 groups of 128 / MXFP4, K = 7168 unless said:
+//   dense, up to 4 rows, n <= 8192: 8 parts of K 5.9 / 5.8 (n = 4096), 8.7 / 8.0 (8192); 2 tiles a wave, 4 parts 9.6 / 9.6, 9.8 / 9.5;  n = 32768: 29.5 / 30.4, 24.4 / 26.0
+//   up to 8 rows, n <= 8192: half the ring for x 6.5 / 6.2 (n = 4096), 9.2 / 9.0 (8192); as for 16 rows 6.9 / 6.8, 9.6 / 9.8
+//   up to 16 rows: 1 tile a workgroup 7.3 / 7.6 (n = 4096), 13.2 / 13.6 (8192); 2 tiles a wave 8.6 / 9.0, 10.0 / 10.8, 17.9 / 19.7 (16384); 2 waves of columns 18.3 / 15.9 (16384),
+//     33 / 33.7 (32768); 4 of them 20.6 / 19.9, 30.1 / 28.8, 62.7 / 62.0 (65536); 4 with 2 tiles each 34.3 / 34.5 (32768), 49.8 / 51.4 (65536)
+//   more rows, in tiles of 32 with 2, 4 or 8 tiles of columns, the fewest that need no more than 256 workgroups, 32 rows: n = 8192 18.0 / 15.9, 19.0 / 16.8, 26.8 / 22.7;
+//     n = 16384 28 / 26, 21.9 / 20.8, 27.4 / 24.2; n = 32768 - / -, 43.9 / -, 36.4 / 34.2; with more, 64 rows by 8 tiles, 16 waves: n = 32768, 64 rows 49.8 / 42.0, against 62.5 / 60.0
+//     in tiles of 32, and 53.5 / 45.5 with 8 waves of 2 tiles each (two waves to a SIMD overlap conversions and products less than four)
+//   grouped, by routes per expert (16 experts of n = 4096, k = 7168, 6 routes a token; then 64 of n = 1024, k = 2048, 8 routes), up projection: 1 token 19.4 / 20.1, with room for 16 26.2 / 22.7;
+//     12 routes: room for 16 71.9 / 74.1, 32 64.0 / 61.0, 64 - / 67.9; 16: 29.8 / 27.4, 25.2 / 21.1, - / 25.6; 24: 107 / 110, 105 / 99, 90.8 / 69.3; 32: 44.1 / 41.9, 45.0 / 36.7, 35.8 / 27.7
+//     down projection, 12 routes: room for 16 38.8 / -, 32 - / 37.7; 16: 22.9 / 20.2, 19.3 / 17.2; 24: 59.5 / -, 51.2 / 45.6
 template <class T, int KIND, bool ZEROS>
 int w4_tile_choose(int out_kind, const W4Rows &rows, const W4Matrix &w, void *out, hipStream_t s)
 {
-#define W4_GO(S, OUT, GROUPED) w4_tile_launch<T, KIND, ZEROS, S, OUT, GROUPED>(rows, w, out, s)
+#define W4_GO(OUT, GROUPED, ...) w4_tile_launch<T, KIND, ZEROS, W4Shape<__VA_ARGS__>, OUT, GROUPED>(rows, w, out, s)
     if (out_kind == W4_OUT_PLAIN) {
-        typedef W4Shape<1, 1, 1, 1, 8> One;
-        typedef W4Shape<2, 1, 1, 1, 4> OneWide;
-        typedef std::conditional_t<KIND == W4_MX, W4Shape<1, 1, 4, 2, 4>, W4Shape<1, 1, 4, 1, 8>> Few;
-        typedef W4Shape<1, 1, 4, 4, 2> FewWide;
-        typedef W4Shape<1, 2, 8, 2, 4> Some;
-        typedef W4Shape<1, 4, 16, 2, 2> Many;
-        typedef W4Shape<2, 4, 16, 4, 2> ManyWide;
-        const bool wide = w.rows >= 16 * 2 * 256;
-        if (rows.rows <= 4) return wide ? W4_GO(OneWide, W4_OUT_PLAIN, false) : W4_GO(One, W4_OUT_PLAIN, false);
-        if (rows.rows <= 16) return wide ? W4_GO(FewWide, W4_OUT_PLAIN, false) : W4_GO(Few, W4_OUT_PLAIN, false);
-        if (rows.rows <= 32) return W4_GO(Some, W4_OUT_PLAIN, false);
-        return wide ? W4_GO(ManyWide, W4_OUT_PLAIN, false) : W4_GO(Many, W4_OUT_PLAIN, false);
+        constexpr bool G = false;
+        const int64_t m = rows.rows, n = w.rows, m32 = (m + 31) / 32;
+        if (m <= 4) return n <= 8192 ? W4_GO(W4_OUT_PLAIN, G, 1, 1, 1, 1, 8) : W4_GO(W4_OUT_PLAIN, G, 2, 1, 1, 1, 4);
+        if (m <= 8 && n <= 8192) return W4_GO(W4_OUT_PLAIN, G, 1, 1, 2, 1, 8);
+        if (m <= 16) {
+            if (n <= 4096) return W4_GO(W4_OUT_PLAIN, G, 1, 1, 4, 1, 8);
+            if (n <= 8192) return W4_GO(W4_OUT_PLAIN, G, 2, 1, 4, 1, 8);
+            if (n <= 16384) return W4_GO(W4_OUT_PLAIN, G, 1, 1, 4, 2, 4);
+            if (n <= 32768) return W4_GO(W4_OUT_PLAIN, G, 1, 1, 4, 4, 2);
+            return W4_GO(W4_OUT_PLAIN, G, 2, 1, 4, 4, 2);
+        }
+        if (m32 * ((n + 31) / 32) <= 256) return W4_GO(W4_OUT_PLAIN, G, 1, 2, 8, 2, 4);
+        if (m32 * ((n + 63) / 64) <= 256) return W4_GO(W4_OUT_PLAIN, G, 1, 2, 8, 4, 4);
+        if (m32 == 1 || m32 * ((n + 127) / 128) <= 256) return W4_GO(W4_OUT_PLAIN, G, 2, 2, 8, 4, 4);
+        return W4_GO(W4_OUT_PLAIN, G, 1, 4, 16, 8, 2);
     }
+    constexpr bool G = true;
     const int64_t tokens = rows.rows / rows.top_k;   // no expert has more of them
-    const bool few = rows.rows <= 8 * rows.num_experts;
-    typedef W4Shape<2, 1, 1, 1, 4> One;
     if (out_kind == W4_OUT_SWIGLU) {
-        typedef W4Shape<2, 1, 4, 4, 2> Few;
-        typedef W4Shape<2, 4, 16, 4, 1> Some;
-        return tokens <= 4 ? W4_GO(One, W4_OUT_SWIGLU, true) : tokens <= 16 || few ? W4_GO(Few, W4_OUT_SWIGLU, true) : W4_GO(Some, W4_OUT_SWIGLU, true);
+        if (tokens <= 4) return W4_GO(W4_OUT_SWIGLU, G, 2, 1, 1, 1, 4);
+        if (tokens <= 16 || rows.rows <= 8 * rows.num_experts) return W4_GO(W4_OUT_SWIGLU, G, 2, 1, 4, 4, 2);
+        if (tokens <= 32 || rows.rows <= 16 * rows.num_experts) return W4_GO(W4_OUT_SWIGLU, G, 2, 2, 8, 4, 1);
+        return W4_GO(W4_OUT_SWIGLU, G, 2, 4, 16, 4, 1);
     }
-    typedef W4Shape<2, 1, 4, 4, 1> Few;
-    typedef W4Shape<1, 2, 8, 4, 1> Some;
-    return tokens <= 4 ? W4_GO(One, W4_OUT_F32, true) : tokens <= 16 || few ? W4_GO(Few, W4_OUT_F32, true) : W4_GO(Some, W4_OUT_F32, true);
+    if (tokens <= 4) return W4_GO(W4_OUT_F32, G, 2, 1, 1, 1, 4);
+    if (tokens <= 16 || rows.rows <= 8 * rows.num_experts) return W4_GO(W4_OUT_F32, G, 2, 1, 4, 4, 1);
+    return W4_GO(W4_OUT_F32, G, 1, 2, 8, 8, 1);
 #undef W4_GO
 }
 
