@@ -7,11 +7,13 @@
 //   dl_te = coef / (S' N_s) p_te (f_se - sum_i p_ti f_si) [(1 - sigmoid(l_te)) for sigmoid scores] + z_coef 2 lse_t softmax(l)_te / N
 // times the loss's own gradient.
 //
-// Forward: a workgroup takes a run of tokens, whatever sequences they belong to; of each of those it leaves the sums of p (fp32 in registers) and the routes
+// Forward, where one workgroup is not enough: a workgroup takes a run of tokens, whatever sequences they belong to; of each of those it leaves the sums of p (fp32 in registers) and the routes
 // (LDS) in the workspace, and a second launch adds a sequence's sums up, in their order, so that the same inputs give the same bits.  The last workgroup of that
 // launch has the loss.  Backward: one pass, logits in, gradient out.
 //
-// Bound by the logits' bytes on paper, by exponentials and the latency of few tokens per wave in fact.
+// Bound by the logits' bytes on paper (16384 tokens of 256 experts, bf16: 8.4 MB read, then 16.8 MB read and written, 5.1 us at the rate of a large copy), by launches
+// and waits for memory in fact: that batch in 13 sequences with sigmoid scores takes 7.3 + 4.2 + 2.5 us forward and 10.0 backward, where an empty launch takes 2.4 and every
+// workgroup has two steps of 16 tokens, the exponentials of all being 1.3 us of the card's time.
 #include <algorithm>
 
 #include "router_lanes.h"
@@ -138,6 +140,114 @@ __device__ __forceinline__ N block_sum(N x, N (&scratch)[WAVES])
     return sum;
 }
 
+// What is read of a token; all of it at once, a step ahead.  (The mask, then the experts of those that it leaves, are two waits for memory in every step:
+// 16384 tokens of 256 experts in 13 sequences 8.3 us at best, against 7.3.)
+template <class T, int V, bool VEC>
+struct TokenIn {
+    LaneRow<T, V, VEC> row;
+    uint32_t mask;
+    int e;
+    __device__ __forceinline__ void load(const T *logits, const uint8_t *token_mask, const int32_t *expert_idx, int t, int at, int experts, int top_k)
+    {
+        row.load(logits + (int64_t)t * experts, at * V, experts);
+        mask = token_mask ? token_mask[t] : 1;
+        e = -1;
+        if (at < top_k) e = expert_idx[(int64_t)t * top_k + at];
+    }
+    __device__ __forceinline__ void load(const T *logits, const uint8_t *token_mask, int t, int at, int experts)
+    {
+        row.load(logits + (int64_t)t * experts, at * V, experts);
+        mask = token_mask ? token_mask[t] : 1;
+    }
+};
+
+// The workgroup's sums over tokens [from, to), STEP at a time, the first of them in `token`: in lanes 0 .. L - 1 of a wave p per expert, in every lane sum of lse^2 and
+// tokens of the wave; routes per expert in LDS.
+template <class T, int V, int L, bool SIGMOID, bool VEC, int STEP>
+__device__ __forceinline__ void add_tokens(TokenIn<T, V, VEC> &token, const T *logits, const int32_t *expert_idx, const uint8_t *token_mask, int from, int to, int mine,
+                                           int experts, int top_k, bool z, int32_t *routes, float (&acc)[V], float &zsum, int &n)
+{
+    const int lane = threadIdx.x & 63, at = lane & (L - 1);
+    zsum = 0.0f;
+    n = 0;
+#pragma unroll
+    for (int i = 0; i < V; i++) acc[i] = 0.0f;
+    for (int t1 = from; t1 < to; t1 += STEP) {
+        const int t = t1 + mine;
+        TokenIn<T, V, VEC> next;
+        next.load(logits, token_mask, expert_idx, min(t + STEP, to - 1), at, experts, top_k);
+        const bool inside = t < to && token.mask != 0;
+        float l[V], rest[V], q[V], lse = 0.0f;
+        token.row.values(at * V, experts, l);
+        const bool valid = token_shares<V, L, SIGMOID>(l, rest, q, lse, z) && inside;
+        if (valid) {
+#pragma unroll
+            for (int i = 0; i < V; i++) acc[i] += l[i];
+            if (at == 0) {
+                n++;
+                if (z) zsum += lse * lse;
+            }
+            if (token.e >= 0 && token.e < experts) atomicAdd(&routes[token.e], 1);
+        }
+        token = next;
+    }
+#pragma unroll
+    for (int off = L; off < 64; off <<= 1) {
+#pragma unroll
+        for (int i = 0; i < V; i++) acc[i] += __shfl_xor(acc[i], off, 64);
+        zsum += __shfl_xor(zsum, off, 64);
+        n += __shfl_xor(n, off, 64);
+    }
+    zsum = __shfl(zsum, 0, 64);
+    n = __shfl(n, 0, 64);
+}
+
+// All of it in one workgroup, for one sequence of few tokens.  In us, sigmoid scores, against the launches below: 512 tokens of 16 experts 5.4 / 6.5, 1024 tokens 7.3 / 6.6;
+// 64 experts, 256 tokens 6.0 / 6.7, 512 tokens 7.9 / 6.9; 256 experts, 128 tokens 8.0 / 10.0, 256 tokens 12.0 / 10.0; 1024 experts, 32 tokens 8.6 / 11.1, 64 tokens
+// 13.5 / 11.2.  So: four steps at most, and 2^14 logits, 2^15 of more than 64 experts, where the launches below are three.
+template <int L>
+constexpr int ONE_THREADS = L > 32 ? 512 : 1024;   // (the waves' sums fit LDS)
+constexpr int ONE_STEPS = 4;
+template <class T, int V, int L, bool SIGMOID, bool VEC>
+__global__ __launch_bounds__(ONE_THREADS<L>) void moe_balance_one_kernel(const T *__restrict__ logits, const int32_t *__restrict__ expert_idx,
+                                                                     const uint8_t *__restrict__ token_mask, const int32_t *__restrict__ seq_offsets, int tokens, int experts,
+                                                                     int top_k, float coef, float z_coef, float *__restrict__ loss, int32_t *__restrict__ counts,
+                                                                     int32_t *__restrict__ seq_tokens)
+{
+    constexpr int THREADS = ONE_THREADS<L>, WAVES = THREADS / 64, TPW = 64 / L, STEP = WAVES * TPW;
+    __shared__ float shares[WAVES][V * L], fs[WAVES];
+    __shared__ int32_t routes[V * L], is[WAVES];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at = lane & (L - 1), mine = wave * TPW + lane / L;
+    const Span span = span_of(seq_offsets, 0, tokens);
+    TokenIn<T, V, VEC> token;
+    if (span.begin < span.end) token.load(logits, token_mask, expert_idx, min(span.begin + mine, span.end - 1), at, experts, top_k);
+    for (int e = threadIdx.x; e < V * L; e += THREADS) routes[e] = 0;
+    __syncthreads();
+    float acc[V], zsum;
+    int n;
+    add_tokens<T, V, L, SIGMOID, VEC, STEP>(token, logits, expert_idx, token_mask, span.begin, span.end, mine, experts, top_k, z_coef != 0, routes, acc, zsum, n);
+    if (lane < L) {
+#pragma unroll
+        for (int i = 0; i < V; i++) shares[wave][at * V + i] = acc[i];
+    }
+    zsum = block_sum(lane == 0 ? zsum : 0.0f, fs);
+    n = block_sum(lane == 0 ? n : 0, is);
+    float sum = 0.0f;
+    for (int e = threadIdx.x; e < experts; e += THREADS) {
+        float p = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) p += shares[w][e];
+        counts[e] = routes[e];
+        sum += p * (float)routes[e];
+    }
+    sum = block_sum(sum, fs);
+    if (threadIdx.x == 0) {
+        const float counted = (float)max(n, 1);
+        *seq_tokens = n;
+        *loss = coef * (sum / counted * ((float)experts / ((float)top_k * counted))) + z_coef * (zsum / counted);
+    }
+}
+
 // Tokens [run * blockIdx.x, ...) of `run`; what they add to sequence s goes to part[(blockIdx.x + s) * (2 experts + 2)]: p per expert, routes per expert, sum of
 // lse^2, tokens.  (Workgroups in order and sequences in order: no two meet.)
 template <class T, int V, int L, bool SIGMOID, bool VEC>
@@ -153,8 +263,8 @@ __global__ __launch_bounds__(BAL_THREADS) void moe_balance_sums_kernel(const T *
     const int mine = wave * TPW + lane / L;
     if (first >= end) return;
     // the first rows are on their way while the sequences are looked at
-    LaneRow<T, V, VEC> row;
-    row.load(logits + (int64_t)min(first + mine, end - 1) * experts, at * V, experts);
+    TokenIn<T, V, VEC> token;
+    token.load(logits, token_mask, expert_idx, min(first + mine, end - 1), at, experts, top_k);
     int s = max(place_of<BAL_THREADS, false, false>(seq_offsets, nullptr, sequences, first, staged, scratch).s, 0);
     const int32_t *const offsets = seq_offsets && sequences < BAL_THREADS ? staged : seq_offsets;
     for (; s < sequences; s++) {
@@ -162,41 +272,12 @@ __global__ __launch_bounds__(BAL_THREADS) void moe_balance_sums_kernel(const T *
         if (span.begin >= end) break;
         const int from = max(span.begin, first), to = min(span.end, end);
         if (from >= to) continue;
-        if (from > first) row.load(logits + (int64_t)min(from + mine, to - 1) * experts, at * V, experts);
+        if (from > first) token.load(logits, token_mask, expert_idx, min(from + mine, to - 1), at, experts, top_k);
         for (int e = threadIdx.x; e < V * L; e += BAL_THREADS) routes[e] = 0;
         __syncthreads();
-        float acc[V], zsum = 0.0f;
-        int n = 0;
-#pragma unroll
-        for (int i = 0; i < V; i++) acc[i] = 0.0f;
-        for (int t1 = from; t1 < to; t1 += STEP) {
-            const int t = t1 + mine;
-            LaneRow<T, V, VEC> next;
-            next.load(logits + (int64_t)min(t + STEP, to - 1) * experts, at * V, experts);
-            const bool inside = t < to && (token_mask == nullptr || token_mask[t] != 0);
-            int e = -1;
-            if (inside && at < top_k) e = expert_idx[(int64_t)t * top_k + at];
-            float l[V], rest[V], q[V], lse = 0.0f;
-            row.values(at * V, experts, l);
-            const bool valid = token_shares<V, L, SIGMOID>(l, rest, q, lse, z) && inside;
-            if (valid) {
-#pragma unroll
-                for (int i = 0; i < V; i++) acc[i] += l[i];
-                if (at == 0) {
-                    n++;
-                    if (z) zsum += lse * lse;
-                }
-                if (e >= 0 && e < experts) atomicAdd(&routes[e], 1);
-            }
-            row = next;
-        }
-#pragma unroll
-        for (int off = L; off < 64; off <<= 1) {
-#pragma unroll
-            for (int i = 0; i < V; i++) acc[i] += __shfl_xor(acc[i], off, 64);
-            zsum += __shfl_xor(zsum, off, 64);
-            n += __shfl_xor(n, off, 64);
-        }
+        float acc[V], zsum;
+        int n;
+        add_tokens<T, V, L, SIGMOID, VEC, STEP>(token, logits, expert_idx, token_mask, from, to, mine, experts, top_k, z, routes, acc, zsum, n);
         if (lane < L) {
 #pragma unroll
             for (int i = 0; i < V; i++) shares[wave][at * V + i] = acc[i];
@@ -323,8 +404,8 @@ __global__ __launch_bounds__(BAL_THREADS) void moe_balance_backward_kernel(const
     __shared__ int scratch[3][BAL_WAVES];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), at = lane & (L - 1);
     const int first = (int)blockIdx.x * run, end = min(first + run, tokens), mine = wave * TPW + lane / L;
-    LaneRow<T, V, VEC> row;
-    row.load(logits + (int64_t)min(first + mine, end - 1) * experts, at * V, experts);
+    TokenIn<T, V, VEC> token;
+    token.load(logits, token_mask, min(first + mine, end - 1), at, experts);
     const float g = *grad_loss;
     const bool z = z_coef != 0;
     const Place place = place_of<BAL_THREADS, true, true>(seq_offsets, seq_tokens, sequences, first, staged, scratch);
@@ -338,7 +419,7 @@ __global__ __launch_bounds__(BAL_THREADS) void moe_balance_backward_kernel(const
         if (span.begin >= end) break;
         const int from = max(span.begin, first), to = min(span.end, end);
         if (from >= to) continue;
-        if (from > first) row.load(logits + (int64_t)min(from + mine, to - 1) * experts, at * V, experts);
+        if (from > first) token.load(logits, token_mask, min(from + mine, to - 1), at, experts);
         float v[V];
         const float n = real ? (float)max(seq_tokens[s], 1) : 1.0f, unit = g * coef / ((float)max(place.alive, 1) * n) * ((float)experts / ((float)top_k * n));
         constexpr int FEW = VEC && V >= 4 ? 4 : VEC ? 2 : 1;   // counts of one access
@@ -352,11 +433,11 @@ __global__ __launch_bounds__(BAL_THREADS) void moe_balance_backward_kernel(const
         }
         for (int t1 = from; t1 < to; t1 += STEP) {
             const int t = t1 + mine;
-            LaneRow<T, V, VEC> next;
-            next.load(logits + (int64_t)min(t + STEP, to - 1) * experts, at * V, experts);
-            const bool inside = real && t < to && (token_mask == nullptr || token_mask[t] != 0);
+            TokenIn<T, V, VEC> next;
+            next.load(logits, token_mask, min(t + STEP, to - 1), at, experts);
+            const bool inside = real && t < to && token.mask != 0;
             float l[V], rest[V], q[V], d[V], lse = 0.0f;
-            row.values(at * V, experts, l);
+            token.row.values(at * V, experts, l);
             const bool valid = token_shares<V, L, SIGMOID>(l, rest, q, lse, z) && inside;
             float dot = 0.0f;
 #pragma unroll
@@ -370,7 +451,7 @@ __global__ __launch_bounds__(BAL_THREADS) void moe_balance_backward_kernel(const
                 if (!valid) d[i] = 0.0f;
             }
             if (t < to) LaneRow<T, V, VEC>::store(grad_logits + (int64_t)t * experts, at * V, experts, d);
-            row = next;
+            token = next;
         }
     }
 }
@@ -439,12 +520,22 @@ extern "C" int cch_moe_balance_loss(const void *logits, int dtype, const int32_t
     float *of_seq = reinterpret_cast<float *>(p), *part = reinterpret_cast<float *>(p + at.part);
     hipStream_t s = static_cast<hipStream_t>(stream);
     int run = 1;
+    bool one = false;
     const int rc = with_logits_type(dtype, [&](auto *type) {
         return with_lanes((int)num_experts, [&](auto v, auto lanes) {
             typedef std::remove_pointer_t<decltype(type)> T;
             constexpr int V = decltype(v)::value, L = decltype(lanes)::value;
             run = balance_run<L>(tokens, BAL_STEPS);
             const bool vec = LanePieces<T, V>::vec(logits, num_experts);
+            // (its comment has both sides)
+            one = tokens > 0 && num_sequences == 1 && tokens <= ONE_STEPS * (ONE_THREADS<L> / L) && tokens * V * L <= (V * L <= 64 ? 1 << 14 : 1 << 15);
+            if (one) {
+                auto kern = scoring == CCH_SCORING_SIGMOID ? (vec ? moe_balance_one_kernel<T, V, L, true, true> : moe_balance_one_kernel<T, V, L, true, false>)
+                                                           : (vec ? moe_balance_one_kernel<T, V, L, false, true> : moe_balance_one_kernel<T, V, L, false, false>);
+                hipLaunchKernelGGL(kern, dim3(1), dim3(ONE_THREADS<L>), 0, s, static_cast<const T *>(logits), expert_idx, token_mask, seq_offsets, (int)tokens, (int)num_experts,
+                                   top_k, coef, z_coef, loss, counts, seq_tokens);
+                return launch_status("moe_balance_one_kernel");
+            }
             auto kern = scoring == CCH_SCORING_SIGMOID ? (vec ? moe_balance_sums_kernel<T, V, L, true, true> : moe_balance_sums_kernel<T, V, L, true, false>)
                                                        : (vec ? moe_balance_sums_kernel<T, V, L, false, true> : moe_balance_sums_kernel<T, V, L, false, false>);
             hipLaunchKernelGGL(kern, dim3((unsigned)std::max<int64_t>(1, (tokens + run - 1) / run)), dim3(BAL_THREADS), 0, s, static_cast<const T *>(logits), expert_idx,
@@ -453,7 +544,7 @@ extern "C" int cch_moe_balance_loss(const void *logits, int dtype, const int32_t
             return launch_status("moe_balance_sums_kernel");
         });
     });
-    if (rc != CCH_OK) return rc;
+    if (rc != CCH_OK || one) return rc;
     const dim3 grid((unsigned)((num_experts + 63) / 64), (unsigned)num_sequences);
     hipLaunchKernelGGL(moe_balance_finish_kernel, grid, dim3(FIN_THREADS), 0, s, part, seq_offsets, (int)tokens, (int)num_experts, top_k, run, coef, z_coef, counts, seq_tokens,
                        of_seq, loss);

@@ -531,18 +531,36 @@ int w4_tile_launch(const W4Rows &rows, const W4Matrix &w, void *out, hipStream_t
     return launch_status("w4_tile_kernel");
 }
 
-// Which shape.  A card of 256 CUs is full with one or two workgroups to a CU; as long as there are fewer, more waves share a tile (K in more parts), and with more
-// tiles a workgroup takes more of them (x from the caches less often, K in fewer parts).  Measured in us, bf16, int4 groups of 128 / MXFP4, K = 7168 unless said:
-//   dense, up to 4 rows, n <= 8192: 8 parts of K 5.9 / 5.8 (n = 4096), 8.7 / 8.0 (8192); 2 tiles a wave, 4 parts 9.6 / 9.6, 9.8 / 9.5;  n = 32768: 29.5 / 30.4, 24.4 / 26.0
-//   up to 8 rows, n <= 8192: half the ring for x 6.5 / 6.2 (n = 4096), 9.2 / 9.0 (8192); as for 16 rows 6.9 / 6.8, 9.6 / 9.8
-//   up to 16 rows: 1 tile a workgroup 7.3 / 7.6 (n = 4096), 13.2 / 13.6 (8192); 2 tiles a wave 8.6 / 9.0, 10.0 / 10.8, 17.9 / 19.7 (16384); 2 waves of columns 18.3 / 15.9 (16384),
-//     33 / 33.7 (32768); 4 of them 20.6 / 19.9, 30.1 / 28.8, 62.7 / 62.0 (65536); 4 with 2 tiles each 34.3 / 34.5 (32768), 49.8 / 51.4 (65536)
-//   more rows, in tiles of 32 with 2, 4 or 8 tiles of columns, the fewest that need no more than 256 workgroups, 32 rows: n = 8192 18.0 / 15.9, 19.0 / 16.8, 26.8 / 22.7;
-//     n = 16384 28 / 26, 21.9 / 20.8, 27.4 / 24.2; n = 32768 - / -, 43.9 / -, 36.4 / 34.2; with more, 64 rows by 8 tiles, 16 waves: n = 32768, 64 rows 49.8 / 42.0, against 62.5 / 60.0
-//     in tiles of 32, and 53.5 / 45.5 with 8 waves of 2 tiles each (two waves to a SIMD overlap conversions and products less than four)
-//   grouped, by routes per expert (16 experts of n = 4096, k = 7168, 6 routes a token; then 64 of n = 1024, k = 2048, 8 routes), up projection: 1 token 19.4 / 20.1, with room for 16 26.2 / 22.7;
-//     12 routes: room for 16 71.9 / 74.1, 32 64.0 / 61.0, 64 - / 67.9; 16: 29.8 / 27.4, 25.2 / 21.1, - / 25.6; 24: 107 / 110, 105 / 99, 90.8 / 69.3; 32: 44.1 / 41.9, 45.0 / 36.7, 35.8 / 27.7
-//     down projection, 12 routes: room for 16 38.8 / -, 32 - / 37.7; 16: 22.9 / 20.2, 19.3 / 17.2; 24: 59.5 / -, 51.2 / 45.6
+// Which shape.  256 CUs are full with one or two workgroups each: as long as there are fewer, more waves share a tile (K in more parts), and where there are more tiles
+// a workgroup takes several (x comes from the caches less often, K is in fewer parts).  Measured in us, int4 in groups of 128 / MXFP4, bf16 x, random codes:
+//
+//   dense, K = 7168, by n:            4096          8192          16384         32768         65536
+//   1 row      1 tile, K in 8      *  6.0 /  5.7  *  9.1 /  7.8    15.3 / 14.4   31.7 / 31.5
+//              2 tiles, K in 4        9.4 /  9.6    10.2 / 10.5  * 14.5 / 13.9 * 27.3 / 27.2
+//   8 rows     1 tile, 8 rows of x *  6.6 /  6.2  *  9.7 /  9.1
+//              1 tile, 16             7.1 /  6.7    12.7 / 12.3
+//   16 rows    1 tile, K in 8      *  7.5 /  7.5    13.8 / 14.0    25.4 / 26.2   60.3 / 61.5   118 / 121
+//              2 tiles, K in 8        8.7 /  9.0  * 10.4 / 11.0    18.7 / 20.1   43.1 / 45.6    84 / 89
+//              2 waves of 1, in 4    11.6 /  9.9    13.4 / 12.6  * 18.8 / 16.2   38.6 / 34.1    74 / 67
+//              4 waves of 1, in 2    16.8 / 14.8    18.6 / 17.9    21.3 / 19.9 * 33.3 / 29.1    65 / 62
+//              4 waves of 2, in 2    23.6 / 22.3    24.0 / 23.4    25.4 / 25.4   35.5 / 34.5  * 53 / 52
+//   32 rows    2 of 1, in 4        * 15.9 / 12.5  * 18.4 / 16.2    34.0 / 30.5   71.5 / 63.0          (more rows: whichever of the three has
+//              4 of 1, in 4          18.3 / 14.6    19.8 / 17.0  * 22.5 / 21.3   48.5 / 42.8           no more than 256 workgroups)
+//              4 of 2, in 4          26.1 / 21.4    27.2 / 22.5    27.7 / 24.1 * 39.4 / 34.4
+//   64 rows    tiles of 32, best   * 17.4 / 13.9  * 21.6 / 18.2  * 31.6 / 25.5   70.3 / 60.2
+//              64 rows, 8 of 1, in 2 44.2 / 30.4    45.2 / 30.8    45.4 / 31.9 * 58.2 / 43.1
+//              64 rows, 4 of 2, in 2 49.5 / 35.6    49.5 / 36.4    49.7 / 37.3   60.3 / 47.0          (two waves to a SIMD, four above)
+//
+//   grouped, 16 experts, K = 7168, n = 4096, 6 routes a token; 64 experts, K = 2048, n = 1024, 8 routes; by the routes of an expert:
+//   up projection     1 token              8 (64 tokens, 64 experts)   12 (32, 16)        16 (128, 64)      24 (64, 16)       32 (256, 64)
+//     4 rows        * 19.2 / 20.0             45.2 / 39.1             152  / 143          67.5 / 61.1       260 / 256         126 / 112
+//     16              30.1 / 29.7           * 18.1 / 17.0              73.0 / 74.5        29.9 / 27.5       110 / 110          44.1 / 41.7
+//     32              46.6 / 44.3             23.4 / 19.9           *  68.7 / 61.8      * 24.3 / 21.1       106 /  98          43.0 / 36.3
+//     64              65.1 / 51.8             32.9 / 24.3             101  /  73.4        33.9 / 25.7     * 101 /  77        * 35.6 / 27.5
+//   down projection
+//     4 rows        * 13.8 / 12.9             35.5 / 33.7              81.5 / 71.9        55.0 / 52.2       142 / 128         106 / 101
+//     16              16.0 / 15.5           * 14.6 / 13.2              40.8 / 41.5        23.1 / 20.6        62 /  61          32.0 / 30.6
+//     32              19.4 / 15.5             18.1 / 16.4           *  44.3 / 38.7      * 19.3 / 17.7     *  52 /  46        * 32.0 / 27.1
 template <class T, int KIND, bool ZEROS>
 int w4_tile_choose(int out_kind, const W4Rows &rows, const W4Matrix &w, void *out, hipStream_t s)
 {
