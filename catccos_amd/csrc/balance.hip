@@ -328,10 +328,21 @@ __global__ __launch_bounds__(FIN_THREADS) void moe_balance_finish_kernel(const f
     float p = 0.0f, zsum = 0.0f;
     int r = 0, n = 0;
     if (e < experts) {
-#pragma unroll 4
-        for (int c = c0 + wave; c < c1; c += FIN_WAVES) {
-            p += mine[(size_t)c * pitch + e];
-            r += __float_as_int(mine[(size_t)c * pitch + experts + e]);
+        constexpr int MANY = 16;   // on their way together
+        for (int first = c0 + wave; first < c1; first += MANY * FIN_WAVES) {
+            float v[MANY];
+            int q[MANY];
+#pragma unroll
+            for (int u = 0; u < MANY; u++) {
+                const float *from = mine + (size_t)min(first + u * FIN_WAVES, c1 - 1) * pitch + e;
+                v[u] = from[0];
+                q[u] = __float_as_int(from[experts]);
+            }
+#pragma unroll
+            for (int u = 0; u < MANY; u++) {
+                p += first + u * FIN_WAVES < c1 ? v[u] : 0.0f;
+                r += first + u * FIN_WAVES < c1 ? q[u] : 0;
+            }
         }
     }
     for (int c = c0 + (int)threadIdx.x; c < c1; c += FIN_THREADS) {
