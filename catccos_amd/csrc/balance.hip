@@ -310,7 +310,8 @@ __global__ __launch_bounds__(BAL_THREADS) void moe_balance_sums_kernel(const T *
     }
 }
 
-// Workgroup (b, s): experts 64 b ... of sequence s, a wave to every sixteenth workgroup's sums.  One workgroup alone has the loss; of several each leaves its
+// Workgroup (b, s): experts 64 b ... of sequence s, a wave to every sixteenth workgroup's sums, sixteen of them on their way together (four: 16384 tokens of 16 experts
+// 9.8 us for the whole forward pass instead of 8.9).  One workgroup alone has the loss; of several each leaves its
 // share, the sum of lse^2 and the tokens in of_seq, for the launch below.  (The last of them to come could add these up instead, but publishing them to one
 // another takes longer than a launch: 9.5 us against 3.0 for 16 experts, the caches of the card's parts being written back.)
 constexpr int FIN_THREADS = 1024, FIN_WAVES = FIN_THREADS / 64;
@@ -480,8 +481,9 @@ static int balance_shape(const char *what, int dtype, int64_t tokens, int64_t ex
     return CCH_OK;
 }
 
-// Tokens of a workgroup: several steps of it, so that the sums left in the workspace stay fewer than the logits, but two workgroups to a CU where there are
-// tokens for them; more steps than `most` only where the launch would have 2^32 threads.
+// Tokens of a workgroup: several steps of it, so that the sums left in the workspace stay fewer than the logits and reading the sequences is paid once, but two
+// workgroups to a CU where there are tokens for them (262144 tokens of 64 experts, forward with up to 4 / 16 / 64 steps 28.7 / 21.6 / 21.7 us, backward with 1 / 4 / 16
+// 20.3 / 15.5 / 16.7; of 256 experts 52.6 / 42.6 / 45.0 and 71 / 44 / 45); more steps than `most` only where the launch would have 2^32 threads.
 template <int L>
 static int balance_run(int64_t tokens, int most)
 {

@@ -11,7 +11,13 @@
 //   softmax, renormalised    dl_j = w_j (g_j - sum_i g_i w_i / scale), the selected experts only
 //   sigmoid                  dl_j = w_j (1 - s_j) g_j
 //   sigmoid, renormalised    dl_j = w_j (1 - s_j) (g_j - sum_i g_i w_i / scale)
-// Everything is fp32 in registers; a row of logits is read once, and in the backward pass of three of the four forms not at all but for the selected ones.
+// Everything is fp32 in registers; a row of logits is read once, and in the backward pass of three of the four forms not at all but for the selected ones.  The
+// selection is top_k times the maximum over a lane's keys and over the lanes, the lowest index that holds it, and that key's removal: for few experts and few routes
+// less than sorting anything, and ties need no extra step.
+//
+// Bound: on paper the bytes (16384 tokens of 64 experts in bf16, 8 routes: 3.1 MB forward, 5.2 MB backward, 1.6 us for both at the rate of a large copy), in fact the
+// launch (an empty one 2.4 us) and the selection's instructions, some 2 V + 20 to a route: that case takes 4.8 + 4.5 us, 4099 tokens of 256 experts (fp32, sigmoid) 5.2 +
+// 5.3, 64 tokens of 16 experts 2.3; 16384 x 1024 28.7 + 23.6 (1.2 and 2.8 TB/s).
 #include <algorithm>
 
 #include "router_lanes.h"
