@@ -736,7 +736,7 @@ def w4a16_matmul(x, w, scales, zeros=None, fmt="int4", group_size=128):
     """x [M, K] (bf16 or half) times 4-bit weights of N rows: the linear layer of a decode step.  Returns [M, N] in x's type; sums in fp32.
 
     w uint8 [N, ceil(K/2)], element 2j in the low nibble.  fmt "int4": an element stands for (code - zero) * scale with scales [N, ceil(K/group_size)]
-    of x's type and zeros uint8 of that shape, or None for 8 everywhere; group_size 32, 64 or 128.  fmt "e2m1": MXFP4, scales E8M0 uint8
+    of x's type and zeros uint8 (0..240) of that shape, or None for 8 everywhere; group_size 32, 64 or 128.  fmt "e2m1": MXFP4, scales E8M0 uint8
     [N, scale_cols(K)], payload and scales as mx_quant(weights [N, K], "e2m1") returns them.  Inference only."""
     r = _direct.w4a16_matmul(x, w, scales, zeros, fmt, group_size)
     if r is not NotImplemented:

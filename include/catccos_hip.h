@@ -399,8 +399,8 @@ int cch_moe_balance_loss_backward(const float *grad_loss, const void *logits, in
  *   zeros    CCH_FMT_INT4: bytes of scales' shape or NULL (8 everywhere): an element stands for (code - zero) * scale
  *   workspace  device memory on a 16-byte boundary of at least cch_w4a16_matmul_workspace_bytes(...) bytes (none for 0); nothing in it has to be
  *            kept or cleared between calls, calls that overlap need one each
- * m below 2^31, n up to 2^25, k below 2^30.  x and w on 16-byte boundaries with k a multiple of 32 below 2^24 (in the FFN below: 2^19 and up) take the
- * tiled kernels, others one with a wave per output element.  Zero points are 0..240 (a byte of more is rounded by the tiled kernels where x is bf16). */
+ * m below 2^31, n up to 2^25, k below 2^30.  x and w on 16-byte boundaries and a k that is a multiple of 32 and below 2^24 (in the FFN below: below 2^19) take the
+ * tiled kernels; anything else takes one with a wave per output element.  Zero points are 0..240: where x is bf16 the tiled kernels round a byte of more. */
 int64_t cch_w4a16_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int cch_w4a16_matmul(const void *x, const void *w, const void *scales, const void *zeros, void *out, int64_t m, int64_t n, int64_t k, int fmt,
                      int group_size, int dtype, void *workspace, int64_t workspace_bytes, void *stream);
