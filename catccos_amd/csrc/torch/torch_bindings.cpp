@@ -23,6 +23,7 @@
 #include <cctype>
 #include <initializer_list>
 #include <mutex>
+#include <optional>
 #include <string>
 #include <tuple>
 
@@ -339,6 +340,200 @@ at::Tensor MoeFfnMxfp8(const at::Tensor &x_in, const at::Tensor &expert_idx_in, 
 }
 
 // ---------------------------------------------------------------------------------------------
+// The MoE gate, its balance loss (each with its gradient as a call of its own) and the products with 4-bit weights
+
+typedef std::optional<at::Tensor> MaybeTensor;
+
+int DtypeCode(const at::Tensor &t)
+{
+    if (t.scalar_type() == at::kBFloat16) return CCH_DTYPE_BF16;
+    if (t.scalar_type() == at::kHalf) return CCH_DTYPE_F16;
+    TORCH_CHECK(t.scalar_type() == at::kFloat, "bfloat16, float16 or float32 expected, got ", t.scalar_type());
+    return CCH_DTYPE_F32;
+}
+int ScoringCode(const std::string &s)
+{
+    TORCH_CHECK(s == "softmax" || s == "sigmoid", "unknown scoring '", s, "' (softmax or sigmoid)");
+    return s == "sigmoid" ? CCH_SCORING_SIGMOID : CCH_SCORING_SOFTMAX;
+}
+void CheckLogits(const at::Tensor &logits)
+{
+    TORCH_CHECK(logits.dim() == 2, "logits must be [tokens, experts]");
+    DtypeCode(logits);
+}
+
+// An optional argument on `like`'s GPU, of the type and number of elements that the kernel takes it to be; contiguous.
+at::Tensor Optional(const char *op, const char *name, const MaybeTensor &t, const at::Tensor &like, std::initializer_list<at::ScalarType> types, int64_t numel)
+{
+    if (!t || !t->defined()) return at::Tensor();
+    SameDevice(op, {{"the first argument", like}, {name, *t}});
+    TORCH_CHECK(std::find(types.begin(), types.end(), t->scalar_type()) != types.end() && t->numel() == numel, "catccos::", op, ": ", name, " must have ", numel,
+                " elements of its type");
+    return t->contiguous();
+}
+template <class T>
+T *PtrOf(const at::Tensor &t)
+{
+    return t.defined() ? static_cast<T *>(t.data_ptr()) : nullptr;
+}
+
+std::tuple<at::Tensor, at::Tensor> MoeRouter(const at::Tensor &logits_in, int64_t top_k, std::string scoring, bool renormalize, double scale, const MaybeTensor &bias_in,
+                                             const MaybeTensor &mask_in)
+{
+    NeedInit();
+    CheckLogits(logits_in);
+    SameDevice("moe_router", {{"logits", logits_in}});
+    c10::DeviceGuard guard(logits_in.device());
+    const at::Tensor logits = logits_in.contiguous();
+    const int64_t tokens = logits.size(0), e = logits.size(1);
+    TORCH_CHECK(top_k >= 1 && top_k <= 8 && top_k <= e, "top_k must be 1..8 and no more than the experts");
+    const at::Tensor bias = Optional("moe_router", "bias", bias_in, logits, {at::kFloat}, e), mask = Optional("moe_router", "token_mask", mask_in, logits, {at::kBool, at::kByte}, tokens);
+    at::Tensor probs = at::empty({tokens, top_k}, logits.options().dtype(at::kFloat)), idx = at::empty({tokens, top_k}, logits.options().dtype(at::kInt));
+    Check(cch_moe_router(logits.data_ptr(), DtypeCode(logits), tokens, e, (int)top_k, ScoringCode(scoring), renormalize, (float)scale, PtrOf<float>(bias), PtrOf<uint8_t>(mask),
+                         probs.data_ptr<float>(), idx.data_ptr<int32_t>(), StreamOf(logits)),
+          "moe_router");
+    return {probs, idx};
+}
+
+at::Tensor MoeRouterBackward(const at::Tensor &grad_in, const at::Tensor &logits_in, const at::Tensor &idx_in, std::string scoring, bool renormalize, double scale)
+{
+    NeedInit();
+    CheckLogits(logits_in);
+    SameDevice("moe_router_backward", {{"grad_probs", grad_in}, {"logits", logits_in}, {"expert_idx", idx_in}});
+    TORCH_CHECK(idx_in.dim() == 2 && idx_in.size(0) == logits_in.size(0) && idx_in.scalar_type() == at::kInt, "expert_idx must be an int32 [tokens, top_k] tensor");
+    TORCH_CHECK(grad_in.sizes() == idx_in.sizes() && grad_in.scalar_type() == at::kFloat, "grad_probs must be a float32 [tokens, top_k] tensor");
+    c10::DeviceGuard guard(logits_in.device());
+    const at::Tensor grad = grad_in.contiguous(), logits = logits_in.contiguous(), idx = idx_in.contiguous();
+    at::Tensor out = at::empty(logits.sizes(), logits.options());
+    Check(cch_moe_router_backward(grad.data_ptr<float>(), logits.data_ptr(), DtypeCode(logits), idx.data_ptr<int32_t>(), logits.size(0), logits.size(1), (int)idx.size(1),
+                                  ScoringCode(scoring), renormalize, (float)scale, out.data_ptr(), StreamOf(logits)),
+          "moe_router_backward");
+    return out;
+}
+
+int64_t Sequences(const MaybeTensor &offsets)
+{
+    if (!offsets || !offsets->defined()) return 1;
+    TORCH_CHECK(offsets->dim() == 1 && offsets->numel() >= 2, "seq_offsets must be an int32 [sequences + 1] tensor");
+    return offsets->numel() - 1;
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> MoeBalanceLoss(const at::Tensor &logits_in, const at::Tensor &idx_in, double coef, double z_coef, std::string scoring,
+                                                              const MaybeTensor &mask_in, const MaybeTensor &offsets_in)
+{
+    NeedInit();
+    CheckLogits(logits_in);
+    SameDevice("moe_balance_loss", {{"logits", logits_in}, {"expert_idx", idx_in}});
+    TORCH_CHECK(idx_in.dim() == 2 && idx_in.size(0) == logits_in.size(0) && idx_in.scalar_type() == at::kInt, "expert_idx must be an int32 [tokens, top_k] tensor");
+    c10::DeviceGuard guard(logits_in.device());
+    const at::Tensor logits = logits_in.contiguous(), idx = idx_in.contiguous();
+    const int64_t tokens = logits.size(0), e = logits.size(1), s = Sequences(offsets_in);
+    const at::Tensor mask = Optional("moe_balance_loss", "token_mask", mask_in, logits, {at::kBool, at::kByte}, tokens);
+    const at::Tensor offsets = Optional("moe_balance_loss", "seq_offsets", offsets_in, logits, {at::kInt}, s + 1);
+    at::Tensor loss = at::empty({}, logits.options().dtype(at::kFloat)), counted = at::empty({s}, logits.options().dtype(at::kInt));
+    at::Tensor counts = offsets.defined() ? at::empty({s, e}, counted.options()) : at::empty({e}, counted.options());
+    const int64_t ws_bytes = cch_moe_balance_loss_workspace_bytes(tokens, e, s);
+    at::Tensor ws = Bytes(logits, {std::max<int64_t>(ws_bytes, 4)});
+    Check(cch_moe_balance_loss(logits.data_ptr(), DtypeCode(logits), idx.data_ptr<int32_t>(), PtrOf<uint8_t>(mask), PtrOf<int32_t>(offsets), tokens, e, (int)idx.size(1), s,
+                               ScoringCode(scoring), (float)coef, (float)z_coef, loss.data_ptr<float>(), counts.data_ptr<int32_t>(), counted.data_ptr<int32_t>(), ws.data_ptr(),
+                               ws.numel(), StreamOf(logits)),
+          "moe_balance_loss");
+    return {loss, counts, counted};
+}
+
+at::Tensor MoeBalanceLossBackward(const at::Tensor &grad_in, const at::Tensor &logits_in, const at::Tensor &counts_in, const at::Tensor &counted_in, int64_t top_k, double coef,
+                                  double z_coef, std::string scoring, const MaybeTensor &mask_in, const MaybeTensor &offsets_in)
+{
+    NeedInit();
+    CheckLogits(logits_in);
+    SameDevice("moe_balance_loss_backward", {{"grad_loss", grad_in}, {"logits", logits_in}, {"counts", counts_in}, {"tokens", counted_in}});
+    c10::DeviceGuard guard(logits_in.device());
+    const at::Tensor grad = grad_in.contiguous(), logits = logits_in.contiguous(), counts = counts_in.contiguous(), counted = counted_in.contiguous();
+    const int64_t tokens = logits.size(0), e = logits.size(1), s = Sequences(offsets_in);
+    TORCH_CHECK(grad.numel() == 1 && grad.scalar_type() == at::kFloat, "grad_loss must be one float32 value");
+    TORCH_CHECK(counts.scalar_type() == at::kInt && counts.numel() == s * e && counted.scalar_type() == at::kInt && counted.numel() == s,
+                "counts must be int32 [sequences, experts] and tokens int32 [sequences]");
+    const at::Tensor mask = Optional("moe_balance_loss_backward", "token_mask", mask_in, logits, {at::kBool, at::kByte}, tokens);
+    const at::Tensor offsets = Optional("moe_balance_loss_backward", "seq_offsets", offsets_in, logits, {at::kInt}, s + 1);
+    at::Tensor out = at::empty(logits.sizes(), logits.options());
+    Check(cch_moe_balance_loss_backward(grad.data_ptr<float>(), logits.data_ptr(), DtypeCode(logits), PtrOf<uint8_t>(mask), PtrOf<int32_t>(offsets), counts.data_ptr<int32_t>(),
+                                        counted.data_ptr<int32_t>(), tokens, e, (int)top_k, s, ScoringCode(scoring), (float)coef, (float)z_coef, out.data_ptr(), StreamOf(logits)),
+          "moe_balance_loss_backward");
+    return out;
+}
+
+// Codes [.., rows, ceil(k/2)], scales and zero points of 4-bit weights, `lead` matrices of `rows` rows.
+void CheckW4(const char *name, const at::Tensor &w, const at::Tensor &scales, const at::Tensor &zeros, int64_t lead, int64_t rows, int64_t k, int fmt, int64_t group,
+             at::ScalarType type)
+{
+    const int64_t groups = fmt == CCH_FMT_INT4 ? (k + group - 1) / group : ScaleCols(k);
+    TORCH_CHECK(w.scalar_type() == at::kByte && w.numel() == lead * rows * ((k + 1) / 2) && w.size(-1) == (k + 1) / 2 && w.size(-2) == rows, name, " must be a uint8 tensor of ",
+                (k + 1) / 2, " bytes a row");
+    TORCH_CHECK(scales.scalar_type() == (fmt == CCH_FMT_INT4 ? type : at::kByte) && scales.numel() == lead * rows * groups && scales.size(-1) == groups, "scales of ", name,
+                " must have ", groups, " columns of ", fmt == CCH_FMT_INT4 ? "the activations' type" : "E8M0 bytes");
+    TORCH_CHECK(!zeros.defined() || (fmt == CCH_FMT_INT4 && zeros.scalar_type() == at::kByte && zeros.sizes() == scales.sizes()), "zeros of ", name,
+                " must be uint8 of the scales' shape, with int4 weights only");
+}
+int W4Format(const std::string &name, int64_t group)
+{
+    TORCH_CHECK(name == "int4" || name == "e2m1" || name == "fp4", "unknown 4-bit weight format '", name, "' (int4 or e2m1)");
+    TORCH_CHECK(name != "int4" || group == 32 || group == 64 || group == 128, "group_size must be 32, 64 or 128");
+    return name == "int4" ? CCH_FMT_INT4 : CCH_FMT_E2M1;
+}
+at::Tensor Zeros(const char *op, const char *name, const MaybeTensor &zeros, const at::Tensor &x)
+{
+    return Optional(op, name, zeros, x, {at::kByte}, zeros && zeros->defined() ? zeros->numel() : 0);
+}
+
+at::Tensor W4A16Matmul(const at::Tensor &x_in, const at::Tensor &w_in, const at::Tensor &scales_in, const MaybeTensor &zeros_in, std::string fmt_name, int64_t group)
+{
+    NeedInit();
+    const int fmt = W4Format(fmt_name, group);
+    TORCH_CHECK(x_in.dim() == 2 && (x_in.scalar_type() == at::kBFloat16 || x_in.scalar_type() == at::kHalf), "x must be a 2-D bfloat16 or float16 tensor");
+    TORCH_CHECK(w_in.dim() == 2 && scales_in.dim() == 2, "w and scales must be 2-D tensors");
+    SameDevice("w4a16_matmul", {{"x", x_in}, {"w", w_in}, {"scales", scales_in}});
+    c10::DeviceGuard guard(x_in.device());
+    const at::Tensor x = x_in.contiguous(), w = w_in.contiguous(), scales = scales_in.contiguous(), zeros = Zeros("w4a16_matmul", "zeros", zeros_in, x);
+    const int64_t m = x.size(0), k = x.size(1), n = w.size(0);
+    CheckW4("w", w, scales, zeros, 1, n, k, fmt, group, x.scalar_type());
+    at::Tensor out = at::empty({m, n}, x.options());
+    const int64_t ws_bytes = cch_w4a16_matmul_workspace_bytes(m, n, k);
+    at::Tensor ws = Bytes(x, {ws_bytes});
+    Check(cch_w4a16_matmul(x.data_ptr(), w.data_ptr(), scales.data_ptr(), PtrOf<void>(zeros), out.data_ptr(), m, n, k, fmt, (int)group, DtypeCode(x), ws.data_ptr(), ws_bytes,
+                           StreamOf(x)),
+          "w4a16_matmul");
+    return out;
+}
+
+at::Tensor MoeFfnW4A16(const at::Tensor &x_in, const at::Tensor &idx_in, const at::Tensor &probs_in, const at::Tensor &w1_in, const at::Tensor &s1_in, const MaybeTensor &z1_in,
+                       const at::Tensor &w2_in, const at::Tensor &s2_in, const MaybeTensor &z2_in, std::string fmt_name, int64_t group)
+{
+    NeedInit();
+    const char *op = "moe_ffn_w4a16";
+    const int fmt = W4Format(fmt_name, group);
+    TORCH_CHECK(x_in.dim() == 2 && (x_in.scalar_type() == at::kBFloat16 || x_in.scalar_type() == at::kHalf), "x must be a 2-D bfloat16 or float16 tensor");
+    TORCH_CHECK(idx_in.dim() == 2 && idx_in.size(0) == x_in.size(0) && idx_in.scalar_type() == at::kInt, "expert_idx must be an int32 [m, top_k] tensor");
+    TORCH_CHECK(probs_in.sizes() == idx_in.sizes() && probs_in.scalar_type() == at::kFloat, "probs must be a float32 [m, top_k] tensor");
+    TORCH_CHECK(w1_in.dim() == 3 && w2_in.dim() == 3 && s1_in.dim() == 3 && s2_in.dim() == 3 && w1_in.size(0) == w2_in.size(0) && w1_in.size(1) % 2 == 0,
+                "w1 and w2 must hold one matrix per expert, w1 gate and up halves");
+    SameDevice(op, {{"x", x_in}, {"expert_idx", idx_in}, {"probs", probs_in}, {"w1", w1_in}, {"scales1", s1_in}, {"w2", w2_in}, {"scales2", s2_in}});
+    c10::DeviceGuard guard(x_in.device());
+    const at::Tensor x = x_in.contiguous(), idx = idx_in.contiguous(), probs = probs_in.contiguous(), w1 = w1_in.contiguous(), s1 = s1_in.contiguous(), w2 = w2_in.contiguous(),
+                     s2 = s2_in.contiguous(), z1 = Zeros(op, "zeros1", z1_in, x), z2 = Zeros(op, "zeros2", z2_in, x);
+    const int64_t m = x.size(0), k = x.size(1), top_k = idx.size(1), e = w1.size(0), n = w1.size(1);
+    TORCH_CHECK(top_k >= 1 && top_k <= 8, "top_k must be 1..8");
+    CheckW4("w1", w1, s1, z1, e, n, k, fmt, group, x.scalar_type());
+    CheckW4("w2", w2, s2, z2, e, k, n / 2, fmt, group, x.scalar_type());
+    at::Tensor out = at::empty({m, k}, x.options());
+    const int64_t ws_bytes = cch_moe_ffn_w4a16_workspace_bytes(m, k, (int)top_k, e, n);
+    at::Tensor ws = Bytes(x, {std::max<int64_t>(ws_bytes, 1)});
+    Check(cch_moe_ffn_w4a16(x.data_ptr(), idx.data_ptr<int32_t>(), probs.data_ptr<float>(), w1.data_ptr(), s1.data_ptr(), PtrOf<void>(z1), w2.data_ptr(), s2.data_ptr(),
+                            PtrOf<void>(z2), out.data_ptr(), m, k, (int)top_k, e, n, fmt, (int)group, DtypeCode(x), ws.data_ptr(), ws.numel(), StreamOf(x)),
+          op);
+    return out;
+}
+
+// ---------------------------------------------------------------------------------------------
 // Meta kernels: output shapes only (reference torch_bindings_meta.cpp:18-30 returns at::empty_symint of the result shape)
 
 c10::SymInt SymScaleCols(const c10::SymInt &k) { return ((k + 63) / 64) * 2; }
@@ -400,6 +595,36 @@ at::Tensor MoeFfnMeta(const at::Tensor &x, const at::Tensor &, const at::Tensor 
     return MetaEmpty(x, x.sym_sizes(), x.scalar_type());
 }
 
+std::tuple<at::Tensor, at::Tensor> MoeRouterMeta(const at::Tensor &logits, int64_t top_k, std::string, bool, double, const MaybeTensor &, const MaybeTensor &)
+{
+    return {MetaEmpty(logits, {logits.sym_size(0), top_k}, at::kFloat), MetaEmpty(logits, {logits.sym_size(0), top_k}, at::kInt)};
+}
+at::Tensor MoeRouterBackwardMeta(const at::Tensor &, const at::Tensor &logits, const at::Tensor &, std::string, bool, double)
+{
+    return MetaEmpty(logits, logits.sym_sizes(), logits.scalar_type());
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor> MoeBalanceLossMeta(const at::Tensor &logits, const at::Tensor &, double, double, std::string, const MaybeTensor &,
+                                                                  const MaybeTensor &offsets)
+{
+    const bool some = offsets && offsets->defined();
+    const c10::SymInt e = logits.sym_size(1), s = some ? offsets->sym_size(0) - 1 : c10::SymInt(1);
+    return {MetaEmpty(logits, {}, at::kFloat), some ? MetaEmpty(logits, {s, e}, at::kInt) : MetaEmpty(logits, {e}, at::kInt), MetaEmpty(logits, {s}, at::kInt)};
+}
+at::Tensor MoeBalanceLossBackwardMeta(const at::Tensor &, const at::Tensor &logits, const at::Tensor &, const at::Tensor &, int64_t, double, double, std::string,
+                                      const MaybeTensor &, const MaybeTensor &)
+{
+    return MetaEmpty(logits, logits.sym_sizes(), logits.scalar_type());
+}
+at::Tensor W4A16Meta(const at::Tensor &x, const at::Tensor &w, const at::Tensor &, const MaybeTensor &, std::string, int64_t)
+{
+    return MetaEmpty(x, {x.sym_size(0), w.sym_size(0)}, x.scalar_type());
+}
+at::Tensor MoeFfnW4A16Meta(const at::Tensor &x, const at::Tensor &, const at::Tensor &, const at::Tensor &, const at::Tensor &, const MaybeTensor &, const at::Tensor &,
+                           const at::Tensor &, const MaybeTensor &, std::string, int64_t)
+{
+    return MetaEmpty(x, x.sym_sizes(), x.scalar_type());
+}
+
 }  // namespace
 
 TORCH_LIBRARY(catccos, m)
@@ -414,6 +639,14 @@ TORCH_LIBRARY(catccos, m)
     m.def("mx_grouped_matmul_swiglu_mx(Tensor a, Tensor sa, Tensor b, Tensor sb, Tensor group_sizes, str fmt, int trans_b, str out_fmt) -> (Tensor, Tensor)");
     m.def("gmm_dequant_swiglu_mx(Tensor x, Tensor w, Tensor group_sizes, Tensor per_tok, Tensor per_ch, int trans_b, str fmt) -> (Tensor, Tensor)");
     m.def("moe_ffn_mxfp8(Tensor x, Tensor expert_idx, Tensor probs, Tensor w1, Tensor sw1, Tensor w2, Tensor sw2, int trans_b) -> Tensor");
+    m.def("moe_router(Tensor logits, int top_k, str scoring, bool renormalize, float scale, Tensor? bias, Tensor? token_mask) -> (Tensor, Tensor)");
+    m.def("moe_router_backward(Tensor grad_probs, Tensor logits, Tensor expert_idx, str scoring, bool renormalize, float scale) -> Tensor");
+    m.def("moe_balance_loss(Tensor logits, Tensor expert_idx, float coef, float z_coef, str scoring, Tensor? token_mask, Tensor? seq_offsets) -> (Tensor, Tensor, Tensor)");
+    m.def("moe_balance_loss_backward(Tensor grad_loss, Tensor logits, Tensor counts, Tensor tokens, int top_k, float coef, float z_coef, str scoring, Tensor? token_mask, "
+          "Tensor? seq_offsets) -> Tensor");
+    m.def("w4a16_matmul(Tensor x, Tensor w, Tensor scales, Tensor? zeros, str fmt, int group_size) -> Tensor");
+    m.def("moe_ffn_w4a16(Tensor x, Tensor expert_idx, Tensor probs, Tensor w1, Tensor scales1, Tensor? zeros1, Tensor w2, Tensor scales2, Tensor? zeros2, str fmt, "
+          "int group_size) -> Tensor");
 }
 
 // init / finalize take no tensors: one kernel for every backend, as in the reference (torch_bindings.cpp:233-238)
@@ -434,6 +667,12 @@ TORCH_LIBRARY_IMPL(catccos, CUDA, m)
     m.impl("mx_grouped_matmul_swiglu_mx", &MxGroupedMatmulSwigluMx);
     m.impl("gmm_dequant_swiglu_mx", &GmmDequantSwigluMx);
     m.impl("moe_ffn_mxfp8", &MoeFfnMxfp8);
+    m.impl("moe_router", &MoeRouter);
+    m.impl("moe_router_backward", &MoeRouterBackward);
+    m.impl("moe_balance_loss", &MoeBalanceLoss);
+    m.impl("moe_balance_loss_backward", &MoeBalanceLossBackward);
+    m.impl("w4a16_matmul", &W4A16Matmul);
+    m.impl("moe_ffn_w4a16", &MoeFfnW4A16);
 }
 
 TORCH_LIBRARY_IMPL(catccos, Meta, m)
@@ -446,4 +685,10 @@ TORCH_LIBRARY_IMPL(catccos, Meta, m)
     m.impl("mx_grouped_matmul_swiglu_mx", &MxGmmSwigluMxMeta);
     m.impl("gmm_dequant_swiglu_mx", &GmmSwigluMxMeta);
     m.impl("moe_ffn_mxfp8", &MoeFfnMeta);
+    m.impl("moe_router", &MoeRouterMeta);
+    m.impl("moe_router_backward", &MoeRouterBackwardMeta);
+    m.impl("moe_balance_loss", &MoeBalanceLossMeta);
+    m.impl("moe_balance_loss_backward", &MoeBalanceLossBackwardMeta);
+    m.impl("w4a16_matmul", &W4A16Meta);
+    m.impl("moe_ffn_w4a16", &MoeFfnW4A16Meta);
 }
