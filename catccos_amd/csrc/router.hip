@@ -16,8 +16,9 @@
 // less than sorting anything, and ties need no extra step.
 //
 // Bound: on paper the bytes (16384 tokens of 64 experts in bf16, 8 routes: 3.1 MB forward, 5.2 MB backward, 1.6 us for both at the rate of a large copy), in fact the
-// launch (an empty one 2.4 us) and the selection's instructions, some 2 V + 20 to a route: that case takes 4.8 + 4.5 us, 4099 tokens of 256 experts (fp32, sigmoid) 5.2 +
-// 5.3, 64 tokens of 16 experts 2.3; 16384 x 1024 28.7 + 23.6 (1.2 and 2.8 TB/s).
+// launch (an empty one 2.4 us) and the selection's instructions, some 2 V + 20 to a route: that case takes 4.8 + 3.9 us, 4099 tokens of 256 experts (fp32, sigmoid) 5.4 +
+// 3.7, 64 tokens of 16 experts 2.2; 16384 x 1024 in bf16 28.0 + 16.7 (1.2 and 4.0 TB/s).  Backward, the selected experts' terms reach the lanes that hold them through LDS: one
+// write for all routes, where comparing every expert with every route is 2 V instructions a route (16384 x 1024 23.6 us, x 256 9.1 against 6.5, x 64 4.3 against 3.8).
 #include <algorithm>
 
 #include "router_lanes.h"
@@ -80,29 +81,24 @@ __global__ __launch_bounds__(ROUTER_THREADS) void moe_router_kernel(const T *__r
 #pragma unroll
         for (int i = 1; i < V; i++) best = fmaxf(best, key[i]);
         const float all = lanes_max<L>(best);
-        int which = 0;
-        float its_l = l[0];
-#pragma unroll
-        for (int i = V - 1; i >= 0; i--)
-            if (key[i] == all) {
-                which = i;
-                its_l = l[i];
-            }
         const uint64_t holders = (__ballot(best == all) >> base) & (L == 64 ? ~0ull : (1ull << (L & 63)) - 1);
         const int owner = __ffsll((unsigned long long)holders) - 1;   // (at least one lane holds the maximum)
         const bool found = all > -INFINITY;
-        const int idx = __shfl(at * V + which, base + owner, 64);
-        const float sel = bias ? __shfl(its_l, base + owner, 64) : all;
-        if (at == j && found) {
-            mine_idx = idx;
-            mine_l = sel;
-        }
+        int which = 0;
+#pragma unroll
+        for (int i = V - 1; i >= 0; i--) which = key[i] == all ? i : which;
         const int taken = found && at == owner ? which : V;
 #pragma unroll
         for (int i = 0; i < V; i++)
             if (i == taken) key[i] = -INFINITY;
+        const int idx = __shfl(at * V + which, base + owner, 64);
+        if (at == j && found) {
+            mine_idx = idx;
+            mine_l = all;
+        }
     }
     const bool there = mine_idx >= 0;
+    if (bias && there) mine_l = to_f32(logits[t * experts + mine_idx]);   // (keys were scores)
     if (RENORM) top = lanes_max<L>(mine_l);
     const float w = route_weight<L, SIGMOID, RENORM>(mine_l, there, top, denominator, scale);
     if (inside && at < top_k) {
@@ -116,7 +112,7 @@ __global__ __launch_bounds__(ROUTER_THREADS) void moe_router_backward_kernel(con
                                                                             const int32_t *__restrict__ expert_idx, T *__restrict__ grad_logits, int tokens, int experts,
                                                                             int top_k, float scale, bool vec)
 {
-    const int lane = threadIdx.x & 63, at = lane & (L - 1), base = lane & ~(L - 1);
+    const int lane = threadIdx.x & 63, at = lane & (L - 1);
     const int64_t t = ((int64_t)blockIdx.x * ROUTER_THREADS + threadIdx.x) / L;
     const bool inside = t < tokens;
     const T *row = logits + (inside ? t : 0) * experts;
@@ -155,13 +151,19 @@ __global__ __launch_bounds__(ROUTER_THREADS) void moe_router_backward_kernel(con
     own = there ? own * scale : 0.0f;
 #pragma unroll
     for (int i = 0; i < V; i++) d[i] = !SIGMOID && !RENORM && dot != 0.0f ? -scale * dot * (d[i] / denominator) : 0.0f;
-    for (int j = 0; j < top_k; j++) {
-        const int e = __shfl(idx, base + j, 64) - at * V;
-        const float x = __shfl(own, base + j, 64);
+    // the selected experts' own terms, by way of the token's row in LDS; its lanes are of one wave, whose LDS accesses are in order
+    // (pieces of four experts, all lanes' first ones first: neighbouring lanes on neighbouring banks)
+    constexpr int PIECE = V < 4 ? V : 4;
+    typedef float Piece __attribute__((ext_vector_type(PIECE)));
+    __shared__ Piece rows[ROUTER_THREADS / L][V / PIECE][L];
+    Piece (*const mine)[L] = rows[threadIdx.x / L];
 #pragma unroll
-        for (int i = 0; i < V; i++)
-            if (e == i) d[i] += x;
-    }
+    for (int c = 0; c < V / PIECE; c++) mine[c][at] = 0.0f;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (there) atomicAdd(reinterpret_cast<float *>(&mine[idx % V / PIECE][idx / V]) + idx % PIECE, own);   // (an expert that a caller names twice gets both)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int i = 0; i < V; i++) d[i] += mine[i / PIECE][at][i % PIECE];
     if (inside) store_row<T, V>(grad_logits + t * experts, at * V, experts, vec, d);
 }
 

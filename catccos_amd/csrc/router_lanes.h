@@ -4,18 +4,18 @@
 // exponential is zero.  A lane's own work grows with V, the steps between lanes, and the lanes that repeat what is done once per token, with L; up to L = 16 such a
 // step is a DPP move.  Measured in us (router forward / backward, balance loss forward / backward, bf16, softmax over the experts, 8 routes):
 //                   16384 tokens                                       64 tokens
-//   64 experts      V 8, L 8    4.6 /  4.3   10.5 /  4.0                3.5 / 3.4    5.3 / 3.5
-//                   V 4, L 16   5.6 /  4.4   10.5 /  4.2                3.3 / 3.1    4.3 / 3.3
-//   128             V 8, L 16   6.7 /  5.9   14.1 /  4.9                3.6 / 3.5    4.9 / 3.5
-//                   V 4, L 32   9.0 /  6.4   15.0 /  5.9                3.8 / 3.1    4.7 / 3.5
-//                   V 16, L 8   6.0 /  6.0   14.8 /  5.2                4.3 / 4.4    6.7 / 3.9
-//   256             V 16, L 16  9.3 /  9.1   15.7 /  6.9                4.3 / 4.6    6.1 / 4.0
-//                   V 8, L 32  11.4 /  9.0   16.1 /  7.3                4.0 / 3.6    5.2 / 3.6
-//                   V 32, L 8   9.0 / 10.2   17.4 /  8.8                5.7 / 6.7   10.1 / 5.4
-//   512             V 16, L 32 16.3 / 15.0   17.8 / 10.5                4.9 / 4.6    6.6 / 4.1
-//                   V 8, L 64  19.3 / 14.9   19.1 / 10.6                4.5 / 3.9    9.7 / 3.7
-//   1024            V 16, L 64 28.7 / 23.6   22.9 / 15.7                5.4 / 4.9   10.8 / 4.1
-//                   V 32, L 32 26.4 / 25.1   23.4 / 23.3                6.4 / 6.9   12.0 / 5.5
+//   64 experts      V 8, L 8    4.6 /  3.8   10.2 /  4.0                3.5 / 3.0    5.1 / 3.4
+//                   V 4, L 16   5.5 /  3.8   10.1 /  4.2                3.3 / 2.6    4.2 / 3.3
+//   128             V 8, L 16   6.7 /  4.5   14.1 /  5.0                3.6 / 2.9    4.8 / 3.5
+//                   V 4, L 32   8.9 /  4.8   14.9 /  5.9                3.8 / 2.7    4.7 / 3.4
+//                   V 16, L 8   6.1 /  4.8   14.6 /  5.2                4.4 / 3.5    6.8 / 3.9
+//   256             V 16, L 16  9.3 /  6.5   15.4 /  7.0                4.4 / 3.4    6.2 / 3.9
+//                   V 8, L 32  11.2 /  6.5   15.8 /  7.5                4.1 / 3.0    5.3 / 3.7
+//                   V 32, L 8   9.3 /  8.0   17.1 /  8.9                6.5 / 4.9   10.0 / 5.4
+//   512             V 16, L 32 16.0 / 10.9   17.7 / 10.5                5.1 / 3.5    6.8 / 4.1
+//                   V 8, L 64  19.0 / 10.9   18.9 / 10.8                4.4 / 3.1   10.6 / 3.8
+//   1024            V 16, L 64 28.0 / 16.7   22.8 / 16.0                5.4 / 3.6   11.8 / 4.1
+//                   V 32, L 32 25.7 / 20.5   23.1 / 19.2                7.1 / 4.9   12.3 / 5.5
 // The first of each is taken: the best or near it where there is work, within a microsecond of the best where launches count.
 #pragma once
 #include <cmath>
@@ -62,8 +62,8 @@ __device__ __forceinline__ float to_f32(__bf16 x) { return (float)x; }
 __device__ __forceinline__ float to_f32(_Float16 x) { return (float)x; }
 
 // This lane's V logits of a row, `experts` long, as they come from memory, so that a row can be on its way while another is worked on.  VEC: rows start and end
-// on boundaries of a lane's loads of up to 16 bytes (router forward / backward, balance forward / backward: 16384 x 64 in bf16 4.5 / 4.1, 10.3 / 4.0 us; one element
-// at a time 5.3 / 5.4, 11.4 / 6.0; 4096 x 256 4.6 / 5.2, 11.9 / 4.5 against 6.2 / 8.5, 15.1 / 10.4).
+// on boundaries of a lane's loads of up to 16 bytes (router forward / backward, balance forward / backward: 16384 x 64 in bf16 4.6 / 3.8, 10.1 / 4.0 us; one element
+// at a time 5.2 / 4.7, 11.1 / 6.0; 4096 x 256 4.7 / 3.9, 11.8 / 4.4 against 6.2 / 7.4, 15.0 / 10.3).
 template <class T, int V>
 struct LanePieces {
     static constexpr int CHUNK = V * (int)sizeof(T) < 16 ? V : 16 / (int)sizeof(T);   // elements of one access
