@@ -575,19 +575,20 @@ int w4_tile_choose(int out_kind, const W4Rows &rows, const W4Matrix &w, void *ou
 #define W4_GO(OUT, GROUPED, ...) w4_tile_launch<T, KIND, ZEROS, W4Shape<__VA_ARGS__>, OUT, GROUPED>(rows, w, out, s)
     if (out_kind == W4_OUT_PLAIN) {
         constexpr bool G = false;
-        const int64_t m = rows.rows, n = w.rows, m32 = (m + 31) / 32;
-        if (m <= 4) return n <= 8192 ? W4_GO(W4_OUT_PLAIN, G, 1, 1, 1, 1, 8) : W4_GO(W4_OUT_PLAIN, G, 2, 1, 1, 1, 4);
-        if (m <= 8 && n <= 8192) return W4_GO(W4_OUT_PLAIN, G, 1, 1, 2, 1, 8);
+        constexpr int64_t CUS = 256;
+        const int64_t m = rows.rows, m32 = (m + 31) / 32, tiles = (w.rows + 15) / 16;
+        if (m <= 4) return tiles <= 2 * CUS ? W4_GO(W4_OUT_PLAIN, G, 1, 1, 1, 1, 8) : W4_GO(W4_OUT_PLAIN, G, 2, 1, 1, 1, 4);
+        if (m <= 8 && tiles <= 2 * CUS) return W4_GO(W4_OUT_PLAIN, G, 1, 1, 2, 1, 8);
         if (m <= 16) {
-            if (n <= 4096) return W4_GO(W4_OUT_PLAIN, G, 1, 1, 4, 1, 8);
-            if (n <= 8192) return W4_GO(W4_OUT_PLAIN, G, 2, 1, 4, 1, 8);
-            if (n <= 16384) return W4_GO(W4_OUT_PLAIN, G, 1, 1, 4, 2, 4);
-            if (n <= 32768) return W4_GO(W4_OUT_PLAIN, G, 1, 1, 4, 4, 2);
+            if (tiles <= CUS) return W4_GO(W4_OUT_PLAIN, G, 1, 1, 4, 1, 8);
+            if (tiles <= 2 * CUS) return W4_GO(W4_OUT_PLAIN, G, 2, 1, 4, 1, 8);
+            if (tiles <= 4 * CUS) return W4_GO(W4_OUT_PLAIN, G, 1, 1, 4, 2, 4);
+            if (tiles <= 8 * CUS) return W4_GO(W4_OUT_PLAIN, G, 1, 1, 4, 4, 2);
             return W4_GO(W4_OUT_PLAIN, G, 2, 1, 4, 4, 2);
         }
-        if (m32 * ((n + 31) / 32) <= 256) return W4_GO(W4_OUT_PLAIN, G, 1, 2, 8, 2, 4);
-        if (m32 * ((n + 63) / 64) <= 256) return W4_GO(W4_OUT_PLAIN, G, 1, 2, 8, 4, 4);
-        if (m32 == 1 || m32 * ((n + 127) / 128) <= 256) return W4_GO(W4_OUT_PLAIN, G, 2, 2, 8, 4, 4);
+        if (m32 * ((tiles + 1) / 2) <= CUS) return W4_GO(W4_OUT_PLAIN, G, 1, 2, 8, 2, 4);
+        if (m32 * ((tiles + 3) / 4) <= CUS) return W4_GO(W4_OUT_PLAIN, G, 1, 2, 8, 4, 4);
+        if (m32 == 1 || m32 * ((tiles + 7) / 8) <= CUS) return W4_GO(W4_OUT_PLAIN, G, 2, 2, 8, 4, 4);
         return W4_GO(W4_OUT_PLAIN, G, 1, 4, 16, 8, 2);
     }
     constexpr bool G = true;
