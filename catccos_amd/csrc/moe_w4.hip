@@ -4,7 +4,7 @@
 // over a token's routes in their order, so that the same inputs give the same bits.
 //
 // Bound by the weights of the experts that some route names, once each: one token, 6 of 16 experts, k = 7168, n = 4096 (132 MB) 19.5 + 13.5 + 3.9 us in its three launches, 4.0 TB/s;
-// 64 tokens (353 MB) 73 + 46 + 5.3 us.  Down projection and sum in one launch, a workgroup having its columns of all routes, measured about the same for one token (14.4 us for 13.2 +
+// 64 tokens (353 MB) 70 + 46 + 4.8 us.  Down projection and sum in one launch, a workgroup having its columns of all routes, measured about the same for one token (14.4 us for 13.2 +
 // 4.7) and far worse for twelve (26 for 11.8 + 4.7, the experts one after another): not kept.
 #include <algorithm>
 

@@ -16,8 +16,8 @@
 // The sums and the groups' scales stay in fp32; rounded to 16 bits are the results alone.  Zero points that -(16 + z) holds exactly, up to 240 in bf16.
 //
 // Bound, one row: the weights' bytes, after a launch, two waits for memory and the sum over K's parts: 4096 x 7168 in 5.9 us, 2.5 TB/s (reading alone 3.6, an empty launch
-// 2.4), 32768 x 7168 in 26 us, 4.6 TB/s.  64 rows x 32768 x 7168: 69 us, 1.7 TB/s and 0.44 PFLOP/s.  A tile of weights and 64 rows of x take, per block of K, 131
-// vector instructions of 4 clocks (conversion 60, scales 32, moving x 16) and 32 matrix instructions of 16, in a SIMD's time nearly one after the other: 16 waves overlap
+// 2.4), 32768 x 7168 in 26 us, 4.6 TB/s.  64 rows x 32768 x 7168: 69 us, 1.7 TB/s and 0.44 PFLOP/s.  A tile of weights and 64 rows of x take, per block of K, about 100
+// vector instructions of 4 clocks (conversion 34, scales 32, x and addresses the rest), 32 matrix instructions of 16 and 18 KB from LDS, in a SIMD's time little overlapped: 16 waves overlap
 // them better than 8 (77 us), whatever order the compiler is asked for.
 #pragma once
 #include <algorithm>
@@ -559,16 +559,17 @@ int w4_tile_launch(const W4Rows &rows, const W4Matrix &w, void *out, hipStream_t
 //              64 rows, 8 of 1, in 2 44.2 / 30.4    45.2 / 30.8    45.4 / 31.9 * 58.2 / 43.1
 //              64 rows, 4 of 2, in 2 49.5 / 35.6    49.5 / 36.4    49.7 / 37.3   60.3 / 47.0          (two waves to a SIMD, four above)
 //
-//   grouped, 16 experts, K = 7168, n = 4096, 6 routes a token; 64 experts, K = 2048, n = 1024, 8 routes; by the routes of an expert:
-//   up projection     1 token              8 (64 tokens, 64 experts)   12 (32, 16)        16 (128, 64)      24 (64, 16)       32 (256, 64)
-//     4 rows        * 19.2 / 20.0             45.2 / 39.1             152  / 143          67.5 / 61.1       260 / 256         126 / 112
-//     16              30.1 / 29.7           * 18.1 / 17.0              73.0 / 74.5        29.9 / 27.5       110 / 110          44.1 / 41.7
-//     32              46.6 / 44.3             23.4 / 19.9           *  68.7 / 61.8      * 24.3 / 21.1       106 /  98          43.0 / 36.3
-//     64              65.1 / 51.8             32.9 / 24.3             101  /  73.4        33.9 / 25.7     * 101 /  77        * 35.6 / 27.5
-//   down projection
-//     4 rows        * 13.8 / 12.9             35.5 / 33.7              81.5 / 71.9        55.0 / 52.2       142 / 128         106 / 101
-//     16              16.0 / 15.5           * 14.6 / 13.2              40.8 / 41.5        23.1 / 20.6        62 /  61          32.0 / 30.6
-//     32              19.4 / 15.5             18.1 / 16.4           *  44.3 / 38.7      * 19.3 / 17.7     *  52 /  46        * 32.0 / 27.1
+//   grouped, 16 experts, K = 7168, n = 4096, 6 routes a token; 64 experts, K = 2048, n = 1024, 8 routes; by an expert's routes, on average (tokens, experts):
+//                  1 token         8 (64, 64)      12 (32, 16)     16 (128, 64)    24 (64, 16)     32 (256, 64)    36 (96, 16)
+//   up, 4 rows   * 19.2 / 20.0     45.2 / 39.1     152 / 143       67.5 / 61.1     260 / 256       126 / 112
+//       16         30.1 / 29.7   * 18.1 / 17.0     73.0 / 74.5     29.9 / 27.5     110 / 110       44.1 / 41.7
+//       32         46.6 / 44.3     23.4 / 19.9   * 68.7 / 61.8   * 24.9 / 21.0     110 / 102       44.3 / 36.6     129 / 113
+//       48                         28.4 / 22.3     88.8 / 67.2     29.3 / 24.0   *  90 /  70     * 32.1 / 25.8   *  93 /  74
+//       64         65.1 / 51.8     33.1 / 24.6     101 / 73.4      34.4 / 25.6     101 /  76       36.3 / 28.1     106 /  77      (48 routes: * 115 / 78, 48 rows 157 / 121)
+//   down, 4 rows * 13.8 / 12.9     35.5 / 33.7     81.5 / 71.9     55.0 / 52.2     142 / 128       106 / 101
+//       16         16.0 / 15.5   * 14.6 / 13.2     40.8 / 41.5     23.1 / 20.6      62 /  61       32.0 / 30.6
+//       32         19.4 / 15.5     17.9 / 16.2   * 44.3 / 38.7   * 19.1 / 17.7   *  53 /  47     * 32.0 / 26.9      81 /  66
+//       48                         25.3 / 20.6     56.1 / 47.5     26.7 / 23.1      59 /  51       31.7 / 26.9   *  63 /  53      (96 routes: * 143 / 114, 32 rows 142 / 117)
 template <class T, int KIND, bool ZEROS>
 int w4_tile_choose(int out_kind, const W4Rows &rows, const W4Matrix &w, void *out, hipStream_t s)
 {
@@ -597,11 +598,13 @@ int w4_tile_choose(int out_kind, const W4Rows &rows, const W4Matrix &w, void *ou
         if (tokens <= 4) return W4_GO(W4_OUT_SWIGLU, G, 2, 1, 1, 1, 4);
         if (tokens <= 16 || rows.rows <= 8 * rows.num_experts) return W4_GO(W4_OUT_SWIGLU, G, 2, 1, 4, 4, 2);
         if (tokens <= 32 || rows.rows <= 16 * rows.num_experts) return W4_GO(W4_OUT_SWIGLU, G, 2, 2, 8, 4, 1);
+        if (tokens <= 48 || rows.rows <= 36 * rows.num_experts) return W4_GO(W4_OUT_SWIGLU, G, 2, 3, 12, 4, 1);
         return W4_GO(W4_OUT_SWIGLU, G, 2, 4, 16, 4, 1);
     }
     if (tokens <= 4) return W4_GO(W4_OUT_F32, G, 2, 1, 1, 1, 4);
     if (tokens <= 16 || rows.rows <= 8 * rows.num_experts) return W4_GO(W4_OUT_F32, G, 2, 1, 4, 4, 1);
-    return W4_GO(W4_OUT_F32, G, 1, 2, 8, 8, 1);
+    if (tokens <= 32 || rows.rows <= 32 * rows.num_experts) return W4_GO(W4_OUT_F32, G, 1, 2, 8, 8, 1);
+    return W4_GO(W4_OUT_F32, G, 2, 3, 12, 4, 1);
 #undef W4_GO
 }
 
