@@ -4,7 +4,7 @@
 // the load (it only selects); weights w_j = scale s_j, or scale s_j / sum of the selected s ("renormalised").  Scores grow with the logits, so
 // without a bias the logits themselves are compared: what is selected then depends on no rounding.  Equal keys go to the lower index.  An expert
 // whose logit is -inf or NaN is not there; where fewer than top_k are, or the token is masked, the remaining routes are -1 with weight 0, which
-// the routing sort drops.
+// the routing sort drops.  With a bias softmax scores are compared over the candidates alone, and logits of +inf share the whole of them.
 //
 // Backward, g the weights' gradient, p = softmax(l):
 //   softmax                  dl_e = p_e (scale g_e [e selected] - sum_j g_j w_j)
@@ -40,6 +40,10 @@ __device__ __forceinline__ float route_weight(float l, bool there, float top, fl
     return there ? scale * (s / sum) : 0.0f;
 }
 
+// e^(key - top) for the scores that a bias is added to: of a logit that is no candidate (key -inf) nothing, of one of +inf (as top is then) 1, the limit.  A weight's
+// denominator takes every logit as it is, so that what is not finite shows there; here it would take all of the token's candidates away.
+__device__ __forceinline__ float candidate_share(float key, float top) { return key == top ? 1.0f : key > -INFINITY ? exp_of(key - top) : 0.0f; }
+
 template <class T, int V, int L, bool SIGMOID, bool RENORM>
 __global__ __launch_bounds__(ROUTER_THREADS) void moe_router_kernel(const T *__restrict__ logits, const float *__restrict__ bias, const uint8_t *__restrict__ token_mask,
                                                                    float *__restrict__ probs, int32_t *__restrict__ expert_idx, int tokens, int experts, int top_k,
@@ -58,7 +62,7 @@ __global__ __launch_bounds__(ROUTER_THREADS) void moe_router_kernel(const T *__r
         top = fmaxf(top, key[i]);
     }
     float denominator = 1.0f;
-    if ((!SIGMOID && !RENORM) || (!SIGMOID && bias)) {
+    if (!SIGMOID && !RENORM) {
         top = lanes_max<L>(top);
         float sum = 0.0f;
 #pragma unroll
@@ -66,11 +70,19 @@ __global__ __launch_bounds__(ROUTER_THREADS) void moe_router_kernel(const T *__r
         denominator = lanes_sum<L>(sum);
     }
     if (bias) {
+        float of_candidates = 1.0f;
+        if (!SIGMOID) {
+            if (RENORM) top = lanes_max<L>(top);
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < V; i++) sum += candidate_share(key[i], top);
+            of_candidates = lanes_sum<L>(sum);
+        }
 #pragma unroll
         for (int i = 0; i < V; i++) {
             const int e = at * V + i;
             if (e >= experts || key[i] == -INFINITY) continue;
-            key[i] = (SIGMOID ? sigmoid(l[i]) : exp_of(l[i] - top) / denominator) + bias[e];
+            key[i] = (SIGMOID ? sigmoid(l[i]) : candidate_share(key[i], top) / of_candidates) + bias[e];
             if (!(key[i] == key[i])) key[i] = -INFINITY;
         }
     }

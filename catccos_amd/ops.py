@@ -569,7 +569,8 @@ def moe_router(logits, top_k, scoring="softmax", renormalize=True, scale=1.0, bi
     top_k largest are taken, by score + bias[e] where a bias (float32 [E]) steers the load, ties to the lower index.  Returns (probs float32
     [tokens, top_k], expert_idx int32 [tokens, top_k]): probs = scale * score, with renormalize divided by the token's sum of selected
     scores.  A logit of -inf or NaN is no candidate, a token whose token_mask is False has none: entries without an expert are -1
-    with weight 0, which the routing sort drops.  Differentiable in the logits."""
+    with weight 0, which the routing sort drops.  What is not finite shows in the weights that it is a part of (all of the token's, or with
+    renormalize the selected ones), never in the others' selection.  Differentiable in the logits."""
     r = _direct.moe_router(logits, top_k, scoring, renormalize, scale, bias, token_mask)
     if r is not NotImplemented:
         return r

@@ -354,7 +354,8 @@ int cch_dyn_quant_i8_rows_smooth(const void *x, const int32_t *src_rows, const f
  * What the reference's examples take from files (examples/utils/gen_data_moe.py:48-57 draws them at random).
  *   logits       [tokens, num_experts] of type `dtype`; tokens up to 2^30, num_experts 1..1024, top_k 1..min(8, num_experts)
  *   scoring      scores s = softmax over the experts, or sigmoid of each logit (fp32)
- *   bias         fp32 [num_experts] or NULL: added to the scores for the selection only
+ *   bias         fp32 [num_experts] or NULL: added to the scores for the selection only (softmax scores of the candidates alone, where logits of +inf share
+ *                the whole; an expert whose bias is -inf or NaN is not selected)
  *   token_mask   bytes [tokens] or NULL: a token whose byte is 0 gets no expert
  *   expert_idx   int32 [tokens, top_k], by falling score (+ bias), ties by rising index.  A logit of -inf or NaN is no candidate;
  *                where fewer than top_k are, the remaining entries are -1 (which cch_moe_init_routing drops)
