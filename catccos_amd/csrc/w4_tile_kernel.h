@@ -284,7 +284,7 @@ __device__ __forceinline__ void w4_sums(const W4Matrix &w, const W4Job &job, con
         w4_u32x4 q[NT], x[MT][4];
         uint32_t p[NT][Tile::IN_WEIGHT ? 1 : Tile::GROUPS];
     };
-    auto read = [&](Operands &o, int slot, int first, int count) {     // first: group of the block in the scales there are
+    auto read = [&](Operands &o, int slot, int first, int own) {       // first: group of the block in the scales there are; own: end of this part's
         const uint8_t *const c = code_ring + slot * NT * W4_CODES, *const xb = x_ring + slot * S::XR * W4_X4;
 #pragma unroll
         for (int j = 0; j < NT; j++) {
@@ -294,13 +294,14 @@ __device__ __forceinline__ void w4_sums(const W4Matrix &w, const W4Job &job, con
             } else {
                 o.q[j] = *reinterpret_cast<const w4_u32x4 *>(c + j * W4_CODES + code_from);
             }
-            // of groups behind K's last one there is no scale: none is needed, but it must be a number
+            // Behind the part's last group, where codes and x read as zeros, lie another part's scale, or the byte that pads MXFP4's rows to pairs: whatever it is (NaN or an
+            // infinity times zero is NaN), none is taken.
             const int row = (j / COLS) * (16 * S::WN * COLS) + 16 * (tile0 + j % COLS) + n;
             if constexpr (Tile::IN_WEIGHT) {
-                o.p[j][0] = first + g < count ? Tile::get_param(params + row * pitch + (first + g) * Tile::PARAM) : 0;
+                o.p[j][0] = first + g < own ? Tile::get_param(params + row * pitch + (first + g) * Tile::PARAM) : 0;
             } else {
 #pragma unroll
-                for (int i = 0; i < Tile::GROUPS; i++) o.p[j][i] = first + i < count ? Tile::get_param(params + row * pitch + (first + i) * Tile::PARAM) : 0;
+                for (int i = 0; i < Tile::GROUPS; i++) o.p[j][i] = first + i < own ? Tile::get_param(params + row * pitch + (first + i) * Tile::PARAM) : 0;
             }
         }
 #pragma unroll
@@ -355,8 +356,8 @@ __device__ __forceinline__ void w4_sums(const W4Matrix &w, const W4Job &job, con
         CCH_WAIT_LGKM0();
         CCH_BARRIER();
         Operands a, b;
-        const int group0 = (begin - b0) * Tile::GROUPS;
-        read(a, 0, group0, count);
+        const int group0 = (begin - b0) * Tile::GROUPS, own = min(end * Tile::GROUPS, (w.k + Tile::GROUP - 1) / Tile::GROUP) - g0;
+        read(a, 0, group0, own);
         // ring slot `SLOT` holds block `step`, whose operands are read or on their way; the other one the next
         auto advance = [&](auto which, Operands &o, int step) {
             constexpr int SLOT = decltype(which)::value;
@@ -366,7 +367,7 @@ __device__ __forceinline__ void w4_sums(const W4Matrix &w, const W4Job &job, con
             CCH_WAIT_LGKM0();          // (and this wave has the operands of block `step`)
             if (S::WN > 1) CCH_BARRIER();
             request(begin + step + 2, end, SLOT);
-            read(o, 1 - SLOT, group0 + (step + 1) * Tile::GROUPS, count);
+            read(o, 1 - SLOT, group0 + (step + 1) * Tile::GROUPS, own);
         };
         for (int step = 0; step < steps; step += 2) {
             advance(IC<0>{}, b, step);

@@ -396,7 +396,8 @@ int cch_moe_balance_loss_backward(const float *grad_loss, const void *logits, in
  *   x        [m, k] of type dtype (CCH_DTYPE_BF16 or CCH_DTYPE_F16), out [m, n] in the same type; sums in fp32
  *   w        [n, ceil(k/2)] bytes, element 2j in the low nibble
  *   scales   CCH_FMT_INT4: [n, ceil(k/group_size)] of x's type, group_size 32, 64 or 128;
- *            CCH_FMT_E2M1: E8M0 [n, 2*ceil(k/64)], groups of 32 (what cch_mx_quant_rows writes for rows of weights)
+ *            CCH_FMT_E2M1: E8M0 [n, 2*ceil(k/64)], groups of 32 (what cch_mx_quant_rows writes for rows of weights); where ceil(k/32) is odd a row's last
+ *            byte is padding, which may hold anything
  *   zeros    CCH_FMT_INT4: bytes of scales' shape or NULL (8 everywhere): an element stands for (code - zero) * scale
  *   workspace  device memory on a 16-byte boundary of at least cch_w4a16_matmul_workspace_bytes(...) bytes (none for 0); nothing in it has to be
  *            kept or cleared between calls, calls that overlap need one each
