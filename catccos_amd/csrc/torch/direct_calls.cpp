@@ -334,10 +334,11 @@ bool W4Format(PyObject *o, int &v)
     return ints || PyUnicode_CompareWithASCIIString(o, "e2m1") == 0;
 }
 int DtypeCode(at::ScalarType t) { return t == at::kHalf ? CCH_DTYPE_F16 : t == at::kBFloat16 ? CCH_DTYPE_BF16 : CCH_DTYPE_F32; }
-// forward: and the call has no gradient to record, which is the general path's.
+// The call has a gradient to record, or a tangent, which are the general path's.
+bool Differentiated(const at::Tensor &t) { return (c10::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined(); }
 bool Logits(PyObject *o, bool forward)
 {
-    return (Plain(o, at::kFloat, 2) || Plain(o, at::kBFloat16, 2) || Plain(o, at::kHalf, 2)) && !(forward && c10::GradMode::is_enabled() && T(o).requires_grad());
+    return (Plain(o, at::kFloat, 2) || Plain(o, at::kBFloat16, 2) || Plain(o, at::kHalf, 2)) && !(forward && Differentiated(T(o)));
 }
 bool Mask(PyObject *o, int64_t tokens, const uint8_t *&p)
 {

@@ -11,6 +11,7 @@ import importlib as _importlib
 import warnings as _warnings
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _abi
 from ._abi import (DTYPE_BF16, DTYPE_F16, DTYPE_F32, FMT_E1M2, FMT_E2M1, FMT_E4M3, FMT_E5M2, FMT_INT4, ROUND_LUT, ROUND_RNE, SCORING_SIGMOID,
@@ -562,6 +563,11 @@ def _recorded(t):
     return torch.is_grad_enabled() and t.requires_grad
 
 
+def _no_tangent(name, *tensors):
+    if any(_forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("%s has no forward-mode derivative" % name)
+
+
 def moe_router(logits, top_k, scoring="softmax", renormalize=True, scale=1.0, bias=None, token_mask=None):
     """The gate: every token's top_k experts and their weights, ready for moe_init_routing, the grouped products and the FFN entry points.
 
@@ -570,12 +576,13 @@ def moe_router(logits, top_k, scoring="softmax", renormalize=True, scale=1.0, bi
     [tokens, top_k], expert_idx int32 [tokens, top_k]): probs = scale * score, with renormalize divided by the token's sum of selected
     scores.  A logit of -inf or NaN is no candidate, a token whose token_mask is False has none: entries without an expert are -1
     with weight 0, which the routing sort drops.  What is not finite shows in the weights that it is a part of (all of the token's, or with
-    renormalize the selected ones), never in the others' selection.  Differentiable in the logits."""
+    renormalize the selected ones), never in the others' selection.  Differentiable in the logits, in reverse mode."""
     r = _direct.moe_router(logits, top_k, scoring, renormalize, scale, bias, token_mask)
     if r is not NotImplemented:
         return r
     _require_gpu(logits, bias, token_mask)
     _check_logits(logits)
+    _no_tangent("moe_router", logits)
     if _recorded(logits):
         return _Router.apply(logits, top_k, scoring, renormalize, scale, bias, token_mask)   # (comes back here without the record)
     tokens, e = logits.shape
@@ -650,7 +657,7 @@ def moe_balance_loss(logits, expert_idx, coef=1.0, z_coef=0.0, scoring="softmax"
     logsumexp(logits)^2.  The batch is one sequence, or seq_offsets (int32 [S + 1], rising) says where the sequences
     begin; tokens in none of them, masked ones (token_mask False) and those without a logit above -inf do not count.
     expert_idx int32 [tokens, top_k], entries outside the experts are no routes.  Returns (loss float32 [], counts int32 [E], or [S, E] with
-    seq_offsets, tokens int32 [1] or [S]: those that counted).  Differentiable in the logits; the same inputs give the same bits."""
+    seq_offsets, tokens int32 [1] or [S]: those that counted).  Differentiable in the logits, in reverse mode; the same inputs give the same bits."""
     r = _direct.moe_balance_loss(logits, expert_idx, coef, z_coef, scoring, token_mask, seq_offsets)
     if r is not NotImplemented:
         return r
@@ -658,6 +665,7 @@ def moe_balance_loss(logits, expert_idx, coef=1.0, z_coef=0.0, scoring="softmax"
     if expert_idx.dtype != torch.int32:
         raise ValueError("expert_idx must be int32 [tokens, top_k]")
     tokens, e, token_mask, offsets, s = _check_balance(logits, expert_idx.shape, token_mask, seq_offsets)
+    _no_tangent("moe_balance_loss", logits)
     if _recorded(logits):
         return _BalanceLoss.apply(logits, expert_idx, coef, z_coef, scoring, token_mask, seq_offsets)
     logits, idx = logits.contiguous(), expert_idx.contiguous()
