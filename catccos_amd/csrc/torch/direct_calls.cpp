@@ -490,7 +490,7 @@ PyObject *W4A16(PyObject *, PyObject *const *v, Py_ssize_t nv)
     HANDLE_TH_ERRORS
     int fmt;
     int64_t group;
-    if (nv != 6 || !PlainThread() || !(Plain(v[0], at::kBFloat16, 2) || Plain(v[0], at::kHalf, 2)) || !W4Format(v[4], fmt) || !Int(v[5], group) ||
+    if (nv != 6 || !PlainThread() || !(Plain(v[0], at::kBFloat16, 2) || Plain(v[0], at::kHalf, 2)) || Differentiated(T(v[0])) || !W4Format(v[4], fmt) || !Int(v[5], group) ||
         !W4Weights(v[1], v[2], v[3], 2, T(v[0]).size(1), fmt, group, T(v[0]).scalar_type()))
         return Decline();
     const at::Tensor &x = T(v[0]), &w = T(v[1]);
@@ -516,7 +516,7 @@ PyObject *MoeFfnW4A16(PyObject *, PyObject *const *v, Py_ssize_t nv)
     int fmt;
     int64_t group;
     if (nv != 11 || !PlainThread() || !(Plain(v[0], at::kBFloat16, 2) || Plain(v[0], at::kHalf, 2)) || !Plain(v[1], at::kInt, 2) || !Plain(v[2], at::kFloat, 2) ||
-        !Plain(v[3], at::kByte, 3) || !W4Format(v[9], fmt) || !Int(v[10], group))
+        Differentiated(T(v[0])) || Differentiated(T(v[2])) || !Plain(v[3], at::kByte, 3) || !W4Format(v[9], fmt) || !Int(v[10], group))
         return Decline();
     const at::Tensor &x = T(v[0]), &idx = T(v[1]), &probs = T(v[2]), &w1 = T(v[3]);
     const int64_t m = x.size(0), k = x.size(1), top_k = idx.size(1), e = w1.size(0), n = w1.size(1);

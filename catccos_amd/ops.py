@@ -714,6 +714,19 @@ class _BalanceLoss(torch.autograd.Function):
         return (moe_balance_loss_backward(grad_loss.float(), logits, counts, tokens, *ctx.options, token_mask, seq_offsets),) + (None,) * 6
 
 
+class _NoGradient(torch.autograd.Function):
+    """What call() returns, recorded as a function of the tensors, whose backward raises: products without a gradient do not lose one in silence."""
+
+    @staticmethod
+    def forward(ctx, name, call, *tensors):
+        ctx.name = name
+        return call()
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise NotImplementedError("%s has no gradient (call it under torch.no_grad() or on detached tensors)" % ctx.name)
+
+
 def _w4_fmt(fmt):
     if fmt in ("int4", FMT_INT4):
         return FMT_INT4
@@ -746,7 +759,7 @@ def w4a16_matmul(x, w, scales, zeros=None, fmt="int4", group_size=128):
 
     w uint8 [N, ceil(K/2)], element 2j in the low nibble.  fmt "int4": an element stands for (code - zero) * scale with scales [N, ceil(K/group_size)]
     of x's type and zeros uint8 (0..240) of that shape, or None for 8 everywhere; group_size 32, 64 or 128.  fmt "e2m1": MXFP4, scales E8M0 uint8
-    [N, scale_cols(K)], payload and scales as mx_quant(weights [N, K], "e2m1") returns them.  Inference only."""
+    [N, scale_cols(K)], payload and scales as mx_quant(weights [N, K], "e2m1") returns them.  Inference only: backward through it raises."""
     r = _direct.w4a16_matmul(x, w, scales, zeros, fmt, group_size)
     if r is not NotImplemented:
         return r
@@ -755,6 +768,9 @@ def w4a16_matmul(x, w, scales, zeros=None, fmt="int4", group_size=128):
     _check_w4_x(x)
     if w.dim() != 2:
         raise ValueError("w must be a 2-D uint8 tensor")
+    _no_tangent("w4a16_matmul", x)
+    if _recorded(x):
+        return _NoGradient.apply("w4a16_matmul", lambda: w4a16_matmul(x.detach(), w, scales, zeros, fmt, group_size), x)
     x = x.contiguous()
     (m, k), n = x.shape, w.shape[0]
     w, scales, zeros = _check_w4("w", w, scales, zeros, (n,), k, fmt, group_size, x.dtype)
@@ -769,7 +785,7 @@ def moe_ffn_w4a16(x, expert_idx, probs, w1, scales1, zeros1, w2, scales2, zeros2
     """The mixture-of-experts feed-forward of few tokens with 4-bit weights, one rank that holds every expert: what moe_ffn_mxfp8 computes, with bf16 or
     half activations throughout.  x [m, k]; expert_idx int32 and probs float32 [m, top_k] (moe_router's; entries outside the experts are
     dropped); w1 [E, n, ceil(k/2)] up projections, gate rows first, w2 [E, k, ceil(n/2/2)] down projections, each with scales and zeros (or
-    None) as in w4a16_matmul.  Returns [m, k] in x's type.  Inference only."""
+    None) as in w4a16_matmul.  Returns [m, k] in x's type.  Inference only: backward through it, to x or probs, raises."""
     r = _direct.moe_ffn_w4a16(x, expert_idx, probs, w1, scales1, zeros1, w2, scales2, zeros2, fmt, group_size)
     if r is not NotImplemented:
         return r
@@ -786,6 +802,10 @@ def moe_ffn_w4a16(x, expert_idx, probs, w1, scales1, zeros1, w2, scales2, zeros2
         raise ValueError("top_k must be 1..8")
     if w1.dim() != 3 or w1.shape[1] % 2:
         raise ValueError("w1 must be a 3-D uint8 tensor of gate and up halves")
+    _no_tangent("moe_ffn_w4a16", x, probs)
+    if _recorded(x) or _recorded(probs):
+        return _NoGradient.apply("moe_ffn_w4a16", lambda: moe_ffn_w4a16(x.detach(), expert_idx, probs.detach(), w1, scales1, zeros1, w2, scales2, zeros2, fmt, group_size),
+                                 x, probs)
     e, n = w1.shape[:2]
     x, expert_idx, probs = x.contiguous(), expert_idx.contiguous(), probs.contiguous()
     w1, scales1, zeros1 = _check_w4("w1", w1, scales1, zeros1, (e, n), k, fmt, group_size, x.dtype)
