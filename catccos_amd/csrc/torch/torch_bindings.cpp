@@ -14,13 +14,18 @@
 // time (:88-95); `finalize` on an uninitialised library returns 0 (:205-207).
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <ATen/core/LegacyTypeDispatch.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
 #include <hip/hip_runtime_api.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
 #include <algorithm>
 #include <atomic>
 #include <cctype>
+#include <functional>
 #include <initializer_list>
 #include <mutex>
 #include <optional>
@@ -625,6 +630,131 @@ at::Tensor MoeFfnW4A16Meta(const at::Tensor &x, const at::Tensor &, const at::Te
     return MetaEmpty(x, x.sym_sizes(), x.scalar_type());
 }
 
+// ---------------------------------------------------------------------------------------------
+// Autograd of the gate, the losses and the 4-bit products: the gradients that catccos_amd.ops' forms have, and an error where there are none.  A call with nothing to
+// differentiate goes on to its kernel as it is.
+
+template <auto F>
+struct Below;   // the operator whose kernel is F, called below autograd
+template <class R, class... A, R (*F)(A...)>
+struct Below<F> {
+    static R call(const char *name, A... a)
+    {
+        static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow(name, "").template typed<R(A...)>();
+        at::AutoDispatchBelowADInplaceOrView below;
+        return op.call(a...);
+    }
+};
+#define CCH_BELOW(f, name, ...) Below<&f>::call("catccos::" name, __VA_ARGS__)
+
+// Some of the tensors are recorded.  A tangent is refused.
+bool Recorded(const char *op, std::initializer_list<at::Tensor> tensors)
+{
+    bool some = false;
+    for (const at::Tensor &t : tensors) {
+        if (!t.defined()) continue;
+        TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), "catccos::", op, " has no forward-mode derivative");
+        some = some || t.requires_grad();
+    }
+    return some && c10::GradMode::is_enabled();
+}
+
+typedef torch::autograd::AutogradContext Context;
+typedef torch::autograd::variable_list Variables;
+
+struct NoGradient : torch::autograd::Function<NoGradient> {
+    static at::Tensor forward(Context *ctx, std::string op, std::function<at::Tensor()> call, const at::Tensor &, const MaybeTensor &)
+    {
+        ctx->saved_data["op"] = op;
+        return call();
+    }
+    static Variables backward(Context *ctx, Variables)
+    {
+        TORCH_CHECK_NOT_IMPLEMENTED(false, "catccos::", ctx->saved_data["op"].toStringRef(), " has no gradient");
+    }
+};
+
+at::Tensor MoeRouterBackwardAutograd(const at::Tensor &grad, const at::Tensor &logits, const at::Tensor &idx, std::string scoring, bool renormalize, double scale)
+{
+    auto call = [&] { return CCH_BELOW(MoeRouterBackward, "moe_router_backward", grad, logits, idx, scoring, renormalize, scale); };
+    return Recorded("moe_router_backward", {grad, logits}) ? NoGradient::apply("moe_router_backward", call, grad, MaybeTensor(logits)) : call();
+}
+at::Tensor MoeBalanceLossBackwardAutograd(const at::Tensor &grad, const at::Tensor &logits, const at::Tensor &counts, const at::Tensor &counted, int64_t top_k, double coef,
+                                          double z_coef, std::string scoring, const MaybeTensor &mask, const MaybeTensor &offsets)
+{
+    auto call = [&] { return CCH_BELOW(MoeBalanceLossBackward, "moe_balance_loss_backward", grad, logits, counts, counted, top_k, coef, z_coef, scoring, mask, offsets); };
+    return Recorded("moe_balance_loss_backward", {grad, logits}) ? NoGradient::apply("moe_balance_loss_backward", call, grad, MaybeTensor(logits)) : call();
+}
+at::Tensor W4A16MatmulAutograd(const at::Tensor &x, const at::Tensor &w, const at::Tensor &scales, const MaybeTensor &zeros, std::string fmt, int64_t group)
+{
+    auto call = [&] { return CCH_BELOW(W4A16Matmul, "w4a16_matmul", x, w, scales, zeros, fmt, group); };
+    return Recorded("w4a16_matmul", {x}) ? NoGradient::apply("w4a16_matmul", call, x, MaybeTensor()) : call();
+}
+at::Tensor MoeFfnW4A16Autograd(const at::Tensor &x, const at::Tensor &idx, const at::Tensor &probs, const at::Tensor &w1, const at::Tensor &s1, const MaybeTensor &z1,
+                               const at::Tensor &w2, const at::Tensor &s2, const MaybeTensor &z2, std::string fmt, int64_t group)
+{
+    auto call = [&] { return CCH_BELOW(MoeFfnW4A16, "moe_ffn_w4a16", x, idx, probs, w1, s1, z1, w2, s2, z2, fmt, group); };
+    return Recorded("moe_ffn_w4a16", {x, probs}) ? NoGradient::apply("moe_ffn_w4a16", call, x, MaybeTensor(probs)) : call();
+}
+
+struct RouterFunction : torch::autograd::Function<RouterFunction> {
+    static Variables forward(Context *ctx, const at::Tensor &logits, int64_t top_k, std::string scoring, bool renormalize, double scale, const MaybeTensor &bias,
+                             const MaybeTensor &mask)
+    {
+        const auto [probs, idx] = CCH_BELOW(MoeRouter, "moe_router", logits, top_k, scoring, renormalize, scale, bias, mask);
+        ctx->save_for_backward({logits, idx});
+        ctx->mark_non_differentiable({idx});
+        ctx->saved_data["scoring"] = scoring;
+        ctx->saved_data["renormalize"] = renormalize;
+        ctx->saved_data["scale"] = scale;
+        return {probs, idx};
+    }
+    static Variables backward(Context *ctx, Variables grads)
+    {
+        const Variables saved = ctx->get_saved_variables();
+        return {MoeRouterBackwardAutograd(grads[0], saved[0], saved[1], ctx->saved_data["scoring"].toStringRef(), ctx->saved_data["renormalize"].toBool(),
+                                          ctx->saved_data["scale"].toDouble()),
+                {}, {}, {}, {}, {}, {}};
+    }
+};
+std::tuple<at::Tensor, at::Tensor> MoeRouterAutograd(const at::Tensor &logits, int64_t top_k, std::string scoring, bool renormalize, double scale, const MaybeTensor &bias,
+                                                     const MaybeTensor &mask)
+{
+    if (!Recorded("moe_router", {logits})) return CCH_BELOW(MoeRouter, "moe_router", logits, top_k, scoring, renormalize, scale, bias, mask);
+    const Variables out = RouterFunction::apply(logits, top_k, scoring, renormalize, scale, bias, mask);
+    return {out[0], out[1]};
+}
+
+struct BalanceLossFunction : torch::autograd::Function<BalanceLossFunction> {
+    static Variables forward(Context *ctx, const at::Tensor &logits, const at::Tensor &idx, double coef, double z_coef, std::string scoring, const MaybeTensor &mask,
+                             const MaybeTensor &offsets)
+    {
+        const auto [loss, counts, counted] = CCH_BELOW(MoeBalanceLoss, "moe_balance_loss", logits, idx, coef, z_coef, scoring, mask, offsets);
+        ctx->save_for_backward({logits, counts, counted, mask.value_or(at::Tensor()), offsets.value_or(at::Tensor())});
+        ctx->mark_non_differentiable({counts, counted});
+        ctx->saved_data["top_k"] = idx.size(1);
+        ctx->saved_data["coef"] = coef;
+        ctx->saved_data["z_coef"] = z_coef;
+        ctx->saved_data["scoring"] = scoring;
+        return {loss, counts, counted};
+    }
+    static Variables backward(Context *ctx, Variables grads)
+    {
+        const Variables saved = ctx->get_saved_variables();
+        const auto maybe = [](const at::Tensor &t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); };
+        return {MoeBalanceLossBackwardAutograd(grads[0], saved[0], saved[1], saved[2], ctx->saved_data["top_k"].toInt(), ctx->saved_data["coef"].toDouble(),
+                                               ctx->saved_data["z_coef"].toDouble(), ctx->saved_data["scoring"].toStringRef(), maybe(saved[3]), maybe(saved[4])),
+                {}, {}, {}, {}, {}, {}};
+    }
+};
+std::tuple<at::Tensor, at::Tensor, at::Tensor> MoeBalanceLossAutograd(const at::Tensor &logits, const at::Tensor &idx, double coef, double z_coef, std::string scoring,
+                                                                      const MaybeTensor &mask, const MaybeTensor &offsets)
+{
+    if (!Recorded("moe_balance_loss", {logits})) return CCH_BELOW(MoeBalanceLoss, "moe_balance_loss", logits, idx, coef, z_coef, scoring, mask, offsets);
+    const Variables out = BalanceLossFunction::apply(logits, idx, coef, z_coef, scoring, mask, offsets);
+    return {out[0], out[1], out[2]};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(catccos, m)
@@ -691,4 +821,14 @@ TORCH_LIBRARY_IMPL(catccos, Meta, m)
     m.impl("moe_balance_loss_backward", &MoeBalanceLossBackwardMeta);
     m.impl("w4a16_matmul", &W4A16Meta);
     m.impl("moe_ffn_w4a16", &MoeFfnW4A16Meta);
+}
+
+TORCH_LIBRARY_IMPL(catccos, Autograd, m)
+{
+    m.impl("moe_router", &MoeRouterAutograd);
+    m.impl("moe_router_backward", &MoeRouterBackwardAutograd);
+    m.impl("moe_balance_loss", &MoeBalanceLossAutograd);
+    m.impl("moe_balance_loss_backward", &MoeBalanceLossBackwardAutograd);
+    m.impl("w4a16_matmul", &W4A16MatmulAutograd);
+    m.impl("moe_ffn_w4a16", &MoeFfnW4A16Autograd);
 }

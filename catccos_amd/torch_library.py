@@ -26,8 +26,8 @@ The operators are a C++ `TORCH_LIBRARY` (catccos_amd/csrc/torch/torch_bindings.c
 `python -m catccos_amd.build` into catccos_amd/libcatccos_torch.so): C++ programs linking libtorch load that
 library directly; importing this module loads it into the Python process (`import catccos_amd` does not).
 Also there: `mx_grouped_matmul_swiglu_mx`, `gmm_dequant_swiglu_mx` (up projections with MX-quantised output) and
-`moe_ffn_mxfp8` (the MXFP8 MoE FFN of one rank, routing to combine); `moe_router`, `moe_balance_loss` and their gradients as calls of their
-own (`..._backward`; the differentiable forms are catccos_amd.ops'); `w4a16_matmul`, `moe_ffn_w4a16`.
+`moe_ffn_mxfp8` (the MXFP8 MoE FFN of one rank, routing to combine); `moe_router`, `moe_balance_loss`, differentiable in the logits in reverse
+mode, and their gradients as calls of their own (`..._backward`); `w4a16_matmul`, `moe_ffn_w4a16`, backward through which raises.
 """
 import os
 
