@@ -367,13 +367,13 @@ void CheckLogits(const at::Tensor &logits)
     DtypeCode(logits);
 }
 
-// An optional argument on `like`'s GPU, of the type and number of elements that the kernel takes it to be; contiguous.
-at::Tensor Optional(const char *op, const char *name, const MaybeTensor &t, const at::Tensor &like, std::initializer_list<at::ScalarType> types, int64_t numel)
+// An optional argument on `like`'s GPU, of the type and shape that the kernel takes it to be; contiguous.
+at::Tensor Optional(const char *op, const char *name, const MaybeTensor &t, const at::Tensor &like, std::initializer_list<at::ScalarType> types, at::IntArrayRef shape)
 {
     if (!t || !t->defined()) return at::Tensor();
     SameDevice(op, {{"the first argument", like}, {name, *t}});
-    TORCH_CHECK(std::find(types.begin(), types.end(), t->scalar_type()) != types.end() && t->numel() == numel, "catccos::", op, ": ", name, " must have ", numel,
-                " elements of its type");
+    TORCH_CHECK(std::find(types.begin(), types.end(), t->scalar_type()) != types.end() && t->sizes() == shape, "catccos::", op, ": ", name, " must be a ", shape,
+                " tensor of its type");
     return t->contiguous();
 }
 template <class T>
@@ -474,8 +474,9 @@ void CheckW4(const char *name, const at::Tensor &w, const at::Tensor &scales, co
     const int64_t groups = fmt == CCH_FMT_INT4 ? (k + group - 1) / group : ScaleCols(k);
     TORCH_CHECK(w.scalar_type() == at::kByte && w.numel() == lead * rows * ((k + 1) / 2) && w.size(-1) == (k + 1) / 2 && w.size(-2) == rows, name, " must be a uint8 tensor of ",
                 (k + 1) / 2, " bytes a row");
-    TORCH_CHECK(scales.scalar_type() == (fmt == CCH_FMT_INT4 ? type : at::kByte) && scales.numel() == lead * rows * groups && scales.size(-1) == groups, "scales of ", name,
-                " must have ", groups, " columns of ", fmt == CCH_FMT_INT4 ? "the activations' type" : "E8M0 bytes");
+    TORCH_CHECK(scales.scalar_type() == (fmt == CCH_FMT_INT4 ? type : at::kByte) && scales.dim() == w.dim() && scales.size(-1) == groups &&
+                    scales.sizes().slice(0, w.dim() - 1) == w.sizes().slice(0, w.dim() - 1),
+                "scales of ", name, " must have a row of ", groups, " for each of its rows, of ", fmt == CCH_FMT_INT4 ? "the activations' type" : "E8M0 bytes");
     TORCH_CHECK(!zeros.defined() || (fmt == CCH_FMT_INT4 && zeros.scalar_type() == at::kByte && zeros.sizes() == scales.sizes()), "zeros of ", name,
                 " must be uint8 of the scales' shape, with int4 weights only");
 }
@@ -487,7 +488,7 @@ int W4Format(const std::string &name, int64_t group)
 }
 at::Tensor Zeros(const char *op, const char *name, const MaybeTensor &zeros, const at::Tensor &x)
 {
-    return Optional(op, name, zeros, x, {at::kByte}, zeros && zeros->defined() ? zeros->numel() : 0);
+    return Optional(op, name, zeros, x, {at::kByte}, zeros && zeros->defined() ? zeros->sizes() : at::IntArrayRef());
 }
 
 at::Tensor W4A16Matmul(const at::Tensor &x_in, const at::Tensor &w_in, const at::Tensor &scales_in, const MaybeTensor &zeros_in, std::string fmt_name, int64_t group)
