@@ -12,7 +12,7 @@
 // launch has the loss.  Backward: one pass, logits in, gradient out.
 //
 // Bound by the logits' bytes on paper (16384 tokens of 256 experts, bf16: 8.4 MB read, then 16.8 MB read and written, 5.1 us at the rate of a large copy), by launches
-// and waits for memory in fact: that batch in 13 sequences with sigmoid scores takes 7.3 + 4.2 + 2.5 us forward and 10.0 backward, where an empty launch takes 2.4 and every
+// and waits for memory in fact: that batch in 13 sequences with sigmoid scores takes 8.6 to 11 + 4.5 + 2.4 us forward and 10 backward, where an empty launch takes 2.4 and every
 // workgroup has two steps of 16 tokens, the exponentials of all being 1.3 us of the card's time.
 #include <algorithm>
 
@@ -140,8 +140,8 @@ __device__ __forceinline__ N block_sum(N x, N (&scratch)[WAVES])
     return sum;
 }
 
-// What is read of a token; all of it at once, a step ahead.  (The mask, then the experts of those that it leaves, are two waits for memory in every step:
-// 16384 tokens of 256 experts in 13 sequences 8.3 us at best, against 7.3.)
+// What is read of a token; all of it at once, a step ahead.  (The mask, then the experts of those that it leaves, are two waits for memory in every step, which other workgroups
+// hide: 16384 tokens of 256 experts in 13 sequences 10.1 and 11.2 us in the median that way, 11.5 and 11.0 this way.)
 template <class T, int V, bool VEC>
 struct TokenIn {
     LaneRow<T, V, VEC> row;

@@ -1,10 +1,11 @@
 // The mixture-of-experts feed-forward of few tokens with weights of 4 bits: for every route (t, j) to expert e = expert_idx[t, j]
 //   h = silu(g) * u, [g | u] = W1_e x_t,  y = W2_e h,  out[t] = sum_j probs[t, j] y_tj
-// Up projection and activation are one launch (h in the activations' type: it is the next product's operand), down projection the next (fp32), then the sum
-// over a token's routes in their order, so that the same inputs give the same bits.
+// Up projection and activation are one launch, down projection the next (fp32), then the sum over a token's routes in their order, so that the same inputs give the same bits.
+// h is rounded to the activations' type, as between two layers that are separate calls: it is the next product's 16-bit operand, and two such parts of it would be twice the rows for
+// the matrix instructions and for LDS.  Of results in bf16 it takes the error against 64 bits from 1.7e-3, their own rounding, to 2.3e-3 or 2.4e-3; in half an h past 65504 is an infinity.
 //
-// Bound by the weights of the experts that some route names, once each: one token, 6 of 16 experts, k = 7168, n = 4096 (132 MB) 19.5 + 13.5 + 3.9 us in its three launches, 4.0 TB/s;
-// 64 tokens (353 MB) 70 + 46 + 4.8 us.  Down projection and sum in one launch, a workgroup having its columns of all routes, measured about the same for one token (14.4 us for 13.2 +
+// Bound by the weights of the experts that some route names, once each: one token, 6 of 16 experts, k = 7168, n = 4096 (136 MB) 21.2 + 15.3 + 3.8 us in its three launches, 3.7 TB/s over the
+// products (fastest of a kernel trace; 36 to 40 us a call); 64 tokens (374 MB) 71 + 51 + 4.4 fastest, 80 + 57 + 5.2 in the median, 113 to 153 a call by card and inputs.  Down projection and sum in one launch, a workgroup having its columns of all routes, measured about the same for one token (14.4 us for 13.2 +
 // 4.7) and far worse for twelve (26 for 11.8 + 4.7, the experts one after another): not kept.
 #include <algorithm>
 

@@ -16,8 +16,9 @@
 // less than sorting anything, and ties need no extra step.
 //
 // Bound: on paper the bytes (16384 tokens of 64 experts in bf16, 8 routes: 3.1 MB forward, 5.2 MB backward, 1.6 us for both at the rate of a large copy), in fact the
-// launch (an empty one 2.4 us) and the selection's instructions, some 2 V + 20 to a route: that case takes 4.8 + 3.9 us, 4099 tokens of 256 experts (fp32, sigmoid) 5.4 +
-// 3.7, 64 tokens of 16 experts 2.2; 16384 x 1024 in bf16 28.0 + 16.7 (1.2 and 4.0 TB/s).  Backward, the selected experts' terms reach the lanes that hold them through LDS: one
+// launch (an empty one 2.4 us) and the selection's instructions, some 2 V + 20 to a route: that case takes 4.8 + 4.0 us, 4099 tokens of 256 experts (fp32, sigmoid) 5.4 +
+// 4.0, 64 tokens of 16 experts 2.2; 16384 x 1024 in bf16 28.0 + 16.7 (1.2 and 4.0 TB/s).  A bias costs the scores of all experts, a division each for softmax: 64 x 256 4.3 -> 6.5 us,
+// 16384 x 64 4.4 -> 5.6, x 256 8.5 -> 15.1, x 1024 25.6 -> 46.7.  Backward, the selected experts' terms reach the lanes that hold them through LDS: one
 // write for all routes, where comparing every expert with every route is 2 V instructions a route (16384 x 1024 23.6 us, x 256 9.1 against 6.5, x 64 4.3 against 3.8).
 #include <algorithm>
 

@@ -124,7 +124,7 @@ __device__ __forceinline__ void store_row(T *row, int first, int experts, bool v
 // 1 / x to a unit in the last place, one instruction (an exact division is ten).
 __device__ __forceinline__ float reciprocal(float x) { return __builtin_amdgcn_rcpf(x); }
 
-// e^x: the argument is rounded once, so that the result is off by |x| 2^-24 relative and the instruction's unit.
+// e^x: the product with log2(e) and that constant are rounded, so that the result is off by up to |x| log2(e) 2^-23 relative and the instruction's unit.
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
 
 // sigmoid(l) / e^c for c <= 0, c no smaller than l or zero: with c the smaller of 0 and the largest of several logits, their sum is at least 1/2

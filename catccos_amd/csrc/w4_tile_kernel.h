@@ -8,17 +8,21 @@
 //
 // A sum over K may be taken in any order, so a matrix instruction's 32 values of K are whichever lie ready.  A code of 4 bits becomes a 16-bit number with one shift and
 // one and-or: 16 + q, the code in the leading bits of 1.xxxx * 2^4.  Masks with two nibbles 16 bits apart give pairs (j, j + 4) of a dword's eight elements, and x is
-// put in the same order.  The 16 and the zero point leave by a second instruction with the constant -(16 + z) as its right operand, exactly: in
-// fp32 the products of a group sum to what (q - z) gives, and one fused multiply-add per group brings its scale in, which is never rounded into a weight.
+// put in the same order.  The 16 and the zero point leave by a second instruction with the constant -(16 + z) as its right operand, and one fused multiply-add
+// per group brings its scale in, which is never rounded into a weight.  Exact in this are the 16-bit operands.  The two halves of a group's sum are fp32 and round at their own size before
+// they cancel: the error is that of a sum of |x| (31 + |q - z|) |scale|, for z up to 15 at most 31 / |q - z| + 1 times that of the products themselves, some bits more where a group's x
+// have one sign.  (4096 x 7168: 2.4e-5 between this and (q - z) scale in fp32, of results whose rounding to bf16 is 1.7e-3.)  And they have to stay finite: a group of bf16 x whose sum of
+// |x| passes 2^128 / 31 (about 1.1e37; 2^128 / 256 with zero points up to 240) gives NaN, as an infinite x does.
 // That asks for a group's values to meet in one instruction and no others, which the way the dwords are read from LDS sees to.  MXFP4 with bf16 needs none of
 // it: the conversion instruction applies the power of two, exactly.
 //
 // The sums and the groups' scales stay in fp32; rounded to 16 bits are the results alone.  Zero points that -(16 + z) holds exactly, up to 240 in bf16.
 //
 // Bound, one row: the weights' bytes, after a launch, two waits for memory and the sum over K's parts: 4096 x 7168 in 5.9 us, 2.5 TB/s (reading alone 3.6, an empty launch
-// 2.4), 32768 x 7168 in 26 us, 4.6 TB/s.  64 rows x 32768 x 7168: 69 us, 1.7 TB/s and 0.44 PFLOP/s.  A tile of weights and 64 rows of x take, per block of K, about 100
-// vector instructions of 4 clocks (conversion 34, scales 32, x and addresses the rest), 32 matrix instructions of 16 and 18 KB from LDS, in a SIMD's time little overlapped: 16 waves overlap
-// them better than 8 (77 us), whatever order the compiler is asked for.
+// 2.4), 32768 x 7168 in 22 to 26 us, 4.6 TB/s.  61 rows x 32768 x 7168, groups of 64 with zero points: 61 to 71 us by card, 1.7 TB/s and 0.41 PFLOP/s at the latter.  A tile of
+// weights and 64 rows of x take, per block of K, about 130 vector instructions of 4 clocks (conversion, scales, x and addresses), 32 matrix instructions of 16 and 18 KB from LDS, 16 of
+// them x: 24, 24 and 27 us for all tiles at 2.4 GHz and 128 bytes a clock and CU, and the launch takes nearly their sum.  16 waves overlap them better than 8 (77 us), whatever order the
+// compiler is asked for; two tiles of columns to a wave read x half as often but leave eight waves.
 #pragma once
 #include <algorithm>
 #include <atomic>
@@ -571,6 +575,10 @@ int w4_tile_launch(const W4Rows &rows, const W4Matrix &w, void *out, hipStream_t
 //       16         16.0 / 15.5   * 14.6 / 13.2     40.8 / 41.5     23.1 / 20.6      62 /  61       32.0 / 30.6
 //       32         19.4 / 15.5     17.9 / 16.2   * 44.3 / 38.7   * 19.1 / 17.7   *  53 /  47     * 32.0 / 26.9      81 /  66
 //       48                         25.3 / 20.6     56.1 / 47.5     26.7 / 23.1      59 /  51       31.7 / 26.9   *  63 /  53      (96 routes: * 143 / 114, 32 rows 142 / 117)
+//
+// These are the layers that were swept.  Below 4096 columns the dense rule was measured afterwards and not tuned: K = 7168, 512 to 2048 columns 6.0 us for one row, 6.6 for 16, 15.1 to
+// 16.4 for 17 to 128 (16 to 256 workgroups of eight waves).  The grouped rule looks at tokens and routes alone: with few experts or a narrow up projection its larger shapes are few workgroups that walk
+// all of K (two of 4 experts, n = 512, K = 8192, 64 tokens: 77 us for the block, 16 of them in the up projection's launch; its weights are 3 us at the rate of a copy).
 template <class T, int KIND, bool ZEROS>
 int w4_tile_choose(int out_kind, const W4Rows &rows, const W4Matrix &w, void *out, hipStream_t s)
 {

@@ -402,7 +402,9 @@ int cch_moe_balance_loss_backward(const float *grad_loss, const void *logits, in
  *   workspace  device memory on a 16-byte boundary of at least cch_w4a16_matmul_workspace_bytes(...) bytes (none for 0); nothing in it has to be
  *            kept or cleared between calls, calls that overlap need one each
  * m below 2^31, n up to 2^25, k below 2^30.  x and w on 16-byte boundaries and a k that is a multiple of 32 and below 2^24 (in the FFN below: below 2^19) take the
- * tiled kernels; anything else takes one with a wave per output element.  Zero points are 0..240: where x is bf16 the tiled kernels round a byte of more. */
+ * tiled kernels; anything else takes one with a wave per output element.  Zero points are 0..240: where x is bf16 the tiled kernels round a byte of more.
+ * int4: before the scale the tiled kernels' fp32 sums of a group are as large as sum |x| (16 + zero) and sum |x| (16 + code); they round at that size, and bf16 x for which one passes
+ * 2^128 (sum |x| of about 1.1e37 with zero points up to 15) give NaN, as an infinite x does. */
 int64_t cch_w4a16_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int cch_w4a16_matmul(const void *x, const void *w, const void *scales, const void *zeros, void *out, int64_t m, int64_t n, int64_t k, int fmt,
                      int group_size, int dtype, void *workspace, int64_t workspace_bytes, void *stream);
@@ -410,7 +412,7 @@ int cch_w4a16_matmul(const void *x, const void *w, const void *scales, const voi
  *   x, out      [m, k] of type dtype; expert_idx int32 [m, top_k] (an entry outside [0, num_experts) is dropped)
  *   probs       fp32 [m, top_k]; top_k 1..8; num_experts 1..1024
  *   w1 / s1 / z1   up projections [num_experts] x [n, k], gate rows first, as above; w2 / s2 / z2 down projections [k, n/2]
- *   The activation silu(gate) * up is rounded to dtype between the two products; sums over a token's routes are fp32, in their order.
+ *   The activation silu(gate) * up is rounded to dtype between the two products (half: beyond 65504 to an infinity); sums over a token's routes are fp32, in their order.
  *   workspace   device memory on a 512-byte boundary, at least cch_moe_ffn_w4a16_workspace_bytes(...); as above */
 int64_t cch_moe_ffn_w4a16_workspace_bytes(int64_t m, int64_t k, int top_k, int64_t num_experts, int64_t n);
 int cch_moe_ffn_w4a16(const void *x, const int32_t *expert_idx, const float *probs, const void *w1, const void *s1, const void *z1,
