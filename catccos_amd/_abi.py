@@ -14,6 +14,8 @@ FMT_E4M3, FMT_E5M2, FMT_E2M1, FMT_E1M2, FMT_INT4 = 0, 1, 2, 3, 4
 ROUND_RNE, ROUND_LUT = 0, 1
 DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2
 SCORING_SOFTMAX, SCORING_SIGMOID = 0, 1
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU, ACT_GELU_TANH = 0, 1, 2, 3, 4
+REDUCE_MEAN, REDUCE_SUM = 0, 1
 
 c = ctypes
 _P, _I64, _I, _SZ, _F = c.c_void_p, c.c_int64, c.c_int, c.c_size_t, c.c_float
@@ -69,12 +71,27 @@ PROTOTYPES = {
     "cch_w4a16_matmul": [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I, _I, _I, _P, _I64, _P],
     "cch_moe_ffn_w4a16_workspace_bytes": [_I64, _I64, _I, _I64, _I64],
     "cch_moe_ffn_w4a16": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I, _I64, _I64, _I, _I, _I, _P, _I64, _P],
+    "cch_grouped_matmul_workspace_bytes": [_I64, _I64, _I64, _I64, _I],
+    "cch_grouped_matmul": [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _I, _P, _I64, _P],
+    "cch_grouped_matmul_backward_workspace_bytes": [_I64, _I64, _I64, _I64, _I],
+    "cch_grouped_matmul_backward": [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _I, _P, _I64, _P],
+    "cch_matmul_bias_act_workspace_bytes": [_I64, _I64, _I64, _I],
+    "cch_matmul_bias_act": [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I, _I, _I, _P, _I64, _P],
+    "cch_matmul_bias_act_backward_workspace_bytes": [_I64, _I64, _I64, _I, _I],
+    "cch_matmul_bias_act_backward": [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I, _I, _I, _P, _I64, _P],
+    "cch_linear_cross_entropy_workspace_bytes": [_I64, _I64, _I64],
+    "cch_linear_cross_entropy": [_P, _P, _P, _I, _P, _P, _P, _P, _I64, _I64, _I64, _I, _F, _I, _P, _I64, _P],
+    "cch_linear_cross_entropy_backward_workspace_bytes": [_I64, _I64, _I64],
+    "cch_linear_cross_entropy_backward": [_P, _P, _P, _P, _I, _P, _P, _P, _P, _I64, _I64, _I64, _I, _F, _I, _P, _I64, _P],
     "cch_set_option": [c.c_char_p, _I],
     "cch_gemm_tail_rows": [_P, _I64, _I64, _I64, _I, _I, _P, _P],
     "cch_gemm_kernel_for": [_I, _I, _I64, _I64, _I64, _I64, _I, _I],
 }
 _RESTYPE = {"cch_last_error": c.c_char_p, "cch_moe_init_routing_workspace_bytes": _I64, "cch_moe_ffn_mxfp8_workspace_bytes": _I64,
-            "cch_moe_balance_loss_workspace_bytes": _I64, "cch_w4a16_matmul_workspace_bytes": _I64, "cch_moe_ffn_w4a16_workspace_bytes": _I64}
+            "cch_moe_balance_loss_workspace_bytes": _I64, "cch_w4a16_matmul_workspace_bytes": _I64, "cch_moe_ffn_w4a16_workspace_bytes": _I64,
+            "cch_grouped_matmul_workspace_bytes": _I64, "cch_grouped_matmul_backward_workspace_bytes": _I64, "cch_matmul_bias_act_workspace_bytes": _I64,
+            "cch_matmul_bias_act_backward_workspace_bytes": _I64, "cch_linear_cross_entropy_workspace_bytes": _I64,
+            "cch_linear_cross_entropy_backward_workspace_bytes": _I64}
 
 _lib = None
 

@@ -1,0 +1,82 @@
+// Products of bf16 or half operands with fp32 sums: the problem that the kernels take (gemm16_kernel.h), how it is launched, and the preparation of
+// operands whose rows start on no 16-byte boundary.
+#pragma once
+#include "common.h"
+
+namespace cch {
+
+constexpr int MAX_GROUPS16 = 1024;
+constexpr int64_t MAX_PITCH16 = (int64_t)1 << 22;   // elements of a row as stored: 256 of them stay below 2^31 bytes, which a request's offset holds
+
+enum Layout16 { ROWS_NK = 0, ROWS_NN = 1, ROWS_TN = 2 };
+// ROWS_NK: A [M, K], B [N, K].  ROWS_NN: A [M, K], B [K, N].  ROWS_TN: A [K, M], B [K, N].
+enum Epilogue16 {
+    EPI16_OUT = 0,    // out = scale * sum, rounded; or fp32 sums kept and added to (`sums`)
+    EPI16_ACT = 1,    // z = sum + bias, kept if asked for; out = act(z) + residual
+    EPI16_STATS = 2,  // cross entropy: a row's largest logit and sum of exponentials per 64 columns, and its target's logit
+    EPI16_GRAD = 3,   // cross entropy: the logits' gradient times grad_scale
+};
+
+struct Gemm16 {
+    const uint16_t *a, *b;
+    uint16_t *out;
+    int64_t pitch_a, pitch_b, pitch_out;   // elements between rows as stored: multiples of 8 for a and b, whose addresses are multiples of 16 bytes
+    int m, n, k;                           // with groups: all groups' rows (or, k_grouped, all groups' K)
+    int64_t b_stride, out_stride;          // elements between the groups' B (rows grouped), outputs (K grouped)
+    const int32_t *group_sizes;            // device, or nullptr: one group of everything.  Clipped to 0..what is left
+    int groups;
+    int k_grouped;                         // 0: a group is a range of rows of A and of the output; 1: a range of K (ROWS_TN)
+    int zero_rest;                         // rows behind the last group are written as zeros
+    const int32_t *a_rows;                 // ROWS_NK: row of A that is row i of the product (m_src rows there; below 2^31 bytes), or nullptr
+    int m_src;
+    const int32_t *out_rows;               // row of the output that row i goes to, or nullptr
+    int half;                              // IEEE half, else bf16
+    // EPI16_OUT
+    const float *scale;                    // device, or nullptr: 1
+    float *sums;                           // fp32 [m, n], or nullptr: a product in pieces of K.  sums_in: added to the sum; sums_out: takes it in place of out
+    int sums_in, sums_out;
+    // EPI16_ACT
+    const uint16_t *bias, *residual;
+    uint16_t *preact;
+    int act;
+    // EPI16_STATS, EPI16_GRAD (columns are v0 + 0..n-1 of the vocabulary)
+    int v0;
+    const int32_t *targets;                // per row of the product
+    float2 *stats;                         // [m, stat_cols]
+    int stat_cols;
+    float *target_logit;
+    const float *lse;                      // per row of the product
+    float z2, grad_scale;                  // 2 * z_coef
+};
+
+// Rows of the output, or the groups' K, that a launch may find: its grid's upper bound.
+int gemm16_launch(const Gemm16 &p, int layout, int epilogue, hipStream_t stream);
+
+inline bool whole16(int64_t cols) { return cols % 8 == 0; }
+inline int64_t pitch16(int64_t cols) { return (cols + 7) & ~(int64_t)7; }
+inline int64_t round256(int64_t bytes) { return (bytes + 255) & ~(int64_t)255; }
+// Bytes of the copy that rows of `cols` elements need (0: none, they are whole multiples of 16 bytes).
+inline int64_t padded16_bytes(int64_t rows, int64_t cols) { return whole16(cols) ? 0 : round256(rows * pitch16(cols) * 2); }
+
+// A workspace handed out front to back.
+struct Carve {
+    uint8_t *at;
+    template <class T> T *take(int64_t bytes)
+    {
+        T *p = reinterpret_cast<T *>(at);
+        at += round256(bytes);
+        return p;
+    }
+};
+
+// Rows of `cols` elements copied to rows of pitch16(cols), zeros behind them.
+int pad_rows16(const uint16_t *src, uint16_t *dst, int64_t rows, int64_t cols, hipStream_t stream);
+// `src`, or its padded copy where its rows need one (space from `ws`); the pitch in *pitch.
+int operand16(const uint16_t *src, int64_t rows, int64_t cols, Carve &ws, const uint16_t **out, int64_t *pitch, hipStream_t stream);
+
+int fill_zero16(uint16_t *dst, int64_t n, hipStream_t stream);
+// dz = grad_out * act'(preact) in rows of pitch16(n) and its column sums; either may be left out.  partial: column_sum_bytes(...) of fp32
+int64_t column_sum_bytes(int64_t m, int64_t n);
+int act_backward16(const uint16_t *grad_out, const uint16_t *preact, uint16_t *dz, uint16_t *grad_bias, float *partial, int64_t m, int64_t n, int act, int half, hipStream_t stream);
+
+}  // namespace cch

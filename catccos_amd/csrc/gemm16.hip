@@ -1,0 +1,128 @@
+// What the products of 16-bit operands need around their kernels: the choice by type, copies of operands whose rows start on no 16-byte boundary, and the
+// first step of a layer's backward pass.
+#include <algorithm>
+
+#include "gemm16_device.h"
+
+namespace cch {
+
+int gemm16_launch_bf16(const Gemm16 &p, int layout, int epilogue, hipStream_t stream);   // gemm16_bf16.hip
+int gemm16_launch_f16(const Gemm16 &p, int layout, int epilogue, hipStream_t stream);    // gemm16_f16.hip
+
+int gemm16_launch(const Gemm16 &p, int layout, int epilogue, hipStream_t stream)
+{
+    return p.half ? gemm16_launch_f16(p, layout, epilogue, stream) : gemm16_launch_bf16(p, layout, epilogue, stream);
+}
+
+// One thread, 16 bytes of the copy.
+__global__ __launch_bounds__(256) void pad_rows16_kernel(const uint16_t *__restrict__ src, uint16_t *__restrict__ dst, int64_t chunks, int64_t cols, int64_t per_row)
+{
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < chunks; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / per_row, c = (i - row * per_row) * 8;
+        const uint16_t *s = src + row * cols + c;
+        v4i o;
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+            const uint32_t lo = c + 2 * x < cols ? s[2 * x] : 0u, hi = c + 2 * x + 1 < cols ? s[2 * x + 1] : 0u;
+            o[x] = (int)(lo | hi << 16);
+        }
+        *reinterpret_cast<v4i *>(dst + i * 8) = o;
+    }
+}
+
+int pad_rows16(const uint16_t *src, uint16_t *dst, int64_t rows, int64_t cols, hipStream_t stream)
+{
+    const int64_t per_row = pitch16(cols) / 8, chunks = rows * per_row;
+    if (chunks == 0) return CCH_OK;
+    hipLaunchKernelGGL(pad_rows16_kernel, dim3((unsigned)std::min<int64_t>((chunks + 255) / 256, 1 << 16)), dim3(256), 0, stream, src, dst, chunks, cols, per_row);
+    return launch_status("pad_rows16_kernel");
+}
+
+int operand16(const uint16_t *src, int64_t rows, int64_t cols, Carve &ws, const uint16_t **out, int64_t *pitch, hipStream_t stream)
+{
+    *pitch = pitch16(cols);
+    *out = src;
+    if (whole16(cols)) return CCH_OK;
+    uint16_t *copy = ws.take<uint16_t>(padded16_bytes(rows, cols));
+    *out = copy;
+    return pad_rows16(src, copy, rows, cols, stream);
+}
+
+__global__ __launch_bounds__(256) void fill_zero16_kernel(uint16_t *dst, int64_t n)
+{
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) dst[i] = 0;
+}
+int fill_zero16(uint16_t *dst, int64_t n, hipStream_t stream)
+{
+    hipLaunchKernelGGL(fill_zero16_kernel, dim3((unsigned)std::min<int64_t>((n + 255) / 256, 1 << 14)), dim3(256), 0, stream, dst, n);
+    return launch_status("fill_zero16_kernel");
+}
+
+// ---- dz = grad_out * act'(preact) and the bias' gradient.  A workgroup has 256 columns, 8 to a thread, and a run of rows, every eighth to a thread; its columns' sums over
+// the run go to `partial`, which a second launch adds up in the runs' order.  Sums are of the products before their rounding.  Bound by memory: two reads, one write.
+constexpr int SUM_COLS = 256, SUM_RUNS = 64;
+static int64_t sum_runs(int64_t m) { return std::max<int64_t>(1, std::min<int64_t>((m + 63) / 64, SUM_RUNS)); }
+int64_t column_sum_bytes(int64_t m, int64_t n) { return round256(sum_runs(m) * n * 4); }
+
+template <class T>
+__global__ __launch_bounds__(256) void act_backward16_kernel(const uint16_t *__restrict__ grad, const uint16_t *__restrict__ pre, uint16_t *__restrict__ dz,
+                                                             float *__restrict__ partial, int m, int n, int64_t pitch, int run, int act, bool whole_rows)
+{
+    __shared__ float sums[8][SUM_COLS];
+    const int tc = threadIdx.x & 31, tr = threadIdx.x >> 5;
+    const int c = (int)blockIdx.x * SUM_COLS + tc * 8, left = n - c;
+    const int first = (int)blockIdx.y * run, last = min(m, first + run);
+    const bool whole = whole_rows && left >= 8;
+    float sum[8] = {};
+    if (left > 0)
+        for (int row = first + tr; row < last; row += 8) {
+            float v[8], z[8];
+            load8<T>(grad + (int64_t)row * n + c, whole, left, v);
+            if (act != CCH_ACT_NONE) {
+                load8<T>(pre + (int64_t)row * n + c, whole, left, z);
+#pragma unroll
+                for (int x = 0; x < 8; x++) v[x] = x < left ? v[x] * act_slope(z[x], act) : 0.0f;
+            }
+            if (dz) store8<T>(dz + (int64_t)row * pitch + c, true, 8, v);
+#pragma unroll
+            for (int x = 0; x < 8; x++) sum[x] += v[x];
+        }
+    if (!partial) return;
+#pragma unroll
+    for (int x = 0; x < 8; x++) sums[tr][tc * 8 + x] = sum[x];
+    __syncthreads();
+    const int col = (int)blockIdx.x * SUM_COLS + (int)threadIdx.x;
+    if (col < n) {
+        float s = 0.0f;
+#pragma unroll
+        for (int x = 0; x < 8; x++) s += sums[x][threadIdx.x];
+        partial[(int64_t)blockIdx.y * n + col] = s;
+    }
+}
+
+template <class T> __global__ __launch_bounds__(256) void column_sum16_kernel(const float *__restrict__ partial, uint16_t *__restrict__ out, int n, int runs)
+{
+    const int col = (int)blockIdx.x * 256 + (int)threadIdx.x;
+    if (col >= n) return;
+    float s = 0.0f;
+#pragma unroll 16
+    for (int i = 0; i < runs; i++) s += partial[(int64_t)i * n + col];
+    out[col] = T::from(s);
+}
+
+int act_backward16(const uint16_t *grad_out, const uint16_t *preact, uint16_t *dz, uint16_t *grad_bias, float *partial, int64_t m, int64_t n, int act, int half, hipStream_t stream)
+{
+    if (m == 0 || n == 0 || (!dz && !grad_bias)) return CCH_OK;
+    const int64_t runs = sum_runs(m), run = (m + runs - 1) / runs;
+    const bool whole = n % 8 == 0 && aligned(grad_out, 16) && aligned(preact, 16);
+    auto kern = half ? act_backward16_kernel<F16> : act_backward16_kernel<Bf16>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)((n + SUM_COLS - 1) / SUM_COLS), (unsigned)runs), dim3(256), 0, stream, grad_out, preact, dz, grad_bias ? partial : nullptr, (int)m,
+                       (int)n, pitch16(n), (int)run, act, whole);
+    if (const int rc = launch_status("act_backward16_kernel")) return rc;
+    if (!grad_bias) return CCH_OK;
+    auto sum = half ? column_sum16_kernel<F16> : column_sum16_kernel<Bf16>;
+    hipLaunchKernelGGL(sum, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, partial, grad_bias, (int)n, (int)runs);
+    return launch_status("column_sum16_kernel");
+}
+
+}  // namespace cch

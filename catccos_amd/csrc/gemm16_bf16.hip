@@ -1,0 +1,8 @@
+// Instantiations of gemm16_kernel.h: bf16.
+#include "gemm16_choose.h"
+
+namespace cch {
+
+int gemm16_launch_bf16(const Gemm16 &p, int layout, int epilogue, hipStream_t stream) { return choose16<Bf16>(p, layout, epilogue, stream); }
+
+}  // namespace cch

@@ -1,0 +1,35 @@
+// Which kernel a product of 16-bit operands runs on.
+#pragma once
+#include "gemm16_kernel.h"
+
+namespace cch {
+
+// Tiles that a launch may have: the groups' sizes are on the device.
+inline int64_t tiles16(const Gemm16 &p, int tm, int tn)
+{
+    const int64_t cols = (p.n + tn - 1) / tn;
+    if (p.k_grouped) return (int64_t)p.groups * ((p.m + tm - 1) / tm) * cols;
+    return (p.group_sizes ? p.m / tm + std::min(p.groups, p.m) : (p.m + tm - 1) / tm) * cols;
+}
+
+template <class T, int LAYOUT, int EPI> int shape16(const Gemm16 &p, hipStream_t stream)
+{
+    using Mid = Shape16<2, 2, 2, 2, 2>;
+    return launch16<T, LAYOUT, EPI, Mid>(p, tiles16(p, Mid::TM, Mid::TN), stream);
+}
+
+template <class T> int choose16(const Gemm16 &p, int layout, int epilogue, hipStream_t stream)
+{
+    switch (layout * 4 + epilogue) {
+    case ROWS_NK * 4 + EPI16_OUT: return shape16<T, ROWS_NK, EPI16_OUT>(p, stream);
+    case ROWS_NN * 4 + EPI16_OUT: return shape16<T, ROWS_NN, EPI16_OUT>(p, stream);
+    case ROWS_TN * 4 + EPI16_OUT: return shape16<T, ROWS_TN, EPI16_OUT>(p, stream);
+    case ROWS_NK * 4 + EPI16_ACT: return shape16<T, ROWS_NK, EPI16_ACT>(p, stream);
+    case ROWS_NN * 4 + EPI16_ACT: return shape16<T, ROWS_NN, EPI16_ACT>(p, stream);
+    case ROWS_NK * 4 + EPI16_STATS: return shape16<T, ROWS_NK, EPI16_STATS>(p, stream);
+    case ROWS_NK * 4 + EPI16_GRAD: return shape16<T, ROWS_NK, EPI16_GRAD>(p, stream);
+    }
+    return fail(CCH_EINVAL, "no product of layout %d with epilogue %d", layout, epilogue);
+}
+
+}  // namespace cch

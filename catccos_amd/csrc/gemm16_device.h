@@ -1,0 +1,329 @@
+// What the kernels of 16-bit products share: types, the panels' way from memory through LDS to the matrix instructions' operands, the group table, the
+// activations, and the epilogues.
+#pragma once
+#include "gemm16.h"
+#include "gemm_device.h"
+
+namespace cch {
+
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+struct Bf16 {
+    using V8 = bf16x8;
+    static __device__ __forceinline__ v16f mfma(v4i a, v4i b, v16f c)
+    {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(V8, a), __builtin_bit_cast(V8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint16_t from(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }   // to nearest even
+    static __device__ __forceinline__ float to(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
+};
+struct F16 {
+    using V8 = f16x8;
+    static __device__ __forceinline__ v16f mfma(v4i a, v4i b, v16f c)
+    {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(V8, a), __builtin_bit_cast(V8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint16_t from(float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
+    static __device__ __forceinline__ float to(uint16_t v) { return (float)__builtin_bit_cast(_Float16, v); }
+};
+
+// ---- activations, fp32.  gelu_tanh(z) = z (1 + tanh u) / 2 with u = sqrt(2/pi) (z + 0.044715 z^3), which is z / (1 + exp(-2u)).
+__device__ __forceinline__ float sigmoid16(float v) { return __builtin_amdgcn_rcpf(1.0f + __expf(-v)); }
+constexpr float GELU_A = 1.5957691216057308f, GELU_B = 0.044715f;   // 2 sqrt(2/pi)
+__device__ __forceinline__ float act_value(float z, int act)
+{
+    switch (act) {
+    case CCH_ACT_RELU: return z < 0.0f ? 0.0f : z;
+    case CCH_ACT_SILU: return z * sigmoid16(z);
+    case CCH_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.7071067811865476f));
+    case CCH_ACT_GELU_TANH: return z * sigmoid16(GELU_A * (z + GELU_B * z * z * z));
+    default: return z;
+    }
+}
+__device__ __forceinline__ float act_slope(float z, int act)
+{
+    switch (act) {
+    case CCH_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
+    case CCH_ACT_SILU: {
+        const float s = sigmoid16(z), c = fminf(fmaxf(z, -1e3f), 1e3f);   // (c: past it s (1 - s) is 0, and infinity times it would not be)
+        return s + c * (s * (1.0f - s));
+    }
+    case CCH_ACT_GELU: {
+        const float c = fminf(fmaxf(z, -1e3f), 1e3f);
+        return 0.5f * (1.0f + erff(z * 0.7071067811865476f)) + c * 0.3989422804014327f * __expf(-0.5f * c * c);
+    }
+    case CCH_ACT_GELU_TANH: {
+        const float s = sigmoid16(GELU_A * (z + GELU_B * z * z * z)), c = fminf(fmaxf(z, -1e3f), 1e3f);
+        return s + c * (s * (1.0f - s)) * GELU_A * (1.0f + 3.0f * GELU_B * c * c);
+    }
+    default: return 1.0f;
+    }
+}
+
+// ---- groups.  start[g] .. start[g + 1]: group g's rows (or K); tile[g]: its first row tile among all groups'.
+struct GroupTable16 {
+    int start[MAX_GROUPS16 + 1];
+    int tile[MAX_GROUPS16 + 1];
+};
+// By one wave.  `all`: rows (or K) that there are; sizes are clipped to what the groups before leave.  bm: rows of a tile.
+__device__ inline void build_groups16(GroupTable16 &tab, const int32_t *sizes, int groups, int all, int bm)
+{
+    const int lane = threadIdx.x & 63;
+    uint32_t before = 0;
+    int tiles_before = 0;
+    for (int b = 0; b < groups; b += 64) {
+        const int g = b + lane;
+        uint32_t sz = 0;
+        if (g < groups) sz = sizes ? (uint32_t)min(max(sizes[g], 0), all) : (uint32_t)all;
+        const uint32_t incl = sat_add(before, wave_scan_sat(sz));
+        const uint32_t prev = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)incl, 0x138, 0xF, 0xF, false);   // the neighbour's: wave_shr:1
+        const int hi = (int)min(incl, (uint32_t)all), lo = (int)min(lane == 0 ? before : prev, (uint32_t)all);
+        const int tiles = (hi - lo + bm - 1) / bm;
+        const int tincl = (int)wave_scan_sat((uint32_t)tiles);
+        if (g < groups) {
+            tab.start[g] = lo;
+            tab.tile[g] = tiles_before + tincl - tiles;
+        }
+        before = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
+        tiles_before += __builtin_amdgcn_readlane(tincl, 63);
+    }
+    if (lane == 0) {
+        tab.start[groups] = (int)min(before, (uint32_t)all);
+        tab.tile[groups] = tiles_before;
+    }
+}
+// The last group whose first tile is not behind `t`: the one that t belongs to, as groups without tiles begin where the next one does.
+__device__ __forceinline__ int group_of_tile16(const GroupTable16 &tab, int groups, int t)
+{
+    int lo = 0, hi = groups;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (tab.tile[mid] <= t) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+// Place of the launch's t-th tile in the list of `total`: consecutive workgroups run on the 8 XCDs in turn, and each XCD takes a run of consecutive
+// tiles, so that its L2 sees neighbours.  -1: none.
+__device__ __forceinline__ int64_t place16(int64_t t, int64_t total)
+{
+    const int64_t per = (total + 7) >> 3, i = t >> 3, at = (t & 7) * per + i;
+    return i < per && at < total ? at : -1;
+}
+// Tiles are walked in bands of 8 row tiles, column by column: the 32 to 64 tiles that an XCD works on at a time then share 8 panels of A and 4 to 8 of B.
+constexpr int BAND16 = 8;
+__device__ __forceinline__ void tile_of16(int64_t at, int row_tiles, int col_tiles, int &rt, int &ct)
+{
+    const int64_t per = (int64_t)BAND16 * col_tiles;
+    const int band = (int)(at / per), in = (int)(at - band * per);
+    const int rows = min(BAND16, row_tiles - band * BAND16);
+    ct = in / rows;
+    rt = band * BAND16 + in - ct * rows;
+}
+
+// ---- panels.  A step is 64 elements of K.
+// K contiguous: a row is 128 bytes, its 16-byte chunk c at position c ^ ((row >> 1) & 7) (gemm_device.h).  Lane (r, g) of a 32 x 32 x 16 instruction holds
+// elements 8g..8g+7 of a sixteenth: chunk 2 kk + g.
+// K-major: a K-row is COLS * 2 bytes; a transposing LDS load hands 16 lanes four K-rows of 16 columns, lane i addressing columns 4 (i % 4) .. of row i / 4 and
+// receiving column i.  32 lanes, one pass of the load, touch 64 bytes of each of four rows that lie a multiple of 256 (or 128) bytes apart: the chunk
+// position's bit 2 and 3 (128 bytes: bit 2) are those of the chunk xor the row's, which puts them on all banks once.
+template <int COLS> struct KMajor {
+    static constexpr int ROW = COLS * 2, CHUNKS = COLS / 8, ROWS_PER_KIB = 512 / COLS;
+    static __device__ __forceinline__ uint32_t swizzle(int row) { return COLS >= 128 ? (uint32_t)(row & 3) << 2 : (uint32_t)((row >> 1) & 1) << 2; }
+};
+__device__ __forceinline__ v4i read_transposed(uint32_t addr, uint32_t row_bytes)
+{
+    typedef __attribute__((address_space(3))) v4s *P;
+    const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(uintptr_t)addr);
+    const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(uintptr_t)(addr + 4 * row_bytes));
+    const v2i l = __builtin_bit_cast(v2i, lo), h = __builtin_bit_cast(v2i, hi);
+    return (v4i){l[0], l[1], h[0], h[1]};
+}
+
+// A descriptor of what is left of a K-major operand from K-row k0 and column c0 on: the last of its `k` rows ends with its n-th column (the 16 bytes that hold it).
+__device__ __forceinline__ Rsrc kmajor_rsrc(const uint16_t *base, int64_t pitch, int k0, int k, int c0, int n)
+{
+    const int64_t left = k0 < k ? ((int64_t)(k - k0 - 1) * pitch + (((n + 7) & ~7) - c0)) * 2 : 0;
+    return make_rsrc(base + (int64_t)k0 * pitch + c0, (uint32_t)min(left, (int64_t)0x7FFFFFF0));
+}
+
+// ---- epilogues.  The matrix instructions take B's fragment first: lane (r, g) then holds, of a 32 x 32 block, row r and columns 8 q + 4 g + x at 4 q + x.  Two swaps
+// between the wave's halves make that columns 16 h + 8 g + 0..7 of half h, 16 bytes of output to a lane.
+__device__ __forceinline__ void eight_columns(const v16f &acc, float v[2][8])
+{
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+            const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[8 * h + x]), __float_as_uint(acc[8 * h + 4 + x]), false, false);
+            v[h][x] = __uint_as_float(s[0]);
+            v[h][4 + x] = __uint_as_float(s[1]);
+        }
+}
+template <class T> __device__ __forceinline__ v4i pack8(const float v[8])
+{
+    v4i o;
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = (int)((uint32_t)T::from(v[2 * i]) | (uint32_t)T::from(v[2 * i + 1]) << 16);
+    return o;
+}
+template <class T> __device__ __forceinline__ void unpack8(v4i o, float v[8])
+{
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        v[2 * i] = T::to((uint16_t)(uint32_t)o[i]);
+        v[2 * i + 1] = T::to((uint16_t)((uint32_t)o[i] >> 16));
+    }
+}
+// Eight elements at p, of which the first `there` (1..8) exist; `whole`: all eight do, on a 16-byte boundary.
+template <class T> __device__ __forceinline__ void load8(const uint16_t *p, bool whole, int there, float v[8])
+{
+    if (whole) {
+        unpack8<T>(*reinterpret_cast<const v4i *>(p), v);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = i < there ? T::to(p[i]) : 0.0f;
+}
+template <class T> __device__ __forceinline__ void store8(uint16_t *p, bool whole, int there, const float v[8])
+{
+    const v4i o = pack8<T>(v);
+    if (whole) {
+        *reinterpret_cast<v4i *>(p) = o;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        if (i < there) p[i] = (uint16_t)((uint32_t)o[i >> 1] >> (16 * (i & 1)));
+}
+
+__device__ __forceinline__ bool whole_rows(const Gemm16 &p);
+
+// The results of one wave: MT x NT blocks of 32 x 32 from row m0 and column n0 of the product on, of which rows below m_end exist.  group: the output that K-grouped
+// problems write.
+template <class T, int EPI, int MT, int NT>
+__device__ __forceinline__ void epilogue16(const Gemm16 &p, v16f (&acc)[MT][NT], int group, int m0, int m_end, int n0)
+{
+    const int lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5;
+    if constexpr (EPI == EPI16_STATS) {
+        // 64 columns' largest logit and sum of exponentials (NT is 2, or 1 for 32 columns), the two halves of the wave joined; a target's logit on the way
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+            const int m = m0 + 32 * i + r;
+            const bool there = m < m_end;
+            const int want = there ? p.targets[m] - p.v0 - n0 - 4 * g : -1;
+            float top = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+                for (int x = 0; x < 16; x++) {
+                    const int c = 32 * j + 8 * (x >> 2) + (x & 3);
+                    if (n0 + c + 4 * g >= p.n) acc[i][j][x] = -INFINITY;
+                    top = fmaxf(top, acc[i][j][x]);
+                    if (c == want) p.target_logit[m] = acc[i][j][x];
+                }
+            top = fmaxf(top, __shfl_xor(top, 32));
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+                for (int x = 0; x < 16; x++) sum += __expf(acc[i][j][x] - top);
+            sum += __shfl_xor(sum, 32);
+            if (there && g == 0 && n0 < p.n) p.stats[(int64_t)m * p.stat_cols + (p.v0 + n0) / (32 * NT)] = make_float2(top, sum);
+        }
+        return;
+    } else {
+        const bool rows_whole = whole_rows(p);
+        const float scale = EPI == EPI16_OUT && p.scale ? *p.scale : 1.0f;
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+            const int m = m0 + 32 * i + r;
+            const bool there = m < m_end;
+            int64_t row = m;
+            float lse = 0.0f, slope = 0.0f;
+            int target = -1;
+            if (EPI == EPI16_OUT && p.out_rows) row = there ? p.out_rows[m] : 0;
+            if (EPI == EPI16_GRAD) {
+                lse = there ? p.lse[m] : 0.0f;
+                slope = (1.0f + p.z2 * lse) * p.grad_scale;
+                target = there ? p.targets[m] - p.v0 : -1;
+            }
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+                float v[2][8];
+                eight_columns(acc[i][j], v);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int n = n0 + 32 * j + 16 * h + 8 * g;
+                    const int left = p.n - n;
+                    if (!there || left <= 0) continue;
+                    const bool whole = rows_whole && left >= 8;
+                    if constexpr (EPI == EPI16_OUT) {
+                        if (p.sums) {
+                            float *s = p.sums + (int64_t)m * p.n + n;
+#pragma unroll
+                            for (int x = 0; x < 8; x++)
+                                if (x < left) {
+                                    if (p.sums_in) v[h][x] += s[x];
+                                    if (p.sums_out) s[x] = v[h][x];
+                                }
+                            if (p.sums_out) continue;
+                        }
+#pragma unroll
+                        for (int x = 0; x < 8; x++) v[h][x] *= scale;
+                        store8<T>(p.out + (int64_t)group * p.out_stride + row * p.pitch_out + n, whole, left, v[h]);
+                    } else if constexpr (EPI == EPI16_ACT) {
+                        if (p.bias) {
+                            float b[8];
+                            load8<T>(p.bias + n, whole, left, b);
+#pragma unroll
+                            for (int x = 0; x < 8; x++) v[h][x] += b[x];
+                        }
+                        const int64_t at = row * p.pitch_out + n;
+                        if (p.preact) store8<T>(p.preact + at, whole, left, v[h]);
+#pragma unroll
+                        for (int x = 0; x < 8; x++) v[h][x] = act_value(v[h][x], p.act);
+                        if (p.residual) {
+                            float b[8];
+                            load8<T>(p.residual + at, whole, left, b);
+#pragma unroll
+                            for (int x = 0; x < 8; x++) v[h][x] += b[x];
+                        }
+                        store8<T>(p.out + at, whole, left, v[h]);
+                    } else {
+                        // rows of the gradient end on 16-byte boundaries, zeros behind the last column: the next product reads it along K
+#pragma unroll
+                        for (int x = 0; x < 8; x++) {
+                            const float d = __expf(v[h][x] - lse) * slope - (n + x == target ? p.grad_scale : 0.0f);
+                            v[h][x] = x < left ? d : 0.0f;
+                        }
+                        store8<T>(p.out + row * p.pitch_out + n, true, 8, v[h]);
+                    }
+                }
+            }
+        }
+    }
+}
+// Whether the epilogue's tensors have rows on 16-byte boundaries.
+__device__ __forceinline__ bool whole_rows(const Gemm16 &p)
+{
+    return p.pitch_out % 8 == 0 && ((uintptr_t)p.out & 15) == 0 && p.out_stride % 8 == 0 && (((uintptr_t)p.bias | (uintptr_t)p.residual | (uintptr_t)p.preact) & 15) == 0;
+}
+
+// Rows behind the last group: zeros.
+__device__ __forceinline__ void zero_rest16(const Gemm16 &p, int first)
+{
+    const int64_t begin = (int64_t)first * p.pitch_out, end = (int64_t)p.m * p.pitch_out, threads = (int64_t)gridDim.x * blockDim.x;
+    const int64_t me = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (((uintptr_t)p.out & 15) == 0 && p.pitch_out % 8 == 0) {
+        v4i *o = reinterpret_cast<v4i *>(p.out);
+        for (int64_t i = begin / 8 + me; i < end / 8; i += threads) o[i] = (v4i){0, 0, 0, 0};
+    } else {
+        for (int64_t i = begin + me; i < end; i += threads) p.out[i] = 0;
+    }
+}
+
+}  // namespace cch

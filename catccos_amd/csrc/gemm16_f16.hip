@@ -1,0 +1,8 @@
+// Instantiations of gemm16_kernel.h: IEEE half.
+#include "gemm16_choose.h"
+
+namespace cch {
+
+int gemm16_launch_f16(const Gemm16 &p, int layout, int epilogue, hipStream_t stream) { return choose16<F16>(p, layout, epilogue, stream); }
+
+}  // namespace cch

@@ -1,0 +1,185 @@
+// Products of 16-bit operands on tiles of (32 MT WM) x (32 NT WN): WM x WN waves of MT x NT blocks of 32 x 32, K in steps of 64 elements, two stages in LDS that
+// are filled straight from memory.  A step's requests are issued before the step before it is multiplied; one barrier a step publishes what has landed and
+// frees what was read.  Two workgroups of the 128 x 128 form share a CU, so that one's epilogue and waits pass under the other's matrix instructions.
+#pragma once
+#include <atomic>
+
+#include "gemm16_device.h"
+
+namespace cch {
+
+template <int MT_, int NT_, int WM_, int WN_, int PER_CU_> struct Shape16 {
+    static constexpr int MT = MT_, NT = NT_, WM = WM_, WN = WN_, WAVES = WM * WN, THREADS = 64 * WAVES, PER_CU = PER_CU_;
+    static constexpr int TM = 32 * MT * WM, TN = 32 * NT * WN;      // tile
+    static constexpr int A_BYTES = TM * 128, B_BYTES = TN * 128, STAGE = A_BYTES + B_BYTES, LDS = 2 * STAGE;
+    static constexpr int NJA = A_BYTES / 1024 / WAVES, NJB = B_BYTES / 1024 / WAVES;   // requests of a wave and step
+};
+
+template <class T, int LAYOUT, int EPI, class S>
+__global__ __launch_bounds__(S::THREADS, S::PER_CU * S::WAVES / 4) void gemm16_kernel(Gemm16 p)
+{
+    constexpr bool A_KM = LAYOUT == ROWS_TN, B_KM = LAYOUT != ROWS_NK;   // K-major operands
+    constexpr int MT = S::MT, NT = S::NT, NJA = S::NJA, NJB = S::NJB;
+    using KA = KMajor<S::TM>;
+    using KB = KMajor<S::TN>;
+    __shared__ GroupTable16 tab;
+    const bool rows_grouped = !p.k_grouped;
+    if (threadIdx.x < 64) build_groups16(tab, p.group_sizes, p.groups, rows_grouped ? p.m : p.k, S::TM);
+    __syncthreads();
+    if (p.zero_rest) zero_rest16(p, tab.start[p.groups]);
+
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), wm = wave / S::WN, wn = wave % S::WN;
+    const int r = lane & 31, g = lane >> 5, tq = lane >> 4, ti = lane & 15;
+    const uint32_t lds = (uint32_t)uniform((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)smem);
+    const int col_tiles = (p.n + S::TN - 1) / S::TN;
+    const int row_tiles = uniform(rows_grouped ? tab.tile[p.groups] : (p.m + S::TM - 1) / S::TM);
+    const int64_t total = (int64_t)row_tiles * col_tiles * (rows_grouped ? 1 : p.groups);
+
+    // this lane's fragment reads in stage 0
+    uint32_t fr_a[4], fr_b[4], ft_a[MT], ft_b[NT];
+#pragma unroll
+    for (int kk = 0; kk < 4; kk++) {
+        const uint32_t chunk = ((uint32_t)(2 * kk + g) ^ swizzle_of_row(r)) << 4;
+        fr_a[kk] = lds + (uint32_t)(wm * MT * 32 + r) * 128u + chunk;
+        fr_b[kk] = lds + S::A_BYTES + (uint32_t)(wn * NT * 32 + r) * 128u + chunk;
+    }
+    const int krow = (tq >> 1) * 8 + (ti >> 2);                                 // (and 4 more by the second load)
+    const uint32_t part = (uint32_t)((tq & 1) * 2 + ((ti & 3) >> 1));           // chunk among a block's four
+#pragma unroll
+    for (int i = 0; i < MT; i++) ft_a[i] = lds + (uint32_t)krow * KA::ROW + ((((uint32_t)(wm * MT + i) * 4 + part) ^ KA::swizzle(krow)) << 4) + (ti & 1) * 8u;
+#pragma unroll
+    for (int j = 0; j < NT; j++)
+        ft_b[j] = lds + S::A_BYTES + (uint32_t)krow * KB::ROW + ((((uint32_t)(wn * NT + j) * 4 + part) ^ KB::swizzle(krow)) << 4) + (ti & 1) * 8u;
+
+    for (int64_t t = blockIdx.x; t < ((total + 7) & ~(int64_t)7); t += gridDim.x) {
+        int64_t at = place16(t, total);
+        if (at < 0) continue;
+        int e = 0, rt, ct, m0, m_end, k_begin = 0, k_end = p.k;
+        if (rows_grouped) {
+            tile_of16(at, row_tiles, col_tiles, rt, ct);
+            e = uniform(group_of_tile16(tab, p.groups, rt));
+            m0 = uniform(tab.start[e] + (rt - tab.tile[e]) * S::TM);
+            m_end = uniform(tab.start[e + 1]);
+        } else {
+            const int64_t per = (int64_t)row_tiles * col_tiles;
+            e = (int)(at / per);
+            tile_of16(at - e * per, row_tiles, col_tiles, rt, ct);
+            m0 = rt * S::TM;
+            m_end = p.m;
+            k_begin = uniform(tab.start[e]);
+            k_end = uniform(tab.start[e + 1]);
+        }
+        const int n0 = ct * S::TN;
+        const int rows = min(m_end - m0, S::TM), cols = min(p.n - n0, S::TN), kk_all = k_end - k_begin;
+        const int steps = (kk_all + 63) >> 6;
+
+        // requests: descriptors and this lane's offsets
+        uint32_t off_a[NJA], off_b[NJB];
+        Rsrc rs_a{}, rs_b{};
+        const int k8 = (p.k + 7) & ~7;   // (rows of other lengths are padded with zeros)
+        const uint16_t *a0 = p.a + (A_KM ? (int64_t)k_begin * p.pitch_a : p.a_rows ? 0 : (int64_t)m0 * p.pitch_a);
+        const uint16_t *b0 = p.b + (rows_grouped ? (int64_t)e * p.b_stride : (int64_t)0) + (B_KM ? (int64_t)k_begin * p.pitch_b : (int64_t)n0 * p.pitch_b);
+        if constexpr (!A_KM) {
+            const int last = p.a_rows ? p.m_src - 1 : rows - 1;
+            rs_a = make_rsrc(a0, (uint32_t)min(((int64_t)last * p.pitch_a + k8) * 2, (int64_t)0x7FFFFFF0));
+        }
+        if constexpr (!B_KM) rs_b = make_rsrc(b0, (uint32_t)min(((int64_t)(cols - 1) * p.pitch_b + k8) * 2, (int64_t)0x7FFFFFF0));
+#pragma unroll
+        for (int j = 0; j < NJA; j++) {
+            if constexpr (A_KM) {
+                const int kr = (wave * NJA + j) * KA::ROWS_PER_KIB + lane / KA::CHUNKS;
+                off_a[j] = (uint32_t)kr * (uint32_t)p.pitch_a * 2u + (((uint32_t)(lane % KA::CHUNKS) ^ KA::swizzle(kr)) << 4);
+            } else {
+                const int row = (wave * NJA + j) * 8 + (lane >> 3);
+                uint32_t src = (uint32_t)row;
+                if (p.a_rows) src = row < rows ? (uint32_t)p.a_rows[m0 + row] : 0u;
+                off_a[j] = row < rows ? src * (uint32_t)p.pitch_a * 2u + (((uint32_t)(lane & 7) ^ swizzle_of_row(row)) << 4) : NO_FETCH;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NJB; j++) {
+            if constexpr (B_KM) {
+                const int kr = (wave * NJB + j) * KB::ROWS_PER_KIB + lane / KB::CHUNKS;
+                off_b[j] = (uint32_t)kr * (uint32_t)p.pitch_b * 2u + (((uint32_t)(lane % KB::CHUNKS) ^ KB::swizzle(kr)) << 4);
+            } else {
+                const int row = (wave * NJB + j) * 8 + (lane >> 3);
+                off_b[j] = row < cols ? (uint32_t)row * (uint32_t)p.pitch_b * 2u + (((uint32_t)(lane & 7) ^ swizzle_of_row(row)) << 4) : NO_FETCH;
+            }
+        }
+        // (K contiguous: a lane whose 8 elements begin at or past K fetches nothing; K is a multiple of 8 or its rows are padded with zeros)
+        auto request = [&](int step) {
+            const uint32_t stage = lds + (uint32_t)(step & 1) * S::STAGE;
+            const int k0 = step * 64;
+            if constexpr (A_KM) rs_a = kmajor_rsrc(a0, p.pitch_a, k0, kk_all, m0, p.m);
+            if constexpr (B_KM) rs_b = kmajor_rsrc(b0, p.pitch_b, k0, kk_all, n0, p.n);
+#pragma unroll
+            for (int j = 0; j < NJA; j++) {
+                const int row = (wave * NJA + j) * 8 + (lane >> 3);
+                const bool in = A_KM || (int)(((uint32_t)(lane & 7) ^ swizzle_of_row(row)) * 8u) < p.k - k0;
+                load16_to_lds(rs_a, in ? off_a[j] : NO_FETCH, A_KM ? 0u : (uint32_t)k0 * 2u, stage + (uint32_t)(wave * NJA + j) * 1024u);
+            }
+#pragma unroll
+            for (int j = 0; j < NJB; j++) {
+                const int row = (wave * NJB + j) * 8 + (lane >> 3);
+                const bool in = B_KM || (int)(((uint32_t)(lane & 7) ^ swizzle_of_row(row)) * 8u) < p.k - k0;
+                load16_to_lds(rs_b, in ? off_b[j] : NO_FETCH, B_KM ? 0u : (uint32_t)k0 * 2u, stage + S::A_BYTES + (uint32_t)(wave * NJB + j) * 1024u);
+            }
+        };
+
+        v16f acc[MT][NT];
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int j = 0; j < NT; j++) acc[i][j] = (v16f)(0.0f);
+        if (steps > 0) request(0);
+        for (int step = 0; step < steps; step++) {
+            CCH_WAIT_VM_LGKM0(0);
+            CCH_BARRIER();
+            if (step + 1 < steps) request(step + 1);
+            const uint32_t stage = (uint32_t)(step & 1) * S::STAGE;
+#pragma unroll
+            for (int kk = 0; kk < 4; kk++) {
+                v4i fa[MT], fb[NT];
+#pragma unroll
+                for (int j = 0; j < NT; j++)
+                    fb[j] = B_KM ? read_transposed(ft_b[j] + stage + (uint32_t)kk * 16u * KB::ROW, KB::ROW) : lds_read16_abs(fr_b[kk] + stage + (uint32_t)j * 4096u);
+#pragma unroll
+                for (int i = 0; i < MT; i++)
+                    fa[i] = A_KM ? read_transposed(ft_a[i] + stage + (uint32_t)kk * 16u * KA::ROW, KA::ROW) : lds_read16_abs(fr_a[kk] + stage + (uint32_t)i * 4096u);
+#pragma unroll
+                for (int i = 0; i < MT; i++)
+#pragma unroll
+                    for (int j = 0; j < NT; j++) acc[i][j] = T::mfma(fb[j], fa[i], acc[i][j]);
+            }
+        }
+        CCH_WAIT_LGKM0();
+        CCH_BARRIER();   // (the next tile's requests overwrite the stages)
+        epilogue16<T, EPI, MT, NT>(p, acc, e, m0 + wm * MT * 32, m_end, n0 + wn * NT * 32);
+    }
+}
+
+// Lets a kernel have more than 64 KB of LDS: once per device; doing it twice from two threads is harmless.
+inline int allow_lds16(const void *kernel, int bytes, std::atomic<uint64_t> &done)
+{
+    int dev = 0;
+    CCH_HIP(hipGetDevice(&dev));
+    const uint64_t bit = (uint64_t)1 << (dev & 63);
+    if (dev >= 64 || !(done.load(std::memory_order_acquire) & bit)) {
+        CCH_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        done.fetch_or(bit, std::memory_order_release);
+    }
+    return CCH_OK;
+}
+
+template <class T, int LAYOUT, int EPI, class S> int launch16(const Gemm16 &p, int64_t tiles, hipStream_t stream)
+{
+    static_assert(S::A_BYTES % (1024 * S::WAVES) == 0 && S::B_BYTES % (1024 * S::WAVES) == 0, "whole requests");
+    static std::atomic<uint64_t> attr_set{0};
+    auto kernel = gemm16_kernel<T, LAYOUT, EPI, S>;
+    if (const int rc = allow_lds16(reinterpret_cast<const void *>(kernel), S::LDS, attr_set)) return rc;
+    const int64_t grid = std::min<int64_t>((tiles + 7) & ~(int64_t)7, (int64_t)1 << 22);   // (a multiple of 8: place16)
+    kernel<<<dim3((uint32_t)grid), dim3(S::THREADS), S::LDS, stream>>>(p);
+    return launch_status("gemm16_kernel");
+}
+
+}  // namespace cch

@@ -14,8 +14,8 @@ import torch
 from torch.autograd import forward_ad as _forward_ad
 
 from . import _abi
-from ._abi import (DTYPE_BF16, DTYPE_F16, DTYPE_F32, FMT_E1M2, FMT_E2M1, FMT_E4M3, FMT_E5M2, FMT_INT4, ROUND_LUT, ROUND_RNE, SCORING_SIGMOID,
-                   SCORING_SOFTMAX, check)
+from ._abi import (ACT_GELU, ACT_GELU_TANH, ACT_NONE, ACT_RELU, ACT_SILU, DTYPE_BF16, DTYPE_F16, DTYPE_F32, FMT_E1M2, FMT_E2M1, FMT_E4M3, FMT_E5M2, FMT_INT4, REDUCE_MEAN, REDUCE_SUM, ROUND_LUT, ROUND_RNE,
+                   SCORING_SIGMOID, SCORING_SOFTMAX, check)
 
 _FMT_NAMES = {"e4m3": FMT_E4M3, "e5m2": FMT_E5M2, "e2m1": FMT_E2M1, "e1m2": FMT_E1M2, "fp8": FMT_E4M3, "fp4": FMT_E2M1}
 _FP4 = (FMT_E2M1, FMT_E1M2)   # two codes per byte; E1M2 exists for the quantiser only
@@ -816,3 +816,267 @@ def moe_ffn_w4a16(x, expert_idx, probs, w1, scales1, zeros1, w2, scales2, zeros2
     check(_abi.lib().cch_moe_ffn_w4a16(_ptr(x), _ptr(expert_idx), _ptr(probs), _ptr(w1), _ptr(scales1), _ptr(zeros1), _ptr(w2), _ptr(scales2), _ptr(zeros2), _ptr(out),
                                        m, k, top_k, e, n, fmt, int(group_size), _DTYPES[x.dtype], _ptr(ws), ws.numel(), _stream()))
     return out
+
+
+_ACTIVATIONS = {"none": ACT_NONE, "relu": ACT_RELU, "silu": ACT_SILU, "gelu": ACT_GELU, "gelu_tanh": ACT_GELU_TANH}
+_REDUCTIONS = {"mean": REDUCE_MEAN, "sum": REDUCE_SUM}
+
+
+def _activation(activation):
+    if activation not in _ACTIVATIONS:
+        raise ValueError("unknown activation %r (%s)" % (activation, ", ".join(_ACTIVATIONS)))
+    return _ACTIVATIONS[activation]
+
+
+def _reduction(reduction):
+    if reduction not in _REDUCTIONS:
+        raise ValueError("unknown reduction %r (mean or sum)" % (reduction,))
+    return _REDUCTIONS[reduction]
+
+
+def _one_device(name, first, *others):
+    _require_gpu(first, *others)
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError("%s: tensors on %s and %s" % (name, first.device, t.device))
+
+
+def _whole(t):
+    """t contiguous and on a 16-byte boundary, as the products' requests want their operands."""
+    if t is None:
+        return None
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _launch16(name, device, nbytes, *args):
+    """One library call on `device`'s current stream, its workspace between the arguments and the stream."""
+    with torch.cuda.device(device):
+        ws = torch.empty(int(nbytes), dtype=torch.uint8, device=device)
+        check(getattr(_abi.lib(), name)(*args, _ptr(ws), ws.numel(), _stream()))
+
+
+def _check_x16(x, what="x"):
+    if x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("%s must be a 2-D bfloat16 or float16 tensor" % what)
+
+
+def _check_grouped(x, w, group_sizes, trans_b):
+    _check_x16(x)
+    if w.dim() != 3 or w.dtype != x.dtype:
+        raise ValueError("w must be a 3-D tensor of x's type")
+    if trans_b not in (0, 1):
+        raise ValueError("trans_b must be 0 or 1")
+    e, k, n = w.shape[0], w.shape[2] if trans_b else w.shape[1], w.shape[1] if trans_b else w.shape[2]
+    if x.shape[1] != k:
+        raise ValueError("inner dimensions differ: x has %d columns, w %d" % (x.shape[1], k))
+    if group_sizes.dtype != torch.int32 or tuple(group_sizes.shape) != (e,):
+        raise ValueError("group_sizes must be an int32 tensor with one entry per expert")
+    return e, x.shape[0], n, k
+
+
+def grouped_matmul(x, w, group_sizes, trans_b=0):
+    """Tokens sorted by expert times their expert's weights, in 16 bits: what mx_grouped_matmul and gmm_dequant_swiglu are to quantised operands, for
+    training and for weights that stay as they are.
+
+    x [T, K] bf16 or half, rows of an expert back to back in expert order (moe_init_routing's); w of x's type, [E, K, N] or with trans_b=1 [E, N, K], up to 1024
+    experts; group_sizes int32 [E] on the GPU.  Returns [T, N] in x's type, sums in fp32, zeros behind the last group.  Differentiable in x and w, in reverse mode."""
+    _one_device("grouped_matmul", x, w, group_sizes)
+    e, t, n, k = _check_grouped(x, w, group_sizes, trans_b)
+    _no_tangent("grouped_matmul", x, w)
+    if _recorded(x) or _recorded(w):
+        return _GroupedMatmul.apply(x, w, group_sizes, trans_b)   # (comes back here without the record)
+    x, w, group_sizes = _whole(x), _whole(w), group_sizes.contiguous()
+    out = torch.empty((t, n), dtype=x.dtype, device=x.device)
+    nbytes = _abi.lib().cch_grouped_matmul_workspace_bytes(e, t, n, k, trans_b)
+    _launch16("cch_grouped_matmul", x.device, nbytes, _ptr(x), _ptr(w), _ptr(group_sizes), _ptr(out), e, t, n, k, trans_b, _DTYPES[x.dtype])
+    return out
+
+
+def grouped_matmul_backward(grad_out, x, w, group_sizes, trans_b=0, x_grad=True, w_grad=True):
+    """The gradients of grouped_matmul: (grad_x [T, K], zeros behind the last group, grad_w in w's layout, zeros for an expert without rows), each None
+    where it is not asked for.  What autograd calls; for programs that do without it."""
+    _one_device("grouped_matmul_backward", x, grad_out, w, group_sizes)
+    e, t, n, k = _check_grouped(x, w, group_sizes, trans_b)
+    if grad_out.dtype != x.dtype or tuple(grad_out.shape) != (t, n):
+        raise ValueError("grad_out must be a tensor [%d, %d] of x's type" % (t, n))
+    grad_out, x, w, group_sizes = _whole(grad_out), _whole(x), _whole(w), group_sizes.contiguous()
+    grad_x = torch.empty_like(x) if x_grad else None
+    grad_w = torch.empty_like(w) if w_grad else None
+    nbytes = _abi.lib().cch_grouped_matmul_backward_workspace_bytes(e, t, n, k, trans_b)
+    _launch16("cch_grouped_matmul_backward", x.device, nbytes, _ptr(grad_out), _ptr(x), _ptr(w), _ptr(group_sizes), _ptr(grad_x), _ptr(grad_w), e, t, n, k, trans_b,
+              _DTYPES[x.dtype])
+    return grad_x, grad_w
+
+
+class _GroupedMatmul(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, group_sizes, trans_b):
+        ctx.save_for_backward(x, w, group_sizes)
+        ctx.trans_b = trans_b
+        return grouped_matmul(x.detach(), w.detach(), group_sizes, trans_b)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, w, group_sizes = ctx.saved_tensors
+        return grouped_matmul_backward(grad, x, w, group_sizes, ctx.trans_b, ctx.needs_input_grad[0], ctx.needs_input_grad[1]) + (None, None)
+
+
+def _check_layer(x, w, trans_b):
+    _check_x16(x)
+    if w.dim() != 2 or w.dtype != x.dtype:
+        raise ValueError("w must be a 2-D tensor of x's type")
+    if trans_b not in (0, 1):
+        raise ValueError("trans_b must be 0 or 1")
+    k, n = (w.shape[1], w.shape[0]) if trans_b else w.shape
+    if x.shape[1] != k:
+        raise ValueError("inner dimensions differ: x has %d columns, w %d" % (x.shape[1], k))
+    return x.shape[0], n, k
+
+
+def matmul_bias_act(x, w, bias=None, residual=None, activation="none", trans_b=0, return_preact=False):
+    """A dense layer in one launch: act(x W + bias) + residual, [M, N] in x's type, sums in fp32, rounded once.
+
+    x [M, K] bf16 or half; w of x's type, [K, N] or with trans_b=1 [N, K]; bias [N] and residual [M, N] of x's type or None; activation "none", "relu", "silu", "gelu" (erf) or
+    "gelu_tanh".  With return_preact returns (out, x W + bias rounded to x's type), what matmul_bias_act_backward takes.  Differentiable in x, w, bias and residual, in reverse
+    mode, through out alone (the activation's slope is taken at the rounded x W + bias)."""
+    _one_device("matmul_bias_act", x, w, bias, residual)
+    m, n, k = _check_layer(x, w, trans_b)
+    act = _activation(activation)
+    if bias is not None and (bias.dtype != x.dtype or tuple(bias.shape) != (n,)):
+        raise ValueError("bias must be a tensor [%d] of x's type" % n)
+    if residual is not None and (residual.dtype != x.dtype or tuple(residual.shape) != (m, n)):
+        raise ValueError("residual must be a tensor [%d, %d] of x's type" % (m, n))
+    given = [t for t in (x, w, bias, residual) if t is not None]
+    _no_tangent("matmul_bias_act", *given)
+    if any(_recorded(t) for t in given):
+        out, preact = _MatmulBiasAct.apply(x, w, bias, residual, activation, trans_b, return_preact)
+        return (out, preact) if return_preact else out
+    x, w = _whole(x), _whole(w)
+    bias, residual = (None if t is None else t.contiguous() for t in (bias, residual))
+    out = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    preact = torch.empty_like(out) if return_preact else None
+    nbytes = _abi.lib().cch_matmul_bias_act_workspace_bytes(m, n, k, trans_b)
+    _launch16("cch_matmul_bias_act", x.device, nbytes, _ptr(x), _ptr(w), _ptr(bias), _ptr(residual), _ptr(preact), _ptr(out), m, n, k, trans_b, act, _DTYPES[x.dtype])
+    return (out, preact) if return_preact else out
+
+
+def matmul_bias_act_backward(grad_out, x, w, preact=None, activation="none", trans_b=0, x_grad=True, w_grad=True, bias_grad=True):
+    """The gradients of matmul_bias_act: (grad_x, grad_w in w's layout, grad_bias), in x's type, each None where it is not asked for; the residual's is grad_out.
+    preact as matmul_bias_act returned it, None without an activation.  grad_out * act'(preact) is rounded to x's type before the products and not before the bias' sum.
+    What autograd calls; for programs that do without it."""
+    _one_device("matmul_bias_act_backward", x, grad_out, w, preact)
+    m, n, k = _check_layer(x, w, trans_b)
+    act = _activation(activation)
+    if grad_out.dtype != x.dtype or tuple(grad_out.shape) != (m, n):
+        raise ValueError("grad_out must be a tensor [%d, %d] of x's type" % (m, n))
+    if act == ACT_NONE:
+        preact = None
+    elif preact is None or preact.dtype != x.dtype or tuple(preact.shape) != (m, n):
+        raise ValueError("preact must be a tensor [%d, %d] of x's type" % (m, n))
+    grad_out, x, w = _whole(grad_out), _whole(x), _whole(w)
+    preact = None if preact is None else preact.contiguous()
+    grad_x = torch.empty_like(x) if x_grad else None
+    grad_w = torch.empty_like(w) if w_grad else None
+    grad_bias = torch.empty((n,), dtype=x.dtype, device=x.device) if bias_grad else None
+    nbytes = _abi.lib().cch_matmul_bias_act_backward_workspace_bytes(m, n, k, trans_b, act)
+    _launch16("cch_matmul_bias_act_backward", x.device, nbytes, _ptr(grad_out), _ptr(x), _ptr(w), _ptr(preact), _ptr(grad_x), _ptr(grad_w), _ptr(grad_bias), m, n, k, trans_b, act,
+              _DTYPES[x.dtype])
+    return grad_x, grad_w, grad_bias
+
+
+class _MatmulBiasAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, bias, residual, activation, trans_b, return_preact):
+        keep = activation != "none" and any(ctx.needs_input_grad[:3])
+        out = matmul_bias_act(x.detach(), w.detach(), None if bias is None else bias.detach(), None if residual is None else residual.detach(), activation, trans_b,
+                              keep or return_preact)
+        out, preact = out if keep or return_preact else (out, None)
+        ctx.save_for_backward(x, w, preact if keep else None)
+        ctx.options = (activation, trans_b)
+        ctx.set_materialize_grads(False)
+        if preact is not None:
+            ctx.mark_non_differentiable(preact)
+        return out, preact
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad, _):
+        if grad is None:
+            return (None,) * 7
+        x, w, preact = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        got = matmul_bias_act_backward(grad, x, w, preact, *ctx.options, *need[:3]) if any(need[:3]) else (None,) * 3
+        return got + (grad if need[3] else None, None, None, None)
+
+
+def _check_ce(x, w, targets):
+    _check_x16(x)
+    if w.dim() != 2 or w.dtype != x.dtype or w.shape[1] != x.shape[1]:
+        raise ValueError("w must be a tensor [vocabulary, %d] of x's type" % x.shape[1])
+    if targets.dtype not in (torch.int32, torch.int64) or tuple(targets.shape) != (x.shape[0],):
+        raise ValueError("targets must be an int64 or int32 tensor [tokens]")
+    return x.shape[0], x.shape[1], w.shape[0]
+
+
+def linear_cross_entropy(x, w, targets, reduction="mean", z_coef=0.0):
+    """Softmax cross entropy of hidden states against an output projection, without the logits x w^T ever being kept.
+
+    x [T, H] bf16 or half; w [V, H] of its type; targets int64 or int32 [T]: a token whose target lies outside 0..V-1 (such as -100) does not count, whatever its row of x
+    holds.  Returns (loss float32 [], nll float32 [T], lse float32 [T], tokens int32 [1]): nll = lse - the target's logit with lse = log sum exp of the
+    logits, both 0 for tokens that do not count, tokens how many do, loss the mean (or with reduction "sum" the sum) over them of nll + z_coef * lse^2, 0 if there are
+    none.  loss is differentiable in x and w, in reverse mode.  The same inputs give the same bits."""
+    _one_device("linear_cross_entropy", x, w, targets)
+    t, h, v = _check_ce(x, w, targets)
+    red = _reduction(reduction)
+    _no_tangent("linear_cross_entropy", x, w)
+    if _recorded(x) or _recorded(w):
+        return _LinearCrossEntropy.apply(x, w, targets, reduction, z_coef)
+    x, w, targets = _whole(x), _whole(w), targets.contiguous()
+    loss = torch.empty((), dtype=torch.float32, device=x.device)
+    nll = torch.empty((t,), dtype=torch.float32, device=x.device)
+    lse = torch.empty_like(nll)
+    tokens = torch.empty((1,), dtype=torch.int32, device=x.device)
+    nbytes = _abi.lib().cch_linear_cross_entropy_workspace_bytes(t, h, v)
+    _launch16("cch_linear_cross_entropy", x.device, nbytes, _ptr(x), _ptr(w), _ptr(targets), targets.element_size(), _ptr(loss), _ptr(nll), _ptr(lse), _ptr(tokens), t, h, v, red,
+              float(z_coef), _DTYPES[x.dtype])
+    return loss, nll, lse, tokens
+
+
+def linear_cross_entropy_backward(grad_loss, x, w, targets, lse, tokens, reduction="mean", z_coef=0.0, x_grad=True, w_grad=True):
+    """The gradients of linear_cross_entropy's loss: (grad_x [T, H], grad_w [V, H]) in x's type, each None where it is not asked for.  grad_loss float32 [] on the GPU; lse and
+    tokens as linear_cross_entropy returned them (a mean divides by tokens: a program that shares a batch between GPUs may give all of theirs), the options as
+    they were given to it.  The logits' gradient is computed a piece of the vocabulary at a time and rounded to x's type.  What autograd calls."""
+    _one_device("linear_cross_entropy_backward", x, grad_loss, w, targets, lse, tokens)
+    t, h, v = _check_ce(x, w, targets)
+    red = _reduction(reduction)
+    if grad_loss.dtype != torch.float32 or grad_loss.numel() != 1:
+        raise ValueError("grad_loss must be one float32 value")
+    if lse.dtype != torch.float32 or tuple(lse.shape) != (t,) or tokens.dtype != torch.int32 or tokens.numel() != 1:
+        raise ValueError("lse must be float32 [tokens] and tokens one int32 value")
+    x, w, targets, lse = _whole(x), _whole(w), targets.contiguous(), lse.contiguous()
+    grad_x = torch.empty_like(x) if x_grad else None
+    grad_w = torch.empty_like(w) if w_grad else None
+    nbytes = _abi.lib().cch_linear_cross_entropy_backward_workspace_bytes(t, h, v)
+    _launch16("cch_linear_cross_entropy_backward", x.device, nbytes, _ptr(grad_loss), _ptr(x), _ptr(w), _ptr(targets), targets.element_size(), _ptr(lse), _ptr(tokens), _ptr(grad_x),
+              _ptr(grad_w), t, h, v, red, float(z_coef), _DTYPES[x.dtype])
+    return grad_x, grad_w
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, targets, reduction, z_coef):
+        loss, nll, lse, tokens = linear_cross_entropy(x.detach(), w.detach(), targets, reduction, z_coef)
+        ctx.save_for_backward(x, w, targets, lse, tokens)
+        ctx.options = (reduction, z_coef)
+        ctx.mark_non_differentiable(nll, lse, tokens)
+        ctx.set_materialize_grads(False)
+        return loss, nll, lse, tokens
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_loss, _nll, _lse, _tokens):
+        if grad_loss is None:
+            return (None,) * 5
+        return linear_cross_entropy_backward(grad_loss.float(), *ctx.saved_tensors, *ctx.options, *ctx.needs_input_grad[:2]) + (None,) * 3

@@ -419,6 +419,51 @@ int cch_moe_ffn_w4a16(const void *x, const int32_t *expert_idx, const float *pro
                       const void *w2, const void *s2, const void *z2, void *out, int64_t m, int64_t k, int top_k, int64_t num_experts,
                       int64_t n, int fmt, int group_size, int dtype, void *workspace, int64_t workspace_bytes, void *stream);
 
+/* ---- Products of bf16 or IEEE half operands (dtype CCH_DTYPE_BF16 or CCH_DTYPE_F16), sums in fp32, rounded once; for training and for serving ----
+ * Tensors are contiguous.  x, w and grad_out lie on 16-byte boundaries.  trans_b 1: weights [n, k], 0: [k, n].  Rows up to 2^30, n and k up to 2^22.
+ * workspace: device memory on a 256-byte boundary of at least ..._workspace_bytes(...) bytes (none for 0); nothing in it has to be kept or cleared between calls, calls
+ * that overlap need one each.  Rows of x, w or grad_out that are no multiple of 16 bytes are copied there first.
+ *
+ * Grouped by expert: out[i] = x[i] W_e for the rows of group e, which lie one group behind the other in expert order; group_sizes int32 [num_experts] on the device, clipped to
+ * 0..what is left of t.  Rows behind the last group are written as zeros.  num_experts up to 1024.
+ * Backward: grad_x [t, k] (zeros behind the last group) and grad_w in w's layout (zeros for a group without rows); either may be NULL. */
+int64_t cch_grouped_matmul_workspace_bytes(int64_t num_experts, int64_t t, int64_t n, int64_t k, int trans_b);
+int cch_grouped_matmul(const void *x, const void *w, const int32_t *group_sizes, void *out, int64_t num_experts, int64_t t, int64_t n, int64_t k, int trans_b, int dtype,
+                       void *workspace, int64_t workspace_bytes, void *stream);
+int64_t cch_grouped_matmul_backward_workspace_bytes(int64_t num_experts, int64_t t, int64_t n, int64_t k, int trans_b);
+int cch_grouped_matmul_backward(const void *grad_out, const void *x, const void *w, const int32_t *group_sizes, void *grad_x, void *grad_w, int64_t num_experts, int64_t t,
+                                int64_t n, int64_t k, int trans_b, int dtype, void *workspace, int64_t workspace_bytes, void *stream);
+/* A dense layer: z = x W + bias, out = act(z) + residual.  bias [n], residual [m, n] or NULL; preact: NULL, or [m, n] for z, rounded, which the backward call takes.
+ * Backward: with dz = grad_out * act'(preact), rounded to dtype: grad_x = dz W^T, grad_w = x^T dz in w's layout, grad_bias = column sums of dz before its rounding; each may be
+ * NULL.  The residual's gradient is grad_out.  CCH_ACT_NONE takes no preact.  CCH_ACT_GELU is z (1 + erf(z / sqrt 2)) / 2, CCH_ACT_GELU_TANH its approximation by tanh. */
+#define CCH_ACT_NONE 0
+#define CCH_ACT_RELU 1
+#define CCH_ACT_SILU 2
+#define CCH_ACT_GELU 3
+#define CCH_ACT_GELU_TANH 4
+int64_t cch_matmul_bias_act_workspace_bytes(int64_t m, int64_t n, int64_t k, int trans_b);
+int cch_matmul_bias_act(const void *x, const void *w, const void *bias, const void *residual, void *preact, void *out, int64_t m, int64_t n, int64_t k, int trans_b,
+                        int activation, int dtype, void *workspace, int64_t workspace_bytes, void *stream);
+int64_t cch_matmul_bias_act_backward_workspace_bytes(int64_t m, int64_t n, int64_t k, int trans_b, int activation);
+int cch_matmul_bias_act_backward(const void *grad_out, const void *x, const void *w, const void *preact, void *grad_x, void *grad_w, void *grad_bias, int64_t m, int64_t n,
+                                 int64_t k, int trans_b, int activation, int dtype, void *workspace, int64_t workspace_bytes, void *stream);
+/* Softmax cross entropy of hidden states x [t, h] against an output projection w [v, h], without the logits l = x w^T:
+ *   lse = log sum exp l, nll = lse - l[target]; loss = mean (CCH_REDUCE_MEAN) or sum over the tokens that count of nll + z_coef * lse^2
+ * targets: int32 or int64 [t] (target_bytes 4 or 8); a token whose target lies outside 0..v-1 does not count: its nll and lse are zero, its row of grad_x too, and its
+ * row of x is not looked at.  No token that counts: loss 0.  nll, lse fp32 [t], loss fp32 [1], tokens int32 [1]: how many count.
+ * Backward: grad_loss fp32 [1] on the device, lse as the forward call wrote it, tokens int32 [1], what a mean divides by; grad_x [t, h], grad_w [v, h], either may be NULL.  The logits are
+ * computed again, a piece of the vocabulary at a time, their gradient is rounded to dtype (half: kept times 2^11, which overflows where 1 + 2 z_coef lse passes 31).
+ * t and v up to 2^30, h up to 2^22.  The same inputs give the same bits. */
+#define CCH_REDUCE_MEAN 0
+#define CCH_REDUCE_SUM 1
+int64_t cch_linear_cross_entropy_workspace_bytes(int64_t t, int64_t h, int64_t v);
+int cch_linear_cross_entropy(const void *x, const void *w, const void *targets, int target_bytes, float *loss, float *nll, float *lse, int32_t *tokens, int64_t t, int64_t h,
+                             int64_t v, int reduction, float z_coef, int dtype, void *workspace, int64_t workspace_bytes, void *stream);
+int64_t cch_linear_cross_entropy_backward_workspace_bytes(int64_t t, int64_t h, int64_t v);
+int cch_linear_cross_entropy_backward(const float *grad_loss, const void *x, const void *w, const void *targets, int target_bytes, const float *lse, const int32_t *tokens,
+                                      void *grad_x, void *grad_w, int64_t t, int64_t h, int64_t v, int reduction, float z_coef, int dtype, void *workspace,
+                                      int64_t workspace_bytes, void *stream);
+
 /* Library switches for tests and benchmarks.  They are process-wide (one atomic each, read at
  * every call): two callers that want different settings at the same time race; set them once, or
  * from one thread between calls.  "force_generic_gemm" = 1 routes every GEMM entry
