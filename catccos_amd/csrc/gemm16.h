@@ -1,6 +1,8 @@
 // Products of bf16 or half operands with fp32 sums: the problem that the kernels take (gemm16_kernel.h), how it is launched, and the preparation of
 // operands whose rows start on no 16-byte boundary.
 #pragma once
+#include <atomic>
+
 #include "common.h"
 
 namespace cch {
@@ -16,6 +18,11 @@ enum Epilogue16 {
     EPI16_STATS = 2,  // cross entropy: a row's largest logit and sum of exponentials per 64 columns, and its target's logit
     EPI16_GRAD = 3,   // cross entropy: the logits' gradient times grad_scale
 };
+
+// The kernels, numbered as the switch "matmul16_kernel" names them: tiles of 128 x 128 and 256 x 256.
+enum Kernel16 { KERNEL16_128 = 0, KERNEL16_256 = 1, NUM_KERNELS16 };
+constexpr int64_t BIG_TILES16 = 192;     // tiles of 256 x 256 from which on they are taken: three quarters of the CUs
+extern std::atomic<int> g_kernel16;   // -1: chosen per problem; else that one wherever it takes the problem
 
 struct Gemm16 {
     const uint16_t *a, *b;

@@ -9,6 +9,8 @@ namespace cch {
 int gemm16_launch_bf16(const Gemm16 &p, int layout, int epilogue, hipStream_t stream);   // gemm16_bf16.hip
 int gemm16_launch_f16(const Gemm16 &p, int layout, int epilogue, hipStream_t stream);    // gemm16_f16.hip
 
+std::atomic<int> g_kernel16{-1};
+
 int gemm16_launch(const Gemm16 &p, int layout, int epilogue, hipStream_t stream)
 {
     return p.half ? gemm16_launch_f16(p, layout, epilogue, stream) : gemm16_launch_bf16(p, layout, epilogue, stream);

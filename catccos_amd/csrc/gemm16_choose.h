@@ -1,6 +1,6 @@
 // Which kernel a product of 16-bit operands runs on.
 #pragma once
-#include "gemm16_kernel.h"
+#include "gemm16_big_kernel.h"
 
 namespace cch {
 
@@ -15,6 +15,12 @@ inline int64_t tiles16(const Gemm16 &p, int tm, int tn)
 template <class T, int LAYOUT, int EPI> int shape16(const Gemm16 &p, hipStream_t stream)
 {
     using Mid = Shape16<2, 2, 2, 2, 2>;
+    int dev = 0, cus = 0;
+    CCH_HIP(hipGetDevice(&dev));
+    CCH_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
+    const int64_t big = tiles16(p, 256, 256);
+    const int asked = g_kernel16.load();
+    if (!p.a_rows && (asked == KERNEL16_256 || (asked < 0 && big >= BIG_TILES16))) return launch16_big<T, LAYOUT, EPI>(p, big, cus, stream);
     return launch16<T, LAYOUT, EPI, Mid>(p, tiles16(p, Mid::TM, Mid::TN), stream);
 }
 

@@ -202,9 +202,9 @@ template <class T> __device__ __forceinline__ void store8(uint16_t *p, bool whol
 
 __device__ __forceinline__ bool whole_rows(const Gemm16 &p);
 
-// The results of one wave: MT x NT blocks of 32 x 32 from row m0 and column n0 of the product on, of which rows below m_end exist.  group: the output that K-grouped
+// The results of one wave: MT x NT blocks of 32 x 32, every RS rows from row m0 on and side by side from column n0 of the product, of which rows below m_end exist.  group: the output that K-grouped
 // problems write.
-template <class T, int EPI, int MT, int NT>
+template <class T, int EPI, int MT, int NT, int RS>
 __device__ __forceinline__ void epilogue16(const Gemm16 &p, v16f (&acc)[MT][NT], int group, int m0, int m_end, int n0)
 {
     const int lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5;
@@ -212,7 +212,7 @@ __device__ __forceinline__ void epilogue16(const Gemm16 &p, v16f (&acc)[MT][NT],
         // 64 columns' largest logit and sum of exponentials (NT is 2, or 1 for 32 columns), the two halves of the wave joined; a target's logit on the way
 #pragma unroll
         for (int i = 0; i < MT; i++) {
-            const int m = m0 + 32 * i + r;
+            const int m = m0 + RS * i + r;
             const bool there = m < m_end;
             const int want = there ? p.targets[m] - p.v0 - n0 - 4 * g : -1;
             float top = -INFINITY;
@@ -240,7 +240,7 @@ __device__ __forceinline__ void epilogue16(const Gemm16 &p, v16f (&acc)[MT][NT],
         const float scale = EPI == EPI16_OUT && p.scale ? *p.scale : 1.0f;
 #pragma unroll
         for (int i = 0; i < MT; i++) {
-            const int m = m0 + 32 * i + r;
+            const int m = m0 + RS * i + r;
             const bool there = m < m_end;
             int64_t row = m;
             float lse = 0.0f, slope = 0.0f;

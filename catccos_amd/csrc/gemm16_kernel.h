@@ -154,7 +154,7 @@ __global__ __launch_bounds__(S::THREADS, S::PER_CU * S::WAVES / 4) void gemm16_k
         }
         CCH_WAIT_LGKM0();
         CCH_BARRIER();   // (the next tile's requests overwrite the stages)
-        epilogue16<T, EPI, MT, NT>(p, acc, e, m0 + wm * MT * 32, m_end, n0 + wn * NT * 32);
+        epilogue16<T, EPI, MT, NT, 32>(p, acc, e, m0 + wm * MT * 32, m_end, n0 + wn * NT * 32);
     }
 }
 

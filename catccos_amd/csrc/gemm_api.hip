@@ -3,6 +3,7 @@
 #include <cstring>
 
 #include "common.h"
+#include "gemm16.h"
 #include "gemm_common.h"
 
 namespace cch {
@@ -97,6 +98,11 @@ int cch_set_option(const char *name, int value)
     if (strcmp(name, "gemm_192_tiles") == 0) {
         CCH_REQUIRE(value >= -1 && value <= 1, "cch_set_option: gemm_192_tiles %d outside -1..1", value);
         g_tiles_192.store(value);
+        return CCH_OK;
+    }
+    if (strcmp(name, "matmul16_kernel") == 0) {
+        CCH_REQUIRE(value >= -1 && value < NUM_KERNELS16, "cch_set_option: matmul16_kernel %d outside -1..%d", value, NUM_KERNELS16 - 1);
+        g_kernel16.store(value);
         return CCH_OK;
     }
     if (strcmp(name, "routing_three_launches") == 0) {

@@ -179,8 +179,8 @@ static int ce_gather(const uint16_t *x, const int32_t *pos, uint16_t *rows, uint
     return launch_status("ce_gather_kernel");
 }
 
-// Rows of x are picked by the product's requests where offsets of 32 bits reach them all and none needs padding, else copied.
-static bool ce_picks(int64_t t, int64_t h) { return whole16(h) && t * h * 2 <= 0x7FFFFFF0; }
+// Rows of x are picked by the product's requests where it runs on tiles of 128 x 128, offsets of 32 bits reach them all and none needs padding; else they are copied.
+static bool ce_picks(int64_t t, int64_t h, int64_t v) { return whole16(h) && t * h * 2 <= 0x7FFFFFF0 && ((t + 255) / 256) * ((v + 255) / 256) < BIG_TILES16; }
 
 struct CeWorkspace {
     int64_t src, pos, target, lse, count, scalar, logit, stats, rows, w, d, sums, end;
@@ -197,7 +197,7 @@ static CeWorkspace ce_workspace(int64_t t, int64_t h, int64_t v, bool backward)
     at.target = piece(t * 4);
     at.count = piece(4);
     at.w = piece(padded16_bytes(v, h));
-    if (backward || !ce_picks(t, h)) {
+    if (backward || !ce_picks(t, h, v)) {
         at.pos = piece(t * 4);
         at.rows = piece(t * pitch16(h) * 2);
     }
@@ -245,7 +245,7 @@ extern "C" int cch_linear_cross_entropy(const void *x, const void *w, const void
     uint8_t *ws = static_cast<uint8_t *>(workspace);
     auto i32 = [&](int64_t o) { return reinterpret_cast<int32_t *>(ws + o); };
     auto f32 = [&](int64_t o) { return reinterpret_cast<float *>(ws + o); };
-    const bool picks = ce_picks(t, h);
+    const bool picks = ce_picks(t, h, v);
 
     CeTokens tk{};
     tk.targets = targets;

@@ -7,6 +7,14 @@ from bounds16 import check, rounded, sum_error
 
 pytestmark = pytest.mark.gpu
 
+
+@pytest.fixture(params=[-1, 0, 1], ids=["chosen", "128x128", "256x256"], autouse=True)
+def kernel16(request):
+    """The kernel that a product goes to by itself, and each one."""
+    cc.set_option("matmul16_kernel", request.param)
+    yield
+    cc.set_option("matmul16_kernel", -1)
+
 SIZES = [
     # group sizes, rows behind the last group, k, n
     ([1], 0, 64, 64),

@@ -7,6 +7,14 @@ from bounds16 import check, rounded, sum_error
 
 pytestmark = pytest.mark.gpu
 
+
+@pytest.fixture(params=[-1, 0, 1], ids=["chosen", "128x128", "256x256"], autouse=True)
+def kernel16(request):
+    """The kernel that a product goes to by itself, and each one."""
+    cc.set_option("matmul16_kernel", request.param)
+    yield
+    cc.set_option("matmul16_kernel", -1)
+
 # The sum of a row's exponentials: each is off by a few units in the last place and by its argument's rounding, 2^-24 times an argument that matters up to about 40; a sum of
 # 64 columns, then of their statistics over 64 lanes and along V / 4096 of them: fewer than 128 + V / 4096 additions deep.
 EXP = 2.0 ** -18

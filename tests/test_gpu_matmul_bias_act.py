@@ -7,6 +7,14 @@ from bounds16 import check, rounded, sum_error
 
 pytestmark = pytest.mark.gpu
 
+
+@pytest.fixture(params=[-1, 0, 1], ids=["chosen", "128x128", "256x256"], autouse=True)
+def kernel16(request):
+    """The kernel that a product goes to by itself, and each one."""
+    cc.set_option("matmul16_kernel", request.param)
+    yield
+    cc.set_option("matmul16_kernel", -1)
+
 ACTS = ["none", "relu", "silu", "gelu", "gelu_tanh"]
 # The activations are smooth with a slope below 1.13 everywhere; computed in fp32 with a hardware exponential and reciprocal (a unit or two in the last place each, the exponent's
 # argument off by 2^-22 of itself, and e^-z small where z is large) their own error stays below 2^-19 (|z| + 1).
