@@ -43,6 +43,18 @@ __device__ __forceinline__ float act_value(float z, int act)
     default: return z;
     }
 }
+// (one branch for eight values)
+__device__ __forceinline__ void apply_act(float v[8], int act)
+{
+    switch (act) {
+#define CCH_EACH(ACT) case ACT: for (int x = 0; x < 8; x++) v[x] = act_value(v[x], ACT); break
+    CCH_EACH(CCH_ACT_RELU);
+    CCH_EACH(CCH_ACT_SILU);
+    CCH_EACH(CCH_ACT_GELU);
+    CCH_EACH(CCH_ACT_GELU_TANH);
+#undef CCH_EACH
+    }
+}
 __device__ __forceinline__ float act_slope(float z, int act)
 {
     switch (act) {
@@ -200,16 +212,56 @@ template <class T> __device__ __forceinline__ void store8(uint16_t *p, bool whol
         if (i < there) p[i] = (uint16_t)((uint32_t)o[i >> 1] >> (16 * (i & 1)));
 }
 
-__device__ __forceinline__ bool whole_rows(const Gemm16 &p);
-
-// The results of one wave: MT x NT blocks of 32 x 32, every RS rows from row m0 on and side by side from column n0 of the product, of which rows below m_end exist.  group: the output that K-grouped
-// problems write.
-template <class T, int EPI, int MT, int NT, int RS>
-__device__ __forceinline__ void epilogue16(const Gemm16 &p, v16f (&acc)[MT][NT], int group, int m0, int m_end, int n0)
+// Whether the epilogue's tensors have rows on 16-byte boundaries.
+__device__ __forceinline__ bool whole_rows(const Gemm16 &p)
 {
+    return p.pitch_out % 8 == 0 && ((uintptr_t)p.out & 15) == 0 && p.out_stride % 8 == 0 && (((uintptr_t)p.bias | (uintptr_t)p.residual | (uintptr_t)p.preact) & 15) == 0;
+}
+
+// Between a wave's writes to LDS and its other lanes' reads: for the compiler alone (a wave's LDS operations are in order), which sees one lane's accesses and may
+// otherwise send lanes that branch alike through writes and reads before the others' writes.
+__device__ __forceinline__ void lanes_meet()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// A wave's results on their way to memory, 32 rows of 64 columns, PASS rows at a time through LDS of the wave's own (PASS * 128 bytes at `at`): a lane holds four pieces of 16
+// bytes of one row, a store wants eight lanes to a row, whole lines of 128 bytes.  Stored as the lanes hold them, 32 bytes a row, a 256 x 256 tile's epilogue took 11 us.
+// Pieces lie at position c ^ (row & 7), so that writes and reads spread over all banks.
+template <int PASS, class Store> __device__ __forceinline__ void through_lds(uint32_t at, const v4i piece[2][2], Store &&store)
+{
+    typedef __attribute__((address_space(3))) v4i *P;
     const int lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5;
+#pragma unroll
+    for (int ps = 0; ps < 32 / PASS; ps++) {
+        if (PASS == 32 || (r / PASS) == ps) {
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    *reinterpret_cast<P>((uintptr_t)(at + (uint32_t)(r % PASS) * 128u + (((uint32_t)(4 * j + 2 * h + g) ^ (uint32_t)(r & 7)) << 4))) = piece[j][h];
+        }
+        lanes_meet();
+        v4i o[PASS / 8];
+#pragma unroll
+        for (int q = 0; q < PASS / 8; q++) o[q] = lds_read16_abs(at + (uint32_t)(q * 8 + (lane >> 3)) * 128u + (((uint32_t)(lane & 7) ^ (uint32_t)(lane >> 3)) << 4));
+        lanes_meet();
+#pragma unroll
+        for (int q = 0; q < PASS / 8; q++) store(ps * PASS + q * 8 + (lane >> 3), (lane & 7) * 8, o[q]);
+    }
+}
+
+// The results of one wave: MT x NT blocks of 32 x 32, every RS rows from row m0 on and side by side from column n0 of the product, of which rows below m_end exist.
+// group: the output that K-grouped problems write.  staging: PASS * 128 bytes of LDS of the wave's own.
+template <class T, int EPI, int MT, int NT, int RS, int PASS>
+__device__ __forceinline__ void epilogue16(const Gemm16 &p, v16f (&acc)[MT][NT], int group, int m0, int m_end, int n0, uint32_t staging)
+{
+    static_assert(NT == 2, "64 columns to a wave");
+    const int lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5;
+    if (n0 >= p.n) return;
     if constexpr (EPI == EPI16_STATS) {
-        // 64 columns' largest logit and sum of exponentials (NT is 2, or 1 for 32 columns), the two halves of the wave joined; a target's logit on the way
+        // 64 columns' largest logit and sum of exponentials, the two halves of the wave joined; a target's logit on the way
 #pragma unroll
         for (int i = 0; i < MT; i++) {
             const int m = m0 + RS * i + r;
@@ -232,37 +284,36 @@ __device__ __forceinline__ void epilogue16(const Gemm16 &p, v16f (&acc)[MT][NT],
 #pragma unroll
                 for (int x = 0; x < 16; x++) sum += __expf(acc[i][j][x] - top);
             sum += __shfl_xor(sum, 32);
-            if (there && g == 0 && n0 < p.n) p.stats[(int64_t)m * p.stat_cols + (p.v0 + n0) / (32 * NT)] = make_float2(top, sum);
+            if (there && g == 0) p.stats[(int64_t)m * p.stat_cols + (p.v0 + n0) / (32 * NT)] = make_float2(top, sum);
         }
         return;
     } else {
-        const bool rows_whole = whole_rows(p);
+        const bool whole = whole_rows(p);   // and then p.n is a multiple of 8, or (EPI16_GRAD) the rows have room for whole pieces
         const float scale = EPI == EPI16_OUT && p.scale ? *p.scale : 1.0f;
+        uint16_t *const out = p.out + (int64_t)group * p.out_stride;
 #pragma unroll
         for (int i = 0; i < MT; i++) {
-            const int m = m0 + RS * i + r;
+            const int first = m0 + RS * i, m = first + r;
+            if (first >= m_end) break;
             const bool there = m < m_end;
-            int64_t row = m;
             float lse = 0.0f, slope = 0.0f;
             int target = -1;
-            if (EPI == EPI16_OUT && p.out_rows) row = there ? p.out_rows[m] : 0;
             if (EPI == EPI16_GRAD) {
                 lse = there ? p.lse[m] : 0.0f;
                 slope = (1.0f + p.z2 * lse) * p.grad_scale;
                 target = there ? p.targets[m] - p.v0 : -1;
             }
+            v4i piece[2][2], pre[2][2];
 #pragma unroll
             for (int j = 0; j < NT; j++) {
                 float v[2][8];
                 eight_columns(acc[i][j], v);
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const int n = n0 + 32 * j + 16 * h + 8 * g;
-                    const int left = p.n - n;
-                    if (!there || left <= 0) continue;
-                    const bool whole = rows_whole && left >= 8;
+                    const int n = n0 + 32 * j + 16 * h + 8 * g, left = p.n - n;
+                    const bool in = there && left > 0;
                     if constexpr (EPI == EPI16_OUT) {
-                        if (p.sums) {
+                        if (p.sums && in) {
                             float *s = p.sums + (int64_t)m * p.n + n;
 #pragma unroll
                             for (int x = 0; x < 8; x++)
@@ -270,29 +321,23 @@ __device__ __forceinline__ void epilogue16(const Gemm16 &p, v16f (&acc)[MT][NT],
                                     if (p.sums_in) v[h][x] += s[x];
                                     if (p.sums_out) s[x] = v[h][x];
                                 }
-                            if (p.sums_out) continue;
                         }
 #pragma unroll
                         for (int x = 0; x < 8; x++) v[h][x] *= scale;
-                        store8<T>(p.out + (int64_t)group * p.out_stride + row * p.pitch_out + n, whole, left, v[h]);
                     } else if constexpr (EPI == EPI16_ACT) {
-                        if (p.bias) {
-                            float b[8];
+                        float b[8];
+                        if (p.bias && in) {
                             load8<T>(p.bias + n, whole, left, b);
 #pragma unroll
                             for (int x = 0; x < 8; x++) v[h][x] += b[x];
                         }
-                        const int64_t at = row * p.pitch_out + n;
-                        if (p.preact) store8<T>(p.preact + at, whole, left, v[h]);
-#pragma unroll
-                        for (int x = 0; x < 8; x++) v[h][x] = act_value(v[h][x], p.act);
-                        if (p.residual) {
-                            float b[8];
-                            load8<T>(p.residual + at, whole, left, b);
+                        pre[j][h] = pack8<T>(v[h]);
+                        apply_act(v[h], p.act);
+                        if (p.residual && in) {
+                            load8<T>(p.residual + (int64_t)m * p.pitch_out + n, whole, left, b);
 #pragma unroll
                             for (int x = 0; x < 8; x++) v[h][x] += b[x];
                         }
-                        store8<T>(p.out + at, whole, left, v[h]);
                     } else {
                         // rows of the gradient end on 16-byte boundaries, zeros behind the last column: the next product reads it along K
 #pragma unroll
@@ -300,17 +345,37 @@ __device__ __forceinline__ void epilogue16(const Gemm16 &p, v16f (&acc)[MT][NT],
                             const float d = __expf(v[h][x] - lse) * slope - (n + x == target ? p.grad_scale : 0.0f);
                             v[h][x] = x < left ? d : 0.0f;
                         }
-                        store8<T>(p.out + row * p.pitch_out + n, true, 8, v[h]);
                     }
+                    piece[j][h] = pack8<T>(v[h]);
                 }
+            }
+            if (EPI == EPI16_OUT && p.sums_out) continue;
+            if (whole) {
+                auto put = [&](uint16_t *base) {
+                    return [&, base](int row, int c, v4i o) {
+                        if (first + row >= m_end || n0 + c >= p.n) return;
+                        const int64_t to = EPI == EPI16_OUT && p.out_rows ? p.out_rows[first + row] : first + row;
+                        *reinterpret_cast<v4i *>(base + to * p.pitch_out + n0 + c) = o;
+                    };
+                };
+                if (EPI == EPI16_ACT && p.preact) through_lds<PASS>(staging, pre, put(p.preact));
+                through_lds<PASS>(staging, piece, put(out));
+            } else if (there) {
+                const int64_t to = EPI == EPI16_OUT && p.out_rows ? p.out_rows[m] : m;
+#pragma unroll
+                for (int j = 0; j < NT; j++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int x = 0; x < 8; x++) {
+                            const int n = n0 + 32 * j + 16 * h + 8 * g + x;
+                            if (n >= p.n) continue;
+                            out[to * p.pitch_out + n] = (uint16_t)((uint32_t)piece[j][h][x >> 1] >> (16 * (x & 1)));
+                            if (EPI == EPI16_ACT && p.preact) p.preact[to * p.pitch_out + n] = (uint16_t)((uint32_t)pre[j][h][x >> 1] >> (16 * (x & 1)));
+                        }
             }
         }
     }
-}
-// Whether the epilogue's tensors have rows on 16-byte boundaries.
-__device__ __forceinline__ bool whole_rows(const Gemm16 &p)
-{
-    return p.pitch_out % 8 == 0 && ((uintptr_t)p.out & 15) == 0 && p.out_stride % 8 == 0 && (((uintptr_t)p.bias | (uintptr_t)p.residual | (uintptr_t)p.preact) & 15) == 0;
 }
 
 // Rows behind the last group: zeros.

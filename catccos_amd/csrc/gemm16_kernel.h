@@ -153,8 +153,11 @@ __global__ __launch_bounds__(S::THREADS, S::PER_CU * S::WAVES / 4) void gemm16_k
             }
         }
         CCH_WAIT_LGKM0();
-        CCH_BARRIER();   // (the next tile's requests overwrite the stages)
-        epilogue16<T, EPI, MT, NT, 32>(p, acc, e, m0 + wm * MT * 32, m_end, n0 + wn * NT * 32);
+        CCH_BARRIER();
+        // (results pass through the stages, which the next tile's requests overwrite)
+        epilogue16<T, EPI, MT, NT, 32, 32>(p, acc, e, m0 + wm * MT * 32, m_end, n0 + wn * NT * 32, lds + (uint32_t)wave * 4096u);
+        CCH_WAIT_LGKM0();
+        CCH_BARRIER();
     }
 }
 
