@@ -43,7 +43,7 @@ __global__ __launch_bounds__(Big16::THREADS, 2) void gemm16_big_kernel(Gemm16 p)
     const uint32_t lds = (uint32_t)uniform((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)smem);
     const int col_tiles = (p.n + S::TN - 1) / S::TN;
     const int row_tiles = uniform(rows_grouped ? tab.tile[p.groups] : (p.m + S::TM - 1) / S::TM);
-    const int64_t per_group = (int64_t)row_tiles * col_tiles, total = per_group * (rows_grouped ? 1 : p.groups);
+    const int per_group = row_tiles * col_tiles, total = per_group * (rows_grouped ? 1 : p.groups);   // (below 2^31: the launch checks)
 
     // ---- this lane's fragment reads (the current stage's; moved by a panel from step to step)
     // A, K contiguous: panel position 128 wm + 32 i + r holds tile row 64 i + 32 wm + r; K-major: column = tile row
@@ -101,8 +101,8 @@ __global__ __launch_bounds__(Big16::THREADS, 2) void gemm16_big_kernel(Gemm16 p)
     };
     const int64_t adv_a = A_KM ? p.pitch_a * 128 : 128, adv_b = B_KM ? p.pitch_b * 128 : 128;   // bytes from step to step
     const int k8 = (p.k + 7) & ~7, n8 = (p.n + 7) & ~7, m8 = (p.m + 7) & ~7;
-    auto decode = [&](int64_t t, Tile &c) {
-        const int64_t at = place16(t, total);
+    auto decode = [&](int t, Tile &c) {
+        const int at = place16(t, total);
         c.valid = at >= 0;
         c.steps = 2;
         c.k_len = 0;
@@ -119,7 +119,7 @@ __global__ __launch_bounds__(Big16::THREADS, 2) void gemm16_big_kernel(Gemm16 p)
             c.m0 = uniform(tab.start[c.e] + (rt - tab.tile[c.e]) * S::TM);
             c.m_end = uniform(tab.start[c.e + 1]);
         } else {
-            c.e = (int)(at / per_group);
+            c.e = at / per_group;
             tile_of16(at - c.e * per_group, row_tiles, col_tiles, rt, ct);
             c.m0 = rt * S::TM;
             c.m_end = p.m;
@@ -176,10 +176,10 @@ __global__ __launch_bounds__(Big16::THREADS, 2) void gemm16_big_kernel(Gemm16 p)
     };
 
     Tile cur, nxt;
-    int64_t t = blockIdx.x;
+    int t = (int)blockIdx.x;
     decode(t, cur);
     if (!cur.valid) return;
-    t += gridDim.x;
+    t += (int)gridDim.x;
     decode(t, nxt);
 
     uint32_t stage = 0;   // byte offset of the current step's panels in the ring: 0 or PANEL
@@ -208,156 +208,173 @@ __global__ __launch_bounds__(Big16::THREADS, 2) void gemm16_big_kernel(Gemm16 p)
     if (wm == 1) CCH_BARRIER();   // one slot behind
 
     v16f acc[MT][NT];
-#pragma unroll
-    for (int i = 0; i < MT; i++)
-#pragma unroll
-        for (int j = 0; j < NT; j++) acc[i][j] = (v16f)(0.0f);
+    // Output stores of a wave that its next tile's first step may leave in flight: they are younger than what that step waits for.  Counted only where they are always issued.
+    const bool whole = whole_rows(p), counted = whole && counted_stores<EPI>(p);
+    const int more = !counted ? 0 : EPI == EPI16_ACT && p.preact ? 2 : 1;   // times 16
+    int young = 0;   // what the current tile's first step finds
 
-    while (true) {
-        for (int kt = 0; kt < cur.steps; kt++) {
-            // descriptors: one step ahead are what two steps ahead were
-            ra1 = ra2;
-            rb1 = rb2;
-            k1 = k2;
-            if (kt + 2 == cur.steps) open(nxt);
-            else advance();
-            describe();
-            const uint32_t other = (uint32_t)PANEL - stage;
-            if constexpr (!HALVES) {
-                v4i fb[NT][4], fa[2][4];
-                // L0
+    // What a wait of n requests allows in step `first_c`: those, and in a tile's first step the stores
+    auto wait = [&](auto first_c, auto n_c) {
+        constexpr int n = decltype(n_c)::value;
+        if constexpr (decltype(first_c)::value != 0) {
+            if (young == 2) CCH_WAIT_VM(n + 32);
+            else if (young == 1) CCH_WAIT_VM(n + 16);
+            else CCH_WAIT_VM(n);
+        } else {
+            CCH_WAIT_VM(n);
+        }
+    };
+    auto mma = [&](auto first_c, v16f &c, const v4i &b, const v4i &a) {
+        if constexpr (decltype(first_c)::value != 0) c = T::mfma(b, a, (v16f)(0.0f));
+        else c = T::mfma(b, a, c);
+    };
+    auto step = [&](auto first_c, int kt) {
+        // descriptors: one step ahead are what two steps ahead were
+        ra1 = ra2;
+        rb1 = rb2;
+        k1 = k2;
+        if (kt + 2 == cur.steps) open(nxt);
+        else advance();
+        describe();
+        const uint32_t other = (uint32_t)PANEL - stage;
+        if constexpr (!HALVES) {
+            v4i fb[NT][4], fa[2][4];
+            // L0
 #pragma unroll
-                for (int kk = 0; kk < 4; kk++)
+            for (int kk = 0; kk < 4; kk++)
 #pragma unroll
-                    for (int j = 0; j < NT; j++) fb[j][kk] = lds_read16_abs(fr_b[kk] + (uint32_t)j * 4096u);
+                for (int j = 0; j < NT; j++) fb[j][kk] = lds_read16_abs(fr_b[kk] + (uint32_t)j * 4096u);
 #pragma unroll
-                for (int kk = 0; kk < 4; kk++)
+            for (int kk = 0; kk < 4; kk++)
 #pragma unroll
-                    for (int i = 0; i < 2; i++) fa[i][kk] = lds_read16_abs(fr_a[kk] + (uint32_t)i * 4096u);
+                for (int i = 0; i < 2; i++) fa[i][kk] = lds_read16_abs(fr_a[kk] + (uint32_t)i * 4096u);
+            __builtin_amdgcn_sched_barrier(0);
+            request_a(ra1, k1, other, IC<2>{});
+            request_a(ra1, k1, other, IC<3>{});
+            CCH_WAIT_LGKM0();
+            CCH_BARRIER();
+            // C0
+            static_for<4>([&](auto kk_c) {
+                constexpr int kk = decltype(kk_c)::value;
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int j = 0; j < NT; j++) mma(IC<(kk == 0 && decltype(first_c)::value)>{}, acc[i][j], fb[j][kk], fa[i][kk]);
+                if constexpr (kk == 0) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    request_a(ra2, k2, stage, IC<0>{});
+                    request_a(ra2, k2, stage, IC<1>{});
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            });
+            __builtin_amdgcn_sched_barrier(0);
+            wait(first_c, IC<10>{});
+            CCH_BARRIER();
+            // L1
+#pragma unroll
+            for (int kk = 0; kk < 4; kk++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) fa[i][kk] = lds_read16_abs(fr_a[kk] + (uint32_t)(2 + i) * 4096u);
+            __builtin_amdgcn_sched_barrier(0);
+            request_b(rb2, k2, stage, IC<0>{});
+            request_b(rb2, k2, stage, IC<1>{});
+            wait(first_c, IC<6>{});
+            CCH_WAIT_LGKM0();
+            CCH_BARRIER();
+            // C1
+            static_for<4>([&](auto kk_c) {
+                constexpr int kk = decltype(kk_c)::value;
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int j = 0; j < NT; j++) mma(IC<(kk == 0 && decltype(first_c)::value)>{}, acc[2 + i][j], fb[j][kk], fa[i][kk]);
+                if constexpr (kk == 0) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    request_b(rb2, k2, stage, IC<2>{});
+                    request_b(rb2, k2, stage, IC<3>{});
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            });
+            __builtin_amdgcn_sched_barrier(0);
+        } else {
+            v4i fb[NT][2], fa[MT][2];
+            static_for<2>([&](auto h_c) {
+                constexpr int h = decltype(h_c)::value;
+                // L0, L1
+#pragma unroll
+                for (int kk = 0; kk < 2; kk++)
+#pragma unroll
+                    for (int j = 0; j < NT; j++) fb[j][kk] = read_transposed(ft_b[j] + (uint32_t)(2 * h + kk) * 16u * KM::ROW, KM::ROW);
+#pragma unroll
+                for (int kk = 0; kk < 2; kk++)
+#pragma unroll
+                    for (int i = 0; i < MT; i++)
+                        fa[i][kk] = A_KM ? read_transposed(ft_a[i] + (uint32_t)(2 * h + kk) * 16u * KM::ROW, KM::ROW) : lds_read16_abs(fr_a[2 * h + kk] + (uint32_t)i * 4096u);
                 __builtin_amdgcn_sched_barrier(0);
-                request_a(ra1, k1, other, IC<2>{});
-                request_a(ra1, k1, other, IC<3>{});
-                CCH_WAIT_LGKM0();
-                CCH_BARRIER();
-                // C0
-#pragma unroll
-                for (int kk = 0; kk < 4; kk++) {
-#pragma unroll
-                    for (int i = 0; i < 2; i++)
-#pragma unroll
-                        for (int j = 0; j < NT; j++) acc[i][j] = T::mfma(fb[j][kk], fa[i][kk], acc[i][j]);
-                    if (kk == 0) {
-                        __builtin_amdgcn_sched_barrier(0);
+                if constexpr (h == 0) {
+                    request_b(rb1, k1, other, IC<2>{});
+                    request_b(rb1, k1, other, IC<3>{});
+                    if constexpr (A_KM) {
+                        request_a(ra1, k1, other, IC<2>{});
+                        request_a(ra1, k1, other, IC<3>{});
+                    }
+                } else {
+                    request_b(rb2, k2, stage, IC<0>{});
+                    request_b(rb2, k2, stage, IC<1>{});
+                    if constexpr (A_KM) {
                         request_a(ra2, k2, stage, IC<0>{});
                         request_a(ra2, k2, stage, IC<1>{});
-                        __builtin_amdgcn_sched_barrier(0);
                     }
                 }
-                __builtin_amdgcn_sched_barrier(0);
-                CCH_WAIT_VM(10);
+                if (wm == 1) wait(first_c, IC<8>{});
+                CCH_WAIT_LGKM0();
                 CCH_BARRIER();
-                // L1
+                // C0, C1
+                static_for<2>([&](auto kk_c) {
+                    constexpr int kk = decltype(kk_c)::value;
+                    static_for<MT>([&](auto i_c) {
+                        constexpr int i = decltype(i_c)::value;
 #pragma unroll
-                for (int kk = 0; kk < 4; kk++)
-#pragma unroll
-                    for (int i = 0; i < 2; i++) fa[i][kk] = lds_read16_abs(fr_a[kk] + (uint32_t)(2 + i) * 4096u);
-                __builtin_amdgcn_sched_barrier(0);
-                request_b(rb2, k2, stage, IC<0>{});
-                request_b(rb2, k2, stage, IC<1>{});
-                CCH_WAIT_VM_LGKM0(6);
-                CCH_BARRIER();
-                // C1
-#pragma unroll
-                for (int kk = 0; kk < 4; kk++) {
-#pragma unroll
-                    for (int i = 0; i < 2; i++)
-#pragma unroll
-                        for (int j = 0; j < NT; j++) acc[2 + i][j] = T::mfma(fb[j][kk], fa[i][kk], acc[2 + i][j]);
-                    if (kk == 0) {
-                        __builtin_amdgcn_sched_barrier(0);
-                        request_b(rb2, k2, stage, IC<2>{});
-                        request_b(rb2, k2, stage, IC<3>{});
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            } else {
-                v4i fb[NT][2], fa[MT][2];
-                static_for<2>([&](auto h_c) {
-                    constexpr int h = decltype(h_c)::value;
-                    // L0, L1
-#pragma unroll
-                    for (int kk = 0; kk < 2; kk++)
-#pragma unroll
-                        for (int j = 0; j < NT; j++) fb[j][kk] = read_transposed(ft_b[j] + (uint32_t)(2 * h + kk) * 16u * KM::ROW, KM::ROW);
-#pragma unroll
-                    for (int kk = 0; kk < 2; kk++)
-#pragma unroll
-                        for (int i = 0; i < MT; i++)
-                            fa[i][kk] = A_KM ? read_transposed(ft_a[i] + (uint32_t)(2 * h + kk) * 16u * KM::ROW, KM::ROW) : lds_read16_abs(fr_a[2 * h + kk] + (uint32_t)i * 4096u);
-                    __builtin_amdgcn_sched_barrier(0);
-                    if constexpr (h == 0) {
-                        request_b(rb1, k1, other, IC<2>{});
-                        request_b(rb1, k1, other, IC<3>{});
-                        if constexpr (A_KM) {
-                            request_a(ra1, k1, other, IC<2>{});
-                            request_a(ra1, k1, other, IC<3>{});
+                        for (int j = 0; j < NT; j++) mma(IC<(h == 0 && kk == 0 && decltype(first_c)::value)>{}, acc[i][j], fb[j][kk], fa[i][kk]);
+                        if constexpr (h == 1 && !A_KM && kk == 0) {
+                            __builtin_amdgcn_sched_barrier(0);
+                            request_a(ra2, k2, stage, i_c);
+                            __builtin_amdgcn_sched_barrier(0);
                         }
-                    } else {
-                        request_b(rb2, k2, stage, IC<0>{});
-                        request_b(rb2, k2, stage, IC<1>{});
-                        if constexpr (A_KM) {
-                            request_a(ra2, k2, stage, IC<0>{});
-                            request_a(ra2, k2, stage, IC<1>{});
-                        }
-                    }
-                    CCH_WAIT_VM_LGKM0(8);
-                    CCH_BARRIER();
-                    // C0, C1
-#pragma unroll
-                    for (int kk = 0; kk < 2; kk++)
-#pragma unroll
-                        for (int i = 0; i < MT; i++) {
-#pragma unroll
-                            for (int j = 0; j < NT; j++) acc[i][j] = T::mfma(fb[j][kk], fa[i][kk], acc[i][j]);
-                            if (h == 1 && !A_KM && kk == 0) {
-                                __builtin_amdgcn_sched_barrier(0);
-                                if (i == 0) request_a(ra2, k2, stage, IC<0>{});
-                                if (i == 1) request_a(ra2, k2, stage, IC<1>{});
-                                if (i == 2) request_a(ra2, k2, stage, IC<2>{});
-                                if (i == 3) request_a(ra2, k2, stage, IC<3>{});
-                                __builtin_amdgcn_sched_barrier(0);
-                            }
-                        }
-                    __builtin_amdgcn_sched_barrier(0);
-                    if constexpr (h == 0) CCH_BARRIER();
+                    });
                 });
-                if constexpr (!A_KM) CCH_WAIT_VM(8);
-            }
-            // the other stage
-            const uint32_t move = other - stage;
+                __builtin_amdgcn_sched_barrier(0);
+                if (wm == 0 || (h == 1 && !A_KM)) wait(first_c, IC<8>{});
+                if constexpr (h == 0) CCH_BARRIER();
+            });
+        }
+        // the other stage
+        const uint32_t move = other - stage;
 #pragma unroll
-            for (int x = 0; x < 4; x++) {
-                if (!A_KM) fr_a[x] += move;
-                if (!B_KM) fr_b[x] += move;
-                if (A_KM) ft_a[x] += move;
-            }
+        for (int x = 0; x < 4; x++) {
+            if (!A_KM) fr_a[x] += move;
+            if (!B_KM) fr_b[x] += move;
+            if (A_KM) ft_a[x] += move;
+        }
 #pragma unroll
-            for (int j = 0; j < NT; j++)
-                if (B_KM) ft_b[j] += move;
-            stage = other;
-            if (kt + 1 < cur.steps) CCH_BARRIER();
+        for (int j = 0; j < NT; j++)
+            if (B_KM) ft_b[j] += move;
+        stage = other;
+    };
+
+    while (true) {
+        step(IC<1>{}, 0);
+        for (int kt = 1; kt < cur.steps; kt++) {
+            CCH_BARRIER();
+            step(IC<0>{}, kt);
         }
         // Both groups write their results in the same slot: the first behind the barrier that ends its last matrix slot, the second, one slot behind, before it.
         if (wm == 0) CCH_BARRIER();
-        epilogue16<T, EPI, MT, NT, 64, S::PASS>(p, acc, cur.e, cur.m0 + wm * 32, cur.m_end, cur.n0 + wn * 64, lds + S::STAGING + (uint32_t)wave * (S::PASS * 128u));
-#pragma unroll
-        for (int i = 0; i < MT; i++)
-#pragma unroll
-            for (int j = 0; j < NT; j++) acc[i][j] = (v16f)(0.0f);
+        epilogue16<T, EPI, MT, NT, 64, S::PASS>(p, acc, cur.e, cur.m0, cur.m_end, cur.n0, wm * 32, wn * 64, lds + S::STAGING + (uint32_t)wave * (S::PASS * 128u), whole, counted);
         if (!nxt.valid) break;
+        young = more;
         cur = nxt;
-        t += gridDim.x;
+        t += (int)gridDim.x;
         decode(t, nxt);
         if (wm == 1) CCH_BARRIER();
     }

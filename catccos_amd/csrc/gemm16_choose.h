@@ -20,7 +20,8 @@ template <class T, int LAYOUT, int EPI> int shape16(const Gemm16 &p, hipStream_t
     CCH_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
     const int64_t big = tiles16(p, 256, 256);
     const int asked = g_kernel16.load();
-    if (!p.a_rows && (asked == KERNEL16_256 || (asked < 0 && big >= BIG_TILES16))) return launch16_big<T, LAYOUT, EPI>(p, big, cus, stream);
+    CCH_REQUIRE(tiles16(p, 128, 128) < (int64_t)1 << 31, "a product of %d x %d in %d groups has too many tiles", p.m, p.n, p.groups);
+    if (!p.a_rows && p.pitch_out < MAX_PITCH16 / 2 && (asked == KERNEL16_256 || (asked < 0 && big >= BIG_TILES16))) return launch16_big<T, LAYOUT, EPI>(p, big, cus, stream);
     return launch16<T, LAYOUT, EPI, Mid>(p, tiles16(p, Mid::TM, Mid::TN), stream);
 }
 

@@ -120,17 +120,17 @@ __device__ __forceinline__ int group_of_tile16(const GroupTable16 &tab, int grou
 
 // Place of the launch's t-th tile in the list of `total`: consecutive workgroups run on the 8 XCDs in turn, and each XCD takes a run of consecutive
 // tiles, so that its L2 sees neighbours.  -1: none.
-__device__ __forceinline__ int64_t place16(int64_t t, int64_t total)
+__device__ __forceinline__ int place16(int t, int total)
 {
-    const int64_t per = (total + 7) >> 3, i = t >> 3, at = (t & 7) * per + i;
-    return i < per && at < total ? at : -1;
+    const int per = (int)(((uint32_t)total + 7) >> 3), i = t >> 3;
+    const int64_t at = (int64_t)(t & 7) * per + i;
+    return i < per && at < total ? (int)at : -1;
 }
 // Tiles are walked in bands of 8 row tiles, column by column: the 32 to 64 tiles that an XCD works on at a time then share 8 panels of A and 4 to 8 of B.
 constexpr int BAND16 = 8;
-__device__ __forceinline__ void tile_of16(int64_t at, int row_tiles, int col_tiles, int &rt, int &ct)
+__device__ __forceinline__ void tile_of16(int at, int row_tiles, int col_tiles, int &rt, int &ct)
 {
-    const int64_t per = (int64_t)BAND16 * col_tiles;
-    const int band = (int)(at / per), in = (int)(at - band * per);
+    const int per = BAND16 * col_tiles, band = at / per, in = at - band * per;
     const int rows = min(BAND16, row_tiles - band * BAND16);
     ct = in / rows;
     rt = band * BAND16 + in - ct * rows;
@@ -212,11 +212,13 @@ template <class T> __device__ __forceinline__ void store8(uint16_t *p, bool whol
         if (i < there) p[i] = (uint16_t)((uint32_t)o[i >> 1] >> (16 * (i & 1)));
 }
 
-// Whether the epilogue's tensors have rows on 16-byte boundaries.
+// Whether the epilogue's tensors have rows on 16-byte boundaries: then p.n is a multiple of 8, or (EPI16_GRAD) rows have room for whole pieces.
 __device__ __forceinline__ bool whole_rows(const Gemm16 &p)
 {
     return p.pitch_out % 8 == 0 && ((uintptr_t)p.out & 15) == 0 && p.out_stride % 8 == 0 && (((uintptr_t)p.bias | (uintptr_t)p.residual | (uintptr_t)p.preact) & 15) == 0;
 }
+// Whether every tile of such a problem stores the same number of times, whatever of it exists: 16 stores of a wave with 128 x 64 outputs, twice that with preact.
+template <int EPI> __device__ __forceinline__ bool counted_stores(const Gemm16 &p) { return EPI != EPI16_STATS && !p.sums && !p.out_rows; }
 
 // Between a wave's writes to LDS and its other lanes' reads: for the compiler alone (a wave's LDS operations are in order), which sees one lane's accesses and may
 // otherwise send lanes that branch alike through writes and reads before the others' writes.
@@ -229,10 +231,10 @@ __device__ __forceinline__ void lanes_meet()
 // A wave's results on their way to memory, 32 rows of 64 columns, PASS rows at a time through LDS of the wave's own (PASS * 128 bytes at `at`): a lane holds four pieces of 16
 // bytes of one row, a store wants eight lanes to a row, whole lines of 128 bytes.  Stored as the lanes hold them, 32 bytes a row, a 256 x 256 tile's epilogue took 11 us.
 // Pieces lie at position c ^ (row & 7), so that writes and reads spread over all banks.
-template <int PASS, class Store> __device__ __forceinline__ void through_lds(uint32_t at, const v4i piece[2][2], Store &&store)
+template <int PASS, class Store> __device__ __forceinline__ void through_lds(uint32_t at, int lane, const v4i piece[2][2], Store &&store)
 {
     typedef __attribute__((address_space(3))) v4i *P;
-    const int lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5;
+    const int r = lane & 31, g = lane >> 5;
 #pragma unroll
     for (int ps = 0; ps < 32 / PASS; ps++) {
         if (PASS == 32 || (r / PASS) == ps) {
@@ -248,18 +250,22 @@ template <int PASS, class Store> __device__ __forceinline__ void through_lds(uin
         for (int q = 0; q < PASS / 8; q++) o[q] = lds_read16_abs(at + (uint32_t)(q * 8 + (lane >> 3)) * 128u + (((uint32_t)(lane & 7) ^ (uint32_t)(lane >> 3)) << 4));
         lanes_meet();
 #pragma unroll
-        for (int q = 0; q < PASS / 8; q++) store(ps * PASS + q * 8 + (lane >> 3), (lane & 7) * 8, o[q]);
+        for (int q = 0; q < PASS / 8; q++) store(ps * PASS + q * 8, o[q]);   // its first of eight rows
     }
 }
 
-// The results of one wave: MT x NT blocks of 32 x 32, every RS rows from row m0 on and side by side from column n0 of the product, of which rows below m_end exist.
-// group: the output that K-grouped problems write.  staging: PASS * 128 bytes of LDS of the wave's own.
+// The results of one wave: MT x NT blocks of 32 x 32, every RS rows from row mw on and side by side from column nw of the tile that begins at row m0 and column n0 of the
+// product, of which rows below m_end exist.  group: the output that K-grouped problems write.  staging: PASS * 128 bytes of LDS of the wave's own.  counted: whole pieces are stored
+// by way of a descriptor that drops what lies outside, always the same number of times (counted_stores).
 template <class T, int EPI, int MT, int NT, int RS, int PASS>
-__device__ __forceinline__ void epilogue16(const Gemm16 &p, v16f (&acc)[MT][NT], int group, int m0, int m_end, int n0, uint32_t staging)
+__device__ __forceinline__ void epilogue16(const Gemm16 &p, v16f (&acc)[MT][NT], int group, int tile_m, int m_end, int tile_n, int mw, int nw, uint32_t staging, bool whole, bool counted)
 {
     static_assert(NT == 2, "64 columns to a wave");
-    const int lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5;
-    if (n0 >= p.n) return;
+    // (opaque: what depends on the lane would otherwise be worked out before the loop over tiles and take registers from the loop over K)
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    const int r = lane & 31, g = lane >> 5, m0 = tile_m + mw, n0 = tile_n + nw;
+    if (!counted && n0 >= p.n) return;
     if constexpr (EPI == EPI16_STATS) {
         // 64 columns' largest logit and sum of exponentials, the two halves of the wave joined; a target's logit on the way
 #pragma unroll
@@ -288,13 +294,17 @@ __device__ __forceinline__ void epilogue16(const Gemm16 &p, v16f (&acc)[MT][NT],
         }
         return;
     } else {
-        const bool whole = whole_rows(p);   // and then p.n is a multiple of 8, or (EPI16_GRAD) the rows have room for whole pieces
         const float scale = EPI == EPI16_OUT && p.scale ? *p.scale : 1.0f;
         uint16_t *const out = p.out + (int64_t)group * p.out_stride;
-#pragma unroll
-        for (int i = 0; i < MT; i++) {
+        // counted: descriptors of the tile's rows that exist; a lane whose columns do not starts 2^31 bytes behind, past any of them
+        const int64_t tile_at = (int64_t)tile_m * p.pitch_out + tile_n;
+        const int tile_bytes = (int)min(((int64_t)max(m_end - tile_m, 0) * p.pitch_out - tile_n) * 2, (int64_t)0x7FFFFFF0);
+        const uint32_t pitch = (uint32_t)p.pitch_out * 2u;
+        const uint32_t lane_at = (uint32_t)(mw + (lane >> 3)) * pitch + (uint32_t)(nw + (lane & 7) * 8) * 2u + (n0 + (lane & 7) * 8 < p.n ? 0u : 0x80000000u);
+        static_for<MT>([&](auto i_c) {
+            constexpr int i = decltype(i_c)::value;
             const int first = m0 + RS * i, m = first + r;
-            if (first >= m_end) break;
+            if (!counted && first >= m_end) return;
             const bool there = m < m_end;
             float lse = 0.0f, slope = 0.0f;
             int target = -1;
@@ -349,17 +359,25 @@ __device__ __forceinline__ void epilogue16(const Gemm16 &p, v16f (&acc)[MT][NT],
                     piece[j][h] = pack8<T>(v[h]);
                 }
             }
-            if (EPI == EPI16_OUT && p.sums_out) continue;
-            if (whole) {
+            if (EPI == EPI16_OUT && p.sums_out) return;
+            if (counted) {
                 auto put = [&](uint16_t *base) {
-                    return [&, base](int row, int c, v4i o) {
-                        if (first + row >= m_end || n0 + c >= p.n) return;
-                        const int64_t to = EPI == EPI16_OUT && p.out_rows ? p.out_rows[first + row] : first + row;
-                        *reinterpret_cast<v4i *>(base + to * p.pitch_out + n0 + c) = o;
+                    const auto rs = __builtin_amdgcn_make_buffer_rsrc(base + tile_at, 0, tile_bytes, 0x00020000);
+                    return [=](int row, v4i o) { __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, o), rs, lane_at + (uint32_t)(RS * i + row) * pitch, 0, 0); };
+                };
+                if (EPI == EPI16_ACT && p.preact) through_lds<PASS>(staging, lane, pre, put(p.preact));
+                through_lds<PASS>(staging, lane, piece, put(out));
+            } else if (whole) {
+                auto put = [&](uint16_t *base) {
+                    return [&, base](int row, v4i o) {
+                        const int at = first + row + (lane >> 3), c = n0 + (lane & 7) * 8;
+                        if (at >= m_end || c >= p.n) return;
+                        const int64_t to = EPI == EPI16_OUT && p.out_rows ? p.out_rows[at] : at;
+                        *reinterpret_cast<v4i *>(base + to * p.pitch_out + c) = o;
                     };
                 };
-                if (EPI == EPI16_ACT && p.preact) through_lds<PASS>(staging, pre, put(p.preact));
-                through_lds<PASS>(staging, piece, put(out));
+                if (EPI == EPI16_ACT && p.preact) through_lds<PASS>(staging, lane, pre, put(p.preact));
+                through_lds<PASS>(staging, lane, piece, put(out));
             } else if (there) {
                 const int64_t to = EPI == EPI16_OUT && p.out_rows ? p.out_rows[m] : m;
 #pragma unroll
@@ -374,7 +392,7 @@ __device__ __forceinline__ void epilogue16(const Gemm16 &p, v16f (&acc)[MT][NT],
                             if (EPI == EPI16_ACT && p.preact) p.preact[to * p.pitch_out + n] = (uint16_t)((uint32_t)pre[j][h][x >> 1] >> (16 * (x & 1)));
                         }
             }
-        }
+        });
     }
 }
 

@@ -33,7 +33,8 @@ __global__ __launch_bounds__(S::THREADS, S::PER_CU * S::WAVES / 4) void gemm16_k
     const uint32_t lds = (uint32_t)uniform((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)smem);
     const int col_tiles = (p.n + S::TN - 1) / S::TN;
     const int row_tiles = uniform(rows_grouped ? tab.tile[p.groups] : (p.m + S::TM - 1) / S::TM);
-    const int64_t total = (int64_t)row_tiles * col_tiles * (rows_grouped ? 1 : p.groups);
+    const int total = row_tiles * col_tiles * (rows_grouped ? 1 : p.groups);   // (below 2^31: the launch checks)
+    const bool whole = whole_rows(p);
 
     // this lane's fragment reads in stage 0
     uint32_t fr_a[4], fr_b[4], ft_a[MT], ft_b[NT];
@@ -51,8 +52,8 @@ __global__ __launch_bounds__(S::THREADS, S::PER_CU * S::WAVES / 4) void gemm16_k
     for (int j = 0; j < NT; j++)
         ft_b[j] = lds + S::A_BYTES + (uint32_t)krow * KB::ROW + ((((uint32_t)(wn * NT + j) * 4 + part) ^ KB::swizzle(krow)) << 4) + (ti & 1) * 8u;
 
-    for (int64_t t = blockIdx.x; t < ((total + 7) & ~(int64_t)7); t += gridDim.x) {
-        int64_t at = place16(t, total);
+    for (int64_t t = blockIdx.x; t < ((total + 7) & ~7); t += gridDim.x) {
+        const int at = place16((int)t, total);
         if (at < 0) continue;
         int e = 0, rt, ct, m0, m_end, k_begin = 0, k_end = p.k;
         if (rows_grouped) {
@@ -61,8 +62,8 @@ __global__ __launch_bounds__(S::THREADS, S::PER_CU * S::WAVES / 4) void gemm16_k
             m0 = uniform(tab.start[e] + (rt - tab.tile[e]) * S::TM);
             m_end = uniform(tab.start[e + 1]);
         } else {
-            const int64_t per = (int64_t)row_tiles * col_tiles;
-            e = (int)(at / per);
+            const int per = row_tiles * col_tiles;
+            e = at / per;
             tile_of16(at - e * per, row_tiles, col_tiles, rt, ct);
             m0 = rt * S::TM;
             m_end = p.m;
@@ -155,7 +156,7 @@ __global__ __launch_bounds__(S::THREADS, S::PER_CU * S::WAVES / 4) void gemm16_k
         CCH_WAIT_LGKM0();
         CCH_BARRIER();
         // (results pass through the stages, which the next tile's requests overwrite)
-        epilogue16<T, EPI, MT, NT, 32, 32>(p, acc, e, m0 + wm * MT * 32, m_end, n0 + wn * NT * 32, lds + (uint32_t)wave * 4096u);
+        epilogue16<T, EPI, MT, NT, 32, 32>(p, acc, e, m0, m_end, n0, wm * MT * 32, wn * NT * 32, lds + (uint32_t)wave * 4096u, whole, false);
         CCH_WAIT_LGKM0();
         CCH_BARRIER();
     }
