@@ -19,8 +19,8 @@ enum Epilogue16 {
     EPI16_GRAD = 3,   // cross entropy: the logits' gradient times grad_scale
 };
 
-// The kernels, numbered as the switch "matmul16_kernel" names them: tiles of 128 x 128 and 256 x 256.
-enum Kernel16 { KERNEL16_128 = 0, KERNEL16_256 = 1, NUM_KERNELS16 };
+// The kernels, numbered as the switch "matmul16_kernel" names them: tiles of 128 x 128, 256 x 256, and of few rows.
+enum Kernel16 { KERNEL16_128 = 0, KERNEL16_256 = 1, KERNEL16_ROWS = 2, NUM_KERNELS16 };
 constexpr int64_t BIG_TILES16 = 192;     // tiles of 256 x 256 from which on they are taken: three quarters of the CUs
 extern std::atomic<int> g_kernel16;   // -1: chosen per problem; else that one wherever it takes the problem
 

@@ -1,6 +1,7 @@
 // Which kernel a product of 16-bit operands runs on.
 #pragma once
 #include "gemm16_big_kernel.h"
+#include "gemm16_stream_kernel.h"
 
 namespace cch {
 
@@ -18,6 +19,16 @@ template <class T, int LAYOUT, int EPI> int shape16(const Gemm16 &p, hipStream_t
     int dev = 0, cus = 0;
     CCH_HIP(hipGetDevice(&dev));
     CCH_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
+    if constexpr (LAYOUT != ROWS_TN && (EPI == EPI16_OUT || EPI == EPI16_ACT)) {
+        const int64_t per_group = (p.m + p.groups - 1) / p.groups;
+        const bool plain = !p.a_rows && !p.sums && !p.out_rows && !p.scale;
+        const int asked = g_kernel16.load();
+        if (plain && (asked == KERNEL16_ROWS || (asked < 0 && per_group <= 32))) {
+            if (per_group <= 8) return launch16_stream_rows<T, LAYOUT, EPI, 8>(p, tiles16(p, 8, Stream16<LAYOUT, 8>::TN), stream);
+            if (per_group <= 16) return launch16_stream_rows<T, LAYOUT, EPI, 16>(p, tiles16(p, 16, Stream16<LAYOUT, 16>::TN), stream);
+            return launch16_stream_rows<T, LAYOUT, EPI, 32>(p, tiles16(p, 32, Stream16<LAYOUT, 32>::TN), stream);
+        }
+    }
     const int64_t big = tiles16(p, 256, 256);
     const int asked = g_kernel16.load();
     CCH_REQUIRE(tiles16(p, 128, 128) < (int64_t)1 << 31, "a product of %d x %d in %d groups has too many tiles", p.m, p.n, p.groups);

@@ -8,7 +8,7 @@ from bounds16 import check, rounded, sum_error
 pytestmark = pytest.mark.gpu
 
 
-@pytest.fixture(params=[-1, 0, 1], ids=["chosen", "128x128", "256x256"], autouse=True)
+@pytest.fixture(params=[-1, 0, 1, 2], ids=["chosen", "128x128", "256x256", "rows"], autouse=True)
 def kernel16(request):
     """The kernel that a product goes to by itself, and each one."""
     cc.set_option("matmul16_kernel", request.param)
