@@ -22,6 +22,10 @@ enum Epilogue16 {
 // The kernels, numbered as the switch "matmul16_kernel" names them: tiles of 128 x 128, 256 x 256, and of few rows.
 enum Kernel16 { KERNEL16_128 = 0, KERNEL16_256 = 1, KERNEL16_ROWS = 2, NUM_KERNELS16 };
 constexpr int64_t BIG_TILES16 = 192;     // tiles of 256 x 256 from which on they are taken: three quarters of the CUs
+struct Plan16 {
+    int kernel, splits, deep;   // Kernel16, parts of K, four stages (tiles of 128 x 128)
+};
+Plan16 plan16(const struct Gemm16 &p, int layout, int epilogue);
 extern std::atomic<int> g_kernel16;   // -1: chosen per problem; else that one wherever it takes the problem
 
 struct Gemm16 {
@@ -38,6 +42,9 @@ struct Gemm16 {
     int m_src;
     const int32_t *out_rows;               // row of the output that row i goes to, or nullptr
     int half;                              // IEEE half, else bf16
+    float *partial;                        // fp32, for sums of parts of K; K is not split where partial_bytes are too few
+    int64_t partial_bytes;
+    int splits;                            // parts of K (set by the launch)
     // EPI16_OUT
     const float *scale;                    // device, or nullptr: 1
     float *sums;                           // fp32 [m, n], or nullptr: a product in pieces of K.  sums_in: added to the sum; sums_out: takes it in place of out
@@ -56,8 +63,23 @@ struct Gemm16 {
     float z2, grad_scale;                  // 2 * z_coef
 };
 
-// Rows of the output, or the groups' K, that a launch may find: its grid's upper bound.
+// Bytes of `partial` that the product may use (its sizes, groups and pointers' being there or not as at the launch; no GPU needed).
+int64_t partial16_bytes(const Gemm16 &p, int layout, int epilogue);
 int gemm16_launch(const Gemm16 &p, int layout, int epilogue, hipStream_t stream);
+
+// Tiles that a launch may have: the groups' sizes are on the device.
+inline int64_t tiles16(const Gemm16 &p, int tm, int tn)
+{
+    const int64_t cols = (p.n + tn - 1) / tn;
+    if (p.k_grouped) return (int64_t)p.groups * ((p.m + tm - 1) / tm) * cols;
+    return (p.group_sizes ? p.m / tm + (p.groups < p.m ? p.groups : p.m) : (p.m + tm - 1) / tm) * cols;
+}
+// Rows of a tile of the kernel for few rows: a group's share of them.
+inline int rows16(const Gemm16 &p)
+{
+    const int share = (int)(((int64_t)p.m + p.groups - 1) / p.groups);
+    return share <= 8 ? 8 : share <= 16 ? 16 : 32;
+}
 
 inline bool whole16(int64_t cols) { return cols % 8 == 0; }
 inline int64_t pitch16(int64_t cols) { return (cols + 7) & ~(int64_t)7; }
@@ -73,6 +95,12 @@ struct Carve {
         T *p = reinterpret_cast<T *>(at);
         at += round256(bytes);
         return p;
+    }
+    // What is left of a workspace to a product's parts.
+    void rest(Gemm16 &p, void *workspace, int64_t bytes) const
+    {
+        p.partial = reinterpret_cast<float *>(at);
+        p.partial_bytes = workspace ? static_cast<uint8_t *>(workspace) + bytes - at : 0;
     }
 };
 

@@ -6,14 +6,110 @@
 
 namespace cch {
 
-int gemm16_launch_bf16(const Gemm16 &p, int layout, int epilogue, hipStream_t stream);   // gemm16_bf16.hip
-int gemm16_launch_f16(const Gemm16 &p, int layout, int epilogue, hipStream_t stream);    // gemm16_f16.hip
-
+int gemm16_launch_bf16(const Gemm16 &p, const Plan16 &plan, int layout, int epilogue, hipStream_t stream);   // gemm16_bf16.hip
+int gemm16_launch_f16(const Gemm16 &p, const Plan16 &plan, int layout, int epilogue, hipStream_t stream);    // gemm16_f16.hip
 std::atomic<int> g_kernel16{-1};
 
-int gemm16_launch(const Gemm16 &p, int layout, int epilogue, hipStream_t stream)
+// ---- which kernel, and K in how many parts: by sizes alone, so that what a call's workspace holds does not depend on the device.
+Plan16 plan16(const Gemm16 &p, int layout, int epilogue)
 {
-    return p.half ? gemm16_launch_f16(p, layout, epilogue, stream) : gemm16_launch_bf16(p, layout, epilogue, stream);
+    constexpr int CUS = 256;
+    const int asked = g_kernel16.load();
+    Plan16 plan{KERNEL16_128, 1, 0};
+    const bool results = epilogue == EPI16_OUT || epilogue == EPI16_ACT;
+    if (layout != ROWS_TN && results && !p.a_rows && !p.sums && !p.out_rows && !p.scale &&
+        (asked == KERNEL16_ROWS || (asked < 0 && (int64_t)p.m <= 32 * (int64_t)p.groups)))
+        return {KERNEL16_ROWS, 1, 0};
+    if (!p.a_rows && p.pitch_out < MAX_PITCH16 / 2 && (asked == KERNEL16_256 || (asked < 0 && tiles16(p, 256, 256) >= BIG_TILES16))) return {KERNEL16_256, 1, 0};
+    // tiles of 128 x 128, about: a group's rows or K are taken to be its share
+    const int64_t share = p.k_grouped || !p.group_sizes ? p.m : (p.m + p.groups - 1) / p.groups, each = (share + 127) / 128 * ((p.n + 127) / 128);
+    const int64_t tiles = each * p.groups, steps = ((p.k_grouped ? (p.k + p.groups - 1) / p.groups : p.k) + 63) / 64;
+    if (results && !p.sums && tiles < CUS) {
+        // us: a step of a workgroup with four stages, its first requests and epilogue, the second launch and the parts' way to memory and back
+        const double STEP = 0.27, START = 2.0, JOIN = 2.5, PER_BYTE = 2.0 / 4e6;
+        const double bytes = 4.0 * p.m * p.n * (p.k_grouped ? p.groups : 1);
+        double best = 0;
+        for (int s = 1; s <= 32 && s <= steps; s++) {
+            const double rounds = (double)((tiles * s + CUS - 1) / CUS);
+            const double us = rounds * ((double)((steps + s - 1) / s) * STEP + START) + (s > 1 ? JOIN + s * bytes * PER_BYTE : 0);
+            if (s == 1 || us < best) {
+                best = us;
+                plan.splits = s;
+            }
+        }
+    }
+    plan.deep = tiles * plan.splits <= CUS;
+    return plan;
+}
+
+static int64_t parts_bytes(const Gemm16 &p, int splits) { return splits > 1 ? round256((int64_t)splits * (p.k_grouped ? p.groups : 1) * p.m * p.n * 4) : 0; }
+int64_t partial16_bytes(const Gemm16 &p, int layout, int epilogue) { return parts_bytes(p, plan16(p, layout, epilogue).splits); }
+
+// ---- the parts of K added up in their order, with the product's epilogue.  VEC elements of a row to a thread.
+template <class T, int EPI, int VEC> __global__ __launch_bounds__(256) void join16_kernel(Gemm16 p, int64_t outputs, int64_t per_row)
+{
+    __shared__ int used;
+    if (!p.k_grouped && p.group_sizes) {
+        if (threadIdx.x < 64) {
+            uint32_t sum = 0;
+            for (int g = threadIdx.x; g < p.groups; g += 64) sum = sat_add(sum, (uint32_t)min(max(p.group_sizes[g], 0), p.m));
+            const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan_sat(sum), 63);
+            if (threadIdx.x == 0) used = (int)min(all, (uint32_t)p.m);
+        }
+        __syncthreads();
+    } else {
+        if (threadIdx.x == 0) used = p.m;
+        __syncthreads();
+    }
+    const float scale = EPI == EPI16_OUT && p.scale ? *p.scale : 1.0f;
+    const int64_t one = (int64_t)p.m * p.n, all = one * (p.k_grouped ? p.groups : 1);
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < outputs; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / per_row, m = p.k_grouped ? row % p.m : row, e = p.k_grouped ? row / p.m : 0;
+        const int n = (int)(i - row * per_row) * VEC;
+        if (m >= used && !p.zero_rest) continue;
+        float v[VEC] = {};
+        if (m < used)
+            for (int s = 0; s < p.splits; s++) {
+                typedef float F __attribute__((ext_vector_type(VEC)));
+                const F a = *reinterpret_cast<const F *>(p.partial + s * all + row * p.n + n);
+#pragma unroll
+                for (int x = 0; x < VEC; x++) v[x] += a[x];
+            }
+        const int64_t to = e * p.out_stride + (EPI == EPI16_OUT && p.out_rows ? p.out_rows[m] : m) * p.pitch_out + n;
+#pragma unroll
+        for (int x = 0; x < VEC; x++) {
+            if constexpr (EPI == EPI16_ACT) {
+                if (p.bias) v[x] += T::to(p.bias[n + x]);
+                if (p.preact) p.preact[to + x] = T::from(v[x]);
+                v[x] = act_value(v[x], p.act);
+                if (p.residual) v[x] += T::to(p.residual[to + x]);
+            } else {
+                v[x] *= scale;
+            }
+            p.out[to + x] = T::from(v[x]);
+        }
+    }
+}
+
+template <class T> static int join16(const Gemm16 &p, int epilogue, hipStream_t stream)
+{
+    const bool four = p.n % 4 == 0;
+    const int64_t per_row = four ? p.n / 4 : p.n, outputs = per_row * p.m * (p.k_grouped ? p.groups : 1);
+    auto kern = epilogue == EPI16_ACT ? (four ? join16_kernel<T, EPI16_ACT, 4> : join16_kernel<T, EPI16_ACT, 1>)
+                                      : (four ? join16_kernel<T, EPI16_OUT, 4> : join16_kernel<T, EPI16_OUT, 1>);
+    hipLaunchKernelGGL(kern, dim3((unsigned)std::min<int64_t>((outputs + 255) / 256, 1 << 16)), dim3(256), 0, stream, p, outputs, per_row);
+    return launch_status("join16_kernel");
+}
+
+int gemm16_launch(const Gemm16 &problem, int layout, int epilogue, hipStream_t stream)
+{
+    Gemm16 p = problem;
+    Plan16 plan = plan16(p, layout, epilogue);
+    if (!p.partial || parts_bytes(p, plan.splits) > p.partial_bytes) plan.splits = 1;
+    p.splits = plan.splits;
+    if (const int rc = p.half ? gemm16_launch_f16(p, plan, layout, epilogue, stream) : gemm16_launch_bf16(p, plan, layout, epilogue, stream)) return rc;
+    if (p.splits == 1) return CCH_OK;
+    return p.half ? join16<F16>(p, epilogue, stream) : join16<Bf16>(p, epilogue, stream);
 }
 
 // One thread, 16 bytes of the copy.

@@ -3,6 +3,9 @@
 
 namespace cch {
 
-int gemm16_launch_bf16(const Gemm16 &p, int layout, int epilogue, hipStream_t stream) { return choose16<Bf16>(p, layout, epilogue, stream); }
+int gemm16_launch_bf16(const Gemm16 &p, const Plan16 &plan, int layout, int epilogue, hipStream_t stream)
+{
+    return choose16<Bf16>(p, plan, layout, epilogue, stream);
+}
 
 }  // namespace cch

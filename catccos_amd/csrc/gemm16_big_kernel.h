@@ -381,10 +381,13 @@ __global__ __launch_bounds__(Big16::THREADS, 2) void gemm16_big_kernel(Gemm16 p)
     CCH_WAIT_VM_LGKM0(0);   // (requests past the last tile fetch nothing, but they write zeros to LDS)
 }
 
-template <class T, int LAYOUT, int EPI> int launch16_big(const Gemm16 &p, int64_t tiles, int cus, hipStream_t stream)
+template <class T, int LAYOUT, int EPI> int launch16_big(const Gemm16 &p, int64_t tiles, hipStream_t stream)
 {
     static std::atomic<uint64_t> attr_set{0};
     auto kernel = gemm16_big_kernel<T, LAYOUT, EPI>;
+    int dev = 0, cus = 0;
+    CCH_HIP(hipGetDevice(&dev));
+    CCH_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
     if (const int rc = allow_lds16(reinterpret_cast<const void *>(kernel), Big16::LDS, attr_set)) return rc;
     const int64_t grid = std::min<int64_t>((tiles + 7) & ~(int64_t)7, std::max(cus & ~7, 8));   // (a multiple of 8: place16)
     kernel<<<dim3((uint32_t)grid), dim3(Big16::THREADS), Big16::LDS, stream>>>(p);

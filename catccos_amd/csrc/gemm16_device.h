@@ -396,6 +396,32 @@ __device__ __forceinline__ void epilogue16(const Gemm16 &p, v16f (&acc)[MT][NT],
     }
 }
 
+// The fp32 sums of one part of K: MT x NT blocks from row m0 and column n0 on, rows below m_end, to rows of n.
+template <int MT, int NT> __device__ __forceinline__ void store_part16(const Gemm16 &p, const v16f (&acc)[MT][NT], float *to, int m0, int m_end, int n0)
+{
+    const int lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5;
+#pragma unroll
+    for (int i = 0; i < MT; i++) {
+        const int m = m0 + 32 * i + r;
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const int n = n0 + 32 * j + 8 * q + 4 * g, left = p.n - n;
+                if (m >= m_end || left <= 0) continue;
+                float *s = to + (int64_t)m * p.n + n;
+                const f32x4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                if (p.n % 4 == 0) {
+                    *reinterpret_cast<f32x4 *>(s) = v;
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 4; x++)
+                        if (x < left) s[x] = v[x];
+                }
+            }
+    }
+}
+
 // Rows behind the last group: zeros.
 __device__ __forceinline__ void zero_rest16(const Gemm16 &p, int first)
 {

@@ -1,6 +1,8 @@
-// Products of 16-bit operands on tiles of (32 MT WM) x (32 NT WN): WM x WN waves of MT x NT blocks of 32 x 32, K in steps of 64 elements, two stages in LDS that
-// are filled straight from memory.  A step's requests are issued before the step before it is multiplied; one barrier a step publishes what has landed and
-// frees what was read.  Two workgroups of the 128 x 128 form share a CU, so that one's epilogue and waits pass under the other's matrix instructions.
+// Products of 16-bit operands on tiles of (32 MT WM) x (32 NT WN): WM x WN waves of MT x NT blocks of 32 x 32, K in steps of 64 elements, DEPTH stages in LDS that are
+// filled straight from memory, DEPTH - 1 steps ahead; one barrier a step publishes what has landed and frees what was read.  A 128 x 128 step is 512 clocks of matrix
+// instructions, while memory answers in 1500 to 2500: with two stages two workgroups share a CU, so that one's waits and epilogue pass under the other's matrix instructions; where there are not
+// that many workgroups, one has four stages (256 x 4096 x 7168 on 64 tiles: 97 us with two).  Tiles too few for the chip are split along K (p.splits): each part leaves fp32 sums,
+// which gemm16_join adds up in the parts' order.
 #pragma once
 #include <atomic>
 
@@ -8,10 +10,10 @@
 
 namespace cch {
 
-template <int MT_, int NT_, int WM_, int WN_, int PER_CU_> struct Shape16 {
-    static constexpr int MT = MT_, NT = NT_, WM = WM_, WN = WN_, WAVES = WM * WN, THREADS = 64 * WAVES, PER_CU = PER_CU_;
+template <int MT_, int NT_, int WM_, int WN_, int DEPTH_> struct Shape16 {
+    static constexpr int MT = MT_, NT = NT_, WM = WM_, WN = WN_, WAVES = WM * WN, THREADS = 64 * WAVES, DEPTH = DEPTH_, PER_CU = DEPTH == 2 ? 2 : 1;
     static constexpr int TM = 32 * MT * WM, TN = 32 * NT * WN;      // tile
-    static constexpr int A_BYTES = TM * 128, B_BYTES = TN * 128, STAGE = A_BYTES + B_BYTES, LDS = 2 * STAGE;
+    static constexpr int A_BYTES = TM * 128, B_BYTES = TN * 128, STAGE = A_BYTES + B_BYTES, LDS = DEPTH * STAGE;
     static constexpr int NJA = A_BYTES / 1024 / WAVES, NJB = B_BYTES / 1024 / WAVES;   // requests of a wave and step
 };
 
@@ -45,16 +47,19 @@ __global__ __launch_bounds__(S::THREADS, S::PER_CU * S::WAVES / 4) void gemm16_k
         fr_b[kk] = lds + S::A_BYTES + (uint32_t)(wn * NT * 32 + r) * 128u + chunk;
     }
     const int krow = (tq >> 1) * 8 + (ti >> 2);                                 // (and 4 more by the second load)
-    const uint32_t part = (uint32_t)((tq & 1) * 2 + ((ti & 3) >> 1));           // chunk among a block's four
+    const uint32_t quarter = (uint32_t)((tq & 1) * 2 + ((ti & 3) >> 1));        // chunk among a block's four
 #pragma unroll
-    for (int i = 0; i < MT; i++) ft_a[i] = lds + (uint32_t)krow * KA::ROW + ((((uint32_t)(wm * MT + i) * 4 + part) ^ KA::swizzle(krow)) << 4) + (ti & 1) * 8u;
+    for (int i = 0; i < MT; i++) ft_a[i] = lds + (uint32_t)krow * KA::ROW + ((((uint32_t)(wm * MT + i) * 4 + quarter) ^ KA::swizzle(krow)) << 4) + (ti & 1) * 8u;
 #pragma unroll
     for (int j = 0; j < NT; j++)
-        ft_b[j] = lds + S::A_BYTES + (uint32_t)krow * KB::ROW + ((((uint32_t)(wn * NT + j) * 4 + part) ^ KB::swizzle(krow)) << 4) + (ti & 1) * 8u;
+        ft_b[j] = lds + S::A_BYTES + (uint32_t)krow * KB::ROW + ((((uint32_t)(wn * NT + j) * 4 + quarter) ^ KB::swizzle(krow)) << 4) + (ti & 1) * 8u;
 
-    for (int64_t t = blockIdx.x; t < ((total + 7) & ~7); t += gridDim.x) {
-        const int at = place16((int)t, total);
+    const int parts = p.splits * total;   // (below 2^31)
+    for (int64_t t = blockIdx.x; t < ((parts + 7) & ~7); t += gridDim.x) {
+        int at = place16((int)t, parts);
         if (at < 0) continue;
+        const int part = at % p.splits;
+        at /= p.splits;
         int e = 0, rt, ct, m0, m_end, k_begin = 0, k_end = p.k;
         if (rows_grouped) {
             tile_of16(at, row_tiles, col_tiles, rt, ct);
@@ -71,8 +76,10 @@ __global__ __launch_bounds__(S::THREADS, S::PER_CU * S::WAVES / 4) void gemm16_k
             k_end = uniform(tab.start[e + 1]);
         }
         const int n0 = ct * S::TN;
-        const int rows = min(m_end - m0, S::TM), cols = min(p.n - n0, S::TN), kk_all = k_end - k_begin;
-        const int steps = (kk_all + 63) >> 6;
+        // this part's steps: `first`.. of the group's K
+        const int rows = min(m_end - m0, S::TM), cols = min(p.n - n0, S::TN), k_all = k_end - k_begin, steps_all = (k_all + 63) >> 6;
+        const int each = (steps_all + p.splits - 1) / p.splits, first = min(part * each, steps_all), steps = min(each, steps_all - first);
+        const int k_stop = min((first + steps) * 64, k_all);   // from k_begin
 
         // requests: descriptors and this lane's offsets
         uint32_t off_a[NJA], off_b[NJB];
@@ -109,20 +116,20 @@ __global__ __launch_bounds__(S::THREADS, S::PER_CU * S::WAVES / 4) void gemm16_k
         }
         // (K contiguous: a lane whose 8 elements begin at or past K fetches nothing; K is a multiple of 8 or its rows are padded with zeros)
         auto request = [&](int step) {
-            const uint32_t stage = lds + (uint32_t)(step & 1) * S::STAGE;
-            const int k0 = step * 64;
-            if constexpr (A_KM) rs_a = kmajor_rsrc(a0, p.pitch_a, k0, kk_all, m0, p.m);
-            if constexpr (B_KM) rs_b = kmajor_rsrc(b0, p.pitch_b, k0, kk_all, n0, p.n);
+            const uint32_t stage = lds + (uint32_t)(step % S::DEPTH) * S::STAGE;
+            const int k0 = (first + step) * 64;
+            if constexpr (A_KM) rs_a = kmajor_rsrc(a0, p.pitch_a, k0, k_stop, m0, p.m);
+            if constexpr (B_KM) rs_b = kmajor_rsrc(b0, p.pitch_b, k0, k_stop, n0, p.n);
 #pragma unroll
             for (int j = 0; j < NJA; j++) {
                 const int row = (wave * NJA + j) * 8 + (lane >> 3);
-                const bool in = A_KM || (int)(((uint32_t)(lane & 7) ^ swizzle_of_row(row)) * 8u) < p.k - k0;
+                const bool in = A_KM || (int)(((uint32_t)(lane & 7) ^ swizzle_of_row(row)) * 8u) < k_stop - k0;
                 load16_to_lds(rs_a, in ? off_a[j] : NO_FETCH, A_KM ? 0u : (uint32_t)k0 * 2u, stage + (uint32_t)(wave * NJA + j) * 1024u);
             }
 #pragma unroll
             for (int j = 0; j < NJB; j++) {
                 const int row = (wave * NJB + j) * 8 + (lane >> 3);
-                const bool in = B_KM || (int)(((uint32_t)(lane & 7) ^ swizzle_of_row(row)) * 8u) < p.k - k0;
+                const bool in = B_KM || (int)(((uint32_t)(lane & 7) ^ swizzle_of_row(row)) * 8u) < k_stop - k0;
                 load16_to_lds(rs_b, in ? off_b[j] : NO_FETCH, B_KM ? 0u : (uint32_t)k0 * 2u, stage + S::A_BYTES + (uint32_t)(wave * NJB + j) * 1024u);
             }
         };
@@ -132,12 +139,14 @@ __global__ __launch_bounds__(S::THREADS, S::PER_CU * S::WAVES / 4) void gemm16_k
         for (int i = 0; i < MT; i++)
 #pragma unroll
             for (int j = 0; j < NT; j++) acc[i][j] = (v16f)(0.0f);
-        if (steps > 0) request(0);
+        // (requests past the last step fetch nothing: every wait counts the same)
+#pragma unroll
+        for (int i = 0; i < S::DEPTH - 1; i++) request(i);
         for (int step = 0; step < steps; step++) {
-            CCH_WAIT_VM_LGKM0(0);
+            CCH_WAIT_VM_LGKM0((S::DEPTH - 2) * (NJA + NJB));
             CCH_BARRIER();
-            if (step + 1 < steps) request(step + 1);
-            const uint32_t stage = (uint32_t)(step & 1) * S::STAGE;
+            request(step + S::DEPTH - 1);
+            const uint32_t stage = (uint32_t)(step % S::DEPTH) * S::STAGE;
 #pragma unroll
             for (int kk = 0; kk < 4; kk++) {
                 v4i fa[MT], fb[NT];
@@ -153,8 +162,14 @@ __global__ __launch_bounds__(S::THREADS, S::PER_CU * S::WAVES / 4) void gemm16_k
                     for (int j = 0; j < NT; j++) acc[i][j] = T::mfma(fb[j], fa[i], acc[i][j]);
             }
         }
-        CCH_WAIT_LGKM0();
+        CCH_WAIT_VM_LGKM0(0);
         CCH_BARRIER();
+        if constexpr (EPI == EPI16_OUT || EPI == EPI16_ACT) {
+            if (p.splits > 1) {
+                store_part16<MT, NT>(p, acc, p.partial + ((int64_t)part * (rows_grouped ? 1 : p.groups) + (rows_grouped ? 0 : e)) * p.m * p.n, m0 + wm * MT * 32, m_end, n0 + wn * NT * 32);
+                continue;
+            }
+        }
         // (results pass through the stages, which the next tile's requests overwrite)
         epilogue16<T, EPI, MT, NT, 32, 32>(p, acc, e, m0, m_end, n0, wm * MT * 32, wn * NT * 32, lds + (uint32_t)wave * 4096u, whole, false);
         CCH_WAIT_LGKM0();
@@ -181,7 +196,7 @@ template <class T, int LAYOUT, int EPI, class S> int launch16(const Gemm16 &p, i
     static std::atomic<uint64_t> attr_set{0};
     auto kernel = gemm16_kernel<T, LAYOUT, EPI, S>;
     if (const int rc = allow_lds16(reinterpret_cast<const void *>(kernel), S::LDS, attr_set)) return rc;
-    const int64_t grid = std::min<int64_t>((tiles + 7) & ~(int64_t)7, (int64_t)1 << 22);   // (a multiple of 8: place16)
+    const int64_t grid = std::min<int64_t>((tiles * p.splits + 7) & ~(int64_t)7, (int64_t)1 << 22);   // (a multiple of 8: place16)
     kernel<<<dim3((uint32_t)grid), dim3(S::THREADS), S::LDS, stream>>>(p);
     return launch_status("gemm16_kernel");
 }

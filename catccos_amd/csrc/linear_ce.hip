@@ -182,8 +182,40 @@ static int ce_gather(const uint16_t *x, const int32_t *pos, uint16_t *rows, uint
 // Rows of x are picked by the product's requests where it runs on tiles of 128 x 128, offsets of 32 bits reach them all and none needs padding; else they are copied.
 static bool ce_picks(int64_t t, int64_t h, int64_t v) { return whole16(h) && t * h * 2 <= 0x7FFFFFF0 && ((t + 255) / 256) * ((v + 255) / 256) < BIG_TILES16; }
 
+// The two products of a piece of c columns of the gradient, pointers apart.
+static const int32_t CE_COUNT = 0;   // stands for the number of tokens that count, where only that there is one matters
+static Gemm16 ce_grad_w(const int32_t *count, int64_t t, int64_t h, int64_t c)
+{
+    Gemm16 p{};
+    p.pitch_a = pitch16(c);
+    p.pitch_b = pitch16(h);
+    p.pitch_out = h;
+    p.m = (int)c;
+    p.n = (int)h;
+    p.k = (int)t;
+    p.k_grouped = 1;
+    p.groups = 1;
+    p.group_sizes = count;
+    return p;
+}
+static Gemm16 ce_grad_x(const int32_t *count, const int32_t *src, float *sums, int64_t t, int64_t h, int64_t c)
+{
+    Gemm16 p{};
+    p.pitch_a = pitch16(c);
+    p.pitch_b = pitch16(h);
+    p.pitch_out = h;
+    p.m = (int)t;
+    p.n = (int)h;
+    p.k = (int)c;
+    p.groups = 1;
+    p.group_sizes = count;
+    p.out_rows = src;
+    p.sums = sums;
+    return p;
+}
+
 struct CeWorkspace {
-    int64_t src, pos, target, lse, count, scalar, logit, stats, rows, w, d, sums, end;
+    int64_t src, pos, target, lse, count, scalar, logit, stats, rows, w, d, sums, parts, end;
 };
 static CeWorkspace ce_workspace(int64_t t, int64_t h, int64_t v, bool backward)
 {
@@ -210,6 +242,8 @@ static CeWorkspace ce_workspace(int64_t t, int64_t h, int64_t v, bool backward)
         at.scalar = piece(4);
         at.d = piece(t * pitch16(c) * 2);
         if (c < v) at.sums = piece(t * h * 4);
+        at.parts = piece(std::max(partial16_bytes(ce_grad_w(&CE_COUNT, t, h, c), ROWS_TN, EPI16_OUT),
+                                  c < v ? 0 : partial16_bytes(ce_grad_x(&CE_COUNT, &CE_COUNT, nullptr, t, h, c), ROWS_NN, EPI16_OUT)));
     }
     return at;
 }
@@ -340,11 +374,11 @@ extern "C" int cch_linear_cross_entropy_backward(const float *grad_loss, const v
     const int64_t piece = ce_piece(t, v);
     for (int64_t v0 = 0; v0 < v; v0 += piece) {
         const int64_t c = std::min(piece, v - v0);
-        Gemm16 p{};
-        p.half = half;
-        p.groups = 1;
-        p.group_sizes = tk.count;
         if (t > 0) {
+            Gemm16 p{};
+            p.half = half;
+            p.groups = 1;
+            p.group_sizes = tk.count;
             p.a = rows;
             p.pitch_a = pitch16(h);
             p.b = pw + v0 * ldw;
@@ -361,39 +395,27 @@ extern "C" int cch_linear_cross_entropy_backward(const float *grad_loss, const v
             p.grad_scale = tk.grad_scale;
             if (const int rc = gemm16_launch(p, ROWS_NK, EPI16_GRAD, s)) return rc;
         }
+        const Carve parts{ws + at.parts};
         if (gw) {
-            Gemm16 q = p;
+            Gemm16 q = ce_grad_w(tk.count, t, h, c);
+            q.half = half;
             q.a = d;
-            q.pitch_a = pitch16(c);
             q.b = rows;
-            q.pitch_b = pitch16(h);
             q.out = gw + v0 * h;
-            q.pitch_out = h;
-            q.m = (int)c;
-            q.n = (int)h;
-            q.k = (int)t;
-            q.k_grouped = 1;
             q.scale = tk.scalar;
+            parts.rest(q, workspace, workspace_bytes);
             if (const int rc = gemm16_launch(q, ROWS_TN, EPI16_OUT, s)) return rc;
         }
         if (gx && t > 0) {
-            Gemm16 q = p;
+            Gemm16 q = ce_grad_x(tk.count, tk.src, piece < v ? f32(at.sums) : nullptr, t, h, c);
+            q.half = half;
             q.a = d;
-            q.pitch_a = pitch16(c);
             q.b = pw + v0 * ldw;
-            q.pitch_b = ldw;
             q.out = gx;
-            q.pitch_out = h;
-            q.m = (int)t;
-            q.n = (int)h;
-            q.k = (int)c;
-            q.out_rows = tk.src;
             q.scale = tk.scalar;
-            if (piece < v) {
-                q.sums = f32(at.sums);
-                q.sums_in = v0 > 0;
-                q.sums_out = v0 + piece < v;
-            }
+            q.sums_in = v0 > 0;
+            q.sums_out = v0 + piece < v;
+            parts.rest(q, workspace, workspace_bytes);
             if (const int rc = gemm16_launch(q, ROWS_NN, EPI16_OUT, s)) return rc;
         }
     }

@@ -50,26 +50,60 @@ static Gemm16 product16(const uint16_t *x, int64_t pitch_x, const uint16_t *w, i
     return p;
 }
 
+// The two products of a backward pass, pointers apart: grad_x's and grad_w's.
+static Gemm16 grad_x_product(const int32_t *sizes, int64_t e, int64_t t, int64_t n, int64_t k, int trans_b, int dtype)
+{
+    // W^T of weights [n, k] is weights [k', n'] with k' = n
+    Gemm16 p = product16(nullptr, pitch16(n), nullptr, pitch16(trans_b ? k : n), nullptr, t, k, n, !trans_b, dtype);
+    p.b_stride = (trans_b ? n : k) * p.pitch_b;
+    p.group_sizes = sizes;
+    p.groups = (int)e;
+    p.zero_rest = sizes != nullptr;
+    return p;
+}
+static Gemm16 grad_w_product(const int32_t *sizes, int64_t e, int64_t t, int64_t n, int64_t k, int trans_b, int dtype)
+{
+    Gemm16 p = trans_b ? product16(nullptr, pitch16(n), nullptr, pitch16(k), nullptr, n, k, t, 0, dtype) : product16(nullptr, pitch16(k), nullptr, pitch16(n), nullptr, k, n, t, 0, dtype);
+    p.b_stride = 0;
+    p.out_stride = n * k;
+    p.group_sizes = sizes;
+    p.groups = (int)e;
+    p.k_grouped = 1;
+    return p;
+}
+static Gemm16 grouped_product(const uint16_t *x, const uint16_t *w, const int32_t *sizes, uint16_t *out, int64_t e, int64_t t, int64_t n, int64_t k, int trans_b, int dtype)
+{
+    Gemm16 p = product16(x, pitch16(k), w, pitch16(trans_b ? k : n), out, t, n, k, trans_b, dtype);
+    p.group_sizes = sizes;
+    p.groups = (int)e;
+    p.zero_rest = 1;
+    return p;
+}
+static const int32_t SOME_SIZES = 0;   // stands for sizes that are there, where only that counts
+static int64_t backward_partial16(const int32_t *sizes, int64_t e, int64_t t, int64_t n, int64_t k, int trans_b)
+{
+    return std::max(partial16_bytes(grad_x_product(sizes, e, t, n, k, trans_b, CCH_DTYPE_BF16), trans_b ? ROWS_NN : ROWS_NK, EPI16_OUT),
+                    partial16_bytes(grad_w_product(sizes, e, t, n, k, trans_b, CCH_DTYPE_BF16), ROWS_TN, EPI16_OUT));
+}
+
 // grad_x [t, k] = grad [t, n] W^T and grad_w = x^T grad (or its transpose), per group.
-static int backward_products16(const uint16_t *grad, int64_t pitch_grad, const uint16_t *x, int64_t pitch_x, const uint16_t *w, int64_t pitch_w, const int32_t *sizes, int64_t e,
-                               uint16_t *grad_x, uint16_t *grad_w, int64_t t, int64_t n, int64_t k, int trans_b, int dtype, hipStream_t stream)
+static int backward_products16(const uint16_t *grad, const uint16_t *x, const uint16_t *w, const int32_t *sizes, int64_t e, uint16_t *grad_x, uint16_t *grad_w, int64_t t, int64_t n,
+                               int64_t k, int trans_b, int dtype, const Carve &ws, void *workspace, int64_t workspace_bytes, hipStream_t stream)
 {
     if (grad_x && t > 0 && k > 0) {
-        // W^T of weights [n, k] is weights [k', n'] with k' = n
-        Gemm16 p = product16(grad, pitch_grad, w, pitch_w, grad_x, t, k, n, !trans_b, dtype);
-        p.b_stride = (trans_b ? n : k) * pitch_w;
-        p.group_sizes = sizes;
-        p.groups = (int)e;
-        p.zero_rest = sizes != nullptr;
+        Gemm16 p = grad_x_product(sizes, e, t, n, k, trans_b, dtype);
+        p.a = grad;
+        p.b = w;
+        p.out = grad_x;
+        ws.rest(p, workspace, workspace_bytes);
         if (const int rc = gemm16_launch(p, trans_b ? ROWS_NN : ROWS_NK, EPI16_OUT, stream)) return rc;
     }
     if (grad_w && n > 0 && k > 0) {
-        Gemm16 p = trans_b ? product16(grad, pitch_grad, x, pitch_x, grad_w, n, k, t, 0, dtype) : product16(x, pitch_x, grad, pitch_grad, grad_w, k, n, t, 0, dtype);
-        p.b_stride = 0;
-        p.out_stride = n * k;
-        p.group_sizes = sizes;
-        p.groups = (int)e;
-        p.k_grouped = 1;
+        Gemm16 p = grad_w_product(sizes, e, t, n, k, trans_b, dtype);
+        p.a = trans_b ? grad : x;
+        p.b = trans_b ? x : grad;
+        p.out = grad_w;
+        ws.rest(p, workspace, workspace_bytes);
         if (const int rc = gemm16_launch(p, ROWS_TN, EPI16_OUT, stream)) return rc;
     }
     return CCH_OK;
@@ -82,7 +116,7 @@ using namespace cch;
 extern "C" int64_t cch_grouped_matmul_workspace_bytes(int64_t num_experts, int64_t t, int64_t n, int64_t k, int trans_b)
 {
     if (!fits16(t, n, k) || !groups_fit(num_experts)) return 0;
-    return padded16_bytes(t, k) + weights16_bytes(num_experts, n, k, trans_b);
+    return padded16_bytes(t, k) + weights16_bytes(num_experts, n, k, trans_b) + partial16_bytes(grouped_product(nullptr, nullptr, &SOME_SIZES, nullptr, num_experts, t, n, k, trans_b, CCH_DTYPE_BF16), trans_b ? ROWS_NK : ROWS_NN, EPI16_OUT);
 }
 
 extern "C" int cch_grouped_matmul(const void *x, const void *w, const int32_t *group_sizes, void *out, int64_t num_experts, int64_t t, int64_t n, int64_t k, int trans_b,
@@ -100,17 +134,15 @@ extern "C" int cch_grouped_matmul(const void *x, const void *w, const int32_t *g
     int64_t ldx, ldw;
     if (const int rc = operand16(u16(x), t, k, ws, &px, &ldx, s)) return rc;
     if (const int rc = operand16(u16(w), num_experts * (trans_b ? n : k), trans_b ? k : n, ws, &pw, &ldw, s)) return rc;
-    Gemm16 p = product16(px, ldx, pw, ldw, u16(out), t, n, k, trans_b, dtype);
-    p.group_sizes = group_sizes;
-    p.groups = (int)num_experts;
-    p.zero_rest = 1;
+    Gemm16 p = grouped_product(px, pw, group_sizes, u16(out), num_experts, t, n, k, trans_b, dtype);
+    ws.rest(p, workspace, workspace_bytes);
     return gemm16_launch(p, trans_b ? ROWS_NK : ROWS_NN, EPI16_OUT, s);
 }
 
 extern "C" int64_t cch_grouped_matmul_backward_workspace_bytes(int64_t num_experts, int64_t t, int64_t n, int64_t k, int trans_b)
 {
     if (!fits16(t, n, k) || !groups_fit(num_experts)) return 0;
-    return padded16_bytes(t, k) + padded16_bytes(t, n) + weights16_bytes(num_experts, n, k, trans_b);
+    return padded16_bytes(t, k) + padded16_bytes(t, n) + weights16_bytes(num_experts, n, k, trans_b) + backward_partial16(&SOME_SIZES, num_experts, t, n, k, trans_b);
 }
 
 extern "C" int cch_grouped_matmul_backward(const void *grad_out, const void *x, const void *w, const int32_t *group_sizes, void *grad_x, void *grad_w, int64_t num_experts,
@@ -132,7 +164,7 @@ extern "C" int cch_grouped_matmul_backward(const void *grad_out, const void *x, 
         if (const int rc = operand16(u16(x), t, k, ws, &px, &ldx, s)) return rc;
     if (grad_x)
         if (const int rc = operand16(u16(w), num_experts * (trans_b ? n : k), trans_b ? k : n, ws, &pw, &ldw, s)) return rc;
-    return backward_products16(pg, ldg, px, ldx, pw, ldw, group_sizes, num_experts, u16(grad_x), u16(grad_w), t, n, k, trans_b, dtype, s);
+    return backward_products16(pg, px, pw, group_sizes, num_experts, u16(grad_x), u16(grad_w), t, n, k, trans_b, dtype, ws, workspace, workspace_bytes, s);
 }
 
 static int check_act(const char *what, int act)
@@ -144,7 +176,8 @@ static int check_act(const char *what, int act)
 extern "C" int64_t cch_matmul_bias_act_workspace_bytes(int64_t m, int64_t n, int64_t k, int trans_b)
 {
     if (!fits16(m, n, k)) return 0;
-    return padded16_bytes(m, k) + weights16_bytes(1, n, k, trans_b);
+    return padded16_bytes(m, k) + weights16_bytes(1, n, k, trans_b) +
+           partial16_bytes(product16(nullptr, pitch16(k), nullptr, pitch16(trans_b ? k : n), nullptr, m, n, k, trans_b, CCH_DTYPE_BF16), trans_b ? ROWS_NK : ROWS_NN, EPI16_ACT);
 }
 
 extern "C" int cch_matmul_bias_act(const void *x, const void *w, const void *bias, const void *residual, void *preact, void *out, int64_t m, int64_t n, int64_t k, int trans_b,
@@ -168,6 +201,7 @@ extern "C" int cch_matmul_bias_act(const void *x, const void *w, const void *bia
     p.residual = u16(residual);
     p.preact = u16(preact);
     p.act = activation;
+    ws.rest(p, workspace, workspace_bytes);
     return gemm16_launch(p, trans_b ? ROWS_NK : ROWS_NN, EPI16_ACT, s);
 }
 
@@ -175,7 +209,7 @@ extern "C" int64_t cch_matmul_bias_act_backward_workspace_bytes(int64_t m, int64
 {
     if (!fits16(m, n, k)) return 0;
     const int64_t dz = activation == CCH_ACT_NONE ? padded16_bytes(m, n) : round256(m * pitch16(n) * 2);
-    return dz + column_sum_bytes(m, n) + padded16_bytes(m, k) + weights16_bytes(1, n, k, trans_b);
+    return dz + column_sum_bytes(m, n) + padded16_bytes(m, k) + weights16_bytes(1, n, k, trans_b) + backward_partial16(nullptr, 1, m, n, k, trans_b);
 }
 
 extern "C" int cch_matmul_bias_act_backward(const void *grad_out, const void *x, const void *w, const void *preact, void *grad_x, void *grad_w, void *grad_bias, int64_t m,
@@ -207,5 +241,5 @@ extern "C" int cch_matmul_bias_act_backward(const void *grad_out, const void *x,
         if (const int rc = operand16(u16(x), m, k, ws, &px, &ldx, s)) return rc;
     if (grad_x)
         if (const int rc = operand16(u16(w), trans_b ? n : k, trans_b ? k : n, ws, &pw, &ldw, s)) return rc;
-    return backward_products16(own ? dz : u16(grad_out), pitch16(n), px, ldx, pw, ldw, nullptr, 1, u16(grad_x), u16(grad_w), m, n, k, trans_b, dtype, s);
+    return backward_products16(own ? dz : u16(grad_out), px, pw, nullptr, 1, u16(grad_x), u16(grad_w), m, n, k, trans_b, dtype, ws, workspace, workspace_bytes, s);
 }
