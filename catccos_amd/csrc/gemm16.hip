@@ -25,13 +25,15 @@ Plan16 plan16(const Gemm16 &p, int layout, int epilogue)
     const int64_t share = p.k_grouped || !p.group_sizes ? p.m : (p.m + p.groups - 1) / p.groups, each = (share + 127) / 128 * ((p.n + 127) / 128);
     const int64_t tiles = each * p.groups, steps = ((p.k_grouped ? (p.k + p.groups - 1) / p.groups : p.k) + 63) / 64;
     if (results && !p.sums && tiles < CUS) {
-        // us: a step of a workgroup with four stages, its first requests and epilogue, the second launch and the parts' way to memory and back
-        const double STEP = 0.27, START = 2.0, JOIN = 2.5, PER_BYTE = 2.0 / 4e6;
+        // us beyond what one launch costs in any case: a step of a workgroup with four stages, longer the more of them share the caches, the second launch, and the parts' way
+        // to memory and back (128 x 1024 x 8192 in 1, 2, 4, 8, 16 parts: 47, 30, 21, 17.5, 18.7 us; 256 x 4096 x 7168 in 1, 2, 4, 8: 45, 32, 34, 33; 512 x 1024 x 1024: 12.2,
+        // 13.5, 14.4, 19.9)
+        const double STEP = 0.32, SHARED = 0.18, JOIN = 1.7, PER_BYTE = 0.6e-6;
         const double bytes = 4.0 * p.m * p.n * (p.k_grouped ? p.groups : 1);
         double best = 0;
         for (int s = 1; s <= 32 && s <= steps; s++) {
-            const double rounds = (double)((tiles * s + CUS - 1) / CUS);
-            const double us = rounds * ((double)((steps + s - 1) / s) * STEP + START) + (s > 1 ? JOIN + s * bytes * PER_BYTE : 0);
+            const double fill = (double)(tiles * s) / CUS, rounds = fill <= 1 ? 1 : (double)((tiles * s + CUS - 1) / CUS);
+            const double us = rounds * (double)((steps + s - 1) / s) * (STEP + SHARED * (fill < 1 ? fill : 1)) + (s > 1 ? JOIN + s * bytes * PER_BYTE : 0);
             if (s == 1 || us < best) {
                 best = us;
                 plan.splits = s;

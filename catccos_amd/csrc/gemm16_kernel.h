@@ -10,6 +10,8 @@
 
 namespace cch {
 
+constexpr int min_c(int a, int b) { return a < b ? a : b; }
+
 template <int MT_, int NT_, int WM_, int WN_, int DEPTH_> struct Shape16 {
     static constexpr int MT = MT_, NT = NT_, WM = WM_, WN = WN_, WAVES = WM * WN, THREADS = 64 * WAVES, DEPTH = DEPTH_, PER_CU = DEPTH == 2 ? 2 : 1;
     static constexpr int TM = 32 * MT * WM, TN = 32 * NT * WN;      // tile
@@ -115,23 +117,25 @@ __global__ __launch_bounds__(S::THREADS, S::PER_CU * S::WAVES / 4) void gemm16_k
             }
         }
         // (K contiguous: a lane whose 8 elements begin at or past K fetches nothing; K is a multiple of 8 or its rows are padded with zeros)
-        auto request = [&](int step) {
-            const uint32_t stage = lds + (uint32_t)(step % S::DEPTH) * S::STAGE;
+        int k_left = 0;
+        uint32_t k_at = 0;
+        uint32_t stage_at = 0;
+        auto prepare = [&](int step) {
             const int k0 = (first + step) * 64;
             if constexpr (A_KM) rs_a = kmajor_rsrc(a0, p.pitch_a, k0, k_stop, m0, p.m);
             if constexpr (B_KM) rs_b = kmajor_rsrc(b0, p.pitch_b, k0, k_stop, n0, p.n);
-#pragma unroll
-            for (int j = 0; j < NJA; j++) {
-                const int row = (wave * NJA + j) * 8 + (lane >> 3);
-                const bool in = A_KM || (int)(((uint32_t)(lane & 7) ^ swizzle_of_row(row)) * 8u) < k_stop - k0;
-                load16_to_lds(rs_a, in ? off_a[j] : NO_FETCH, A_KM ? 0u : (uint32_t)k0 * 2u, stage + (uint32_t)(wave * NJA + j) * 1024u);
-            }
-#pragma unroll
-            for (int j = 0; j < NJB; j++) {
-                const int row = (wave * NJB + j) * 8 + (lane >> 3);
-                const bool in = B_KM || (int)(((uint32_t)(lane & 7) ^ swizzle_of_row(row)) * 8u) < k_stop - k0;
-                load16_to_lds(rs_b, in ? off_b[j] : NO_FETCH, B_KM ? 0u : (uint32_t)k0 * 2u, stage + S::A_BYTES + (uint32_t)(wave * NJB + j) * 1024u);
-            }
+            k_left = k_stop - k0;
+            k_at = (uint32_t)k0 * 2u;
+            stage_at = lds + (uint32_t)(step % S::DEPTH) * S::STAGE;
+        };
+        // request q of a wave's NJA + NJB of a step
+        auto request = [&](auto q_c) {
+            constexpr int q = decltype(q_c)::value, j = q < NJA ? q : q - NJA;
+            constexpr bool is_a = q < NJA, km = is_a ? A_KM : B_KM;
+            const int row = (wave * (is_a ? NJA : NJB) + j) * 8 + (lane >> 3);
+            const bool in = km || (int)(((uint32_t)(lane & 7) ^ swizzle_of_row(row)) * 8u) < k_left;
+            const uint32_t off = is_a ? off_a[j] : off_b[j];
+            load16_to_lds(is_a ? rs_a : rs_b, in ? off : NO_FETCH, km ? 0u : k_at, stage_at + (is_a ? 0u : (uint32_t)S::A_BYTES) + (uint32_t)(wave * (is_a ? NJA : NJB) + j) * 1024u);
         };
 
         v16f acc[MT][NT];
@@ -139,29 +143,43 @@ __global__ __launch_bounds__(S::THREADS, S::PER_CU * S::WAVES / 4) void gemm16_k
         for (int i = 0; i < MT; i++)
 #pragma unroll
             for (int j = 0; j < NT; j++) acc[i][j] = (v16f)(0.0f);
-        // (requests past the last step fetch nothing: every wait counts the same)
-#pragma unroll
-        for (int i = 0; i < S::DEPTH - 1; i++) request(i);
-        for (int step = 0; step < steps; step++) {
+        // Operands are read a step ahead: while one set is multiplied the other is filled, and the step's requests, DEPTH ahead into the stage that was read last, go
+        // between the matrix instructions too.  (Requests past the last step fetch nothing: every wait counts the same.)
+        static_for<S::DEPTH>([&](auto i) { prepare(i); static_for<NJA + NJB>(request); });
+        CCH_WAIT_VM((S::DEPTH - 1) * (NJA + NJB));
+        CCH_BARRIER();
+        v4i fa[2][MT][4], fb[2][NT][4];
+        uint32_t read_at = 0;   // the stage to read next
+        auto read = [&](auto set_c, auto i_c) {   // the i-th of a step's fragments, sixteenth by sixteenth
+            constexpr int set = decltype(set_c)::value, kk = decltype(i_c)::value / (MT + NT), f = decltype(i_c)::value % (MT + NT);
+            if constexpr (f < NT) fb[set][f][kk] = B_KM ? read_transposed(ft_b[f] + read_at + (uint32_t)kk * 16u * KB::ROW, KB::ROW) : lds_read16_abs(fr_b[kk] + read_at + (uint32_t)f * 4096u);
+            else fa[set][f - NT][kk] = A_KM ? read_transposed(ft_a[f - NT] + read_at + (uint32_t)kk * 16u * KA::ROW, KA::ROW) : lds_read16_abs(fr_a[kk] + read_at + (uint32_t)(f - NT) * 4096u);
+        };
+        constexpr int READS = 4 * (MT + NT), MMAS = 4 * MT * NT;
+        static_for<READS>([&](auto i) { read(IC<0>{}, i); });
+        auto multiply = [&](auto set_c, int step) {
+            constexpr int set = decltype(set_c)::value;
+            read_at = read_at + S::STAGE == S::LDS ? 0u : read_at + (uint32_t)S::STAGE;
             CCH_WAIT_VM_LGKM0((S::DEPTH - 2) * (NJA + NJB));
             CCH_BARRIER();
-            request(step + S::DEPTH - 1);
-            const uint32_t stage = (uint32_t)(step % S::DEPTH) * S::STAGE;
-#pragma unroll
-            for (int kk = 0; kk < 4; kk++) {
-                v4i fa[MT], fb[NT];
-#pragma unroll
-                for (int j = 0; j < NT; j++)
-                    fb[j] = B_KM ? read_transposed(ft_b[j] + stage + (uint32_t)kk * 16u * KB::ROW, KB::ROW) : lds_read16_abs(fr_b[kk] + stage + (uint32_t)j * 4096u);
-#pragma unroll
-                for (int i = 0; i < MT; i++)
-                    fa[i] = A_KM ? read_transposed(ft_a[i] + stage + (uint32_t)kk * 16u * KA::ROW, KA::ROW) : lds_read16_abs(fr_a[kk] + stage + (uint32_t)i * 4096u);
-#pragma unroll
-                for (int i = 0; i < MT; i++)
-#pragma unroll
-                    for (int j = 0; j < NT; j++) acc[i][j] = T::mfma(fb[j], fa[i], acc[i][j]);
-            }
+            prepare(step + S::DEPTH);
+            static_for<MMAS>([&](auto m_c) {
+                constexpr int m = decltype(m_c)::value, kk = m / (MT * NT), i = m / NT % MT, j = m % NT;
+                acc[i][j] = T::mfma(fb[set][j][kk], fa[set][i][kk], acc[i][j]);
+                // reads in the first three quarters, requests over all
+                constexpr int r0 = min_c(m * READS * 4 / (MMAS * 3), READS), r1 = min_c((m + 1) * READS * 4 / (MMAS * 3), READS);
+                static_for<r1 - r0>([&](auto x) { read(IC<1 - set>{}, IC<r0 + decltype(x)::value>{}); });
+                constexpr int q0 = m * (NJA + NJB) / MMAS, q1 = (m + 1) * (NJA + NJB) / MMAS;
+                static_for<q1 - q0>([&](auto x) { request(IC<q0 + decltype(x)::value>{}); });
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        };
+        int step = 0;
+        for (; step + 2 <= steps; step += 2) {
+            multiply(IC<0>{}, step);
+            multiply(IC<1>{}, step + 1);
         }
+        if (step < steps) multiply(IC<0>{}, step);
         CCH_WAIT_VM_LGKM0(0);
         CCH_BARRIER();
         if constexpr (EPI == EPI16_OUT || EPI == EPI16_ACT) {

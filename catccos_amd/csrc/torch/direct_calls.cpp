@@ -537,6 +537,236 @@ PyObject *MoeFfnW4A16(PyObject *, PyObject *const *v, Py_ssize_t nv)
     END_HANDLE_TH_ERRORS
 }
 
+// ---- Products of 16-bit operands.  All tensors on the current device (whose stream the call takes), operands on 16-byte boundaries.
+bool Here(std::initializer_list<PyObject *> tensors)
+{
+    const int64_t device = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().device_index();
+    for (PyObject *o : tensors)
+        if (o != Py_None && T(o).device().index() != device) return false;
+    return true;
+}
+bool Whole(PyObject *o) { return ((uintptr_t)T(o).data_ptr() & 15) == 0; }
+bool Sixteen(PyObject *o, int64_t dim, bool forward) { return (Plain(o, at::kBFloat16, dim) || Plain(o, at::kHalf, dim)) && Whole(o) && !(forward && Differentiated(T(o))); }
+// of x's type and rank `dim`
+bool Like(PyObject *o, const at::Tensor &x, int64_t dim, bool forward) { return Plain(o, x.scalar_type(), dim) && !(forward && Differentiated(T(o))); }
+bool Activation(PyObject *o, int &v)
+{
+    static const char *const names[] = {"none", "relu", "silu", "gelu", "gelu_tanh"};   // in the order of CCH_ACT_*
+    if (!PyUnicode_Check(o)) return false;
+    for (v = CCH_ACT_NONE; v <= CCH_ACT_GELU_TANH; v++)
+        if (PyUnicode_CompareWithASCIIString(o, names[v]) == 0) return true;
+    return false;
+}
+bool Reduction(PyObject *o, int &v)
+{
+    if (!PyUnicode_Check(o)) return false;
+    v = PyUnicode_CompareWithASCIIString(o, "mean") == 0 ? CCH_REDUCE_MEAN : CCH_REDUCE_SUM;
+    return v == CCH_REDUCE_MEAN || PyUnicode_CompareWithASCIIString(o, "sum") == 0;
+}
+struct Space {
+    at::Tensor t;
+    int64_t bytes;
+    Space(const at::Tensor &like, int64_t n) : bytes(n)
+    {
+        if (n > 0) t = New(like, {n}, at::kByte);
+    }
+    void *p() const { return bytes > 0 ? t.data_ptr() : nullptr; }
+};
+// Tensors and Nones as a tuple.
+PyObject *Several(std::initializer_list<at::Tensor> list)
+{
+    PyObject *t = PyTuple_New((Py_ssize_t)list.size());
+    Py_ssize_t i = 0;
+    for (const at::Tensor &v : list) {
+        PyObject *o = t == nullptr ? nullptr : v.defined() ? THPVariable_Wrap(v) : (Py_INCREF(Py_None), Py_None);
+        if (o == nullptr) {
+            Py_XDECREF(t);
+            return nullptr;
+        }
+        PyTuple_SET_ITEM(t, i++, o);
+    }
+    return t;
+}
+void *DataOf(const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+bool Grouped(PyObject *x, PyObject *w, PyObject *sizes, PyObject *trans, bool forward, int &trans_b, int64_t &e, int64_t &t, int64_t &n, int64_t &k)
+{
+    if (!Sixteen(x, 2, forward) || !Like(w, T(x), 3, forward) || !Whole(w) || !Plain(sizes, at::kInt, 1) || !Flag(trans, trans_b) || !Here({x, w, sizes})) return false;
+    t = T(x).size(0);
+    k = T(x).size(1);
+    e = T(w).size(0);
+    n = T(w).size(trans_b ? 1 : 2);
+    return T(w).size(trans_b ? 2 : 1) == k && T(sizes).size(0) == e;
+}
+
+// grouped_matmul(x, w, group_sizes, trans_b)
+PyObject *GroupedMatmul(PyObject *, PyObject *const *v, Py_ssize_t nv)
+{
+    HANDLE_TH_ERRORS
+    int trans_b;
+    int64_t e, t, n, k;
+    if (nv != 4 || !PlainThread() || !Grouped(v[0], v[1], v[2], v[3], true, trans_b, e, t, n, k)) return Decline();
+    const at::Tensor &x = T(v[0]);
+    at::Tensor out;
+    int rc;
+    {
+        pybind11::gil_scoped_release nogil;
+        const Space ws(x, cch_grouped_matmul_workspace_bytes(e, t, n, k, trans_b));
+        out = New(x, {t, n}, x.scalar_type());
+        rc = cch_grouped_matmul(x.data_ptr(), T(v[1]).data_ptr(), P<const int32_t>(T(v[2])), out.data_ptr(), e, t, n, k, trans_b, DtypeCode(x.scalar_type()), ws.p(), ws.bytes,
+                                Stream());
+    }
+    return rc == CCH_OK ? THPVariable_Wrap(out) : Decline();
+    END_HANDLE_TH_ERRORS
+}
+
+// grouped_matmul_backward(grad_out, x, w, group_sizes, trans_b, x_grad, w_grad)
+PyObject *GroupedMatmulBackward(PyObject *, PyObject *const *v, Py_ssize_t nv)
+{
+    HANDLE_TH_ERRORS
+    int trans_b, x_grad, w_grad;
+    int64_t e, t, n, k;
+    if (nv != 7 || !PlainThread() || !Grouped(v[1], v[2], v[3], v[4], false, trans_b, e, t, n, k) || !Like(v[0], T(v[1]), 2, false) || !Whole(v[0]) || !Here({v[0]}) ||
+        T(v[0]).size(0) != t || T(v[0]).size(1) != n || !Flag(v[5], x_grad) || !Flag(v[6], w_grad))
+        return Decline();
+    const at::Tensor &x = T(v[1]), &w = T(v[2]);
+    at::Tensor gx, gw;
+    int rc;
+    {
+        pybind11::gil_scoped_release nogil;
+        const Space ws(x, cch_grouped_matmul_backward_workspace_bytes(e, t, n, k, trans_b));
+        if (x_grad) gx = New(x, x.sizes(), x.scalar_type());
+        if (w_grad) gw = New(w, w.sizes(), w.scalar_type());
+        rc = cch_grouped_matmul_backward(T(v[0]).data_ptr(), x.data_ptr(), w.data_ptr(), P<const int32_t>(T(v[3])), DataOf(gx), DataOf(gw), e, t, n, k, trans_b,
+                                         DtypeCode(x.scalar_type()), ws.p(), ws.bytes, Stream());
+    }
+    return rc == CCH_OK ? Several({gx, gw}) : Decline();
+    END_HANDLE_TH_ERRORS
+}
+
+bool Layer(PyObject *x, PyObject *w, PyObject *trans, bool forward, int &trans_b, int64_t &m, int64_t &n, int64_t &k)
+{
+    if (!Sixteen(x, 2, forward) || !Like(w, T(x), 2, forward) || !Whole(w) || !Flag(trans, trans_b) || !Here({x, w})) return false;
+    m = T(x).size(0);
+    k = T(x).size(1);
+    n = T(w).size(trans_b ? 0 : 1);
+    return T(w).size(trans_b ? 1 : 0) == k;
+}
+
+// matmul_bias_act(x, w, bias, residual, activation, trans_b, return_preact)
+PyObject *MatmulBiasAct(PyObject *, PyObject *const *v, Py_ssize_t nv)
+{
+    HANDLE_TH_ERRORS
+    int trans_b, act, keep;
+    int64_t m, n, k;
+    if (nv != 7 || !PlainThread() || !Layer(v[0], v[1], v[5], true, trans_b, m, n, k) || !Activation(v[4], act) || !Flag(v[6], keep)) return Decline();
+    const at::Tensor &x = T(v[0]);
+    if (v[2] != Py_None && (!Like(v[2], x, 1, true) || T(v[2]).size(0) != n)) return Decline();
+    if (v[3] != Py_None && (!Like(v[3], x, 2, true) || T(v[3]).size(0) != m || T(v[3]).size(1) != n)) return Decline();
+    if (!Here({v[2], v[3]})) return Decline();
+    at::Tensor out, pre;
+    int rc;
+    {
+        pybind11::gil_scoped_release nogil;
+        const Space ws(x, cch_matmul_bias_act_workspace_bytes(m, n, k, trans_b));
+        out = New(x, {m, n}, x.scalar_type());
+        if (keep) pre = New(x, {m, n}, x.scalar_type());
+        rc = cch_matmul_bias_act(x.data_ptr(), T(v[1]).data_ptr(), Data(v[2]), Data(v[3]), DataOf(pre), out.data_ptr(), m, n, k, trans_b, act, DtypeCode(x.scalar_type()), ws.p(),
+                                 ws.bytes, Stream());
+    }
+    return rc != CCH_OK ? Decline() : keep ? Pair(out, pre) : THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// matmul_bias_act_backward(grad_out, x, w, preact, activation, trans_b, x_grad, w_grad, bias_grad)
+PyObject *MatmulBiasActBackward(PyObject *, PyObject *const *v, Py_ssize_t nv)
+{
+    HANDLE_TH_ERRORS
+    int trans_b, act, x_grad, w_grad, b_grad;
+    int64_t m, n, k;
+    if (nv != 9 || !PlainThread() || !Layer(v[1], v[2], v[5], false, trans_b, m, n, k) || !Activation(v[4], act) || !Like(v[0], T(v[1]), 2, false) || !Whole(v[0]) ||
+        T(v[0]).size(0) != m || T(v[0]).size(1) != n || !Here({v[0]}) || !Flag(v[6], x_grad) || !Flag(v[7], w_grad) || !Flag(v[8], b_grad))
+        return Decline();
+    const at::Tensor &x = T(v[1]), &w = T(v[2]);
+    if (act != CCH_ACT_NONE && (v[3] == Py_None || !Like(v[3], x, 2, false) || T(v[3]).sizes() != T(v[0]).sizes() || !Here({v[3]}))) return Decline();
+    at::Tensor gx, gw, gb;
+    int rc;
+    {
+        pybind11::gil_scoped_release nogil;
+        const Space ws(x, cch_matmul_bias_act_backward_workspace_bytes(m, n, k, trans_b, act));
+        if (x_grad) gx = New(x, x.sizes(), x.scalar_type());
+        if (w_grad) gw = New(w, w.sizes(), w.scalar_type());
+        if (b_grad) gb = New(x, {n}, x.scalar_type());
+        rc = cch_matmul_bias_act_backward(T(v[0]).data_ptr(), x.data_ptr(), w.data_ptr(), act == CCH_ACT_NONE ? nullptr : T(v[3]).data_ptr(), DataOf(gx), DataOf(gw), DataOf(gb), m, n,
+                                          k, trans_b, act, DtypeCode(x.scalar_type()), ws.p(), ws.bytes, Stream());
+    }
+    return rc == CCH_OK ? Several({gx, gw, gb}) : Decline();
+    END_HANDLE_TH_ERRORS
+}
+
+bool Entropy(PyObject *x, PyObject *w, PyObject *targets, PyObject *reduction, PyObject *z_coef, bool forward, int &red, float &z, int64_t &t, int64_t &h, int64_t &voc)
+{
+    if (!Sixteen(x, 2, forward) || !Like(w, T(x), 2, forward) || !Whole(w) || (!Plain(targets, at::kLong, 1) && !Plain(targets, at::kInt, 1)) || !Reduction(reduction, red) ||
+        !Real(z_coef, z) || !Here({x, w, targets}))
+        return false;
+    t = T(x).size(0);
+    h = T(x).size(1);
+    voc = T(w).size(0);
+    return T(w).size(1) == h && T(targets).size(0) == t;
+}
+
+// linear_cross_entropy(x, w, targets, reduction, z_coef)
+PyObject *LinearCrossEntropy(PyObject *, PyObject *const *v, Py_ssize_t nv)
+{
+    HANDLE_TH_ERRORS
+    int red;
+    float z;
+    int64_t t, h, voc;
+    if (nv != 5 || !PlainThread() || !Entropy(v[0], v[1], v[2], v[3], v[4], true, red, z, t, h, voc)) return Decline();
+    const at::Tensor &x = T(v[0]), &targets = T(v[2]);
+    at::Tensor loss, nll, lse, tokens;
+    int rc;
+    {
+        pybind11::gil_scoped_release nogil;
+        const Space ws(x, cch_linear_cross_entropy_workspace_bytes(t, h, voc));
+        loss = New(x, {}, at::kFloat);
+        nll = New(x, {t}, at::kFloat);
+        lse = New(x, {t}, at::kFloat);
+        tokens = New(x, {1}, at::kInt);
+        rc = cch_linear_cross_entropy(x.data_ptr(), T(v[1]).data_ptr(), targets.data_ptr(), targets.scalar_type() == at::kLong ? 8 : 4, P<float>(loss), P<float>(nll), P<float>(lse),
+                                      P<int32_t>(tokens), t, h, voc, red, z, DtypeCode(x.scalar_type()), ws.p(), ws.bytes, Stream());
+    }
+    return rc == CCH_OK ? Several({loss, nll, lse, tokens}) : Decline();
+    END_HANDLE_TH_ERRORS
+}
+
+// linear_cross_entropy_backward(grad_loss, x, w, targets, lse, tokens, reduction, z_coef, x_grad, w_grad)
+PyObject *LinearCrossEntropyBackward(PyObject *, PyObject *const *v, Py_ssize_t nv)
+{
+    HANDLE_TH_ERRORS
+    int red, x_grad, w_grad;
+    float z;
+    int64_t t, h, voc;
+    if (nv != 10 || !PlainThread() || !Entropy(v[1], v[2], v[3], v[6], v[7], false, red, z, t, h, voc) || !Plain(v[0], at::kFloat, -1) || T(v[0]).numel() != 1 ||
+        !Plain(v[4], at::kFloat, 1) || T(v[4]).size(0) != t || !Plain(v[5], at::kInt, -1) || T(v[5]).numel() != 1 || !Here({v[0], v[4], v[5]}) || !Flag(v[8], x_grad) ||
+        !Flag(v[9], w_grad))
+        return Decline();
+    const at::Tensor &x = T(v[1]), &w = T(v[2]), &targets = T(v[3]);
+    at::Tensor gx, gw;
+    int rc;
+    {
+        pybind11::gil_scoped_release nogil;
+        const Space ws(x, cch_linear_cross_entropy_backward_workspace_bytes(t, h, voc));
+        if (x_grad) gx = New(x, x.sizes(), x.scalar_type());
+        if (w_grad) gw = New(w, w.sizes(), w.scalar_type());
+        rc = cch_linear_cross_entropy_backward(P<const float>(T(v[0])), x.data_ptr(), w.data_ptr(), targets.data_ptr(), targets.scalar_type() == at::kLong ? 8 : 4,
+                                               P<const float>(T(v[4])), P<const int32_t>(T(v[5])), DataOf(gx), DataOf(gw), t, h, voc, red, z, DtypeCode(x.scalar_type()), ws.p(),
+                                               ws.bytes, Stream());
+    }
+    return rc == CCH_OK ? Several({gx, gw}) : Decline();
+    END_HANDLE_TH_ERRORS
+}
+
 #define CCH_FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr
 PyMethodDef methods[] = {
     {"mx_quant", CCH_FAST(MxQuant)},
@@ -553,6 +783,12 @@ PyMethodDef methods[] = {
     {"moe_balance_loss_backward", CCH_FAST(MoeBalanceLossBackward)},
     {"w4a16_matmul", CCH_FAST(W4A16)},
     {"moe_ffn_w4a16", CCH_FAST(MoeFfnW4A16)},
+    {"grouped_matmul", CCH_FAST(GroupedMatmul)},
+    {"grouped_matmul_backward", CCH_FAST(GroupedMatmulBackward)},
+    {"matmul_bias_act", CCH_FAST(MatmulBiasAct)},
+    {"matmul_bias_act_backward", CCH_FAST(MatmulBiasActBackward)},
+    {"linear_cross_entropy", CCH_FAST(LinearCrossEntropy)},
+    {"linear_cross_entropy_backward", CCH_FAST(LinearCrossEntropyBackward)},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_direct", "native form of the tensor-level entry points", -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -53,7 +53,8 @@ class _Direct:
 
     def __getattr__(self, name):
         names = ("mx_quant", "dynamic_quant_i8", "moe_init_routing", "w8a8_matmul_dequant", "gmm_i8", "mx_matmul", "mx_grouped_matmul", "moe_ffn_mxfp8",
-                 "moe_router", "moe_router_backward", "moe_balance_loss", "moe_balance_loss_backward", "w4a16_matmul", "moe_ffn_w4a16")
+                 "moe_router", "moe_router_backward", "moe_balance_loss", "moe_balance_loss_backward", "w4a16_matmul", "moe_ffn_w4a16", "grouped_matmul",
+                 "grouped_matmul_backward", "matmul_bias_act", "matmul_bias_act_backward", "linear_cross_entropy", "linear_cross_entropy_backward")
         if name not in names:
             raise AttributeError(name)
         try:
@@ -881,6 +882,9 @@ def grouped_matmul(x, w, group_sizes, trans_b=0):
 
     x [T, K] bf16 or half, rows of an expert back to back in expert order (moe_init_routing's); w of x's type, [E, K, N] or with trans_b=1 [E, N, K], up to 1024
     experts; group_sizes int32 [E] on the GPU.  Returns [T, N] in x's type, sums in fp32, zeros behind the last group.  Differentiable in x and w, in reverse mode."""
+    r = _direct.grouped_matmul(x, w, group_sizes, trans_b)
+    if r is not NotImplemented:
+        return r
     _one_device("grouped_matmul", x, w, group_sizes)
     e, t, n, k = _check_grouped(x, w, group_sizes, trans_b)
     _no_tangent("grouped_matmul", x, w)
@@ -896,6 +900,9 @@ def grouped_matmul(x, w, group_sizes, trans_b=0):
 def grouped_matmul_backward(grad_out, x, w, group_sizes, trans_b=0, x_grad=True, w_grad=True):
     """The gradients of grouped_matmul: (grad_x [T, K], zeros behind the last group, grad_w in w's layout, zeros for an expert without rows), each None
     where it is not asked for.  What autograd calls; for programs that do without it."""
+    r = _direct.grouped_matmul_backward(grad_out, x, w, group_sizes, trans_b, x_grad, w_grad)
+    if r is not NotImplemented:
+        return r
     _one_device("grouped_matmul_backward", x, grad_out, w, group_sizes)
     e, t, n, k = _check_grouped(x, w, group_sizes, trans_b)
     if grad_out.dtype != x.dtype or tuple(grad_out.shape) != (t, n):
@@ -941,6 +948,9 @@ def matmul_bias_act(x, w, bias=None, residual=None, activation="none", trans_b=0
     x [M, K] bf16 or half; w of x's type, [K, N] or with trans_b=1 [N, K]; bias [N] and residual [M, N] of x's type or None; activation "none", "relu", "silu", "gelu" (erf) or
     "gelu_tanh".  With return_preact returns (out, x W + bias rounded to x's type), what matmul_bias_act_backward takes.  Differentiable in x, w, bias and residual, in reverse
     mode, through out alone (the activation's slope is taken at the rounded x W + bias)."""
+    r = _direct.matmul_bias_act(x, w, bias, residual, activation, trans_b, return_preact)
+    if r is not NotImplemented:
+        return r
     _one_device("matmul_bias_act", x, w, bias, residual)
     m, n, k = _check_layer(x, w, trans_b)
     act = _activation(activation)
@@ -966,6 +976,9 @@ def matmul_bias_act_backward(grad_out, x, w, preact=None, activation="none", tra
     """The gradients of matmul_bias_act: (grad_x, grad_w in w's layout, grad_bias), in x's type, each None where it is not asked for; the residual's is grad_out.
     preact as matmul_bias_act returned it, None without an activation.  grad_out * act'(preact) is rounded to x's type before the products and not before the bias' sum.
     What autograd calls; for programs that do without it."""
+    r = _direct.matmul_bias_act_backward(grad_out, x, w, preact, activation, trans_b, x_grad, w_grad, bias_grad)
+    if r is not NotImplemented:
+        return r
     _one_device("matmul_bias_act_backward", x, grad_out, w, preact)
     m, n, k = _check_layer(x, w, trans_b)
     act = _activation(activation)
@@ -1027,6 +1040,9 @@ def linear_cross_entropy(x, w, targets, reduction="mean", z_coef=0.0):
     holds.  Returns (loss float32 [], nll float32 [T], lse float32 [T], tokens int32 [1]): nll = lse - the target's logit with lse = log sum exp of the
     logits, both 0 for tokens that do not count, tokens how many do, loss the mean (or with reduction "sum" the sum) over them of nll + z_coef * lse^2, 0 if there are
     none.  loss is differentiable in x and w, in reverse mode.  The same inputs give the same bits."""
+    r = _direct.linear_cross_entropy(x, w, targets, reduction, z_coef)
+    if r is not NotImplemented:
+        return r
     _one_device("linear_cross_entropy", x, w, targets)
     t, h, v = _check_ce(x, w, targets)
     red = _reduction(reduction)
@@ -1048,6 +1064,9 @@ def linear_cross_entropy_backward(grad_loss, x, w, targets, lse, tokens, reducti
     """The gradients of linear_cross_entropy's loss: (grad_x [T, H], grad_w [V, H]) in x's type, each None where it is not asked for.  grad_loss float32 [] on the GPU; lse and
     tokens as linear_cross_entropy returned them (a mean divides by tokens: a program that shares a batch between GPUs may give all of theirs), the options as
     they were given to it.  The logits' gradient is computed a piece of the vocabulary at a time and rounded to x's type.  What autograd calls."""
+    r = _direct.linear_cross_entropy_backward(grad_loss, x, w, targets, lse, tokens, reduction, z_coef, x_grad, w_grad)
+    if r is not NotImplemented:
+        return r
     _one_device("linear_cross_entropy_backward", x, grad_loss, w, targets, lse, tokens)
     t, h, v = _check_ce(x, w, targets)
     red = _reduction(reduction)
