@@ -22,7 +22,7 @@ namespace cch {
 
 struct Big16 {
     static constexpr int MT = 4, NT = 2, TM = 256, TN = 256, THREADS = 512;
-    static constexpr int PANEL = 32768, A_AT = 0, B_AT = 2 * PANEL, PASS = 16, STAGING = 4 * PANEL, TABLE = STAGING + 8 * PASS * 128, LDS = TABLE + (int)sizeof(GroupTable16);
+    static constexpr int PANEL = 32768, A_AT = 0, B_AT = 2 * PANEL, TABLE = 4 * PANEL, LDS = TABLE + (int)sizeof(GroupTable16);
 };
 
 template <class T, int LAYOUT, int EPI>
@@ -370,7 +370,7 @@ __global__ __launch_bounds__(Big16::THREADS, 2) void gemm16_big_kernel(Gemm16 p)
         }
         // Both groups write their results in the same slot: the first behind the barrier that ends its last matrix slot, the second, one slot behind, before it.
         if (wm == 0) CCH_BARRIER();
-        epilogue16<T, EPI, MT, NT, 64, S::PASS>(p, acc, cur.e, cur.m0, cur.m_end, cur.n0, wm * 32, wn * 64, lds + S::STAGING + (uint32_t)wave * (S::PASS * 128u), whole, counted);
+        epilogue16<T, EPI, MT, NT, 64>(p, acc, cur.e, cur.m0, cur.m_end, cur.n0, wm * 32, wn * 64, whole, counted);
         if (!nxt.valid) break;
         young = more;
         cur = nxt;

@@ -220,45 +220,27 @@ __device__ __forceinline__ bool whole_rows(const Gemm16 &p)
 // Whether every tile of such a problem stores the same number of times, whatever of it exists: 16 stores of a wave with 128 x 64 outputs, twice that with preact.
 template <int EPI> __device__ __forceinline__ bool counted_stores(const Gemm16 &p) { return EPI != EPI16_STATS && !p.sums && !p.out_rows; }
 
-// Between a wave's writes to LDS and its other lanes' reads: for the compiler alone (a wave's LDS operations are in order), which sees one lane's accesses and may
-// otherwise send lanes that branch alike through writes and reads before the others' writes.
-__device__ __forceinline__ void lanes_meet()
+// A wave's results on their way to memory, 32 rows of 32 columns: a lane holds two pieces of 16 bytes of one row, h = 0 and 1, columns 16 h + 8 g.  Swapping rows of 16 lanes between
+// the two brings four lanes to a row, 64 bytes, 16 rows to a store: store(first row, piece), the lane's row being (lane & 15) of it and its columns those of lane_columns().
+// Stored as the lanes hold them, 32 bytes a row, a 256 x 256 tile's epilogue took 11 us.
+__device__ __forceinline__ int lane_columns(int lane) { return (lane >> 4 & 1) * 16 + (lane >> 5) * 8; }
+template <class Store> __device__ __forceinline__ void by_rows(v4i x, v4i y, Store &&store)
 {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
-// A wave's results on their way to memory, 32 rows of 64 columns, PASS rows at a time through LDS of the wave's own (PASS * 128 bytes at `at`): a lane holds four pieces of 16
-// bytes of one row, a store wants eight lanes to a row, whole lines of 128 bytes.  Stored as the lanes hold them, 32 bytes a row, a 256 x 256 tile's epilogue took 11 us.
-// Pieces lie at position c ^ (row & 7), so that writes and reads spread over all banks.
-template <int PASS, class Store> __device__ __forceinline__ void through_lds(uint32_t at, int lane, const v4i piece[2][2], Store &&store)
-{
-    typedef __attribute__((address_space(3))) v4i *P;
-    const int r = lane & 31, g = lane >> 5;
 #pragma unroll
-    for (int ps = 0; ps < 32 / PASS; ps++) {
-        if (PASS == 32 || (r / PASS) == ps) {
-#pragma unroll
-            for (int j = 0; j < 2; j++)
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-                    *reinterpret_cast<P>((uintptr_t)(at + (uint32_t)(r % PASS) * 128u + (((uint32_t)(4 * j + 2 * h + g) ^ (uint32_t)(r & 7)) << 4))) = piece[j][h];
-        }
-        lanes_meet();
-        v4i o[PASS / 8];
-#pragma unroll
-        for (int q = 0; q < PASS / 8; q++) o[q] = lds_read16_abs(at + (uint32_t)(q * 8 + (lane >> 3)) * 128u + (((uint32_t)(lane & 7) ^ (uint32_t)(lane >> 3)) << 4));
-        lanes_meet();
-#pragma unroll
-        for (int q = 0; q < PASS / 8; q++) store(ps * PASS + q * 8, o[q]);   // its first of eight rows
+    for (int d = 0; d < 4; d++) {
+        const auto s = __builtin_amdgcn_permlane16_swap((uint32_t)x[d], (uint32_t)y[d], false, false);
+        x[d] = (int)s[0];
+        y[d] = (int)s[1];
     }
+    store(0, x);
+    store(16, y);
 }
 
 // The results of one wave: MT x NT blocks of 32 x 32, every RS rows from row mw on and side by side from column nw of the tile that begins at row m0 and column n0 of the
-// product, of which rows below m_end exist.  group: the output that K-grouped problems write.  staging: PASS * 128 bytes of LDS of the wave's own.  counted: whole pieces are stored
+// product, of which rows below m_end exist.  group: the output that K-grouped problems write.  counted: whole pieces are stored
 // by way of a descriptor that drops what lies outside, always the same number of times (counted_stores).
-template <class T, int EPI, int MT, int NT, int RS, int PASS>
-__device__ __forceinline__ void epilogue16(const Gemm16 &p, v16f (&acc)[MT][NT], int group, int tile_m, int m_end, int tile_n, int mw, int nw, uint32_t staging, bool whole, bool counted)
+template <class T, int EPI, int MT, int NT, int RS>
+__device__ __forceinline__ void epilogue16(const Gemm16 &p, v16f (&acc)[MT][NT], int group, int tile_m, int m_end, int tile_n, int mw, int nw, bool whole, bool counted)
 {
     static_assert(NT == 2, "64 columns to a wave");
     // (opaque: what depends on the lane would otherwise be worked out before the loop over tiles and take registers from the loop over K)
@@ -300,7 +282,10 @@ __device__ __forceinline__ void epilogue16(const Gemm16 &p, v16f (&acc)[MT][NT],
         const int64_t tile_at = (int64_t)tile_m * p.pitch_out + tile_n;
         const int tile_bytes = (int)min(((int64_t)max(m_end - tile_m, 0) * p.pitch_out - tile_n) * 2, (int64_t)0x7FFFFFF0);
         const uint32_t pitch = (uint32_t)p.pitch_out * 2u;
-        const uint32_t lane_at = (uint32_t)(mw + (lane >> 3)) * pitch + (uint32_t)(nw + (lane & 7) * 8) * 2u + (n0 + (lane & 7) * 8 < p.n ? 0u : 0x80000000u);
+        const int lc = lane_columns(lane);
+        uint32_t lane_at[NT];
+#pragma unroll
+        for (int j = 0; j < NT; j++) lane_at[j] = (uint32_t)(mw + (lane & 15)) * pitch + (uint32_t)(nw + 32 * j + lc) * 2u + (n0 + 32 * j + lc < p.n ? 0u : 0x80000000u);
         static_for<MT>([&](auto i_c) {
             constexpr int i = decltype(i_c)::value;
             const int first = m0 + RS * i, m = first + r;
@@ -361,23 +346,29 @@ __device__ __forceinline__ void epilogue16(const Gemm16 &p, v16f (&acc)[MT][NT],
             }
             if (EPI == EPI16_OUT && p.sums_out) return;
             if (counted) {
-                auto put = [&](uint16_t *base) {
+                auto put = [&](uint16_t *base, const v4i (&what)[2][2]) {
                     const auto rs = __builtin_amdgcn_make_buffer_rsrc(base + tile_at, 0, tile_bytes, 0x00020000);
-                    return [=](int row, v4i o) { __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, o), rs, lane_at + (uint32_t)(RS * i + row) * pitch, 0, 0); };
+#pragma unroll
+                    for (int j = 0; j < NT; j++)
+                        by_rows(what[j][0], what[j][1], [&](int row, v4i o) {
+                            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, o), rs, lane_at[j] + (uint32_t)(RS * i + row) * pitch, 0, 0);
+                        });
                 };
-                if (EPI == EPI16_ACT && p.preact) through_lds<PASS>(staging, lane, pre, put(p.preact));
-                through_lds<PASS>(staging, lane, piece, put(out));
+                if (EPI == EPI16_ACT && p.preact) put(p.preact, pre);
+                put(out, piece);
             } else if (whole) {
-                auto put = [&](uint16_t *base) {
-                    return [&, base](int row, v4i o) {
-                        const int at = first + row + (lane >> 3), c = n0 + (lane & 7) * 8;
-                        if (at >= m_end || c >= p.n) return;
-                        const int64_t to = EPI == EPI16_OUT && p.out_rows ? p.out_rows[at] : at;
-                        *reinterpret_cast<v4i *>(base + to * p.pitch_out + c) = o;
-                    };
+                auto put = [&](uint16_t *base, const v4i (&what)[2][2]) {
+#pragma unroll
+                    for (int j = 0; j < NT; j++)
+                        by_rows(what[j][0], what[j][1], [&](int row, v4i o) {
+                            const int at = first + row + (lane & 15), c = n0 + 32 * j + lc;
+                            if (at >= m_end || c >= p.n) return;
+                            const int64_t to = EPI == EPI16_OUT && p.out_rows ? p.out_rows[at] : at;
+                            *reinterpret_cast<v4i *>(base + to * p.pitch_out + c) = o;
+                        });
                 };
-                if (EPI == EPI16_ACT && p.preact) through_lds<PASS>(staging, lane, pre, put(p.preact));
-                through_lds<PASS>(staging, lane, piece, put(out));
+                if (EPI == EPI16_ACT && p.preact) put(p.preact, pre);
+                put(out, piece);
             } else if (there) {
                 const int64_t to = EPI == EPI16_OUT && p.out_rows ? p.out_rows[m] : m;
 #pragma unroll

@@ -188,10 +188,7 @@ __global__ __launch_bounds__(S::THREADS, S::PER_CU * S::WAVES / 4) void gemm16_k
                 continue;
             }
         }
-        // (results pass through the stages, which the next tile's requests overwrite)
-        epilogue16<T, EPI, MT, NT, 32, 32>(p, acc, e, m0, m_end, n0, wm * MT * 32, wn * NT * 32, lds + (uint32_t)wave * 4096u, whole, false);
-        CCH_WAIT_LGKM0();
-        CCH_BARRIER();
+        epilogue16<T, EPI, MT, NT, 32>(p, acc, e, m0, m_end, n0, wm * MT * 32, wn * NT * 32, whole, false);
     }
 }
 
