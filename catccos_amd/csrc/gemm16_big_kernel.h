@@ -43,7 +43,7 @@ __global__ __launch_bounds__(Big16::THREADS, 2) void gemm16_big_kernel(Gemm16 p)
     const uint32_t lds = (uint32_t)uniform((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)smem);
     const int col_tiles = (p.n + S::TN - 1) / S::TN;
     const int row_tiles = uniform(rows_grouped ? tab.tile[p.groups] : (p.m + S::TM - 1) / S::TM);
-    const int per_group = row_tiles * col_tiles, total = per_group * (rows_grouped ? 1 : p.groups);   // (below 2^31: the launch checks)
+    const int per_list = row_tiles * col_tiles, end = lists_end16(per_list, rows_grouped ? 1 : p.groups);   // (below 2^31: the launch checks)
 
     // ---- this lane's fragment reads (the current stage's; moved by a panel from step to step)
     // A, K contiguous: panel position 128 wm + 32 i + r holds tile row 64 i + 32 wm + r; K-major: column = tile row
@@ -101,8 +101,13 @@ __global__ __launch_bounds__(Big16::THREADS, 2) void gemm16_big_kernel(Gemm16 p)
     };
     const int64_t adv_a = A_KM ? p.pitch_a * 128 : 128, adv_b = B_KM ? p.pitch_b * 128 : 128;   // bytes from step to step
     const int k8 = (p.k + 7) & ~7, n8 = (p.n + 7) & ~7, m8 = (p.m + 7) & ~7;
-    auto decode = [&](int t, Tile &c) {
-        const int at = place16(t, total);
+    // The tile at t, or the next one there is of this workgroup's (t moves on).
+    auto decode = [&](int &t, Tile &c) {
+        int at = -1, list = 0;
+        for (; t < end; t += (int)gridDim.x) {
+            at = place_in_lists16(t, per_list, list);
+            if (at >= 0) break;
+        }
         c.valid = at >= 0;
         c.steps = 2;
         c.k_len = 0;
@@ -113,14 +118,13 @@ __global__ __launch_bounds__(Big16::THREADS, 2) void gemm16_big_kernel(Gemm16 p)
         if (!c.valid) return;
         int rt, ct, k0 = 0;
         c.k_len = p.k;
+        tile_of16(at, row_tiles, col_tiles, rt, ct);
         if (rows_grouped) {
-            tile_of16(at, row_tiles, col_tiles, rt, ct);
             c.e = uniform(group_of_tile16(tab, p.groups, rt));
             c.m0 = uniform(tab.start[c.e] + (rt - tab.tile[c.e]) * S::TM);
             c.m_end = uniform(tab.start[c.e + 1]);
         } else {
-            c.e = at / per_group;
-            tile_of16(at - c.e * per_group, row_tiles, col_tiles, rt, ct);
+            c.e = list;
             c.m0 = rt * S::TM;
             c.m_end = p.m;
             k0 = uniform(tab.start[c.e]);

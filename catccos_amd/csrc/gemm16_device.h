@@ -18,6 +18,7 @@ struct Bf16 {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(V8, a), __builtin_bit_cast(V8, b), c, 0, 0, 0);
     }
     static __device__ __forceinline__ uint16_t from(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }   // to nearest even
+    static __device__ __forceinline__ uint32_t two(float a, float b) { return __builtin_bit_cast(uint32_t, (bf16x2){(__bf16)a, (__bf16)b}); }
     static __device__ __forceinline__ float to(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
 };
 struct F16 {
@@ -27,6 +28,7 @@ struct F16 {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(V8, a), __builtin_bit_cast(V8, b), c, 0, 0, 0);
     }
     static __device__ __forceinline__ uint16_t from(float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
+    static __device__ __forceinline__ uint32_t two(float a, float b) { return __builtin_bit_cast(uint32_t, (f16x2){(_Float16)a, (_Float16)b}); }
     static __device__ __forceinline__ float to(uint16_t v) { return (float)__builtin_bit_cast(_Float16, v); }
 };
 
@@ -43,11 +45,11 @@ __device__ __forceinline__ float act_value(float z, int act)
     default: return z;
     }
 }
-// (one branch for eight values)
-__device__ __forceinline__ void apply_act(float v[8], int act)
+// (one branch for all of them)
+template <int N> __device__ __forceinline__ void apply_act(float (&v)[N], int act)
 {
     switch (act) {
-#define CCH_EACH(ACT) case ACT: for (int x = 0; x < 8; x++) v[x] = act_value(v[x], ACT); break
+#define CCH_EACH(ACT) case ACT: _Pragma("unroll") for (int x = 0; x < N; x++) v[x] = act_value(v[x], ACT); break
     CCH_EACH(CCH_ACT_RELU);
     CCH_EACH(CCH_ACT_SILU);
     CCH_EACH(CCH_ACT_GELU);
@@ -126,6 +128,16 @@ __device__ __forceinline__ int place16(int t, int total)
     const int64_t at = (int64_t)(t & 7) * per + i;
     return i < per && at < total ? (int)at : -1;
 }
+// The launch's t-th tile of `groups` lists of `per` tiles each: the list in `e`, the place in it returned, -1 for none.  Every list is spread over all XCDs, as lists
+// whose tiles take different times (groups of K) would otherwise leave some XCDs behind.  `lists_end`: from where on there is none.
+__device__ __forceinline__ int lists_end16(int per, int groups) { return ((per + 7) & ~7) * groups; }
+__device__ __forceinline__ int place_in_lists16(int t, int per, int &e)
+{
+    const int whole = (per + 7) & ~7;
+    e = t / whole;
+    return place16(t - e * whole, per);
+}
+
 // Tiles are walked in bands of 8 row tiles, column by column: the 32 to 64 tiles that an XCD works on at a time then share 8 panels of A and 4 to 8 of B.
 constexpr int BAND16 = 8;
 __device__ __forceinline__ void tile_of16(int at, int row_tiles, int col_tiles, int &rt, int &ct)
@@ -162,19 +174,7 @@ __device__ __forceinline__ Rsrc kmajor_rsrc(const uint16_t *base, int64_t pitch,
     return make_rsrc(base + (int64_t)k0 * pitch + c0, (uint32_t)min(left, (int64_t)0x7FFFFFF0));
 }
 
-// ---- epilogues.  The matrix instructions take B's fragment first: lane (r, g) then holds, of a 32 x 32 block, row r and columns 8 q + 4 g + x at 4 q + x.  Two swaps
-// between the wave's halves make that columns 16 h + 8 g + 0..7 of half h, 16 bytes of output to a lane.
-__device__ __forceinline__ void eight_columns(const v16f &acc, float v[2][8])
-{
-#pragma unroll
-    for (int h = 0; h < 2; h++)
-#pragma unroll
-        for (int x = 0; x < 4; x++) {
-            const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[8 * h + x]), __float_as_uint(acc[8 * h + 4 + x]), false, false);
-            v[h][x] = __uint_as_float(s[0]);
-            v[h][4 + x] = __uint_as_float(s[1]);
-        }
-}
+// ---- epilogues.  The matrix instructions take B's fragment first: lane (r, g) then holds, of a 32 x 32 block, row r and columns 8 q + 4 g + x at 4 q + x.
 template <class T> __device__ __forceinline__ v4i pack8(const float v[8])
 {
     v4i o;
@@ -220,20 +220,63 @@ __device__ __forceinline__ bool whole_rows(const Gemm16 &p)
 // Whether every tile of such a problem stores the same number of times, whatever of it exists: 16 stores of a wave with 128 x 64 outputs, twice that with preact.
 template <int EPI> __device__ __forceinline__ bool counted_stores(const Gemm16 &p) { return EPI != EPI16_STATS && !p.sums && !p.out_rows; }
 
-// A wave's results on their way to memory, 32 rows of 32 columns: a lane holds two pieces of 16 bytes of one row, h = 0 and 1, columns 16 h + 8 g.  Swapping rows of 16 lanes between
-// the two brings four lanes to a row, 64 bytes, 16 rows to a store: store(first row, piece), the lane's row being (lane & 15) of it and its columns those of lane_columns().
-// Stored as the lanes hold them, 32 bytes a row, a 256 x 256 tile's epilogue took 11 us.
+// A block's 16 values of a lane as memory wants them.  Rounded to pairs (q, w) of columns 8 q + 4 g + 2 w, + 1; a swap between the wave's halves of pairs 2 h and 2 h + 1 makes that 16 bytes of
+// columns 16 h + 8 g; a swap of rows of 16 lanes between h = 0 and 1 then brings four lanes, 64 bytes, to a row: out[0] has rows 0..15 of the block, out[1] rows 16..31, the lane's row among them
+// being lane & 15 and its columns lane_columns(lane) + 0..7.  Both swaps undo themselves.  Pairs are swapped, not the fp32 values: the epilogue of a tile is its vector instructions, four clocks
+// each and two waves to a SIMD.  (Stored as the lanes hold them, 32 bytes a row, a 256 x 256 tile's epilogue took 11 us; 64 bytes a row is as fast as whole lines by way of LDS.)
 __device__ __forceinline__ int lane_columns(int lane) { return (lane >> 4 & 1) * 16 + (lane >> 5) * 8; }
-template <class Store> __device__ __forceinline__ void by_rows(v4i x, v4i y, Store &&store)
+__device__ __forceinline__ void swap32(uint32_t &x, uint32_t &y)
 {
+    const auto s = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+    x = s[0];
+    y = s[1];
+}
+__device__ __forceinline__ void swap16(uint32_t &x, uint32_t &y)
+{
+    const auto s = __builtin_amdgcn_permlane16_swap(x, y, false, false);
+    x = s[0];
+    y = s[1];
+}
+template <class T> __device__ __forceinline__ void to_rows(const float (&v)[16], v4i (&out)[2])
+{
+    uint32_t p[4][2];
 #pragma unroll
-    for (int d = 0; d < 4; d++) {
-        const auto s = __builtin_amdgcn_permlane16_swap((uint32_t)x[d], (uint32_t)y[d], false, false);
-        x[d] = (int)s[0];
-        y[d] = (int)s[1];
-    }
-    store(0, x);
-    store(16, y);
+    for (int q = 0; q < 4; q++)
+#pragma unroll
+        for (int w = 0; w < 2; w++) p[q][w] = T::two(v[4 * q + 2 * w], v[4 * q + 2 * w + 1]);
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int w = 0; w < 2; w++) swap32(p[2 * h][w], p[2 * h + 1][w]);
+#pragma unroll
+    for (int q = 0; q < 2; q++)
+#pragma unroll
+        for (int w = 0; w < 2; w++) swap16(p[q][w], p[q + 2][w]);
+#pragma unroll
+    for (int h = 0; h < 2; h++) out[h] = (v4i){(int)p[2 * h][0], (int)p[2 * h][1], (int)p[2 * h + 1][0], (int)p[2 * h + 1][1]};
+}
+template <class T> __device__ __forceinline__ void from_rows(const v4i (&in)[2], float (&v)[16])
+{
+    uint32_t p[4][2];
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int x = 0; x < 4; x++) p[2 * h + (x >> 1)][x & 1] = (uint32_t)in[h][x];
+#pragma unroll
+    for (int q = 0; q < 2; q++)
+#pragma unroll
+        for (int w = 0; w < 2; w++) swap16(p[q][w], p[q + 2][w]);
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int w = 0; w < 2; w++) swap32(p[2 * h][w], p[2 * h + 1][w]);
+#pragma unroll
+    for (int q = 0; q < 4; q++)
+#pragma unroll
+        for (int w = 0; w < 2; w++) {
+            v[4 * q + 2 * w] = T::to((uint16_t)p[q][w]);
+            v[4 * q + 2 * w + 1] = T::to((uint16_t)(p[q][w] >> 16));
+        }
 }
 
 // The results of one wave: MT x NT blocks of 32 x 32, every RS rows from row mw on and side by side from column nw of the tile that begins at row m0 and column n0 of the
@@ -248,23 +291,36 @@ __device__ __forceinline__ void epilogue16(const Gemm16 &p, v16f (&acc)[MT][NT],
     asm volatile("" : "+v"(lane));
     const int r = lane & 31, g = lane >> 5, m0 = tile_m + mw, n0 = tile_n + nw;
     if (!counted && n0 >= p.n) return;
+    // this lane's columns of block j: n0 + 32 j + 8 q + 4 g + x at 4 q + x; those from `left` on do not exist
+    const int left = p.n - n0 - 4 * g;
+    auto column = [](int j, int x) { return 32 * j + 8 * (x >> 2) + (x & 3); };
+    const bool edge = n0 + 32 * NT > p.n;
     if constexpr (EPI == EPI16_STATS) {
         // 64 columns' largest logit and sum of exponentials, the two halves of the wave joined; a target's logit on the way
-#pragma unroll
-        for (int i = 0; i < MT; i++) {
+        static_for<MT>([&](auto i_c) {
+            constexpr int i = decltype(i_c)::value;
             const int m = m0 + RS * i + r;
             const bool there = m < m_end;
             const int want = there ? p.targets[m] - p.v0 - n0 - 4 * g : -1;
+            if (__any(want >= 0 && want < 32 * NT)) {
+#pragma unroll
+                for (int j = 0; j < NT; j++)
+#pragma unroll
+                    for (int x = 0; x < 16; x++)
+                        if (column(j, x) == want) p.target_logit[m] = acc[i][j][x];
+            }
+            if (edge) {
+#pragma unroll
+                for (int j = 0; j < NT; j++)
+#pragma unroll
+                    for (int x = 0; x < 16; x++)
+                        if (column(j, x) >= left) acc[i][j][x] = -INFINITY;
+            }
             float top = -INFINITY;
 #pragma unroll
             for (int j = 0; j < NT; j++)
 #pragma unroll
-                for (int x = 0; x < 16; x++) {
-                    const int c = 32 * j + 8 * (x >> 2) + (x & 3);
-                    if (n0 + c + 4 * g >= p.n) acc[i][j][x] = -INFINITY;
-                    top = fmaxf(top, acc[i][j][x]);
-                    if (c == want) p.target_logit[m] = acc[i][j][x];
-                }
+                for (int x = 0; x < 16; x++) top = fmaxf(top, acc[i][j][x]);
             top = fmaxf(top, __shfl_xor(top, 32));
             float sum = 0.0f;
 #pragma unroll
@@ -273,116 +329,145 @@ __device__ __forceinline__ void epilogue16(const Gemm16 &p, v16f (&acc)[MT][NT],
                 for (int x = 0; x < 16; x++) sum += __expf(acc[i][j][x] - top);
             sum += __shfl_xor(sum, 32);
             if (there && g == 0) p.stats[(int64_t)m * p.stat_cols + (p.v0 + n0) / (32 * NT)] = make_float2(top, sum);
-        }
-        return;
+        });
     } else {
-        const float scale = EPI == EPI16_OUT && p.scale ? *p.scale : 1.0f;
         uint16_t *const out = p.out + (int64_t)group * p.out_stride;
+        const bool scaled = EPI == EPI16_OUT && p.scale, summed = EPI == EPI16_OUT && p.sums;
+        const float scale = scaled ? *p.scale : 1.0f;
+        const int lc = lane_columns(lane);
         // counted: descriptors of the tile's rows that exist; a lane whose columns do not starts 2^31 bytes behind, past any of them
         const int64_t tile_at = (int64_t)tile_m * p.pitch_out + tile_n;
         const int tile_bytes = (int)min(((int64_t)max(m_end - tile_m, 0) * p.pitch_out - tile_n) * 2, (int64_t)0x7FFFFFF0);
         const uint32_t pitch = (uint32_t)p.pitch_out * 2u;
-        const int lc = lane_columns(lane);
         uint32_t lane_at[NT];
 #pragma unroll
         for (int j = 0; j < NT; j++) lane_at[j] = (uint32_t)(mw + (lane & 15)) * pitch + (uint32_t)(nw + 32 * j + lc) * 2u + (n0 + 32 * j + lc < p.n ? 0u : 0x80000000u);
+        float bias[NT][16];
+        if constexpr (EPI == EPI16_ACT) {
+            if (p.bias) {
+#pragma unroll
+                for (int j = 0; j < NT; j++)
+#pragma unroll
+                    for (int x = 0; x < 16; x++) bias[j][x] = column(j, x) < left ? T::to(p.bias[n0 + 4 * g + column(j, x)]) : 0.0f;
+            }
+        }
         static_for<MT>([&](auto i_c) {
             constexpr int i = decltype(i_c)::value;
             const int first = m0 + RS * i, m = first + r;
             if (!counted && first >= m_end) return;
             const bool there = m < m_end;
             float lse = 0.0f, slope = 0.0f;
-            int target = -1;
-            if (EPI == EPI16_GRAD) {
+            int want = -1;
+            bool wanted = false;
+            if constexpr (EPI == EPI16_GRAD) {
                 lse = there ? p.lse[m] : 0.0f;
                 slope = (1.0f + p.z2 * lse) * p.grad_scale;
-                target = there ? p.targets[m] - p.v0 : -1;
+                want = there ? p.targets[m] - p.v0 - n0 - 4 * g : -1;
+                wanted = __any(want >= 0 && want < 32 * NT);
             }
-            v4i piece[2][2], pre[2][2];
+            static_for<NT>([&](auto j_c) {
+                constexpr int j = decltype(j_c)::value;
+                float v[16];
 #pragma unroll
-            for (int j = 0; j < NT; j++) {
-                float v[2][8];
-                eight_columns(acc[i][j], v);
+                for (int x = 0; x < 16; x++) v[x] = acc[i][j][x];
+                // sixteen bytes of `base` in rows' layout: store (or load) row `row` of the block, columns lane_at
+                auto each_row = [&](auto &&at_row) {
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const int n = n0 + 32 * j + 16 * h + 8 * g, left = p.n - n;
-                    const bool in = there && left > 0;
-                    if constexpr (EPI == EPI16_OUT) {
-                        if (p.sums && in) {
-                            float *s = p.sums + (int64_t)m * p.n + n;
-#pragma unroll
-                            for (int x = 0; x < 8; x++)
-                                if (x < left) {
-                                    if (p.sums_in) v[h][x] += s[x];
-                                    if (p.sums_out) s[x] = v[h][x];
-                                }
-                        }
-#pragma unroll
-                        for (int x = 0; x < 8; x++) v[h][x] *= scale;
-                    } else if constexpr (EPI == EPI16_ACT) {
-                        float b[8];
-                        if (p.bias && in) {
-                            load8<T>(p.bias + n, whole, left, b);
-#pragma unroll
-                            for (int x = 0; x < 8; x++) v[h][x] += b[x];
-                        }
-                        pre[j][h] = pack8<T>(v[h]);
-                        apply_act(v[h], p.act);
-                        if (p.residual && in) {
-                            load8<T>(p.residual + (int64_t)m * p.pitch_out + n, whole, left, b);
-#pragma unroll
-                            for (int x = 0; x < 8; x++) v[h][x] += b[x];
-                        }
-                    } else {
-                        // rows of the gradient end on 16-byte boundaries, zeros behind the last column: the next product reads it along K
-#pragma unroll
-                        for (int x = 0; x < 8; x++) {
-                            const float d = __expf(v[h][x] - lse) * slope - (n + x == target ? p.grad_scale : 0.0f);
-                            v[h][x] = x < left ? d : 0.0f;
-                        }
+                    for (int h = 0; h < 2; h++) {
+                        const int at = first + 16 * h + (lane & 15), c = n0 + 32 * j + lc;
+                        if (at >= m_end || c >= p.n) continue;
+                        const int64_t to = EPI == EPI16_OUT && p.out_rows ? p.out_rows[at] : at;
+                        at_row(h, to * p.pitch_out + c);
                     }
-                    piece[j][h] = pack8<T>(v[h]);
-                }
-            }
-            if (EPI == EPI16_OUT && p.sums_out) return;
-            if (counted) {
-                auto put = [&](uint16_t *base, const v4i (&what)[2][2]) {
-                    const auto rs = __builtin_amdgcn_make_buffer_rsrc(base + tile_at, 0, tile_bytes, 0x00020000);
-#pragma unroll
-                    for (int j = 0; j < NT; j++)
-                        by_rows(what[j][0], what[j][1], [&](int row, v4i o) {
-                            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, o), rs, lane_at[j] + (uint32_t)(RS * i + row) * pitch, 0, 0);
-                        });
                 };
-                if (EPI == EPI16_ACT && p.preact) put(p.preact, pre);
-                put(out, piece);
-            } else if (whole) {
-                auto put = [&](uint16_t *base, const v4i (&what)[2][2]) {
+                auto store = [&](uint16_t *base) {
+                    if (whole) {
+                        v4i rows[2];
+                        to_rows<T>(v, rows);
+                        if (counted) {
+                            const auto rs = __builtin_amdgcn_make_buffer_rsrc(base + tile_at, 0, tile_bytes, 0x00020000);
 #pragma unroll
-                    for (int j = 0; j < NT; j++)
-                        by_rows(what[j][0], what[j][1], [&](int row, v4i o) {
-                            const int at = first + row + (lane & 15), c = n0 + 32 * j + lc;
-                            if (at >= m_end || c >= p.n) return;
-                            const int64_t to = EPI == EPI16_OUT && p.out_rows ? p.out_rows[at] : at;
-                            *reinterpret_cast<v4i *>(base + to * p.pitch_out + c) = o;
-                        });
-                };
-                if (EPI == EPI16_ACT && p.preact) put(p.preact, pre);
-                put(out, piece);
-            } else if (there) {
-                const int64_t to = EPI == EPI16_OUT && p.out_rows ? p.out_rows[m] : m;
-#pragma unroll
-                for (int j = 0; j < NT; j++)
-#pragma unroll
-                    for (int h = 0; h < 2; h++)
-#pragma unroll
-                        for (int x = 0; x < 8; x++) {
-                            const int n = n0 + 32 * j + 16 * h + 8 * g + x;
-                            if (n >= p.n) continue;
-                            out[to * p.pitch_out + n] = (uint16_t)((uint32_t)piece[j][h][x >> 1] >> (16 * (x & 1)));
-                            if (EPI == EPI16_ACT && p.preact) p.preact[to * p.pitch_out + n] = (uint16_t)((uint32_t)pre[j][h][x >> 1] >> (16 * (x & 1)));
+                            for (int h = 0; h < 2; h++)
+                                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, rows[h]), rs, lane_at[j] + (uint32_t)(RS * i + 16 * h) * pitch, 0, 0);
+                        } else {
+                            each_row([&](int h, int64_t at) { *reinterpret_cast<v4i *>(base + at) = rows[h]; });
                         }
-            }
+                    } else if (there) {
+                        const int64_t to = (EPI == EPI16_OUT && p.out_rows ? p.out_rows[m] : m) * p.pitch_out + n0 + 4 * g;
+#pragma unroll
+                        for (int x = 0; x < 16; x++)
+                            if (column(j, x) < left) base[to + column(j, x)] = T::from(v[x]);
+                    }
+                };
+                if constexpr (EPI == EPI16_OUT) {
+                    if (summed) {
+                        float *s = p.sums + (int64_t)m * p.n + n0 + 4 * g;
+                        if (there)
+#pragma unroll
+                            for (int q = 0; q < 4; q++) {
+                                const int c = column(j, 4 * q);
+                                if (p.n % 4 == 0 && c < left) {
+                                    f32x4 *at = reinterpret_cast<f32x4 *>(s + c);
+                                    f32x4 a = {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+                                    if (p.sums_in) a += *at;
+                                    if (p.sums_out) *at = a;
+#pragma unroll
+                                    for (int x = 0; x < 4; x++) v[4 * q + x] = a[x];
+                                } else {
+#pragma unroll
+                                    for (int x = 0; x < 4; x++)
+                                        if (c + x < left) {
+                                            if (p.sums_in) v[4 * q + x] += s[c + x];
+                                            if (p.sums_out) s[c + x] = v[4 * q + x];
+                                        }
+                                }
+                            }
+                        if (p.sums_out) return;
+                    }
+                    if (scaled) {
+#pragma unroll
+                        for (int x = 0; x < 16; x++) v[x] *= scale;
+                    }
+                    store(out);
+                } else if constexpr (EPI == EPI16_ACT) {
+                    if (p.bias) {
+#pragma unroll
+                        for (int x = 0; x < 16; x++) v[x] += bias[j][x];
+                    }
+                    if (p.preact) store(p.preact);
+                    apply_act(v, p.act);
+                    if (p.residual) {
+                        float add[16] = {};
+                        if (whole) {
+                            v4i rows[2] = {};
+                            each_row([&](int h, int64_t at) { rows[h] = *reinterpret_cast<const v4i *>(p.residual + at); });
+                            from_rows<T>(rows, add);
+                        } else if (there) {
+#pragma unroll
+                            for (int x = 0; x < 16; x++)
+                                if (column(j, x) < left) add[x] = T::to(p.residual[(int64_t)m * p.pitch_out + n0 + 4 * g + column(j, x)]);
+                        }
+#pragma unroll
+                        for (int x = 0; x < 16; x++) v[x] += add[x];
+                    }
+                    store(out);
+                } else {
+                    // rows of the gradient end on 16-byte boundaries, zeros behind the last column: the next product reads it along K
+#pragma unroll
+                    for (int x = 0; x < 16; x++) v[x] = __expf(v[x] - lse) * slope;
+                    if (wanted) {
+#pragma unroll
+                        for (int x = 0; x < 16; x++)
+                            if (column(j, x) == want) v[x] -= p.grad_scale;
+                    }
+                    if (edge) {
+#pragma unroll
+                        for (int x = 0; x < 16; x++)
+                            if (column(j, x) >= left) v[x] = 0.0f;
+                    }
+                    store(out);
+                }
+            });
         });
     }
 }

@@ -37,7 +37,7 @@ __global__ __launch_bounds__(S::THREADS, S::PER_CU * S::WAVES / 4) void gemm16_k
     const uint32_t lds = (uint32_t)uniform((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)smem);
     const int col_tiles = (p.n + S::TN - 1) / S::TN;
     const int row_tiles = uniform(rows_grouped ? tab.tile[p.groups] : (p.m + S::TM - 1) / S::TM);
-    const int total = row_tiles * col_tiles * (rows_grouped ? 1 : p.groups);   // (below 2^31: the launch checks)
+    const int per_list = row_tiles * col_tiles * p.splits, end = lists_end16(per_list, rows_grouped ? 1 : p.groups);   // (below 2^31: the launch checks)
     const bool whole = whole_rows(p);
 
     // this lane's fragment reads in stage 0
@@ -56,22 +56,17 @@ __global__ __launch_bounds__(S::THREADS, S::PER_CU * S::WAVES / 4) void gemm16_k
     for (int j = 0; j < NT; j++)
         ft_b[j] = lds + S::A_BYTES + (uint32_t)krow * KB::ROW + ((((uint32_t)(wn * NT + j) * 4 + quarter) ^ KB::swizzle(krow)) << 4) + (ti & 1) * 8u;
 
-    const int parts = p.splits * total;   // (below 2^31)
-    for (int64_t t = blockIdx.x; t < ((parts + 7) & ~7); t += gridDim.x) {
-        int at = place16((int)t, parts);
+    for (int64_t t = blockIdx.x; t < end; t += gridDim.x) {
+        int e = 0, rt, ct, m0, m_end, k_begin = 0, k_end = p.k;
+        const int at = place_in_lists16((int)t, per_list, e);
         if (at < 0) continue;
         const int part = at % p.splits;
-        at /= p.splits;
-        int e = 0, rt, ct, m0, m_end, k_begin = 0, k_end = p.k;
+        tile_of16(at / p.splits, row_tiles, col_tiles, rt, ct);
         if (rows_grouped) {
-            tile_of16(at, row_tiles, col_tiles, rt, ct);
             e = uniform(group_of_tile16(tab, p.groups, rt));
             m0 = uniform(tab.start[e] + (rt - tab.tile[e]) * S::TM);
             m_end = uniform(tab.start[e + 1]);
         } else {
-            const int per = row_tiles * col_tiles;
-            e = at / per;
-            tile_of16(at - e * per, row_tiles, col_tiles, rt, ct);
             m0 = rt * S::TM;
             m_end = p.m;
             k_begin = uniform(tab.start[e]);
@@ -211,7 +206,7 @@ template <class T, int LAYOUT, int EPI, class S> int launch16(const Gemm16 &p, i
     static std::atomic<uint64_t> attr_set{0};
     auto kernel = gemm16_kernel<T, LAYOUT, EPI, S>;
     if (const int rc = allow_lds16(reinterpret_cast<const void *>(kernel), S::LDS, attr_set)) return rc;
-    const int64_t grid = std::min<int64_t>((tiles * p.splits + 7) & ~(int64_t)7, (int64_t)1 << 22);   // (a multiple of 8: place16)
+    const int64_t groups = p.k_grouped ? p.groups : 1, grid = std::min<int64_t>((tiles / groups * p.splits + 7) / 8 * 8 * groups, (int64_t)1 << 22);   // (a multiple of 8: place16)
     kernel<<<dim3((uint32_t)grid), dim3(S::THREADS), S::LDS, stream>>>(p);
     return launch_status("gemm16_kernel");
 }
