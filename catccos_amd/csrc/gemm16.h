@@ -104,10 +104,13 @@ struct Carve {
     }
 };
 
-// Rows of `cols` elements copied to rows of pitch16(cols), zeros behind them.
-int pad_rows16(const uint16_t *src, uint16_t *dst, int64_t rows, int64_t cols, hipStream_t stream);
-// `src`, or its padded copy where its rows need one (space from `ws`); the pitch in *pitch.
-int operand16(const uint16_t *src, int64_t rows, int64_t cols, Carve &ws, const uint16_t **out, int64_t *pitch, hipStream_t stream);
+// An operand's rows of `cols` elements, back to back.  `whole_operands16` makes copies in rows of pitch16(cols), zeros behind them, of those that are no whole multiples of 16 bytes
+// (space from `ws`), and points `at` there; an operand that is not there (nullptr) stays so.
+struct Operand16 {
+    const uint16_t *at;
+    int64_t rows, cols;
+};
+int whole_operands16(Operand16 *operands, int n, Carve &ws, hipStream_t stream);
 
 int fill_zero16(uint16_t *dst, int64_t n, hipStream_t stream);
 // dz = grad_out * act'(preact) in rows of pitch16(n) and its column sums; either may be left out.  partial: column_sum_bytes(...) of fp32

@@ -114,38 +114,52 @@ int gemm16_launch(const Gemm16 &problem, int layout, int epilogue, hipStream_t s
     return p.half ? join16<F16>(p, epilogue, stream) : join16<Bf16>(p, epilogue, stream);
 }
 
-// One thread, 16 bytes of the copy.
-__global__ __launch_bounds__(256) void pad_rows16_kernel(const uint16_t *__restrict__ src, uint16_t *__restrict__ dst, int64_t chunks, int64_t cols, int64_t per_row)
+// One thread, 16 bytes of a copy; up to two operands in a launch.
+struct PadRows16 {
+    const uint16_t *src;
+    uint16_t *dst;
+    int64_t chunks, cols, per_row;
+};
+__global__ __launch_bounds__(256) void pad_rows16_kernel(PadRows16 a, PadRows16 b)
 {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < chunks; i += (int64_t)gridDim.x * 256) {
-        const int64_t row = i / per_row, c = (i - row * per_row) * 8;
-        const uint16_t *s = src + row * cols + c;
-        v4i o;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.chunks + b.chunks; i += (int64_t)gridDim.x * 256) {
+        const bool second = i >= a.chunks;
+        const PadRows16 &o = second ? b : a;
+        const int64_t at = second ? i - a.chunks : i, row = at / o.per_row, c = (at - row * o.per_row) * 8;
+        const uint16_t *s = o.src + row * o.cols + c;
+        v4i v;
 #pragma unroll
         for (int x = 0; x < 4; x++) {
-            const uint32_t lo = c + 2 * x < cols ? s[2 * x] : 0u, hi = c + 2 * x + 1 < cols ? s[2 * x + 1] : 0u;
-            o[x] = (int)(lo | hi << 16);
+            const uint32_t lo = c + 2 * x < o.cols ? s[2 * x] : 0u, hi = c + 2 * x + 1 < o.cols ? s[2 * x + 1] : 0u;
+            v[x] = (int)(lo | hi << 16);
         }
-        *reinterpret_cast<v4i *>(dst + i * 8) = o;
+        *reinterpret_cast<v4i *>(o.dst + at * 8) = v;
     }
 }
 
-int pad_rows16(const uint16_t *src, uint16_t *dst, int64_t rows, int64_t cols, hipStream_t stream)
+int whole_operands16(Operand16 *operands, int n, Carve &ws, hipStream_t stream)
 {
-    const int64_t per_row = pitch16(cols) / 8, chunks = rows * per_row;
-    if (chunks == 0) return CCH_OK;
-    hipLaunchKernelGGL(pad_rows16_kernel, dim3((unsigned)std::min<int64_t>((chunks + 255) / 256, 1 << 16)), dim3(256), 0, stream, src, dst, chunks, cols, per_row);
-    return launch_status("pad_rows16_kernel");
-}
-
-int operand16(const uint16_t *src, int64_t rows, int64_t cols, Carve &ws, const uint16_t **out, int64_t *pitch, hipStream_t stream)
-{
-    *pitch = pitch16(cols);
-    *out = src;
-    if (whole16(cols)) return CCH_OK;
-    uint16_t *copy = ws.take<uint16_t>(padded16_bytes(rows, cols));
-    *out = copy;
-    return pad_rows16(src, copy, rows, cols, stream);
+    PadRows16 pads[2] = {};
+    int used = 0;
+    for (int i = 0; i < n; i++) {
+        Operand16 &o = operands[i];
+        if (!o.at || whole16(o.cols) || o.rows == 0 || o.cols == 0) continue;
+        uint16_t *copy = ws.take<uint16_t>(padded16_bytes(o.rows, o.cols));
+        pads[used++] = PadRows16{o.at, copy, o.rows * (pitch16(o.cols) / 8), o.cols, pitch16(o.cols) / 8};
+        o.at = copy;
+        if (used == 2 || i + 1 == n) {
+            const int64_t chunks = pads[0].chunks + pads[1].chunks;
+            hipLaunchKernelGGL(pad_rows16_kernel, dim3((unsigned)std::min<int64_t>((chunks + 255) / 256, 1 << 16)), dim3(256), 0, stream, pads[0], pads[1]);
+            if (const int rc = launch_status("pad_rows16_kernel")) return rc;
+            pads[0] = pads[1] = PadRows16{};
+            used = 0;
+        }
+    }
+    if (used) {
+        hipLaunchKernelGGL(pad_rows16_kernel, dim3((unsigned)std::min<int64_t>((pads[0].chunks + 255) / 256, 1 << 16)), dim3(256), 0, stream, pads[0], pads[1]);
+        return launch_status("pad_rows16_kernel");
+    }
+    return CCH_OK;
 }
 
 __global__ __launch_bounds__(256) void fill_zero16_kernel(uint16_t *dst, int64_t n)
@@ -161,7 +175,7 @@ int fill_zero16(uint16_t *dst, int64_t n, hipStream_t stream)
 // ---- dz = grad_out * act'(preact) and the bias' gradient.  A workgroup has 256 columns, 8 to a thread, and a run of rows, every eighth to a thread; its columns' sums over
 // the run go to `partial`, which a second launch adds up in the runs' order.  Sums are of the products before their rounding.  Bound by memory: two reads, one write.
 constexpr int SUM_COLS = 256, SUM_RUNS = 64;
-static int64_t sum_runs(int64_t m) { return std::max<int64_t>(1, std::min<int64_t>((m + 63) / 64, SUM_RUNS)); }
+static int64_t sum_runs(int64_t m) { return std::max<int64_t>(1, std::min<int64_t>((m + 7) / 8, SUM_RUNS)); }
 int64_t column_sum_bytes(int64_t m, int64_t n) { return round256(sum_runs(m) * n * 4); }
 
 template <class T>

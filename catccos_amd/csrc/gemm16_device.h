@@ -82,16 +82,24 @@ struct GroupTable16 {
     int start[MAX_GROUPS16 + 1];
     int tile[MAX_GROUPS16 + 1];
 };
-// By one wave.  `all`: rows (or K) that there are; sizes are clipped to what the groups before leave.  bm: rows of a tile.
+// By one wave.  `all`: rows (or K) that there are; sizes are clipped to what the groups before leave (no sizes: one group of all).  bm: rows of a tile.
 __device__ inline void build_groups16(GroupTable16 &tab, const int32_t *sizes, int groups, int all, int bm)
 {
     const int lane = threadIdx.x & 63;
+    if (!sizes) {
+        if (lane == 0) {
+            tab.start[0] = tab.tile[0] = 0;
+            tab.start[1] = all;
+            tab.tile[1] = (all + bm - 1) / bm;
+        }
+        return;
+    }
     uint32_t before = 0;
     int tiles_before = 0;
     for (int b = 0; b < groups; b += 64) {
         const int g = b + lane;
         uint32_t sz = 0;
-        if (g < groups) sz = sizes ? (uint32_t)min(max(sizes[g], 0), all) : (uint32_t)all;
+        if (g < groups) sz = (uint32_t)min(max(sizes[g], 0), all);
         const uint32_t incl = sat_add(before, wave_scan_sat(sz));
         const uint32_t prev = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)incl, 0x138, 0xF, 0xF, false);   // the neighbour's: wave_shr:1
         const int hi = (int)min(incl, (uint32_t)all), lo = (int)min(lane == 0 ? before : prev, (uint32_t)all);

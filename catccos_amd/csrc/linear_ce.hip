@@ -308,7 +308,10 @@ extern "C" int cch_linear_cross_entropy(const void *x, const void *w, const void
             p.a = rows;
         }
         Carve wc{ws + at.w};
-        if (const int rc = operand16(static_cast<const uint16_t *>(w), v, h, wc, &p.b, &p.pitch_b, s)) return rc;
+        Operand16 in{static_cast<const uint16_t *>(w), v, h};
+        if (const int rc = whole_operands16(&in, 1, wc, s)) return rc;
+        p.b = in.at;
+        p.pitch_b = pitch16(h);
         p.m = (int)t;
         p.n = (int)v;
         p.k = (int)h;
@@ -366,10 +369,11 @@ extern "C" int cch_linear_cross_entropy_backward(const float *grad_loss, const v
     if (const int rc = launch_status("ce_tokens_kernel")) return rc;
     uint16_t *rows = reinterpret_cast<uint16_t *>(ws + at.rows), *d = reinterpret_cast<uint16_t *>(ws + at.d);
     if (const int rc = ce_gather(static_cast<const uint16_t *>(x), tk.pos, rows, gx, t, h, s)) return rc;
-    const uint16_t *pw;
-    int64_t ldw;
+    Operand16 in{static_cast<const uint16_t *>(w), v, h};
     Carve wc{ws + at.w};
-    if (const int rc = operand16(static_cast<const uint16_t *>(w), v, h, wc, &pw, &ldw, s)) return rc;
+    if (const int rc = whole_operands16(&in, 1, wc, s)) return rc;
+    const uint16_t *pw = in.at;
+    const int64_t ldw = pitch16(h);
 
     const int64_t piece = ce_piece(t, v);
     for (int64_t v0 = 0; v0 < v; v0 += piece) {

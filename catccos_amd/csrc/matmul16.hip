@@ -130,11 +130,9 @@ extern "C" int cch_grouped_matmul(const void *x, const void *w, const int32_t *g
     if (const int rc = check_workspace16("cch_grouped_matmul", workspace, workspace_bytes, cch_grouped_matmul_workspace_bytes(num_experts, t, n, k, trans_b))) return rc;
     hipStream_t s = static_cast<hipStream_t>(stream);
     Carve ws{static_cast<uint8_t *>(workspace)};
-    const uint16_t *px, *pw;
-    int64_t ldx, ldw;
-    if (const int rc = operand16(u16(x), t, k, ws, &px, &ldx, s)) return rc;
-    if (const int rc = operand16(u16(w), num_experts * (trans_b ? n : k), trans_b ? k : n, ws, &pw, &ldw, s)) return rc;
-    Gemm16 p = grouped_product(px, pw, group_sizes, u16(out), num_experts, t, n, k, trans_b, dtype);
+    Operand16 in[2] = {{u16(x), t, k}, {u16(w), num_experts * (trans_b ? n : k), trans_b ? k : n}};
+    if (const int rc = whole_operands16(in, 2, ws, s)) return rc;
+    Gemm16 p = grouped_product(in[0].at, in[1].at, group_sizes, u16(out), num_experts, t, n, k, trans_b, dtype);
     ws.rest(p, workspace, workspace_bytes);
     return gemm16_launch(p, trans_b ? ROWS_NK : ROWS_NN, EPI16_OUT, s);
 }
@@ -157,14 +155,9 @@ extern "C" int cch_grouped_matmul_backward(const void *grad_out, const void *x, 
         return rc;
     hipStream_t s = static_cast<hipStream_t>(stream);
     Carve ws{static_cast<uint8_t *>(workspace)};
-    const uint16_t *pg, *px = nullptr, *pw = nullptr;
-    int64_t ldg, ldx = pitch16(k), ldw = pitch16(trans_b ? k : n);
-    if (const int rc = operand16(u16(grad_out), t, n, ws, &pg, &ldg, s)) return rc;
-    if (grad_w)
-        if (const int rc = operand16(u16(x), t, k, ws, &px, &ldx, s)) return rc;
-    if (grad_x)
-        if (const int rc = operand16(u16(w), num_experts * (trans_b ? n : k), trans_b ? k : n, ws, &pw, &ldw, s)) return rc;
-    return backward_products16(pg, px, pw, group_sizes, num_experts, u16(grad_x), u16(grad_w), t, n, k, trans_b, dtype, ws, workspace, workspace_bytes, s);
+    Operand16 in[3] = {{u16(grad_out), t, n}, {grad_w ? u16(x) : nullptr, t, k}, {grad_x ? u16(w) : nullptr, num_experts * (trans_b ? n : k), trans_b ? k : n}};
+    if (const int rc = whole_operands16(in, 3, ws, s)) return rc;
+    return backward_products16(in[0].at, in[1].at, in[2].at, group_sizes, num_experts, u16(grad_x), u16(grad_w), t, n, k, trans_b, dtype, ws, workspace, workspace_bytes, s);
 }
 
 static int check_act(const char *what, int act)
@@ -192,11 +185,9 @@ extern "C" int cch_matmul_bias_act(const void *x, const void *w, const void *bia
     if (const int rc = check_workspace16("cch_matmul_bias_act", workspace, workspace_bytes, cch_matmul_bias_act_workspace_bytes(m, n, k, trans_b))) return rc;
     hipStream_t s = static_cast<hipStream_t>(stream);
     Carve ws{static_cast<uint8_t *>(workspace)};
-    const uint16_t *px, *pw;
-    int64_t ldx, ldw;
-    if (const int rc = operand16(u16(x), m, k, ws, &px, &ldx, s)) return rc;
-    if (const int rc = operand16(u16(w), trans_b ? n : k, trans_b ? k : n, ws, &pw, &ldw, s)) return rc;
-    Gemm16 p = product16(px, ldx, pw, ldw, u16(out), m, n, k, trans_b, dtype);
+    Operand16 in[2] = {{u16(x), m, k}, {u16(w), trans_b ? n : k, trans_b ? k : n}};
+    if (const int rc = whole_operands16(in, 2, ws, s)) return rc;
+    Gemm16 p = product16(in[0].at, pitch16(k), in[1].at, pitch16(trans_b ? k : n), u16(out), m, n, k, trans_b, dtype);
     p.bias = u16(bias);
     p.residual = u16(residual);
     p.preact = u16(preact);
@@ -235,11 +226,7 @@ extern "C" int cch_matmul_bias_act_backward(const void *grad_out, const void *x,
         if (const int rc = fill_zero16(u16(grad_bias), n, s)) return rc;
     }
     if (const int rc = act_backward16(u16(grad_out), u16(preact), dz, u16(grad_bias), partial, m, n, activation, dtype == CCH_DTYPE_F16, s)) return rc;
-    const uint16_t *px = nullptr, *pw = nullptr;
-    int64_t ldx = pitch16(k), ldw = pitch16(trans_b ? k : n);
-    if (grad_w)
-        if (const int rc = operand16(u16(x), m, k, ws, &px, &ldx, s)) return rc;
-    if (grad_x)
-        if (const int rc = operand16(u16(w), trans_b ? n : k, trans_b ? k : n, ws, &pw, &ldw, s)) return rc;
-    return backward_products16(own ? dz : u16(grad_out), px, pw, nullptr, 1, u16(grad_x), u16(grad_w), m, n, k, trans_b, dtype, ws, workspace, workspace_bytes, s);
+    Operand16 in[2] = {{grad_w ? u16(x) : nullptr, m, k}, {grad_x ? u16(w) : nullptr, trans_b ? n : k, trans_b ? k : n}};
+    if (const int rc = whole_operands16(in, 2, ws, s)) return rc;
+    return backward_products16(own ? dz : u16(grad_out), in[0].at, in[1].at, nullptr, 1, u16(grad_x), u16(grad_w), m, n, k, trans_b, dtype, ws, workspace, workspace_bytes, s);
 }
