@@ -70,13 +70,20 @@ template <class T, int EPI, int VEC> __global__ __launch_bounds__(256) void join
         const int n = (int)(i - row * per_row) * VEC;
         if (m >= used && !p.zero_rest) continue;
         float v[VEC] = {};
-        if (m < used)
-            for (int s = 0; s < p.splits; s++) {
-                typedef float F __attribute__((ext_vector_type(VEC)));
-                const F a = *reinterpret_cast<const F *>(p.partial + s * all + row * p.n + n);
+        if (m < used) {
+            typedef float F __attribute__((ext_vector_type(VEC)));
+            const float *from = p.partial + row * p.n + n;
+            // (eight parts' loads on their way together; those past the last are not added)
+            for (int s = 0; s < p.splits; s += 8) {
+                F part[8];
 #pragma unroll
-                for (int x = 0; x < VEC; x++) v[x] += a[x];
+                for (int y = 0; y < 8; y++) part[y] = *reinterpret_cast<const F *>(from + min(s + y, p.splits - 1) * all);
+#pragma unroll
+                for (int y = 0; y < 8; y++)
+#pragma unroll
+                    for (int x = 0; x < VEC; x++) v[x] = s + y < p.splits ? v[x] + part[y][x] : v[x];
             }
+        }
         const int64_t to = e * p.out_stride + (EPI == EPI16_OUT && p.out_rows ? p.out_rows[m] : m) * p.pitch_out + n;
 #pragma unroll
         for (int x = 0; x < VEC; x++) {
