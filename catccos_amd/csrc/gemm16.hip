@@ -11,36 +11,47 @@ int gemm16_launch_f16(const Gemm16 &p, const Plan16 &plan, int layout, int epilo
 std::atomic<int> g_kernel16{-1};
 
 // ---- which kernel, and K in how many parts: by sizes alone, so that what a call's workspace holds does not depend on the device.
+// Estimates in us beyond an empty launch, fitted to products of 1 to 512 rows, 512 to 7168 columns and K of 512 to 8192.
 Plan16 plan16(const Gemm16 &p, int layout, int epilogue)
 {
     constexpr int CUS = 256;
+    constexpr double MEMORY = 5.1e6;   // bytes a us
     const int asked = g_kernel16.load();
     Plan16 plan{KERNEL16_128, 1, 0};
     const bool results = epilogue == EPI16_OUT || epilogue == EPI16_ACT;
-    if (layout != ROWS_TN && results && !p.a_rows && !p.sums && !p.out_rows && !p.scale &&
-        (asked == KERNEL16_ROWS || (asked < 0 && (int64_t)p.m <= 32 * (int64_t)p.groups)))
-        return {KERNEL16_ROWS, 1, 0};
+    const bool rows_kernel = layout != ROWS_TN && results && !p.a_rows && !p.sums && !p.out_rows && !p.scale;
+    if (rows_kernel && asked == KERNEL16_ROWS) return {KERNEL16_ROWS, 1, 0};
     if (!p.a_rows && p.pitch_out < MAX_PITCH16 / 2 && (asked == KERNEL16_256 || (asked < 0 && tiles16(p, 256, 256) >= BIG_TILES16))) return {KERNEL16_256, 1, 0};
     // tiles of 128 x 128, about: a group's rows or K are taken to be its share
-    const int64_t share = p.k_grouped || !p.group_sizes ? p.m : (p.m + p.groups - 1) / p.groups, each = (share + 127) / 128 * ((p.n + 127) / 128);
-    const int64_t tiles = each * p.groups, steps = ((p.k_grouped ? (p.k + p.groups - 1) / p.groups : p.k) + 63) / 64;
-    if (results && !p.sums && tiles < CUS) {
-        // us beyond what one launch costs in any case: a step of a workgroup with four stages, longer the more of them share the caches, the second launch, and the parts' way
-        // to memory and back (128 x 1024 x 8192 in 1, 2, 4, 8, 16 parts: 47, 30, 21, 17.5, 18.7 us; 256 x 4096 x 7168 in 1, 2, 4, 8: 45, 32, 34, 33; 512 x 1024 x 1024: 12.2,
-        // 13.5, 14.4, 19.9)
+    const int64_t groups = p.k_grouped || !p.group_sizes ? p.groups : std::max(std::min(p.groups, p.m), 1);   // that may have rows
+    const int64_t share = p.k_grouped || !p.group_sizes ? p.m : (p.m + groups - 1) / groups, each = (share + 127) / 128 * ((p.n + 127) / 128);
+    const int64_t tiles = each * groups, steps = ((p.k_grouped ? (p.k + groups - 1) / groups : p.k) + 63) / 64;
+    const double weights = 2.0 * p.n * p.k * groups / MEMORY;
+    double best = 0;
+    for (int s = 1; s <= 32 && (s == 1 || (s <= steps && results && !p.sums && tiles < CUS)); s++) {
+        // a step of a workgroup with four stages, longer the more of them share the caches; the second launch, and the parts' way to memory and back (128 x 1024 x 8192 in 1, 2,
+        // 4, 8, 16 parts: 47, 30, 21, 17.5, 18.7 us; 256 x 4096 x 7168 in 1, 2, 4, 8: 45, 32, 34, 33; 512 x 1024 x 1024: 12.2, 13.5, 14.4, 19.9)
         const double STEP = 0.32, SHARED = 0.18, JOIN = 1.7, PER_BYTE = 0.6e-6;
-        const double bytes = 4.0 * p.m * p.n * (p.k_grouped ? p.groups : 1);
-        double best = 0;
-        for (int s = 1; s <= 32 && s <= steps; s++) {
-            const double fill = (double)(tiles * s) / CUS, rounds = fill <= 1 ? 1 : (double)((tiles * s + CUS - 1) / CUS);
-            const double us = rounds * (double)((steps + s - 1) / s) * (STEP + SHARED * (fill < 1 ? fill : 1)) + (s > 1 ? JOIN + s * bytes * PER_BYTE : 0);
-            if (s == 1 || us < best) {
-                best = us;
-                plan.splits = s;
-            }
+        const double fill = (double)(tiles * s) / CUS, rounds = fill <= 1 ? 1 : (double)((tiles * s + CUS - 1) / CUS);
+        const double us = rounds * (double)((steps + s - 1) / s) * (STEP + SHARED * (fill < 1 ? fill : 1)) +
+                          (s > 1 ? JOIN + s * 4.0 * p.m * p.n * (p.k_grouped ? groups : 1) * PER_BYTE : 0);
+        if (s == 1 || us < best) {
+            best = us;
+            plan.splits = s;
         }
     }
     plan.deep = tiles * plan.splits <= CUS;
+    if (rows_kernel && asked < 0 && share <= 128) {
+        // The kernel for few rows: an eighth of the steps in a row, or the weights' way from memory, again for every tile of rows (from the caches).  K-major weights come in half
+        // lines.  4096 x 7168: 1 row 15.4 us (128 x 128 tiles 18.3), 32 22.4 (19.3), K-major 29 (18.7); 7168 x 2048: 1 row 8.7 (13.9), 64 17.1 (16.7), K-major 12.1 (13.8);
+        // 1024 x 1024: 1 row 4.9 (9.4), 96 5.9 (11.3), K-major 6.0 (9.5).  Its launch, prologue and epilogue take 2 us less than the others'.
+        const int mr = rows16(p);
+        const int64_t row_tiles = (share + mr - 1) / mr, workgroups = row_tiles * groups * ((p.n + 31) / 32);
+        const double step = (layout == ROWS_NN ? 0.9 : 0.31) * (mr == 32 ? 1.2 : 1.0) * (double)((workgroups + CUS - 1) / CUS);
+        const double fetch = weights * (layout == ROWS_NN ? 2.0 : 1.0) * (1 + 0.4 * (row_tiles - 1));
+        const double us = std::max((double)((steps + 7) / 8) * step, fetch);
+        if (us <= std::max(best, weights) + 2.0) return {KERNEL16_ROWS, 1, 0};
+    }
     return plan;
 }
 

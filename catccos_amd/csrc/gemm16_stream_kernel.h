@@ -1,4 +1,4 @@
-// Products of a few rows: bound by the weights' way from memory.  A workgroup has MR rows (8, 16 or 32) of a group and 32 NB columns; its waves take K's steps of 64 elements in
+// Products of a few rows: bound by the weights' way from memory.  A workgroup has MR rows (8, 16 or 32) of a group and 32 columns; its waves take K's steps of 64 elements in
 // turn, each with a ring of DEPTH stages in LDS of its own that is filled straight from memory, so that the loop over K has no barrier and 64 KiB or more of weights are on their way to
 // a CU at any time.  In the end the waves' sums are added up in LDS, in their order.
 #pragma once
@@ -8,20 +8,20 @@
 
 namespace cch {
 
-// K-contiguous weights come 32 rows of 128 bytes to a wave's step; of K-major ones 32 columns would be half lines, so a tile has 64.
+// A step's weights are 32 rows of 128 bytes, or (K-major) 64 of 64: half lines, whose other halves a neighbouring workgroup of the same XCD asks for.
 template <int LAYOUT, int MR_> struct Stream16 {
-    static constexpr int MR = MR_, NB = LAYOUT == ROWS_NK ? 1 : 2, WAVES = LAYOUT == ROWS_NK ? 8 : 4, THREADS = 64 * WAVES, TN = 32 * NB;
+    static constexpr int MR = MR_, WAVES = 8, THREADS = 64 * WAVES, TN = 32;
     static constexpr int W_BYTES = TN * 128, X_BYTES = MR * 128, STAGE = W_BYTES + X_BYTES;
-    static constexpr int DEPTH = LAYOUT == ROWS_NK && MR == 32 ? 2 : 3, RW = W_BYTES / 1024, RX = X_BYTES / 1024;
-    static constexpr int RING = WAVES * DEPTH * STAGE, SUMS = WAVES * NB * 4096, LDS = (RING > SUMS ? RING : SUMS);
+    static constexpr int DEPTH = MR == 32 ? 2 : 3, RW = W_BYTES / 1024, RX = X_BYTES / 1024;
+    static constexpr int RING = WAVES * DEPTH * STAGE, PITCH = 36, SUMS = WAVES * 32 * PITCH * 4, LDS = (RING > SUMS ? RING : SUMS);
 };
 
 template <class T, int LAYOUT, int EPI, class S>
 __global__ __launch_bounds__(S::THREADS) void gemm16_stream_kernel(Gemm16 p)
 {
     constexpr bool B_KM = LAYOUT != ROWS_NK;
-    constexpr int NB = S::NB, DEPTH = S::DEPTH;
-    using KB = KMajor<64>;
+    constexpr int DEPTH = S::DEPTH;
+    using KB = KMajor<S::TN>;
     __shared__ GroupTable16 tab;
     if (threadIdx.x < 64) build_groups16(tab, p.group_sizes, p.groups, p.m, S::MR);
     __syncthreads();
@@ -35,7 +35,7 @@ __global__ __launch_bounds__(S::THREADS) void gemm16_stream_kernel(Gemm16 p)
     const int steps = (p.k + 63) >> 6, mine = (steps - wave + S::WAVES - 1) / S::WAVES;   // of this wave: wave, wave + WAVES, ...
     const int k8 = (p.k + 7) & ~7;
 
-    uint32_t fr_x[4], fr_w[4], ft_w[NB];
+    uint32_t fr_x[4], fr_w[4];
 #pragma unroll
     for (int kk = 0; kk < 4; kk++) {
         const int row = r & (S::MR - 1);   // (rows of the block that there are none of are not stored: any will do)
@@ -43,9 +43,7 @@ __global__ __launch_bounds__(S::THREADS) void gemm16_stream_kernel(Gemm16 p)
         fr_x[kk] = ring + S::W_BYTES + (uint32_t)row * 128u + (((uint32_t)(2 * kk + g) ^ swizzle_of_row(row)) << 4);
     }
     const int krow = (tq >> 1) * 8 + (ti >> 2);
-#pragma unroll
-    for (int j = 0; j < NB; j++)
-        ft_w[j] = ring + (uint32_t)krow * KB::ROW + ((((uint32_t)j * 4 + (uint32_t)((tq & 1) * 2 + ((ti & 3) >> 1))) ^ KB::swizzle(krow)) << 4) + (ti & 1) * 8u;
+    const uint32_t ft_w = ring + (uint32_t)krow * KB::ROW + ((uint32_t)((tq & 1) * 2 + ((ti & 3) >> 1)) << 4) + (ti & 1) * 8u;
 
     for (int64_t t = blockIdx.x; t < ((total + 7) & ~7); t += gridDim.x) {
         const int at = place16((int)t, total);
@@ -67,7 +65,10 @@ __global__ __launch_bounds__(S::THREADS) void gemm16_stream_kernel(Gemm16 p)
 #pragma unroll
         for (int q = 0; q < S::RW; q++) {
             const int row = q * 8 + (lane >> 3);
-            if (B_KM) off_w[q] = (uint32_t)row * (uint32_t)p.pitch_b * 2u + (((uint32_t)(lane & 7) ^ KB::swizzle(row)) << 4);
+            if (B_KM) {
+                const int kr = q * KB::ROWS_PER_KIB + lane / KB::CHUNKS;
+                off_w[q] = (uint32_t)kr * (uint32_t)p.pitch_b * 2u + (((uint32_t)(lane % KB::CHUNKS) ^ KB::swizzle(kr)) << 4);
+            }
             else off_w[q] = row < cols ? (uint32_t)row * (uint32_t)p.pitch_b * 2u + (((uint32_t)(lane & 7) ^ swizzle_of_row(row)) << 4) : NO_FETCH;
         }
         // the wave's i-th step into stage `at`; past the last one nothing is fetched, so that waits count the same
@@ -85,9 +86,7 @@ __global__ __launch_bounds__(S::THREADS) void gemm16_stream_kernel(Gemm16 p)
                 load16_to_lds(rs_x, in ? off_x[q] : NO_FETCH, (uint32_t)k0 * 2u, ring + at + (uint32_t)(S::W_BYTES + q * 1024));
             }
         };
-        v16f acc[NB];
-#pragma unroll
-        for (int j = 0; j < NB; j++) acc[j] = (v16f)(0.0f);
+        v16f acc = (v16f)(0.0f);
 #pragma unroll
         for (int i = 0; i < DEPTH; i++) request(i, (uint32_t)(i * S::STAGE));
         uint32_t stage = 0;
@@ -95,12 +94,11 @@ __global__ __launch_bounds__(S::THREADS) void gemm16_stream_kernel(Gemm16 p)
             CCH_WAIT_VM((DEPTH - 1) * (S::RW + S::RX));
             __builtin_amdgcn_sched_barrier(0);
             asm volatile("" ::: "memory");
-            v4i fx[4], fw[NB][4];
+            v4i fx[4], fw[4];
 #pragma unroll
             for (int kk = 0; kk < 4; kk++) {
                 fx[kk] = lds_read16_abs(fr_x[kk] + stage);
-#pragma unroll
-                for (int j = 0; j < NB; j++) fw[j][kk] = B_KM ? read_transposed(ft_w[j] + stage + (uint32_t)kk * 16u * KB::ROW, KB::ROW) : lds_read16_abs(fr_w[kk] + stage);
+                fw[kk] = B_KM ? read_transposed(ft_w + stage + (uint32_t)kk * 16u * KB::ROW, KB::ROW) : lds_read16_abs(fr_w[kk] + stage);
             }
             __builtin_amdgcn_sched_barrier(0);
             CCH_WAIT_LGKM0();   // (in registers: the stage is free)
@@ -108,18 +106,15 @@ __global__ __launch_bounds__(S::THREADS) void gemm16_stream_kernel(Gemm16 p)
             request(i + DEPTH, stage);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int kk = 0; kk < 4; kk++)
-#pragma unroll
-                for (int j = 0; j < NB; j++) acc[j] = T::mfma(fw[j][kk], fx[kk], acc[j]);
+            for (int kk = 0; kk < 4; kk++) acc = T::mfma(fw[kk], fx[kk], acc);
             stage = stage + S::STAGE == DEPTH * S::STAGE ? 0u : stage + S::STAGE;
         }
         CCH_WAIT_VM_LGKM0(0);
-        CCH_BARRIER();   // all rings are done with: the sums take their place, [wave][block][32 columns][32 rows]
+        CCH_BARRIER();   // all rings are done with: the sums take their place, [wave][32 rows][32 columns and 4 more, so that rows begin on other banks]
         float *sums = reinterpret_cast<float *>(smem);
 #pragma unroll
-        for (int j = 0; j < NB; j++)
-#pragma unroll
-            for (int x = 0; x < 16; x++) sums[((wave * NB + j) * 32 + 8 * (x >> 2) + 4 * g + (x & 3)) * 32 + r] = acc[j][x];
+        for (int q = 0; q < 4; q++)
+            *reinterpret_cast<f32x4 *>(sums + (wave * 32 + r) * S::PITCH + 8 * q + 4 * g) = (f32x4){acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
         CCH_WAIT_LGKM0();
         CCH_BARRIER();
         for (int i = threadIdx.x; i < rows * S::TN; i += S::THREADS) {
@@ -127,7 +122,7 @@ __global__ __launch_bounds__(S::THREADS) void gemm16_stream_kernel(Gemm16 p)
             if (n >= p.n) continue;
             float v = 0.0f;
 #pragma unroll
-            for (int w = 0; w < S::WAVES; w++) v += sums[(w * NB * 32 + col) * 32 + row];
+            for (int w = 0; w < S::WAVES; w++) v += sums[(w * 32 + row) * S::PITCH + col];
             const int64_t to = (int64_t)m * p.pitch_out + n;
             if constexpr (EPI == EPI16_ACT) {
                 if (p.bias) v += T::to(p.bias[n]);
