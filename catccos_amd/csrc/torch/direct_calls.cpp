@@ -688,7 +688,7 @@ PyObject *MatmulBiasActBackward(PyObject *, PyObject *const *v, Py_ssize_t nv)
         T(v[0]).size(0) != m || T(v[0]).size(1) != n || !Here({v[0]}) || !Flag(v[6], x_grad) || !Flag(v[7], w_grad) || !Flag(v[8], b_grad))
         return Decline();
     const at::Tensor &x = T(v[1]), &w = T(v[2]);
-    if (act != CCH_ACT_NONE && (v[3] == Py_None || !Like(v[3], x, 2, false) || T(v[3]).sizes() != T(v[0]).sizes() || !Here({v[3]}))) return Decline();
+    if (v[3] == Py_None ? act != CCH_ACT_NONE : !Like(v[3], x, 2, false) || T(v[3]).sizes() != T(v[0]).sizes() || !Here({v[3]})) return Decline();
     at::Tensor gx, gw, gb;
     int rc;
     {

@@ -540,6 +540,190 @@ at::Tensor MoeFfnW4A16(const at::Tensor &x_in, const at::Tensor &idx_in, const a
 }
 
 // ---------------------------------------------------------------------------------------------
+// Products of 16-bit operands, the dense layer and the loss of an output projection, each with its gradients as a call of its own.  What is not asked for is an empty tensor.
+
+// Contiguous and on a 16-byte boundary, as the products' requests want their operands.
+at::Tensor Whole(const at::Tensor &t)
+{
+    const at::Tensor c = t.contiguous();
+    return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
+}
+at::Tensor Empty0(const at::Tensor &like) { return at::empty({0}, like.options()); }
+void *PtrIf(const at::Tensor &t, bool wanted) { return wanted ? t.data_ptr() : nullptr; }
+
+void CheckX16(const at::Tensor &x)
+{
+    TORCH_CHECK(x.dim() == 2 && (x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf), "x must be a 2-D bfloat16 or float16 tensor");
+}
+void CheckTrans(int64_t trans_b) { TORCH_CHECK(trans_b == 0 || trans_b == 1, "trans_b must be 0 or 1"); }
+int ActivationCode(const std::string &a)
+{
+    if (a == "none") return CCH_ACT_NONE;
+    if (a == "relu") return CCH_ACT_RELU;
+    if (a == "silu") return CCH_ACT_SILU;
+    if (a == "gelu") return CCH_ACT_GELU;
+    TORCH_CHECK(a == "gelu_tanh", "unknown activation '", a, "' (none, relu, silu, gelu or gelu_tanh)");
+    return CCH_ACT_GELU_TANH;
+}
+int ReductionCode(const std::string &r)
+{
+    TORCH_CHECK(r == "mean" || r == "sum", "unknown reduction '", r, "' (mean or sum)");
+    return r == "sum" ? CCH_REDUCE_SUM : CCH_REDUCE_MEAN;
+}
+void CheckLike(const char *name, const at::Tensor &t, const at::Tensor &x, at::IntArrayRef shape)
+{
+    TORCH_CHECK(t.scalar_type() == x.scalar_type() && t.sizes() == shape, name, " must be a tensor ", shape, " of x's type");
+}
+
+struct GroupedShape {
+    int64_t e, t, n, k;
+};
+GroupedShape CheckGrouped(const at::Tensor &x, const at::Tensor &w, const at::Tensor &sizes, int64_t trans_b)
+{
+    CheckX16(x);
+    CheckTrans(trans_b);
+    TORCH_CHECK(w.dim() == 3 && w.scalar_type() == x.scalar_type(), "w must be a 3-D tensor of x's type");
+    const GroupedShape s{w.size(0), x.size(0), w.size(trans_b ? 1 : 2), x.size(1)};
+    TORCH_CHECK(w.size(trans_b ? 2 : 1) == s.k, "inner dimensions differ: x has ", s.k, " columns, w ", w.size(trans_b ? 2 : 1));
+    TORCH_CHECK(sizes.scalar_type() == at::kInt && sizes.dim() == 1 && sizes.size(0) == s.e, "group_sizes must be an int32 tensor with one entry per expert");
+    return s;
+}
+
+at::Tensor GroupedMatmul(const at::Tensor &x_in, const at::Tensor &w_in, const at::Tensor &sizes_in, int64_t trans_b)
+{
+    NeedInit();
+    SameDevice("grouped_matmul", {{"x", x_in}, {"w", w_in}, {"group_sizes", sizes_in}});
+    const GroupedShape s = CheckGrouped(x_in, w_in, sizes_in, trans_b);
+    c10::DeviceGuard guard(x_in.device());
+    const at::Tensor x = Whole(x_in), w = Whole(w_in), sizes = sizes_in.contiguous();
+    at::Tensor out = at::empty({s.t, s.n}, x.options());
+    at::Tensor ws = Bytes(x, {cch_grouped_matmul_workspace_bytes(s.e, s.t, s.n, s.k, (int)trans_b)});
+    Check(cch_grouped_matmul(x.data_ptr(), w.data_ptr(), sizes.data_ptr<int32_t>(), out.data_ptr(), s.e, s.t, s.n, s.k, (int)trans_b, DtypeCode(x), ws.data_ptr(), ws.numel(),
+                             StreamOf(x)),
+          "grouped_matmul");
+    return out;
+}
+
+std::tuple<at::Tensor, at::Tensor> GroupedMatmulBackward(const at::Tensor &grad_in, const at::Tensor &x_in, const at::Tensor &w_in, const at::Tensor &sizes_in, int64_t trans_b,
+                                                         bool x_grad, bool w_grad)
+{
+    NeedInit();
+    SameDevice("grouped_matmul_backward", {{"x", x_in}, {"grad_out", grad_in}, {"w", w_in}, {"group_sizes", sizes_in}});
+    const GroupedShape s = CheckGrouped(x_in, w_in, sizes_in, trans_b);
+    CheckLike("grad_out", grad_in, x_in, {s.t, s.n});
+    c10::DeviceGuard guard(x_in.device());
+    const at::Tensor grad = Whole(grad_in), x = Whole(x_in), w = Whole(w_in), sizes = sizes_in.contiguous();
+    at::Tensor gx = x_grad ? at::empty(x.sizes(), x.options()) : Empty0(x), gw = w_grad ? at::empty(w.sizes(), w.options()) : Empty0(w);
+    at::Tensor ws = Bytes(x, {cch_grouped_matmul_backward_workspace_bytes(s.e, s.t, s.n, s.k, (int)trans_b)});
+    Check(cch_grouped_matmul_backward(grad.data_ptr(), x.data_ptr(), w.data_ptr(), sizes.data_ptr<int32_t>(), PtrIf(gx, x_grad), PtrIf(gw, w_grad), s.e, s.t, s.n, s.k, (int)trans_b,
+                                      DtypeCode(x), ws.data_ptr(), ws.numel(), StreamOf(x)),
+          "grouped_matmul_backward");
+    return {gx, gw};
+}
+
+struct LayerShape {
+    int64_t m, n, k;
+};
+LayerShape CheckLayer(const at::Tensor &x, const at::Tensor &w, int64_t trans_b)
+{
+    CheckX16(x);
+    CheckTrans(trans_b);
+    TORCH_CHECK(w.dim() == 2 && w.scalar_type() == x.scalar_type(), "w must be a 2-D tensor of x's type");
+    TORCH_CHECK(w.size(trans_b ? 1 : 0) == x.size(1), "inner dimensions differ: x has ", x.size(1), " columns, w ", w.size(trans_b ? 1 : 0));
+    return {x.size(0), w.size(trans_b ? 0 : 1), x.size(1)};
+}
+
+std::tuple<at::Tensor, at::Tensor> MatmulBiasAct(const at::Tensor &x_in, const at::Tensor &w_in, const MaybeTensor &bias_in, const MaybeTensor &residual_in, std::string activation,
+                                                 int64_t trans_b, bool return_preact)
+{
+    NeedInit();
+    const char *op = "matmul_bias_act";
+    SameDevice(op, {{"x", x_in}, {"w", w_in}});
+    const LayerShape s = CheckLayer(x_in, w_in, trans_b);
+    const int act = ActivationCode(activation);
+    c10::DeviceGuard guard(x_in.device());
+    const at::Tensor x = Whole(x_in), w = Whole(w_in), bias = Optional(op, "bias", bias_in, x, {x.scalar_type()}, {s.n}),
+                     residual = Optional(op, "residual", residual_in, x, {x.scalar_type()}, {s.m, s.n});
+    at::Tensor out = at::empty({s.m, s.n}, x.options()), preact = return_preact ? at::empty({s.m, s.n}, x.options()) : Empty0(x);
+    at::Tensor ws = Bytes(x, {cch_matmul_bias_act_workspace_bytes(s.m, s.n, s.k, (int)trans_b)});
+    Check(cch_matmul_bias_act(x.data_ptr(), w.data_ptr(), PtrOf<void>(bias), PtrOf<void>(residual), PtrIf(preact, return_preact), out.data_ptr(), s.m, s.n, s.k, (int)trans_b, act,
+                              DtypeCode(x), ws.data_ptr(), ws.numel(), StreamOf(x)),
+          op);
+    return {out, preact};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> MatmulBiasActBackward(const at::Tensor &grad_in, const at::Tensor &x_in, const at::Tensor &w_in, const MaybeTensor &preact_in,
+                                                                     std::string activation, int64_t trans_b, bool x_grad, bool w_grad, bool bias_grad)
+{
+    NeedInit();
+    const char *op = "matmul_bias_act_backward";
+    SameDevice(op, {{"x", x_in}, {"grad_out", grad_in}, {"w", w_in}});
+    const LayerShape s = CheckLayer(x_in, w_in, trans_b);
+    const int act = ActivationCode(activation);
+    CheckLike("grad_out", grad_in, x_in, {s.m, s.n});
+    TORCH_CHECK(act == CCH_ACT_NONE || (preact_in && preact_in->defined()), "an activation's gradient takes preact");
+    c10::DeviceGuard guard(x_in.device());
+    const at::Tensor grad = Whole(grad_in), x = Whole(x_in), w = Whole(w_in);
+    const at::Tensor preact = act == CCH_ACT_NONE ? at::Tensor() : Optional(op, "preact", preact_in, x, {x.scalar_type()}, {s.m, s.n});
+    at::Tensor gx = x_grad ? at::empty(x.sizes(), x.options()) : Empty0(x), gw = w_grad ? at::empty(w.sizes(), w.options()) : Empty0(w),
+               gb = bias_grad ? at::empty({s.n}, x.options()) : Empty0(x);
+    at::Tensor ws = Bytes(x, {cch_matmul_bias_act_backward_workspace_bytes(s.m, s.n, s.k, (int)trans_b, act)});
+    Check(cch_matmul_bias_act_backward(grad.data_ptr(), x.data_ptr(), w.data_ptr(), PtrOf<void>(preact), PtrIf(gx, x_grad), PtrIf(gw, w_grad), PtrIf(gb, bias_grad), s.m, s.n, s.k,
+                                       (int)trans_b, act, DtypeCode(x), ws.data_ptr(), ws.numel(), StreamOf(x)),
+          op);
+    return {gx, gw, gb};
+}
+
+void CheckCe(const at::Tensor &x, const at::Tensor &w, const at::Tensor &targets)
+{
+    CheckX16(x);
+    TORCH_CHECK(w.dim() == 2 && w.scalar_type() == x.scalar_type() && w.size(1) == x.size(1), "w must be a tensor [vocabulary, ", x.size(1), "] of x's type");
+    TORCH_CHECK((targets.scalar_type() == at::kInt || targets.scalar_type() == at::kLong) && targets.dim() == 1 && targets.size(0) == x.size(0),
+                "targets must be an int64 or int32 tensor [tokens]");
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> LinearCrossEntropy(const at::Tensor &x_in, const at::Tensor &w_in, const at::Tensor &targets_in, std::string reduction,
+                                                                              double z_coef)
+{
+    NeedInit();
+    SameDevice("linear_cross_entropy", {{"x", x_in}, {"w", w_in}, {"targets", targets_in}});
+    CheckCe(x_in, w_in, targets_in);
+    const int red = ReductionCode(reduction);
+    c10::DeviceGuard guard(x_in.device());
+    const at::Tensor x = Whole(x_in), w = Whole(w_in), targets = targets_in.contiguous();
+    const int64_t t = x.size(0), h = x.size(1), v = w.size(0);
+    at::Tensor loss = at::empty({}, x.options().dtype(at::kFloat)), nll = at::empty({t}, loss.options()), lse = at::empty({t}, loss.options()),
+               tokens = at::empty({1}, x.options().dtype(at::kInt));
+    at::Tensor ws = Bytes(x, {cch_linear_cross_entropy_workspace_bytes(t, h, v)});
+    Check(cch_linear_cross_entropy(x.data_ptr(), w.data_ptr(), targets.data_ptr(), (int)targets.element_size(), loss.data_ptr<float>(), nll.data_ptr<float>(), lse.data_ptr<float>(),
+                                   tokens.data_ptr<int32_t>(), t, h, v, red, (float)z_coef, DtypeCode(x), ws.data_ptr(), ws.numel(), StreamOf(x)),
+          "linear_cross_entropy");
+    return {loss, nll, lse, tokens};
+}
+
+std::tuple<at::Tensor, at::Tensor> LinearCrossEntropyBackward(const at::Tensor &grad_in, const at::Tensor &x_in, const at::Tensor &w_in, const at::Tensor &targets_in,
+                                                              const at::Tensor &lse_in, const at::Tensor &tokens_in, std::string reduction, double z_coef, bool x_grad, bool w_grad)
+{
+    NeedInit();
+    SameDevice("linear_cross_entropy_backward", {{"x", x_in}, {"grad_loss", grad_in}, {"w", w_in}, {"targets", targets_in}, {"lse", lse_in}, {"tokens", tokens_in}});
+    CheckCe(x_in, w_in, targets_in);
+    const int red = ReductionCode(reduction);
+    const int64_t t = x_in.size(0), h = x_in.size(1), v = w_in.size(0);
+    TORCH_CHECK(grad_in.scalar_type() == at::kFloat && grad_in.numel() == 1, "grad_loss must be one float32 value");
+    TORCH_CHECK(lse_in.scalar_type() == at::kFloat && lse_in.dim() == 1 && lse_in.size(0) == t && tokens_in.scalar_type() == at::kInt && tokens_in.numel() == 1,
+                "lse must be float32 [tokens] and tokens one int32 value");
+    c10::DeviceGuard guard(x_in.device());
+    const at::Tensor x = Whole(x_in), w = Whole(w_in), targets = targets_in.contiguous(), lse = lse_in.contiguous();
+    at::Tensor gx = x_grad ? at::empty(x.sizes(), x.options()) : Empty0(x), gw = w_grad ? at::empty(w.sizes(), w.options()) : Empty0(w);
+    at::Tensor ws = Bytes(x, {cch_linear_cross_entropy_backward_workspace_bytes(t, h, v)});
+    Check(cch_linear_cross_entropy_backward(grad_in.data_ptr<float>(), x.data_ptr(), w.data_ptr(), targets.data_ptr(), (int)targets.element_size(), lse.data_ptr<float>(),
+                                            tokens_in.data_ptr<int32_t>(), PtrIf(gx, x_grad), PtrIf(gw, w_grad), t, h, v, red, (float)z_coef, DtypeCode(x), ws.data_ptr(), ws.numel(),
+                                            StreamOf(x)),
+          "linear_cross_entropy_backward");
+    return {gx, gw};
+}
+
+// ---------------------------------------------------------------------------------------------
 // Meta kernels: output shapes only (reference torch_bindings_meta.cpp:18-30 returns at::empty_symint of the result shape)
 
 c10::SymInt SymScaleCols(const c10::SymInt &k) { return ((k + 63) / 64) * 2; }
@@ -631,8 +815,43 @@ at::Tensor MoeFfnW4A16Meta(const at::Tensor &x, const at::Tensor &, const at::Te
     return MetaEmpty(x, x.sym_sizes(), x.scalar_type());
 }
 
+at::Tensor Meta0(const at::Tensor &like) { return MetaEmpty(like, {0}, like.scalar_type()); }
+at::Tensor MetaLike(const at::Tensor &t, bool wanted) { return wanted ? MetaEmpty(t, t.sym_sizes(), t.scalar_type()) : Meta0(t); }
+at::Tensor GroupedMatmulMeta(const at::Tensor &x, const at::Tensor &w, const at::Tensor &, int64_t trans_b)
+{
+    return MetaEmpty(x, {x.sym_size(0), w.sym_size(trans_b ? 1 : 2)}, x.scalar_type());
+}
+std::tuple<at::Tensor, at::Tensor> GroupedMatmulBackwardMeta(const at::Tensor &, const at::Tensor &x, const at::Tensor &w, const at::Tensor &, int64_t, bool x_grad, bool w_grad)
+{
+    return {MetaLike(x, x_grad), MetaLike(w, w_grad)};
+}
+std::tuple<at::Tensor, at::Tensor> MatmulBiasActMeta(const at::Tensor &x, const at::Tensor &w, const MaybeTensor &, const MaybeTensor &, std::string activation, int64_t trans_b,
+                                                     bool return_preact)
+{
+    ActivationCode(activation);
+    const at::Tensor out = MetaEmpty(x, {x.sym_size(0), w.sym_size(trans_b ? 0 : 1)}, x.scalar_type());
+    return {out, MetaLike(out, return_preact)};
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor> MatmulBiasActBackwardMeta(const at::Tensor &, const at::Tensor &x, const at::Tensor &w, const MaybeTensor &, std::string activation,
+                                                                         int64_t trans_b, bool x_grad, bool w_grad, bool bias_grad)
+{
+    ActivationCode(activation);
+    return {MetaLike(x, x_grad), MetaLike(w, w_grad), bias_grad ? MetaEmpty(x, {w.sym_size(trans_b ? 0 : 1)}, x.scalar_type()) : Meta0(x)};
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> LinearCrossEntropyMeta(const at::Tensor &x, const at::Tensor &, const at::Tensor &, std::string reduction, double)
+{
+    ReductionCode(reduction);
+    return {MetaEmpty(x, {}, at::kFloat), MetaEmpty(x, {x.sym_size(0)}, at::kFloat), MetaEmpty(x, {x.sym_size(0)}, at::kFloat), MetaEmpty(x, {1}, at::kInt)};
+}
+std::tuple<at::Tensor, at::Tensor> LinearCrossEntropyBackwardMeta(const at::Tensor &, const at::Tensor &x, const at::Tensor &w, const at::Tensor &, const at::Tensor &,
+                                                                  const at::Tensor &, std::string reduction, double, bool x_grad, bool w_grad)
+{
+    ReductionCode(reduction);
+    return {MetaLike(x, x_grad), MetaLike(w, w_grad)};
+}
+
 // ---------------------------------------------------------------------------------------------
-// Autograd of the gate, the losses and the 4-bit products: the gradients that catccos_amd.ops' forms have, and an error where there are none.  A call with nothing to
+// Autograd of the gate, the losses and the products with 16- and 4-bit weights: the gradients that catccos_amd.ops' forms have, and an error where there are none.  A call with nothing to
 // differentiate goes on to its kernel as it is.
 
 template <auto F>
@@ -756,6 +975,143 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> MoeBalanceLossAutograd(const at::
     return {out[0], out[1], out[2]};
 }
 
+// Several outputs, none of which has a gradient.
+struct NoGradients : torch::autograd::Function<NoGradients> {
+    static Variables forward(Context *ctx, std::string op, std::function<Variables()> call, const at::Tensor &, const at::Tensor &, const at::Tensor &, const MaybeTensor &)
+    {
+        ctx->saved_data["op"] = op;
+        return call();
+    }
+    static Variables backward(Context *ctx, Variables)
+    {
+        TORCH_CHECK_NOT_IMPLEMENTED(false, "catccos::", ctx->saved_data["op"].toStringRef(), " has no gradient");
+    }
+};
+
+// What a node's backward has to work out: which inputs were recorded when it was made.
+bool Wants(const at::Tensor &t) { return t.defined() && t.requires_grad(); }
+bool Wants(const MaybeTensor &t) { return t && Wants(*t); }
+at::Tensor If(bool wanted, const at::Tensor &t) { return wanted ? t : at::Tensor(); }
+
+std::tuple<at::Tensor, at::Tensor> GroupedMatmulBackwardAutograd(const at::Tensor &grad, const at::Tensor &x, const at::Tensor &w, const at::Tensor &sizes, int64_t trans_b,
+                                                                 bool x_grad, bool w_grad)
+{
+    auto call = [&] { return CCH_BELOW(GroupedMatmulBackward, "grouped_matmul_backward", grad, x, w, sizes, trans_b, x_grad, w_grad); };
+    if (!Recorded("grouped_matmul_backward", {grad, x, w})) return call();
+    const Variables out = NoGradients::apply(
+        "grouped_matmul_backward", [&]() -> Variables { const auto [gx, gw] = call(); return {gx, gw}; }, grad, x, w, MaybeTensor());
+    return {out[0], out[1]};
+}
+struct GroupedMatmulFunction : torch::autograd::Function<GroupedMatmulFunction> {
+    static at::Tensor forward(Context *ctx, const at::Tensor &x, const at::Tensor &w, const at::Tensor &sizes, int64_t trans_b)
+    {
+        ctx->save_for_backward({x, w, sizes});
+        ctx->saved_data["trans_b"] = trans_b;
+        ctx->saved_data["x"] = Wants(x);
+        ctx->saved_data["w"] = Wants(w);
+        return CCH_BELOW(GroupedMatmul, "grouped_matmul", x, w, sizes, trans_b);
+    }
+    static Variables backward(Context *ctx, Variables grads)
+    {
+        const Variables saved = ctx->get_saved_variables();
+        const bool x = ctx->saved_data["x"].toBool(), w = ctx->saved_data["w"].toBool();
+        const auto [gx, gw] = GroupedMatmulBackwardAutograd(grads[0], saved[0], saved[1], saved[2], ctx->saved_data["trans_b"].toInt(), x, w);
+        return {If(x, gx), If(w, gw), {}, {}};
+    }
+};
+at::Tensor GroupedMatmulAutograd(const at::Tensor &x, const at::Tensor &w, const at::Tensor &sizes, int64_t trans_b)
+{
+    if (!Recorded("grouped_matmul", {x, w})) return CCH_BELOW(GroupedMatmul, "grouped_matmul", x, w, sizes, trans_b);
+    return GroupedMatmulFunction::apply(x, w, sizes, trans_b);
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> MatmulBiasActBackwardAutograd(const at::Tensor &grad, const at::Tensor &x, const at::Tensor &w, const MaybeTensor &preact,
+                                                                             std::string activation, int64_t trans_b, bool x_grad, bool w_grad, bool bias_grad)
+{
+    auto call = [&] { return CCH_BELOW(MatmulBiasActBackward, "matmul_bias_act_backward", grad, x, w, preact, activation, trans_b, x_grad, w_grad, bias_grad); };
+    if (!Recorded("matmul_bias_act_backward", {grad, x, w, preact.value_or(at::Tensor())})) return call();
+    const Variables out = NoGradients::apply(
+        "matmul_bias_act_backward", [&]() -> Variables { const auto [gx, gw, gb] = call(); return {gx, gw, gb}; }, grad, x, w, preact);
+    return {out[0], out[1], out[2]};
+}
+struct MatmulBiasActFunction : torch::autograd::Function<MatmulBiasActFunction> {
+    static Variables forward(Context *ctx, const at::Tensor &x, const at::Tensor &w, const MaybeTensor &bias, const MaybeTensor &residual, std::string activation, int64_t trans_b,
+                             bool return_preact)
+    {
+        const bool keep = activation != "none" && (Wants(x) || Wants(w) || Wants(bias));
+        const auto [out, preact] = CCH_BELOW(MatmulBiasAct, "matmul_bias_act", x, w, bias, residual, activation, trans_b, keep || return_preact);
+        ctx->save_for_backward({x, w, keep ? preact : at::Tensor()});
+        ctx->saved_data["activation"] = activation;
+        ctx->saved_data["trans_b"] = trans_b;
+        ctx->saved_data["x"] = Wants(x);
+        ctx->saved_data["w"] = Wants(w);
+        ctx->saved_data["bias"] = Wants(bias);
+        ctx->saved_data["residual"] = Wants(residual);
+        ctx->mark_non_differentiable({preact});
+        ctx->set_materialize_grads(false);
+        return {out, preact};
+    }
+    static Variables backward(Context *ctx, Variables grads)
+    {
+        if (!grads[0].defined()) return {{}, {}, {}, {}, {}, {}, {}};
+        const Variables saved = ctx->get_saved_variables();
+        const bool x = ctx->saved_data["x"].toBool(), w = ctx->saved_data["w"].toBool(), b = ctx->saved_data["bias"].toBool();
+        at::Tensor gx, gw, gb;
+        if (x || w || b)
+            std::tie(gx, gw, gb) = MatmulBiasActBackwardAutograd(grads[0], saved[0], saved[1], saved[2].defined() ? MaybeTensor(saved[2]) : MaybeTensor(),
+                                                                 ctx->saved_data["activation"].toStringRef(), ctx->saved_data["trans_b"].toInt(), x, w, b);
+        return {If(x, gx), If(w, gw), If(b, gb), If(ctx->saved_data["residual"].toBool(), grads[0]), {}, {}, {}};
+    }
+};
+std::tuple<at::Tensor, at::Tensor> MatmulBiasActAutograd(const at::Tensor &x, const at::Tensor &w, const MaybeTensor &bias, const MaybeTensor &residual, std::string activation,
+                                                         int64_t trans_b, bool return_preact)
+{
+    if (!Recorded("matmul_bias_act", {x, w, bias.value_or(at::Tensor()), residual.value_or(at::Tensor())}))
+        return CCH_BELOW(MatmulBiasAct, "matmul_bias_act", x, w, bias, residual, activation, trans_b, return_preact);
+    const Variables out = MatmulBiasActFunction::apply(x, w, bias, residual, activation, trans_b, return_preact);
+    return {out[0], return_preact ? out[1] : at::empty_symint({0}, out[1].options())};
+}
+
+std::tuple<at::Tensor, at::Tensor> LinearCrossEntropyBackwardAutograd(const at::Tensor &grad, const at::Tensor &x, const at::Tensor &w, const at::Tensor &targets,
+                                                                      const at::Tensor &lse, const at::Tensor &tokens, std::string reduction, double z_coef, bool x_grad, bool w_grad)
+{
+    auto call = [&] { return CCH_BELOW(LinearCrossEntropyBackward, "linear_cross_entropy_backward", grad, x, w, targets, lse, tokens, reduction, z_coef, x_grad, w_grad); };
+    if (!Recorded("linear_cross_entropy_backward", {grad, x, w, lse})) return call();
+    const Variables out = NoGradients::apply(
+        "linear_cross_entropy_backward", [&]() -> Variables { const auto [gx, gw] = call(); return {gx, gw}; }, grad, x, w, MaybeTensor(lse));
+    return {out[0], out[1]};
+}
+struct LinearCrossEntropyFunction : torch::autograd::Function<LinearCrossEntropyFunction> {
+    static Variables forward(Context *ctx, const at::Tensor &x, const at::Tensor &w, const at::Tensor &targets, std::string reduction, double z_coef)
+    {
+        const auto [loss, nll, lse, tokens] = CCH_BELOW(LinearCrossEntropy, "linear_cross_entropy", x, w, targets, reduction, z_coef);
+        ctx->save_for_backward({x, w, targets, lse, tokens});
+        ctx->saved_data["reduction"] = reduction;
+        ctx->saved_data["z_coef"] = z_coef;
+        ctx->saved_data["x"] = Wants(x);
+        ctx->saved_data["w"] = Wants(w);
+        ctx->mark_non_differentiable({nll, lse, tokens});
+        ctx->set_materialize_grads(false);
+        return {loss, nll, lse, tokens};
+    }
+    static Variables backward(Context *ctx, Variables grads)
+    {
+        if (!grads[0].defined()) return {{}, {}, {}, {}, {}};
+        const Variables saved = ctx->get_saved_variables();
+        const bool x = ctx->saved_data["x"].toBool(), w = ctx->saved_data["w"].toBool();
+        const auto [gx, gw] = LinearCrossEntropyBackwardAutograd(grads[0], saved[0], saved[1], saved[2], saved[3], saved[4], ctx->saved_data["reduction"].toStringRef(),
+                                                                 ctx->saved_data["z_coef"].toDouble(), x, w);
+        return {If(x, gx), If(w, gw), {}, {}, {}};
+    }
+};
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> LinearCrossEntropyAutograd(const at::Tensor &x, const at::Tensor &w, const at::Tensor &targets, std::string reduction,
+                                                                                      double z_coef)
+{
+    if (!Recorded("linear_cross_entropy", {x, w})) return CCH_BELOW(LinearCrossEntropy, "linear_cross_entropy", x, w, targets, reduction, z_coef);
+    const Variables out = LinearCrossEntropyFunction::apply(x, w, targets, reduction, z_coef);
+    return {out[0], out[1], out[2], out[3]};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(catccos, m)
@@ -778,6 +1134,14 @@ TORCH_LIBRARY(catccos, m)
     m.def("w4a16_matmul(Tensor x, Tensor w, Tensor scales, Tensor? zeros, str fmt, int group_size) -> Tensor");
     m.def("moe_ffn_w4a16(Tensor x, Tensor expert_idx, Tensor probs, Tensor w1, Tensor scales1, Tensor? zeros1, Tensor w2, Tensor scales2, Tensor? zeros2, str fmt, "
           "int group_size) -> Tensor");
+    m.def("grouped_matmul(Tensor x, Tensor w, Tensor group_sizes, int trans_b) -> Tensor");
+    m.def("grouped_matmul_backward(Tensor grad_out, Tensor x, Tensor w, Tensor group_sizes, int trans_b, bool x_grad, bool w_grad) -> (Tensor, Tensor)");
+    m.def("matmul_bias_act(Tensor x, Tensor w, Tensor? bias, Tensor? residual, str activation, int trans_b, bool return_preact) -> (Tensor, Tensor)");
+    m.def("matmul_bias_act_backward(Tensor grad_out, Tensor x, Tensor w, Tensor? preact, str activation, int trans_b, bool x_grad, bool w_grad, bool bias_grad) -> "
+          "(Tensor, Tensor, Tensor)");
+    m.def("linear_cross_entropy(Tensor x, Tensor w, Tensor targets, str reduction, float z_coef) -> (Tensor, Tensor, Tensor, Tensor)");
+    m.def("linear_cross_entropy_backward(Tensor grad_loss, Tensor x, Tensor w, Tensor targets, Tensor lse, Tensor tokens, str reduction, float z_coef, bool x_grad, "
+          "bool w_grad) -> (Tensor, Tensor)");
 }
 
 // init / finalize take no tensors: one kernel for every backend, as in the reference (torch_bindings.cpp:233-238)
@@ -804,6 +1168,12 @@ TORCH_LIBRARY_IMPL(catccos, CUDA, m)
     m.impl("moe_balance_loss_backward", &MoeBalanceLossBackward);
     m.impl("w4a16_matmul", &W4A16Matmul);
     m.impl("moe_ffn_w4a16", &MoeFfnW4A16);
+    m.impl("grouped_matmul", &GroupedMatmul);
+    m.impl("grouped_matmul_backward", &GroupedMatmulBackward);
+    m.impl("matmul_bias_act", &MatmulBiasAct);
+    m.impl("matmul_bias_act_backward", &MatmulBiasActBackward);
+    m.impl("linear_cross_entropy", &LinearCrossEntropy);
+    m.impl("linear_cross_entropy_backward", &LinearCrossEntropyBackward);
 }
 
 TORCH_LIBRARY_IMPL(catccos, Meta, m)
@@ -822,6 +1192,12 @@ TORCH_LIBRARY_IMPL(catccos, Meta, m)
     m.impl("moe_balance_loss_backward", &MoeBalanceLossBackwardMeta);
     m.impl("w4a16_matmul", &W4A16Meta);
     m.impl("moe_ffn_w4a16", &MoeFfnW4A16Meta);
+    m.impl("grouped_matmul", &GroupedMatmulMeta);
+    m.impl("grouped_matmul_backward", &GroupedMatmulBackwardMeta);
+    m.impl("matmul_bias_act", &MatmulBiasActMeta);
+    m.impl("matmul_bias_act_backward", &MatmulBiasActBackwardMeta);
+    m.impl("linear_cross_entropy", &LinearCrossEntropyMeta);
+    m.impl("linear_cross_entropy_backward", &LinearCrossEntropyBackwardMeta);
 }
 
 TORCH_LIBRARY_IMPL(catccos, Autograd, m)
@@ -832,4 +1208,10 @@ TORCH_LIBRARY_IMPL(catccos, Autograd, m)
     m.impl("moe_balance_loss_backward", &MoeBalanceLossBackwardAutograd);
     m.impl("w4a16_matmul", &W4A16MatmulAutograd);
     m.impl("moe_ffn_w4a16", &MoeFfnW4A16Autograd);
+    m.impl("grouped_matmul", &GroupedMatmulAutograd);
+    m.impl("grouped_matmul_backward", &GroupedMatmulBackwardAutograd);
+    m.impl("matmul_bias_act", &MatmulBiasActAutograd);
+    m.impl("matmul_bias_act_backward", &MatmulBiasActBackwardAutograd);
+    m.impl("linear_cross_entropy", &LinearCrossEntropyAutograd);
+    m.impl("linear_cross_entropy_backward", &LinearCrossEntropyBackwardAutograd);
 }

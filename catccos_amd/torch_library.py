@@ -27,7 +27,9 @@ The operators are a C++ `TORCH_LIBRARY` (catccos_amd/csrc/torch/torch_bindings.c
 library directly; importing this module loads it into the Python process (`import catccos_amd` does not).
 Also there: `mx_grouped_matmul_swiglu_mx`, `gmm_dequant_swiglu_mx` (up projections with MX-quantised output) and
 `moe_ffn_mxfp8` (the MXFP8 MoE FFN of one rank, routing to combine); `moe_router`, `moe_balance_loss`, differentiable in the logits in reverse
-mode, and their gradients as calls of their own (`..._backward`); `w4a16_matmul`, `moe_ffn_w4a16`, backward through which raises.
+mode, and their gradients as calls of their own (`..._backward`); `w4a16_matmul`, `moe_ffn_w4a16`, backward through which raises; `grouped_matmul`, `matmul_bias_act` and
+`linear_cross_entropy`, differentiable in reverse mode as `catccos_amd`'s forms are, and their gradients (`..._backward`), where a result that is not asked for
+is an empty tensor.
 """
 import os
 
