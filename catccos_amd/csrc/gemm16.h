@@ -24,7 +24,26 @@ enum Kernel16 { KERNEL16_128 = 0, KERNEL16_256 = 1, KERNEL16_ROWS = 2, NUM_KERNE
 constexpr int64_t BIG_TILES16 = 192;     // tiles of 256 x 256 from which on they are taken: three quarters of the CUs
 struct Plan16 {
     int kernel, splits, deep;   // Kernel16, parts of K, four stages (tiles of 128 x 128)
+    int tail;                   // tiles of 256 x 256: how many parts of its last round's tiles there may be (0: that round is not split)
 };
+// Tiles of 256 x 256: in how many parts the K of the last round's `left` tiles is worked on by `grid` workgroups, at most `most` parts in all.  In ns, measured: a step of a tile; a
+// part's sums to memory and back (256 KiB each way); the second launch.  Integers: the product's kernel and the one that joins the parts decide it alike.
+constexpr int TAIL16_MOST = 8, TAIL16_STEPS = 64;   // (from TAIL16_MOST^2 steps on every part has some)
+constexpr int64_t TAIL16_BYTES = 256 * 256 * 4;
+__host__ __device__ inline int tail_parts16(int left, int grid, int steps, int most)
+{
+    constexpr int STEP = 1450, PART = 110, JOIN = 6000;
+    int parts = 1, best = STEP * steps;
+    if (left <= 0 || steps < TAIL16_STEPS) return 1;
+    for (int s = 2; s <= TAIL16_MOST && left * s <= most; s++) {
+        const int ns = (left * s + grid - 1) / grid * ((steps + s - 1) / s) * STEP + left * s * PART + JOIN;
+        if (ns < best) {
+            best = ns;
+            parts = s;
+        }
+    }
+    return parts;
+}
 Plan16 plan16(const struct Gemm16 &p, int layout, int epilogue);
 extern std::atomic<int> g_kernel16;   // -1: chosen per problem; else that one wherever it takes the problem
 
@@ -45,6 +64,7 @@ struct Gemm16 {
     float *partial;                        // fp32, for sums of parts of K; K is not split where partial_bytes are too few
     int64_t partial_bytes;
     int splits;                            // parts of K (set by the launch)
+    int tail;                              // Plan16::tail (set by the launch)
     // EPI16_OUT
     const float *scale;                    // device, or nullptr: 1
     float *sums;                           // fp32 [m, n], or nullptr: a product in pieces of K.  sums_in: added to the sum; sums_out: takes it in place of out

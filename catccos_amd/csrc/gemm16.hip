@@ -17,11 +17,19 @@ Plan16 plan16(const Gemm16 &p, int layout, int epilogue)
     constexpr int CUS = 256;
     constexpr double MEMORY = 5.1e6;   // bytes a us
     const int asked = g_kernel16.load();
-    Plan16 plan{KERNEL16_128, 1, 0};
+    Plan16 plan{KERNEL16_128, 1, 0, 0};
     const bool results = epilogue == EPI16_OUT || epilogue == EPI16_ACT;
     const bool rows_kernel = layout != ROWS_TN && results && !p.a_rows && !p.sums && !p.out_rows && !p.scale;
-    if (rows_kernel && asked == KERNEL16_ROWS) return {KERNEL16_ROWS, 1, 0};
-    if (!p.a_rows && p.pitch_out < MAX_PITCH16 / 2 && (asked == KERNEL16_256 || (asked < 0 && tiles16(p, 256, 256) >= BIG_TILES16))) return {KERNEL16_256, 1, 0};
+    if (rows_kernel && asked == KERNEL16_ROWS) return {KERNEL16_ROWS, 1, 0, 0};
+    const bool big = !p.a_rows && p.pitch_out < MAX_PITCH16 / 2;
+    const int64_t big_tiles = tiles16(p, 256, 256);
+    Plan16 on_big{KERNEL16_256, 1, 0, 0};
+    const int big_steps = (p.k + 63) / 64;
+    if (layout != ROWS_TN && results && big_steps >= TAIL16_STEPS) {
+        on_big.tail = (int)std::min<int64_t>(2 * CUS, TAIL16_MOST * big_tiles);
+        if (!p.group_sizes && tail_parts16((int)(big_tiles % CUS), CUS, big_steps, on_big.tail) == 1) on_big.tail = 0;
+    }
+    if (big && (asked == KERNEL16_256 || (asked < 0 && big_tiles >= BIG_TILES16))) return on_big;
     // tiles of 128 x 128, about: a group's rows or K are taken to be its share
     const int64_t groups = p.k_grouped || !p.group_sizes ? p.groups : std::max(std::min(p.groups, p.m), 1);   // that may have rows
     const int64_t share = p.k_grouped || !p.group_sizes ? p.m : (p.m + groups - 1) / groups, each = (share + 127) / 128 * ((p.n + 127) / 128);
@@ -40,6 +48,12 @@ Plan16 plan16(const Gemm16 &p, int layout, int epilogue)
             plan.splits = s;
         }
     }
+    if (big && asked < 0 && on_big.tail) {
+        // Few tiles of 256 x 256 and a long K, whose parts fill the chip (2000 of 4999 rows x 1984, K = 20011: 289 us on tiles of 128 x 128)
+        const int parts = tail_parts16((int)big_tiles, CUS, big_steps, on_big.tail);
+        const double us = (double)((big_tiles * parts + CUS - 1) / CUS) * ((big_steps + parts - 1) / parts) * 1.45 + (double)big_tiles * parts * 0.11 + 12;
+        if (us < best) return on_big;
+    }
     plan.deep = tiles * plan.splits <= CUS;
     if (rows_kernel && asked < 0 && share <= 128) {
         // The kernel for few rows: an eighth of the steps in a row, or the weights' way from memory, again for every tile of rows (from the caches).  K-major weights come in half
@@ -50,13 +64,17 @@ Plan16 plan16(const Gemm16 &p, int layout, int epilogue)
         const double step = (layout == ROWS_NN ? 0.9 : 0.31) * (mr == 32 ? 1.2 : 1.0) * (double)((workgroups + CUS - 1) / CUS);
         const double fetch = weights * (layout == ROWS_NN ? 2.0 : 1.0) * (1 + 0.4 * (row_tiles - 1));
         const double us = std::max((double)((steps + 7) / 8) * step, fetch);
-        if (us <= std::max(best, weights) + 2.0) return {KERNEL16_ROWS, 1, 0};
+        if (us <= std::max(best, weights) + 2.0) return {KERNEL16_ROWS, 1, 0, 0};
     }
     return plan;
 }
 
 static int64_t parts_bytes(const Gemm16 &p, int splits) { return splits > 1 ? round256((int64_t)splits * (p.k_grouped ? p.groups : 1) * p.m * p.n * 4) : 0; }
-int64_t partial16_bytes(const Gemm16 &p, int layout, int epilogue) { return parts_bytes(p, plan16(p, layout, epilogue).splits); }
+int64_t partial16_bytes(const Gemm16 &p, int layout, int epilogue)
+{
+    const Plan16 plan = plan16(p, layout, epilogue);
+    return std::max(parts_bytes(p, plan.splits), plan.tail * TAIL16_BYTES);
+}
 
 // ---- the parts of K added up in their order, with the product's epilogue.  VEC elements of a row to a thread.
 template <class T, int EPI, int VEC> __global__ __launch_bounds__(256) void join16_kernel(Gemm16 p, int64_t outputs, int64_t per_row)
@@ -126,6 +144,7 @@ int gemm16_launch(const Gemm16 &problem, int layout, int epilogue, hipStream_t s
     Gemm16 p = problem;
     Plan16 plan = plan16(p, layout, epilogue);
     if (!p.partial || parts_bytes(p, plan.splits) > p.partial_bytes) plan.splits = 1;
+    if (!p.partial || plan.tail * TAIL16_BYTES > p.partial_bytes) plan.tail = 0;
     p.splits = plan.splits;
     if (const int rc = p.half ? gemm16_launch_f16(p, plan, layout, epilogue, stream) : gemm16_launch_bf16(p, plan, layout, epilogue, stream)) return rc;
     if (p.splits == 1) return CCH_OK;

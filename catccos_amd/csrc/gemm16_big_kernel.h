@@ -10,6 +10,8 @@
 //   ROWS_NK  L0: A blocks 2-3 of s + 1   C0: A blocks 0-1 of s + 2   L1, C1: half of B of s + 2 each; L0 reads all of B and A blocks 0-1, L1 A blocks 2-3
 //   ROWS_NN  L0: second half of B of s + 1   L1: first half of B of s + 2   C1: A of s + 2; L0 reads the first half of the step, L1 the second
 //   ROWS_TN  L0: second halves of A and B of s + 1   L1: first halves of s + 2; reads likewise
+// Where the tiles leave part of the last round's workgroups idle and K is long, that round's tiles are worked on in parts of K (tail_parts16): each leaves its fp32 sums as its lanes hold them, and a
+// second launch adds a tile's parts up in their order and writes the results.
 // A group's A rows are read by that group alone (K contiguous), so they are free one slot earlier than B.  Every wave issues the same number of requests in every step (what lies
 // past the operand fetches nothing), so every wait is a constant: requests complete in order.  The last two steps of a tile request the next one's first two; past the last tile
 // the descriptors are empty.
@@ -30,6 +32,7 @@ __global__ __launch_bounds__(Big16::THREADS, 2) void gemm16_big_kernel(Gemm16 p)
 {
     using S = Big16;
     constexpr bool A_KM = LAYOUT == ROWS_TN, B_KM = LAYOUT != ROWS_NK, HALVES = LAYOUT != ROWS_NK;
+    constexpr bool TAIL = LAYOUT != ROWS_TN && (EPI == EPI16_OUT || EPI == EPI16_ACT);
     constexpr int MT = S::MT, NT = S::NT, PANEL = S::PANEL;
     using KM = KMajor<256>;
     GroupTable16 &tab = *reinterpret_cast<GroupTable16 *>(smem + S::TABLE);
@@ -44,6 +47,14 @@ __global__ __launch_bounds__(Big16::THREADS, 2) void gemm16_big_kernel(Gemm16 p)
     const int col_tiles = (p.n + S::TN - 1) / S::TN;
     const int row_tiles = uniform(rows_grouped ? tab.tile[p.groups] : (p.m + S::TM - 1) / S::TM);
     const int per_list = row_tiles * col_tiles, end = lists_end16(per_list, rows_grouped ? 1 : p.groups);   // (below 2^31: the launch checks)
+
+    int parts = 1, left = 0, full = 0;   // of K; tiles of the last round, and before it
+    if (TAIL && p.tail) {
+        left = per_list % (int)gridDim.x;
+        full = per_list - left;
+        parts = uniform(tail_parts16(left, (int)gridDim.x, (p.k + 63) >> 6, p.tail));
+    }
+    const int tiles_end = TAIL && parts > 1 ? full + ((left * parts + 7) & ~7) : end, part_k = TAIL ? (((p.k + 63) >> 6) + parts - 1) / parts * 64 : 0;
 
     // ---- this lane's fragment reads (the current stage's; moved by a panel from step to step)
     // A, K contiguous: panel position 128 wm + 32 i + r holds tile row 64 i + 32 wm + r; K-major: column = tile row
@@ -95,6 +106,7 @@ __global__ __launch_bounds__(Big16::THREADS, 2) void gemm16_big_kernel(Gemm16 p)
 
     struct Tile {
         bool valid;
+        int slot;                    // of a part of K: where its sums go; else -1
         int e, m0, m_end, n0, k_len, steps;
         const uint16_t *a, *b;       // first element of the first step
         int64_t left_a, left_b;      // bytes from there to the operand's end
@@ -103,9 +115,21 @@ __global__ __launch_bounds__(Big16::THREADS, 2) void gemm16_big_kernel(Gemm16 p)
     const int k8 = (p.k + 7) & ~7, n8 = (p.n + 7) & ~7, m8 = (p.m + 7) & ~7;
     // The tile at t, or the next one there is of this workgroup's (t moves on).
     auto decode = [&](int &t, Tile &c) {
-        int at = -1, list = 0;
-        for (; t < end; t += (int)gridDim.x) {
-            at = place_in_lists16(t, per_list, list);
+        int at = -1, list = 0, part = 0;
+        c.slot = -1;
+        for (; t < tiles_end; t += (int)gridDim.x) {
+            if (!TAIL || parts == 1) {
+                at = place_in_lists16(t, per_list, list);
+            } else if (t < full) {
+                at = place16(t, full);
+            } else {
+                const int v = place16(t - full, left * parts);
+                if (v >= 0) {
+                    part = v / left;
+                    at = full + v - part * left;
+                    c.slot = v;
+                }
+            }
             if (at >= 0) break;
         }
         c.valid = at >= 0;
@@ -123,6 +147,10 @@ __global__ __launch_bounds__(Big16::THREADS, 2) void gemm16_big_kernel(Gemm16 p)
             c.e = uniform(group_of_tile16(tab, p.groups, rt));
             c.m0 = uniform(tab.start[c.e] + (rt - tab.tile[c.e]) * S::TM);
             c.m_end = uniform(tab.start[c.e + 1]);
+            if (TAIL && c.slot >= 0) {
+                k0 = part * part_k;
+                c.k_len = min(p.k - k0, part_k);
+            }
         } else {
             c.e = list;
             c.m0 = rt * S::TM;
@@ -136,16 +164,16 @@ __global__ __launch_bounds__(Big16::THREADS, 2) void gemm16_big_kernel(Gemm16 p)
             c.a = p.a + (int64_t)k0 * p.pitch_a + c.m0;
             c.left_a = c.k_len ? ((int64_t)(c.k_len - 1) * p.pitch_a + m8 - c.m0) * 2 : 0;
         } else {
-            c.a = p.a + (int64_t)c.m0 * p.pitch_a;
-            c.left_a = ((int64_t)(min(c.m_end - c.m0, S::TM) - 1) * p.pitch_a + k8) * 2;
+            c.a = p.a + (int64_t)c.m0 * p.pitch_a + k0;
+            c.left_a = ((int64_t)(min(c.m_end - c.m0, S::TM) - 1) * p.pitch_a + k8 - k0) * 2;
         }
         const uint16_t *b = p.b + (rows_grouped ? (int64_t)c.e * p.b_stride : (int64_t)0);
         if (B_KM) {
             c.b = b + (int64_t)k0 * p.pitch_b + c.n0;
             c.left_b = c.k_len ? ((int64_t)(c.k_len - 1) * p.pitch_b + n8 - c.n0) * 2 : 0;
         } else {
-            c.b = b + (int64_t)c.n0 * p.pitch_b;
-            c.left_b = ((int64_t)(min(p.n - c.n0, S::TN) - 1) * p.pitch_b + k8) * 2;
+            c.b = b + (int64_t)c.n0 * p.pitch_b + k0;
+            c.left_b = ((int64_t)(min(p.n - c.n0, S::TN) - 1) * p.pitch_b + k8 - k0) * 2;
         }
     };
 
@@ -374,7 +402,19 @@ __global__ __launch_bounds__(Big16::THREADS, 2) void gemm16_big_kernel(Gemm16 p)
         }
         // Both groups write their results in the same slot: the first behind the barrier that ends its last matrix slot, the second, one slot behind, before it.
         if (wm == 0) CCH_BARRIER();
-        epilogue16<T, EPI, MT, NT, 64>(p, acc, cur.e, cur.m0, cur.m_end, cur.n0, wm * 32, wn * 64, whole, counted);
+        if (TAIL && cur.slot >= 0) {
+            // (32 stores, no fewer than `more` counts)
+            f32x4 *to = reinterpret_cast<f32x4 *>(p.partial) + (int64_t)cur.slot * (TAIL16_BYTES / 16) + threadIdx.x;
+            static_for<MT>([&](auto i_c) {
+                static_for<NT>([&](auto j_c) {
+                    constexpr int i = decltype(i_c)::value, j = decltype(j_c)::value;
+#pragma unroll
+                    for (int q = 0; q < 4; q++) to[((i * NT + j) * 4 + q) * S::THREADS] = (f32x4){acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                });
+            });
+        } else {
+            epilogue16<T, EPI, MT, NT, 64>(p, acc, cur.e, cur.m0, cur.m_end, cur.n0, wm * 32, wn * 64, whole, counted);
+        }
         if (!nxt.valid) break;
         young = more;
         cur = nxt;
@@ -385,6 +425,41 @@ __global__ __launch_bounds__(Big16::THREADS, 2) void gemm16_big_kernel(Gemm16 p)
     CCH_WAIT_VM_LGKM0(0);   // (requests past the last tile fetch nothing, but they write zeros to LDS)
 }
 
+// The last round's tiles whose K was split: their parts added up in order, 64 rows (a block of each group of waves) to a workgroup and turn, then what the product does with a result.
+template <class T, int EPI> __global__ __launch_bounds__(Big16::THREADS) void gemm16_tail_kernel(Gemm16 p, int grid)
+{
+    using S = Big16;
+    __shared__ GroupTable16 tab;
+    if (threadIdx.x < 64) build_groups16(tab, p.group_sizes, p.groups, p.m, S::TM);
+    __syncthreads();
+    const int wave = uniform(threadIdx.x >> 6), wm = wave >> 2, wn = wave & 3;
+    const int row_tiles = uniform(tab.tile[p.groups]), col_tiles = (p.n + S::TN - 1) / S::TN, all = row_tiles * col_tiles, left = all % grid;
+    const int parts = uniform(tail_parts16(left, grid, (p.k + 63) >> 6, p.tail));
+    if (parts == 1) return;
+    const bool whole = whole_rows(p);
+    for (int t = blockIdx.x; t < left * S::MT; t += gridDim.x) {
+        const int tile = t / S::MT, i = t % S::MT;
+        int rt, ct;
+        tile_of16(all - left + tile, row_tiles, col_tiles, rt, ct);
+        const int e = uniform(group_of_tile16(tab, p.groups, rt)), m0 = uniform(tab.start[e] + (rt - tab.tile[e]) * S::TM), m_end = uniform(tab.start[e + 1]);
+        if (m0 + i * 64 >= m_end) continue;
+        const f32x4 *from = reinterpret_cast<const f32x4 *>(p.partial) + (int64_t)tile * (TAIL16_BYTES / 16) + i * (S::NT * 4 * S::THREADS) + threadIdx.x;
+        f32x4 sum[S::NT * 4];
+#pragma unroll
+        for (int q = 0; q < S::NT * 4; q++) sum[q] = from[q * S::THREADS];
+#pragma unroll 2
+        for (int s = 1; s < parts; s++)
+#pragma unroll
+            for (int q = 0; q < S::NT * 4; q++) sum[q] += from[(int64_t)s * left * (TAIL16_BYTES / 16) + q * S::THREADS];
+        v16f acc[1][S::NT];
+#pragma unroll
+        for (int q = 0; q < S::NT * 4; q++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) acc[0][q >> 2][4 * (q & 3) + x] = sum[q][x];
+        epilogue16<T, EPI, 1, S::NT, 64>(p, acc, e, m0, m_end, ct * S::TN, wm * 32 + i * 64, wn * 64, whole, false);
+    }
+}
+
 template <class T, int LAYOUT, int EPI> int launch16_big(const Gemm16 &p, int64_t tiles, hipStream_t stream)
 {
     static std::atomic<uint64_t> attr_set{0};
@@ -393,9 +468,16 @@ template <class T, int LAYOUT, int EPI> int launch16_big(const Gemm16 &p, int64_
     CCH_HIP(hipGetDevice(&dev));
     CCH_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
     if (const int rc = allow_lds16(reinterpret_cast<const void *>(kernel), Big16::LDS, attr_set)) return rc;
-    const int64_t grid = std::min<int64_t>((tiles + 7) & ~(int64_t)7, std::max(cus & ~7, 8));   // (a multiple of 8: place16)
+    const int64_t most = std::max(cus & ~7, 8), grid = p.tail ? most : std::min<int64_t>((tiles + 7) & ~(int64_t)7, most);   // (a multiple of 8: place16)
     kernel<<<dim3((uint32_t)grid), dim3(Big16::THREADS), Big16::LDS, stream>>>(p);
-    return launch_status("gemm16_big_kernel");
+    if (const int rc = launch_status("gemm16_big_kernel")) return rc;
+    if constexpr (LAYOUT != ROWS_TN && (EPI == EPI16_OUT || EPI == EPI16_ACT)) {
+        if (p.tail) {
+            gemm16_tail_kernel<T, EPI><<<dim3((uint32_t)(2 * grid)), dim3(Big16::THREADS), 0, stream>>>(p, (int)grid);
+            return launch_status("gemm16_tail_kernel");
+        }
+    }
+    return CCH_OK;
 }
 
 }  // namespace cch

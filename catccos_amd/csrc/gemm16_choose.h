@@ -9,6 +9,7 @@ template <class T, int LAYOUT, int EPI> int shape16(Gemm16 p, const Plan16 &plan
 {
     CCH_REQUIRE((tiles16(p, 128, 128) + 8 * (int64_t)p.groups) * plan.splits < (int64_t)1 << 31, "a product of %d x %d in %d groups has too many tiles", p.m, p.n, p.groups);
     p.splits = plan.splits;
+    p.tail = plan.tail;
     if constexpr (LAYOUT != ROWS_TN && (EPI == EPI16_OUT || EPI == EPI16_ACT)) {
         if (plan.kernel == KERNEL16_ROWS) {
             const int rows = rows16(p);

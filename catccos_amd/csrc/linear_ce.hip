@@ -238,12 +238,13 @@ static CeWorkspace ce_workspace(int64_t t, int64_t h, int64_t v, bool backward)
         at.stats = piece(t * ((v + CE_STAT - 1) / CE_STAT) * 8);
     } else {
         const int64_t c = ce_piece(t, v);
+        float some;   // (stands for sums that are there)
         at.lse = piece(t * 4);
         at.scalar = piece(4);
         at.d = piece(t * pitch16(c) * 2);
         if (c < v) at.sums = piece(t * h * 4);
         at.parts = piece(std::max(partial16_bytes(ce_grad_w(&CE_COUNT, t, h, c), ROWS_TN, EPI16_OUT),
-                                  c < v ? 0 : partial16_bytes(ce_grad_x(&CE_COUNT, &CE_COUNT, nullptr, t, h, c), ROWS_NN, EPI16_OUT)));
+                                  partial16_bytes(ce_grad_x(&CE_COUNT, &CE_COUNT, c < v ? &some : nullptr, t, h, c), ROWS_NN, EPI16_OUT)));
     }
     return at;
 }

@@ -326,10 +326,53 @@ def test_long_sums(m, k, n, trans_b):
     assert not gx.any()
 
 
+@pytest.fixture
+def big_tiles():
+    cc.set_option("matmul16_kernel", 1)
+    yield
+    cc.set_option("matmul16_kernel", -1)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-def test_a_vocabulary_of_several_pieces(dtype):
-    """Enough tokens that the gradient of the logits is worked on in three pieces, whose shares of grad_x are added up."""
-    x, w, tg = loss_test._case(66000, 24, 3700, dtype, 0.6)
+@pytest.mark.parametrize("trans_b", [0, 1])
+@pytest.mark.parametrize("sizes,rest,k,n", [([300, 1, 0, 129, 600], 7, 4096, 520), ([40], 0, 9999, 33), ([2000, 0, 900, 1800], 5, 4424, 4400)])
+def test_tiles_of_256_and_a_long_k_in_groups(big_tiles, sizes, rest, k, n, trans_b, dtype):
+    """K is worked on in parts where the last round of tiles leaves workgroups idle: behind whole rounds (some 340 tiles) and alone."""
+    x, w, g, gs = (v.cuda() for v in grouped._case(sizes, rest, k, n, trans_b, dtype))
+    out = cc.grouped_matmul(x, w, gs, trans_b)
+    grads = cc.grouped_matmul_backward(g, x, w, gs, trans_b)
+    assert same(out, cc.grouped_matmul(x, w, gs, trans_b))
+    for (a, b), i in zip(grouped._ranges(sizes, x.shape[0]), range(len(sizes))):
+        m = (w[i].t() if trans_b else w[i]).double()
+        want = x[a:b].double() @ m
+        check(out[a:b], want, rounded(want, sum_error(x[a:b].double(), m), dtype), "out %d" % i)
+        want = g[a:b].double() @ m.t()
+        check(grads[0][a:b], want, rounded(want, sum_error(g[a:b].double(), m.t()), dtype), "grad_x %d" % i)
+    assert not out[sum(sizes):].any() and not grads[0][sum(sizes):].any()
+
+
+@pytest.mark.parametrize("m,k,n,act", [(700, 4200, 520, "gelu"), (4400, 4096, 4100, "silu"), (1, 20000, 8, "none"), (257, 65600, 256, "relu")])
+@pytest.mark.parametrize("trans_b", [0, 1])
+def test_tiles_of_256_and_a_long_k_in_a_layer(big_tiles, m, k, n, act, trans_b):
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    new = lambda *shape: torch.randn(*shape, device="cuda", generator=gen)   # noqa: E731
+    x, w, b, r = new(m, k).bfloat16(), (new(*((n, k) if trans_b else (k, n))) * k ** -0.5).bfloat16(), new(n).bfloat16(), new(m, n).bfloat16()
+    wk = (w.t() if trans_b else w).double()
+    z = x.double() @ wk + b.double()
+    ez = sum_error(x.double(), wk) + 2.0 ** -23 * z.abs()
+    y = {"gelu": torch.nn.functional.gelu, "silu": torch.nn.functional.silu, "relu": torch.relu, "none": lambda v: v}[act](z) + r.double()
+    out, pre = cc.matmul_bias_act(x, w, b, r, act, trans_b, True)
+    check(pre, z, rounded(z, ez, torch.bfloat16), "preact")
+    check(out, y, rounded(y, 1.13 * ez + 2.0 ** -19 * (z.abs() + 1) + 2.0 ** -23 * y.abs(), torch.bfloat16), "out")
+    assert all(same(a, c) for a, c in zip((out, pre), cc.matmul_bias_act(x, w, b, r, act, trans_b, True)))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("t,h,v", [(66000, 24, 3700), (16000, 264, 9000)])
+def test_a_vocabulary_of_several_pieces(t, h, v, dtype):
+    """Enough tokens that the gradient of the logits is worked on in several pieces, whose shares of grad_x are added up; the second, of pieces of more than 4096
+    columns, sums them in parts."""
+    x, w, tg = loss_test._case(t, h, v, dtype, 0.6)
     scale = 1024.0 if dtype == torch.float16 else 1.0
     got = cc.linear_cross_entropy(x.cuda(), w.cuda(), tg.cuda(), reduction="sum", z_coef=1e-4)
     grads = cc.linear_cross_entropy_backward(torch.full((), scale, device="cuda"), x.cuda(), w.cuda(), tg.cuda(), got[2], got[3], reduction="sum", z_coef=1e-4)
