@@ -160,11 +160,12 @@ __device__ __forceinline__ void tile_of16(int at, int row_tiles, int col_tiles, 
 // K contiguous: a row is 128 bytes, its 16-byte chunk c at position c ^ ((row >> 1) & 7) (gemm_device.h).  Lane (r, g) of a 32 x 32 x 16 instruction holds
 // elements 8g..8g+7 of a sixteenth: chunk 2 kk + g.
 // K-major: a K-row is COLS * 2 bytes; a transposing LDS load hands 16 lanes four K-rows of 16 columns, lane i addressing columns 4 (i % 4) .. of row i / 4 and
-// receiving column i.  32 lanes, one pass of the load, touch 64 bytes of each of four rows that lie a multiple of 256 (or 128) bytes apart: the chunk
-// position's bit 2 and 3 (128 bytes: bit 2) are those of the chunk xor the row's, which puts them on all banks once.  (Four rows of 64 bytes are on all banks as they are.)
+// receiving column i.  32 lanes, one pass of the load, touch 64 bytes of each of four rows that lie a multiple of 256 bytes apart: the chunk
+// position's bits 2 and 3 are those of the chunk xor the row's, which puts them on all banks once.  (Four rows of 64 bytes are on all banks as they are.)
 template <int COLS> struct KMajor {
     static constexpr int ROW = COLS * 2, CHUNKS = COLS / 8, ROWS_PER_KIB = 512 / COLS;
-    static __device__ __forceinline__ uint32_t swizzle(int row) { return COLS >= 128 ? (uint32_t)(row & 3) << 2 : COLS == 64 ? (uint32_t)((row >> 1) & 1) << 2 : 0u; }
+    static_assert(COLS == 32 || COLS % 128 == 0, "64 columns would need a swizzle of their own");
+    static __device__ __forceinline__ uint32_t swizzle(int row) { return COLS >= 128 ? (uint32_t)(row & 3) << 2 : 0u; }
 };
 __device__ __forceinline__ v4i read_transposed(uint32_t addr, uint32_t row_bytes)
 {

@@ -3,7 +3,8 @@
 // and ctypes 10 us of host time (checks, allocations, argument conversion, stream look-up), so that the host was what such a step
 // waited for.  Measured, host time of a call: mx_quant 11.6 -> 4.3 us, mx_matmul 10.3 -> 4.1, dynamic_quant_i8 9.9 -> 4.1,
 // moe_init_routing 11.9 -> 5.2, moe_ffn_mxfp8 56 -> 17.5 (of which three quarters are allocations and launches), moe_router 11.3 -> 4.6 (its backward 9.7 ->
-// 4.0), moe_balance_loss 14.4 -> 5.7 (10.1 -> 4.3), w4a16_matmul 11.2 -> 3.8, moe_ffn_w4a16 19.4 -> 9.8.
+// 4.0), moe_balance_loss 14.4 -> 5.7 (10.1 -> 4.3), w4a16_matmul 11.2 -> 3.8, moe_ffn_w4a16 19.4 -> 9.8, grouped_matmul 14.5 -> 4.7
+// (backward 17.3 -> 8.3), matmul_bias_act 14.8 -> 4.4 (24.4 -> 15.7, five launches), linear_cross_entropy 34.6 -> 15.1, four launches (33.6 -> 17.7).
 //
 // Every function here answers Py_NotImplemented to a call it does not recognise as one of those, or that the library refuses,
 // before or without any effect that outlives the call: the caller (ops.py) then takes the general path, which makes inputs

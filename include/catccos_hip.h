@@ -489,6 +489,9 @@ int cch_linear_cross_entropy_backward(const float *grad_loss, const void *x, con
  * writes fp16, the vector epilogue widens it; the golden generator's option,
  * examples/utils/gen_data_dispatch_gmm_dequant_swiglu.py:309-310); 0 (default) keeps fp32 throughout, the golden
  * generator's default path - this one switch does change results, by at most 2^-11 relative;
+ * "matmul16_kernel" = 0..2 asks for one of the kernels of the products of bf16 or half operands (0: tiles of 128 x 128, 1: of 256 x 256, 2: few rows) wherever that kernel takes
+ * the problem, -1 (default) chooses per problem.  They add up K in different orders (all in fp32), as 0, 1 and their parts of K do by the problem's size: a result's last bit can
+ * depend on how many rows the call has; a workspace is as large as the choice at the time of the query asks for (a launch with less runs, with fewer parts of K, or is refused);
  * "gemm_nt_output" = 1 / 0 gives or denies the output stores the non-temporal hint, -1 (default) gives it to the MXFP4 kernels, where it measured
  * 3-4 % faster (no difference for the others); "quant_integer_encoder" = 1 runs the E4M3
  * round-to-nearest-even quantiser through the integer encoder instead of the hardware conversion (an
