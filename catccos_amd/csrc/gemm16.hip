@@ -151,52 +151,60 @@ int gemm16_launch(const Gemm16 &problem, int layout, int epilogue, hipStream_t s
     return p.half ? join16<F16>(p, epilogue, stream) : join16<Bf16>(p, epilogue, stream);
 }
 
-// One thread, 16 bytes of a copy; up to two operands in a launch.
+// Copies of rows; up to two operands in a launch.  A row has a power of two of a workgroup's threads, 16 bytes to each and turn, so that no thread divides (2684
+// rows, 20 experts' 3840 x 1449: one chunk of the whole copy to a thread 247 us a call, so 210).
 struct PadRows16 {
     const uint16_t *src;
     uint16_t *dst;
-    int64_t chunks, cols, per_row;
+    int64_t rows, cols, per_row;
+    int threads_log2;
+    const int32_t *sizes;
+    int64_t group_rows;
 };
 __global__ __launch_bounds__(256) void pad_rows16_kernel(PadRows16 a, PadRows16 b)
 {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.chunks + b.chunks; i += (int64_t)gridDim.x * 256) {
-        const bool second = i >= a.chunks;
-        const PadRows16 &o = second ? b : a;
-        const int64_t at = second ? i - a.chunks : i, row = at / o.per_row, c = (at - row * o.per_row) * 8;
-        const uint16_t *s = o.src + row * o.cols + c;
-        v4i v;
+    const PadRows16 &o = blockIdx.y ? b : a;
+    const int threads = 1 << o.threads_log2, at_once = 256 >> o.threads_log2;
+    for (int64_t row = (int64_t)blockIdx.x * at_once + (threadIdx.x >> o.threads_log2); row < o.rows; row += (int64_t)gridDim.x * at_once) {
+        if (o.sizes && o.sizes[row / o.group_rows] <= 0) continue;
+        const uint16_t *s = o.src + row * o.cols;
+        uint16_t *d = o.dst + row * o.per_row * 8;
+        for (int64_t c = (threadIdx.x & (threads - 1)) * 8; c < o.per_row * 8; c += threads * 8) {
+            v4i v = {};
+            if (c + 8 <= o.cols) v = reinterpret_cast<const Unaligned16 *>(s + c)->v;
+            else
 #pragma unroll
-        for (int x = 0; x < 4; x++) {
-            const uint32_t lo = c + 2 * x < o.cols ? s[2 * x] : 0u, hi = c + 2 * x + 1 < o.cols ? s[2 * x + 1] : 0u;
-            v[x] = (int)(lo | hi << 16);
+                for (int x = 0; x < 7; x++)
+                    if (c + x < o.cols) v[x >> 1] |= (int)((uint32_t)s[c + x] << (16 * (x & 1)));
+            *reinterpret_cast<v4i *>(d + c) = v;
         }
-        *reinterpret_cast<v4i *>(o.dst + at * 8) = v;
     }
 }
 
 int whole_operands16(Operand16 *operands, int n, Carve &ws, hipStream_t stream)
 {
-    PadRows16 pads[2] = {};
+    PadRows16 pads[2];
     int used = 0;
+    auto copy = [&] {
+        int64_t blocks = 1;
+        for (int i = 0; i < used; i++) blocks = std::max(blocks, (pads[i].rows << pads[i].threads_log2) / 256 + 1);
+        hipLaunchKernelGGL(pad_rows16_kernel, dim3((unsigned)std::min<int64_t>(blocks, 2048), (unsigned)used), dim3(256), 0, stream, pads[0], pads[used - 1]);
+        used = 0;
+        return launch_status("pad_rows16_kernel");
+    };
     for (int i = 0; i < n; i++) {
         Operand16 &o = operands[i];
         if (!o.at || whole16(o.cols) || o.rows == 0 || o.cols == 0) continue;
-        uint16_t *copy = ws.take<uint16_t>(padded16_bytes(o.rows, o.cols));
-        pads[used++] = PadRows16{o.at, copy, o.rows * (pitch16(o.cols) / 8), o.cols, pitch16(o.cols) / 8};
-        o.at = copy;
-        if (used == 2 || i + 1 == n) {
-            const int64_t chunks = pads[0].chunks + pads[1].chunks;
-            hipLaunchKernelGGL(pad_rows16_kernel, dim3((unsigned)std::min<int64_t>((chunks + 255) / 256, 1 << 16)), dim3(256), 0, stream, pads[0], pads[1]);
-            if (const int rc = launch_status("pad_rows16_kernel")) return rc;
-            pads[0] = pads[1] = PadRows16{};
-            used = 0;
-        }
+        uint16_t *to = ws.take<uint16_t>(padded16_bytes(o.rows, o.cols));
+        const int64_t per_row = pitch16(o.cols) / 8;
+        int log2 = 0;
+        while (log2 < 8 && (1 << log2) < per_row) log2++;
+        pads[used++] = PadRows16{o.at, to, o.rows, o.cols, per_row, log2, o.sizes, o.group_rows};
+        o.at = to;
+        if (used == 2)
+            if (const int rc = copy()) return rc;
     }
-    if (used) {
-        hipLaunchKernelGGL(pad_rows16_kernel, dim3((unsigned)std::min<int64_t>((pads[0].chunks + 255) / 256, 1 << 16)), dim3(256), 0, stream, pads[0], pads[1]);
-        return launch_status("pad_rows16_kernel");
-    }
-    return CCH_OK;
+    return used ? copy() : CCH_OK;
 }
 
 __global__ __launch_bounds__(256) void fill_zero16_kernel(uint16_t *dst, int64_t n)
@@ -217,24 +225,23 @@ int64_t column_sum_bytes(int64_t m, int64_t n) { return round256(sum_runs(m) * n
 
 template <class T>
 __global__ __launch_bounds__(256) void act_backward16_kernel(const uint16_t *__restrict__ grad, const uint16_t *__restrict__ pre, uint16_t *__restrict__ dz,
-                                                             float *__restrict__ partial, int m, int n, int64_t pitch, int run, int act, bool whole_rows)
+                                                             float *__restrict__ partial, int m, int n, int64_t pitch, int run, int act)
 {
     __shared__ float sums[8][SUM_COLS];
     const int tc = threadIdx.x & 31, tr = threadIdx.x >> 5;
     const int c = (int)blockIdx.x * SUM_COLS + tc * 8, left = n - c;
     const int first = (int)blockIdx.y * run, last = min(m, first + run);
-    const bool whole = whole_rows && left >= 8;
     float sum[8] = {};
     if (left > 0)
         for (int row = first + tr; row < last; row += 8) {
             float v[8], z[8];
-            load8<T>(grad + (int64_t)row * n + c, whole, left, v);
+            load8<T>(grad + (int64_t)row * n + c, left, v);
             if (act != CCH_ACT_NONE) {
-                load8<T>(pre + (int64_t)row * n + c, whole, left, z);
+                load8<T>(pre + (int64_t)row * n + c, left, z);
 #pragma unroll
                 for (int x = 0; x < 8; x++) v[x] = x < left ? v[x] * act_slope(z[x], act) : 0.0f;
             }
-            if (dz) store8<T>(dz + (int64_t)row * pitch + c, true, 8, v);
+            if (dz) *reinterpret_cast<v4i *>(dz + (int64_t)row * pitch + c) = pack8<T>(v);
 #pragma unroll
             for (int x = 0; x < 8; x++) sum[x] += v[x];
         }
@@ -265,10 +272,9 @@ int act_backward16(const uint16_t *grad_out, const uint16_t *preact, uint16_t *d
 {
     if (m == 0 || n == 0 || (!dz && !grad_bias)) return CCH_OK;
     const int64_t runs = sum_runs(m), run = (m + runs - 1) / runs;
-    const bool whole = n % 8 == 0 && aligned(grad_out, 16) && aligned(preact, 16);
     auto kern = half ? act_backward16_kernel<F16> : act_backward16_kernel<Bf16>;
     hipLaunchKernelGGL(kern, dim3((unsigned)((n + SUM_COLS - 1) / SUM_COLS), (unsigned)runs), dim3(256), 0, stream, grad_out, preact, dz, grad_bias ? partial : nullptr, (int)m,
-                       (int)n, pitch16(n), (int)run, act, whole);
+                       (int)n, pitch16(n), (int)run, act);
     if (const int rc = launch_status("act_backward16_kernel")) return rc;
     if (!grad_bias) return CCH_OK;
     auto sum = half ? column_sum16_kernel<F16> : column_sum16_kernel<Bf16>;

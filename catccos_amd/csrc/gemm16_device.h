@@ -183,6 +183,11 @@ __device__ __forceinline__ Rsrc kmajor_rsrc(const uint16_t *base, int64_t pitch,
     return make_rsrc(base + (int64_t)k0 * pitch + c0, (uint32_t)min(left, (int64_t)0x7FFFFFF0));
 }
 
+// Sixteen bytes anywhere: global memory takes them on any element's address, where rows do not start on 16-byte boundaries (1733 x 307, K = 512, with a residual and preact: 18.8 us, element by element 35.8).
+struct __attribute__((packed, aligned(2))) Unaligned16 {
+    v4i v;
+};
+
 // ---- epilogues.  The matrix instructions take B's fragment first: lane (r, g) then holds, of a 32 x 32 block, row r and columns 8 q + 4 g + x at 4 q + x.
 template <class T> __device__ __forceinline__ v4i pack8(const float v[8])
 {
@@ -199,26 +204,15 @@ template <class T> __device__ __forceinline__ void unpack8(v4i o, float v[8])
         v[2 * i + 1] = T::to((uint16_t)((uint32_t)o[i] >> 16));
     }
 }
-// Eight elements at p, of which the first `there` (1..8) exist; `whole`: all eight do, on a 16-byte boundary.
-template <class T> __device__ __forceinline__ void load8(const uint16_t *p, bool whole, int there, float v[8])
+// Eight elements, of which `there` exist.
+template <class T> __device__ __forceinline__ void load8(const uint16_t *p, int there, float v[8])
 {
-    if (whole) {
-        unpack8<T>(*reinterpret_cast<const v4i *>(p), v);
+    if (there >= 8) {
+        unpack8<T>(reinterpret_cast<const Unaligned16 *>(p)->v, v);
         return;
     }
 #pragma unroll
     for (int i = 0; i < 8; i++) v[i] = i < there ? T::to(p[i]) : 0.0f;
-}
-template <class T> __device__ __forceinline__ void store8(uint16_t *p, bool whole, int there, const float v[8])
-{
-    const v4i o = pack8<T>(v);
-    if (whole) {
-        *reinterpret_cast<v4i *>(p) = o;
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-        if (i < there) p[i] = (uint16_t)((uint32_t)o[i >> 1] >> (16 * (i & 1)));
 }
 
 // Whether the epilogue's tensors have rows on 16-byte boundaries: then p.n is a multiple of 8, or (EPI16_GRAD) rows have room for whole pieces.
@@ -287,11 +281,6 @@ template <class T> __device__ __forceinline__ void from_rows(const v4i (&in)[2],
             v[4 * q + 2 * w + 1] = T::to((uint16_t)(p[q][w] >> 16));
         }
 }
-
-// Sixteen bytes anywhere: global memory takes them on any element's address, where rows do not start on 16-byte boundaries (1733 x 307, K = 512, with a residual and preact: 18.8 us, element by element 35.8).
-struct __attribute__((packed, aligned(2))) Unaligned16 {
-    v4i v;
-};
 
 // The results of one wave: MT x NT blocks of 32 x 32, every RS rows from row mw on and side by side from column nw of the tile that begins at row m0 and column n0 of the
 // product, of which rows below m_end exist.  group: the output that K-grouped problems write.  counted: whole pieces are stored

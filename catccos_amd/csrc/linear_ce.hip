@@ -140,7 +140,7 @@ __global__ __launch_bounds__(CE_THREADS) void ce_loss_kernel(const float *__rest
 
 // Rows of x that count, one behind the other (rows of pitch16(h), zeros behind h); the others' rows of grad_x are zeros.  pos: a token's place or -1.
 __global__ __launch_bounds__(256) void ce_gather_kernel(const uint16_t *__restrict__ x, const int32_t *__restrict__ pos, uint16_t *__restrict__ rows, uint16_t *__restrict__ grad_x,
-                                                        int64_t chunks, int64_t h, int64_t per_row, bool whole)
+                                                        int64_t chunks, int64_t h, int64_t per_row)
 {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < chunks; i += (int64_t)gridDim.x * 256) {
         const int64_t t = i / per_row, c = (i - t * per_row) * 8;
@@ -149,23 +149,20 @@ __global__ __launch_bounds__(256) void ce_gather_kernel(const uint16_t *__restri
         if (at >= 0) {
             if (!rows) continue;
             const uint16_t *s = x + t * h + c;
-            v4i o;
-            if (whole) {
-                o = *reinterpret_cast<const v4i *>(s);
-            } else {
+            v4i o = {};
+            if (left >= 8) o = reinterpret_cast<const Unaligned16 *>(s)->v;
+            else
 #pragma unroll
-                for (int k = 0; k < 4; k++) o[k] = (int)((2 * k < left ? (uint32_t)s[2 * k] : 0u) | (2 * k + 1 < left ? (uint32_t)s[2 * k + 1] << 16 : 0u));
-            }
+                for (int k = 0; k < 7; k++)
+                    if (k < left) o[k >> 1] |= (int)((uint32_t)s[k] << (16 * (k & 1)));
             *reinterpret_cast<v4i *>(rows + (int64_t)at * per_row * 8 + c) = o;
         } else if (grad_x) {
             uint16_t *o = grad_x + t * h + c;
-            if (whole) {
-                *reinterpret_cast<v4i *>(o) = (v4i){0, 0, 0, 0};
-            } else {
+            if (left >= 8) reinterpret_cast<Unaligned16 *>(o)->v = (v4i){0, 0, 0, 0};
+            else
 #pragma unroll
-                for (int k = 0; k < 8; k++)
+                for (int k = 0; k < 7; k++)
                     if (k < left) o[k] = 0;
-            }
         }
     }
 }
@@ -174,8 +171,7 @@ static int ce_gather(const uint16_t *x, const int32_t *pos, uint16_t *rows, uint
 {
     const int64_t per_row = pitch16(h) / 8, chunks = t * per_row;
     if (chunks == 0) return CCH_OK;
-    const bool whole = h % 8 == 0 && aligned(x, 16) && aligned(grad_x, 16);
-    hipLaunchKernelGGL(ce_gather_kernel, dim3((unsigned)std::min<int64_t>((chunks + 255) / 256, 1 << 16)), dim3(256), 0, s, x, pos, rows, grad_x, chunks, h, per_row, whole);
+    hipLaunchKernelGGL(ce_gather_kernel, dim3((unsigned)std::min<int64_t>((chunks + 255) / 256, 1 << 16)), dim3(256), 0, s, x, pos, rows, grad_x, chunks, h, per_row);
     return launch_status("ce_gather_kernel");
 }
 

@@ -130,7 +130,7 @@ extern "C" int cch_grouped_matmul(const void *x, const void *w, const int32_t *g
     if (const int rc = check_workspace16("cch_grouped_matmul", workspace, workspace_bytes, cch_grouped_matmul_workspace_bytes(num_experts, t, n, k, trans_b))) return rc;
     hipStream_t s = static_cast<hipStream_t>(stream);
     Carve ws{static_cast<uint8_t *>(workspace)};
-    Operand16 in[2] = {{u16(x), t, k}, {u16(w), num_experts * (trans_b ? n : k), trans_b ? k : n}};
+    Operand16 in[2] = {{u16(x), t, k}, {u16(w), num_experts * (trans_b ? n : k), trans_b ? k : n, group_sizes, trans_b ? n : k}};
     if (const int rc = whole_operands16(in, 2, ws, s)) return rc;
     Gemm16 p = grouped_product(in[0].at, in[1].at, group_sizes, u16(out), num_experts, t, n, k, trans_b, dtype);
     ws.rest(p, workspace, workspace_bytes);
@@ -155,7 +155,7 @@ extern "C" int cch_grouped_matmul_backward(const void *grad_out, const void *x, 
         return rc;
     hipStream_t s = static_cast<hipStream_t>(stream);
     Carve ws{static_cast<uint8_t *>(workspace)};
-    Operand16 in[3] = {{u16(grad_out), t, n}, {grad_w ? u16(x) : nullptr, t, k}, {grad_x ? u16(w) : nullptr, num_experts * (trans_b ? n : k), trans_b ? k : n}};
+    Operand16 in[3] = {{u16(grad_out), t, n}, {grad_w ? u16(x) : nullptr, t, k}, {grad_x ? u16(w) : nullptr, num_experts * (trans_b ? n : k), trans_b ? k : n, group_sizes, trans_b ? n : k}};
     if (const int rc = whole_operands16(in, 3, ws, s)) return rc;
     return backward_products16(in[0].at, in[1].at, in[2].at, group_sizes, num_experts, u16(grad_x), u16(grad_w), t, n, k, trans_b, dtype, ws, workspace, workspace_bytes, s);
 }
