@@ -40,6 +40,7 @@ __global__ __launch_bounds__(Big16::THREADS, 2) void gemm16_big_kernel(Gemm16 p)
     if (threadIdx.x < 64) build_groups16(tab, p.group_sizes, p.groups, rows_grouped ? p.m : p.k, S::TM);
     __syncthreads();
     if (p.zero_rest) zero_rest16(p, uniform(tab.start[p.groups]));
+    if (!rows_grouped) zero_groups16(p, tab);
 
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), wm = wave >> 2, wn = wave & 3;
     const int r = lane & 31, g = lane >> 5, tq = lane >> 4, ti = lane & 15;
@@ -120,6 +121,7 @@ __global__ __launch_bounds__(Big16::THREADS, 2) void gemm16_big_kernel(Gemm16 p)
         for (; t < tiles_end; t += (int)gridDim.x) {
             if (!TAIL || parts == 1) {
                 at = place_in_lists16(t, per_list, list);
+                if (!rows_grouped && uniform(tab.start[list + 1] - tab.start[list]) == 0) at = -1;   // (zero_groups16)
             } else if (t < full) {
                 at = place16(t, full);
             } else {

@@ -519,4 +519,16 @@ __device__ __forceinline__ void zero_rest16(const Gemm16 &p, int first)
     }
 }
 
+// K grouped: zeros to the outputs of groups without a K, which the kernel then leaves out (backward of 9 rows over 128 experts, 1152 x 1007: 190 -> 127 us).
+__device__ __forceinline__ void zero_groups16(const Gemm16 &p, const GroupTable16 &tab)
+{
+    const int64_t n = (int64_t)p.m * p.pitch_out, threads = (int64_t)gridDim.x * blockDim.x, me = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    for (int g = 0; g < p.groups; g++) {
+        if (uniform(tab.start[g + 1] - tab.start[g]) > 0) continue;
+        uint16_t *o = p.out + g * p.out_stride;
+        for (int64_t i = me; i < n / 8; i += threads) reinterpret_cast<Unaligned16 *>(o)[i].v = (v4i){0, 0, 0, 0};
+        if (me < n % 8) o[n / 8 * 8 + me] = 0;
+    }
+}
+
 }  // namespace cch

@@ -31,6 +31,8 @@ __global__ __launch_bounds__(S::THREADS, S::PER_CU * S::WAVES / 4) void gemm16_k
     if (threadIdx.x < 64) build_groups16(tab, p.group_sizes, p.groups, rows_grouped ? p.m : p.k, S::TM);
     __syncthreads();
     if (p.zero_rest) zero_rest16(p, tab.start[p.groups]);
+    const bool leave_empty = !rows_grouped && p.splits == 1;
+    if (leave_empty) zero_groups16(p, tab);
 
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), wm = wave / S::WN, wn = wave % S::WN;
     const int r = lane & 31, g = lane >> 5, tq = lane >> 4, ti = lane & 15;
@@ -71,6 +73,7 @@ __global__ __launch_bounds__(S::THREADS, S::PER_CU * S::WAVES / 4) void gemm16_k
             m_end = p.m;
             k_begin = uniform(tab.start[e]);
             k_end = uniform(tab.start[e + 1]);
+            if (leave_empty && k_end == k_begin) continue;
         }
         const int n0 = ct * S::TN;
         // this part's steps: `first`.. of the group's K
