@@ -23,6 +23,7 @@
 #include <cstring>
 
 #include "catccos_hip.h"
+#include "recorded_backward.h"
 
 namespace {
 
@@ -768,6 +769,15 @@ PyObject *LinearCrossEntropyBackward(PyObject *, PyObject *const *v, Py_ssize_t 
     END_HANDLE_TH_ERRORS
 }
 
+// accumulates_on_default_stream(): of the node whose backward runs (recorded_backward.h)
+PyObject *AccumulatesOnDefault(PyObject *, PyObject *const *, Py_ssize_t nv)
+{
+    HANDLE_TH_ERRORS
+    if (nv != 0) return Decline();
+    return PyBool_FromLong(AccumulatesOnDefaultStream());
+    END_HANDLE_TH_ERRORS
+}
+
 #define CCH_FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr
 PyMethodDef methods[] = {
     {"mx_quant", CCH_FAST(MxQuant)},
@@ -790,6 +800,7 @@ PyMethodDef methods[] = {
     {"matmul_bias_act_backward", CCH_FAST(MatmulBiasActBackward)},
     {"linear_cross_entropy", CCH_FAST(LinearCrossEntropy)},
     {"linear_cross_entropy_backward", CCH_FAST(LinearCrossEntropyBackward)},
+    {"accumulates_on_default_stream", CCH_FAST(AccumulatesOnDefault)},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_direct", "native form of the tensor-level entry points", -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -33,6 +33,7 @@
 #include <tuple>
 
 #include "catccos_hip.h"
+#include "recorded_backward.h"
 
 namespace {
 
@@ -988,6 +989,15 @@ struct NoGradients : torch::autograd::Function<NoGradients> {
     }
 };
 
+// Called in a node's backward (recorded_backward.h).
+void CheckRecording(const char *op, const at::Tensor &grad)
+{
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (!grad.is_cuda() || hipStreamIsCapturing(c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(grad.device().index()).stream(), &status) != hipSuccess) return;
+    TORCH_CHECK(status == hipStreamCaptureStatusNone || !AccumulatesOnDefaultStream(), "catccos::", op,
+                ": its backward pass is being recorded into a graph while an eager graph of the same leaves is alive; drop that graph or use fresh leaves");
+}
+
 // What a node's backward has to work out: which inputs were recorded when it was made.
 bool Wants(const at::Tensor &t) { return t.defined() && t.requires_grad(); }
 bool Wants(const MaybeTensor &t) { return t && Wants(*t); }
@@ -1013,6 +1023,7 @@ struct GroupedMatmulFunction : torch::autograd::Function<GroupedMatmulFunction> 
     }
     static Variables backward(Context *ctx, Variables grads)
     {
+        CheckRecording("grouped_matmul", grads[0]);
         const Variables saved = ctx->get_saved_variables();
         const bool x = ctx->saved_data["x"].toBool(), w = ctx->saved_data["w"].toBool();
         const auto [gx, gw] = GroupedMatmulBackwardAutograd(grads[0], saved[0], saved[1], saved[2], ctx->saved_data["trans_b"].toInt(), x, w);
@@ -1054,6 +1065,7 @@ struct MatmulBiasActFunction : torch::autograd::Function<MatmulBiasActFunction> 
     static Variables backward(Context *ctx, Variables grads)
     {
         if (!grads[0].defined()) return {{}, {}, {}, {}, {}, {}, {}};
+        CheckRecording("matmul_bias_act", grads[0]);
         const Variables saved = ctx->get_saved_variables();
         const bool x = ctx->saved_data["x"].toBool(), w = ctx->saved_data["w"].toBool(), b = ctx->saved_data["bias"].toBool();
         at::Tensor gx, gw, gb;
@@ -1097,6 +1109,7 @@ struct LinearCrossEntropyFunction : torch::autograd::Function<LinearCrossEntropy
     static Variables backward(Context *ctx, Variables grads)
     {
         if (!grads[0].defined()) return {{}, {}, {}, {}, {}};
+        CheckRecording("linear_cross_entropy", grads[0]);
         const Variables saved = ctx->get_saved_variables();
         const bool x = ctx->saved_data["x"].toBool(), w = ctx->saved_data["w"].toBool();
         const auto [gx, gw] = LinearCrossEntropyBackwardAutograd(grads[0], saved[0], saved[1], saved[2], saved[3], saved[4], ctx->saved_data["reduction"].toStringRef(),

@@ -54,7 +54,8 @@ class _Direct:
     def __getattr__(self, name):
         names = ("mx_quant", "dynamic_quant_i8", "moe_init_routing", "w8a8_matmul_dequant", "gmm_i8", "mx_matmul", "mx_grouped_matmul", "moe_ffn_mxfp8",
                  "moe_router", "moe_router_backward", "moe_balance_loss", "moe_balance_loss_backward", "w4a16_matmul", "moe_ffn_w4a16", "grouped_matmul",
-                 "grouped_matmul_backward", "matmul_bias_act", "matmul_bias_act_backward", "linear_cross_entropy", "linear_cross_entropy_backward")
+                 "grouped_matmul_backward", "matmul_bias_act", "matmul_bias_act_backward", "linear_cross_entropy", "linear_cross_entropy_backward",
+                 "accumulates_on_default_stream")
         if name not in names:
             raise AttributeError(name)
         try:
@@ -829,6 +830,13 @@ def _activation(activation):
     return _ACTIVATIONS[activation]
 
 
+def _check_recording(name):
+    """In a node's backward: where it is being recorded into a graph and adds to a leaf that an eager graph still holds, whose gradients are accumulated on the default stream, torch would have
+    that stream wait for the recording one, which ends the process."""
+    if torch.cuda.is_current_stream_capturing() and _direct.accumulates_on_default_stream() is True:
+        raise RuntimeError("%s: its backward pass is being recorded into a graph while an eager graph of the same leaves is alive; drop that graph or use fresh leaves" % name)
+
+
 def _reduction(reduction):
     if reduction not in _REDUCTIONS:
         raise ValueError("unknown reduction %r (mean or sum)" % (reduction,))
@@ -926,6 +934,7 @@ class _GroupedMatmul(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
+        _check_recording("grouped_matmul")
         x, w, group_sizes = ctx.saved_tensors
         return grouped_matmul_backward(grad, x, w, group_sizes, ctx.trans_b, ctx.needs_input_grad[0], ctx.needs_input_grad[1]) + (None, None)
 
@@ -1018,6 +1027,7 @@ class _MatmulBiasAct(torch.autograd.Function):
     def backward(ctx, grad, _):
         if grad is None:
             return (None,) * 7
+        _check_recording("matmul_bias_act")
         x, w, preact = ctx.saved_tensors
         need = ctx.needs_input_grad
         got = matmul_bias_act_backward(grad, x, w, preact, *ctx.options, *need[:3]) if any(need[:3]) else (None,) * 3
@@ -1098,4 +1108,5 @@ class _LinearCrossEntropy(torch.autograd.Function):
     def backward(ctx, grad_loss, _nll, _lse, _tokens):
         if grad_loss is None:
             return (None,) * 5
+        _check_recording("linear_cross_entropy")
         return linear_cross_entropy_backward(grad_loss.float(), *ctx.saved_tensors, *ctx.options, *ctx.needs_input_grad[:2]) + (None,) * 3

@@ -243,6 +243,52 @@ def test_a_recorded_autograd_step():
         assert all(same(a, b) for a, b in zip(held, step()))
 
 
+@pytest.mark.parametrize("lib", ["python", "torch.ops"])
+def test_a_recorded_backward_of_leaves_that_an_eager_graph_holds_is_refused(lib):
+    """The check itself, outside any capture: where the node for a leaf was made on the default stream it says so, else not."""
+    x, w = torch.randn(8, 64, device="cuda").bfloat16(), torch.randn(64, 32, device="cuda").bfloat16()
+    seen = []
+
+    class Look(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, v):
+            return v.clone()
+
+        @staticmethod
+        def backward(ctx, g):
+            seen.append(ops._direct.accumulates_on_default_stream())
+            return g
+
+    leaf = x.clone().requires_grad_()
+    Look.apply(leaf).sum().backward()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        fresh = x.clone().requires_grad_()
+        Look.apply(fresh).sum().backward()
+        Look.apply(fresh * 2).sum().backward()
+    torch.cuda.current_stream().wait_stream(side)
+    assert seen == [True, False, False]
+    assert ops._direct.accumulates_on_default_stream() is False   # (no node runs)
+    # what the operators make of it, the capture being told by the test
+    leaf = w.clone().requires_grad_()
+    if lib == "python":
+        y = cc.matmul_bias_act(x, leaf)
+        with pytest.MonkeyPatch.context() as patch:
+            patch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+            with pytest.raises(RuntimeError, match="eager graph"):
+                y.sum().backward()
+            with torch.cuda.stream(side):
+                ours = w.clone().requires_grad_()
+                cc.matmul_bias_act(x, ours).sum().backward()
+        torch.cuda.synchronize()
+        assert ours.grad is not None
+    else:
+        assert OPS.init(0, 1, 1 << 20, "tcp://127.0.0.1:8666") == 0
+        OPS.matmul_bias_act(x, leaf, None, None, "none", 0, False)[0].sum().backward()
+        assert OPS.finalize() == 0 and leaf.grad is not None
+
+
 def test_a_training_step_of_experts():
     """Gate, routing, the experts' two products, the layer behind them and the loss, with the balance loss: every stage's result and gradient is that of its formula at the
     values that reached it."""
