@@ -325,11 +325,13 @@ __device__ __forceinline__ void epilogue16(const Gemm16 &p, v16f (&acc)[MT][NT],
 #pragma unroll
                 for (int x = 0; x < 16; x++) top = fmaxf(top, acc[i][j][x]);
             top = fmaxf(top, __shfl_xor(top, 32));
+            // (all of them -inf: a sum of 0; a NaN among them: NaN)
+            const float base = top > -INFINITY ? top : 0.0f;
             float sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < NT; j++)
 #pragma unroll
-                for (int x = 0; x < 16; x++) sum += __expf(acc[i][j][x] - top);
+                for (int x = 0; x < 16; x++) sum += __expf(acc[i][j][x] - base);
             sum += __shfl_xor(sum, 32);
             if (there && g == 0) p.stats[(int64_t)m * p.stat_cols + (p.v0 + n0) / (32 * NT)] = make_float2(top, sum);
         });

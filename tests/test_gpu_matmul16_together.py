@@ -427,6 +427,31 @@ def test_a_vocabulary_of_several_pieces(t, h, v, dtype):
     assert all(same(a, b) for a, b in zip(grads, again))
 
 
+@pytest.mark.parametrize("kernel", [0, 1])
+def test_logits_of_minus_infinity_count_nothing(kernel):
+    """Columns whose logit is -inf for every token, a whole run of 64 of them among others: the loss is that without them; a NaN logit is not lost there."""
+    gen = torch.Generator().manual_seed(12)
+    x = (torch.rand(70, 40, generator=gen) + 0.1).bfloat16()
+    w = (torch.randn(400, 40, generator=gen) * 0.2).bfloat16()
+    out = torch.zeros(400, dtype=torch.bool)
+    out[64:128] = out[200:210] = out[399] = True
+    tg = torch.arange(400)[~out][torch.randint(int((~out).sum()), (70,), generator=gen)]
+    w[out, 3] = float("-inf")
+    l = x.double() @ w[~out].double().t()
+    el = sum_error(x.double(), w[~out].double().t())
+    want = torch.logsumexp(l, 1)
+    bound = el.amax(1) + loss_test.EXP + 130 * 2.0 ** -24 + 2.0 ** -22 * want.abs()
+    cc.set_option("matmul16_kernel", kernel)
+    try:
+        got = cc.linear_cross_entropy(x.cuda(), w.cuda(), tg.cuda())
+        check(got[2], want, bound, "lse")
+        x[5, 3] = float("nan")
+        lse = cc.linear_cross_entropy(x.cuda(), w.cuda(), tg.cuda())[2]
+    finally:
+        cc.set_option("matmul16_kernel", -1)
+    assert torch.isnan(lse[5]) and int(torch.isnan(lse).sum()) == 1
+
+
 @pytest.mark.parametrize("trans_b", [0, 1])
 def test_tensors_past_32_bits(trans_b):
     """x, out and the weights each beyond 2^31 bytes: what lies behind that is where it belongs."""
