@@ -405,11 +405,12 @@ __global__ __launch_bounds__(Big16::THREADS, 2) void gemm16_big_kernel(Gemm16 p)
         // Both groups write their results in the same slot: the first behind the barrier that ends its last matrix slot, the second, one slot behind, before it.
         if (wm == 0) CCH_BARRIER();
         if (TAIL && cur.slot >= 0) {
-            // (32 stores, no fewer than `more` counts)
+            // (blocks of rows that there are none of stay out, so these stores are not counted on)
             f32x4 *to = reinterpret_cast<f32x4 *>(p.partial) + (int64_t)cur.slot * (TAIL16_BYTES / 16) + threadIdx.x;
             static_for<MT>([&](auto i_c) {
                 static_for<NT>([&](auto j_c) {
                     constexpr int i = decltype(i_c)::value, j = decltype(j_c)::value;
+                    if (cur.m0 + wm * 32 + i * 64 >= cur.m_end) return;
 #pragma unroll
                     for (int q = 0; q < 4; q++) to[((i * NT + j) * 4 + q) * S::THREADS] = (f32x4){acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
                 });
@@ -418,7 +419,7 @@ __global__ __launch_bounds__(Big16::THREADS, 2) void gemm16_big_kernel(Gemm16 p)
             epilogue16<T, EPI, MT, NT, 64>(p, acc, cur.e, cur.m0, cur.m_end, cur.n0, wm * 32, wn * 64, whole, counted);
         }
         if (!nxt.valid) break;
-        young = more;
+        young = TAIL && cur.slot >= 0 ? 0 : more;
         cur = nxt;
         t += (int)gridDim.x;
         decode(t, nxt);
