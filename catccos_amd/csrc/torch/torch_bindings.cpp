@@ -993,7 +993,11 @@ struct NoGradients : torch::autograd::Function<NoGradients> {
 void CheckRecording(const char *op, const at::Tensor &grad)
 {
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    if (!grad.is_cuda() || hipStreamIsCapturing(c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(grad.device().index()).stream(), &status) != hipSuccess) return;
+    if (!grad.is_cuda()) return;
+    if (hipStreamIsCapturing(c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(grad.device().index()).stream(), &status) != hipSuccess) {
+        (void)hipGetLastError();   // (the default stream while another thread records: not this call's matter)
+        return;
+    }
     TORCH_CHECK(status == hipStreamCaptureStatusNone || !AccumulatesOnDefaultStream(), "catccos::", op,
                 ": its backward pass is being recorded into a graph while an eager graph of the same leaves is alive; drop that graph or use fresh leaves");
 }
