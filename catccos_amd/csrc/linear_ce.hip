@@ -92,31 +92,33 @@ __global__ __launch_bounds__(CE_THREADS) void ce_tokens_kernel(CeTokens p)
     }
 }
 
-// One wave to a counted token: its partial statistics joined.
+// One wave to a counted token and turn: its partial statistics joined.  (A launch holds fewer than 2^32 threads: beyond, it is cut short without an error.)
+constexpr int CE_JOIN_BLOCKS = 1 << 16;
 __global__ __launch_bounds__(256) void ce_join_kernel(const float2 *__restrict__ stats, const float *__restrict__ logit, const int32_t *__restrict__ src,
                                                       const int32_t *__restrict__ count, float *__restrict__ nll, float *__restrict__ lse, int cols)
 {
-    const int i = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (i >= count[0]) return;
-    const float2 *s = stats + (int64_t)i * cols;
-    float top = -INFINITY, sum = 0.0f;
-    for (int c = lane; c < cols; c += 64) {
-        const float2 v = s[c];
-        const float m = fmaxf(top, v.x);
-        sum = (top > -INFINITY || sum != sum ? sum * __expf(top - m) : 0.0f) + (v.x > -INFINITY || v.y != v.y ? v.y * __expf(v.x - m) : 0.0f);
-        top = m;
-    }
+    const int lane = threadIdx.x & 63, tokens = count[0];
+    for (int i = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6); i < tokens; i += (int)gridDim.x * 4) {
+        const float2 *s = stats + (int64_t)i * cols;
+        float top = -INFINITY, sum = 0.0f;
+        for (int c = lane; c < cols; c += 64) {
+            const float2 v = s[c];
+            const float m = fmaxf(top, v.x);
+            sum = (top > -INFINITY || sum != sum ? sum * __expf(top - m) : 0.0f) + (v.x > -INFINITY || v.y != v.y ? v.y * __expf(v.x - m) : 0.0f);
+            top = m;
+        }
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-        const float ot = __shfl_xor(top, d), os = __shfl_xor(sum, d), m = fmaxf(top, ot);
-        sum = (sum == 0.0f ? 0.0f : sum * __expf(top - m)) + (os == 0.0f ? 0.0f : os * __expf(ot - m));
-        top = m;
-    }
-    if (lane == 0) {
-        const float l = top + logf(sum);
-        const int t = src[i];
-        lse[t] = l;
-        nll[t] = l - logit[i];
+        for (int d = 32; d > 0; d >>= 1) {
+            const float ot = __shfl_xor(top, d), os = __shfl_xor(sum, d), m = fmaxf(top, ot);
+            sum = (sum == 0.0f ? 0.0f : sum * __expf(top - m)) + (os == 0.0f ? 0.0f : os * __expf(ot - m));
+            top = m;
+        }
+        if (lane == 0) {
+            const float l = top + logf(sum);
+            const int t = src[i];
+            lse[t] = l;
+            nll[t] = l - logit[i];
+        }
     }
 }
 
@@ -320,7 +322,7 @@ extern "C" int cch_linear_cross_entropy(const void *x, const void *w, const void
         p.stats = reinterpret_cast<float2 *>(ws + at.stats);
         p.stat_cols = (int)((v + CE_STAT - 1) / CE_STAT);
         if (const int rc = gemm16_launch(p, ROWS_NK, EPI16_STATS, s)) return rc;
-        hipLaunchKernelGGL(ce_join_kernel, dim3((unsigned)((t + 3) / 4)), dim3(256), 0, s, p.stats, p.target_logit, tk.src, tk.count, nll, lse, p.stat_cols);
+        hipLaunchKernelGGL(ce_join_kernel, dim3((unsigned)std::min<int64_t>((t + 3) / 4, CE_JOIN_BLOCKS)), dim3(256), 0, s, p.stats, p.target_logit, tk.src, tk.count, nll, lse, p.stat_cols);
         if (const int rc = launch_status("ce_join_kernel")) return rc;
     }
     hipLaunchKernelGGL(ce_loss_kernel, dim3(1), dim3(CE_THREADS), 0, s, nll, lse, tokens, loss, (int)t, z_coef, (int)(reduction == CCH_REDUCE_MEAN));
