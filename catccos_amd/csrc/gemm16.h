@@ -80,7 +80,8 @@ struct Gemm16 {
     int stat_cols;
     float *target_logit;
     const float *lse;                      // per row of the product
-    float z2, grad_scale;                  // 2 * z_coef
+    float z2;                              // 2 * z_coef
+    const float *grad_scale;               // device, or nullptr: 1
 };
 
 // Bytes of `partial` that the product may use (its sizes, groups and pointers' being there or not as at the launch; no GPU needed).

@@ -338,7 +338,7 @@ __device__ __forceinline__ void epilogue16(const Gemm16 &p, v16f (&acc)[MT][NT],
     } else {
         uint16_t *const out = p.out + (int64_t)group * p.out_stride;
         const bool scaled = EPI == EPI16_OUT && p.scale, summed = EPI == EPI16_OUT && p.sums;
-        const float scale = scaled ? *p.scale : 1.0f;
+        const float scale = scaled ? *p.scale : 1.0f, grad_scale = EPI == EPI16_GRAD && p.grad_scale ? *p.grad_scale : 1.0f;
         const int lc = lane_columns(lane);
         // counted: descriptors of the tile's rows that exist; a lane whose columns do not starts 2^31 bytes behind, past any of them
         const int64_t tile_at = (int64_t)tile_m * p.pitch_out + tile_n;
@@ -366,7 +366,7 @@ __device__ __forceinline__ void epilogue16(const Gemm16 &p, v16f (&acc)[MT][NT],
             bool wanted = false;
             if constexpr (EPI == EPI16_GRAD) {
                 lse = there ? p.lse[m] : 0.0f;
-                slope = (1.0f + p.z2 * lse) * p.grad_scale;
+                slope = (1.0f + p.z2 * lse) * grad_scale;
                 want = there ? p.targets[m] - p.v0 - n0 - 4 * g : -1;
                 wanted = __any(want >= 0 && want < 32 * NT);
             }
@@ -468,7 +468,7 @@ __device__ __forceinline__ void epilogue16(const Gemm16 &p, v16f (&acc)[MT][NT],
                     if (wanted) {
 #pragma unroll
                         for (int x = 0; x < 16; x++)
-                            if (column(j, x) == want) v[x] -= p.grad_scale;
+                            if (column(j, x) == want) v[x] -= grad_scale;
                     }
                     if (edge) {
 #pragma unroll

@@ -14,8 +14,9 @@ namespace cch {
 constexpr int64_t CE_MAX_TOKENS = (int64_t)1 << 30, CE_MAX_VOCAB = (int64_t)1 << 30;
 constexpr int CE_STAT = 64;                                   // columns of one pair of statistics
 constexpr int64_t CE_PIECE_BYTES = (int64_t)256 << 20;        // of d at a time
-// Half cannot hold p of a large vocabulary: d is kept times 2^11 there, which leaves it within 2^16 up to 1 + 2 z lse = 31 and p above 2^-25 at full precision.
-static float ce_grad_scale(int half) { return half ? 2048.0f : 1.0f; }
+// Half cannot hold p of a large vocabulary: d is kept times 2^11 there, which leaves p above 2^-25 at full precision.  |d| can be as large as |1 + 2 z lse|, or as that
+// number's distance to 1: where this passes 31 for some token, d is kept times the largest power of two that leaves it at 31 * 2^11 or less (half ends at 65504).
+constexpr float CE_HALF_SCALE = 2048.0f, CE_HALF_MOST = 31.0f;
 
 static int64_t ce_piece(int64_t t, int64_t v)
 {
@@ -25,8 +26,8 @@ static int64_t ce_piece(int64_t t, int64_t v)
     return std::min<int64_t>(((v + pieces - 1) / pieces + 255) / 256 * 256, v);
 }
 
-// ---- the tokens that count, in their order: src[i] the i-th one, target[i] its target, count[0] how many; scalars[0] what the gradient's products are multiplied by.  The
-// others' nll and lse are zero.  One workgroup, four tokens to a thread and round.
+// ---- the tokens that count, in their order: src[i] the i-th one, target[i] its target, count[0] how many; scalars[0] what the gradient's products are multiplied by, scalars[1]
+// what d is kept times.  The others' nll and lse are zero.  One workgroup, four tokens to a thread and round.
 constexpr int CE_THREADS = 1024, CE_PER = 4;
 struct CeTokens {
     const void *targets;
@@ -39,15 +40,17 @@ struct CeTokens {
     int32_t *tokens;             // forward
     const float *grad_loss;      // backward
     const int32_t *divisor;
-    float *scalar;
-    float grad_scale;
-    int mean;
+    float *scalars;
+    float z2;                    // 2 * z_coef
+    int half, mean;
 };
 __global__ __launch_bounds__(CE_THREADS) void ce_tokens_kernel(CeTokens p)
 {
     __shared__ int sums[2][CE_THREADS / 64];
+    __shared__ float largest[CE_THREADS / 64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int before = 0, par = 0;
+    float most = 0.0f;   // of |d|, this thread's tokens
     for (int base = 0; base < p.t; base += CE_THREADS * CE_PER, par ^= 1) {
         const int first = base + (int)threadIdx.x * CE_PER;
         int64_t tg[CE_PER];
@@ -77,7 +80,11 @@ __global__ __launch_bounds__(CE_THREADS) void ce_tokens_kernel(CeTokens p)
             if (tg[i] >= 0) {
                 p.src[at] = t;
                 p.target[at] = (int32_t)tg[i];
-                if (p.lse) p.lse[at] = p.lse_in[t];
+                if (p.lse) {
+                    const float lse = p.lse_in[t], f = 1.0f + p.z2 * lse, d = fmaxf(f, 1.0f - f);
+                    p.lse[at] = lse;
+                    if (d < INFINITY) most = fmaxf(most, d);   // (not a NaN's either: such a token's row says so itself)
+                }
                 at++;
             } else if (p.nll_out) {
                 p.nll_out[t] = 0.0f;
@@ -88,7 +95,18 @@ __global__ __launch_bounds__(CE_THREADS) void ce_tokens_kernel(CeTokens p)
     if (threadIdx.x == 0) {
         p.count[0] = before;
         if (p.tokens) p.tokens[0] = before;
-        if (p.scalar) p.scalar[0] = p.grad_loss[0] / (p.mean ? (float)max(p.divisor[0], 1) : 1.0f) / p.grad_scale;
+    }
+    if (!p.scalars) return;
+    for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
+    if (lane == 0) largest[wave] = most;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        float scale = p.half ? CE_HALF_SCALE : 1.0f;
+        for (int w = 0; w < CE_THREADS / 64; w++) most = fmaxf(most, largest[w]);
+        if (p.half)
+            for (; most > CE_HALF_MOST; most *= 0.5f) scale *= 0.5f;
+        p.scalars[0] = p.grad_loss[0] / (p.mean ? (float)max(p.divisor[0], 1) : 1.0f) / scale;
+        p.scalars[1] = scale;
     }
 }
 
@@ -213,7 +231,7 @@ static Gemm16 ce_grad_x(const int32_t *count, const int32_t *src, float *sums, i
 }
 
 struct CeWorkspace {
-    int64_t src, pos, target, lse, count, scalar, logit, stats, rows, w, d, sums, parts, end;
+    int64_t src, pos, target, lse, count, scalars, logit, stats, rows, w, d, sums, parts, end;
 };
 static CeWorkspace ce_workspace(int64_t t, int64_t h, int64_t v, bool backward)
 {
@@ -238,7 +256,7 @@ static CeWorkspace ce_workspace(int64_t t, int64_t h, int64_t v, bool backward)
         const int64_t c = ce_piece(t, v);
         float some;   // (stands for sums that are there)
         at.lse = piece(t * 4);
-        at.scalar = piece(4);
+        at.scalars = piece(8);
         at.d = piece(t * pitch16(c) * 2);
         if (c < v) at.sums = piece(t * h * 4);
         at.parts = piece(std::max(partial16_bytes(ce_grad_w(&CE_COUNT, t, h, c), ROWS_TN, EPI16_OUT),
@@ -361,8 +379,9 @@ extern "C" int cch_linear_cross_entropy_backward(const float *grad_loss, const v
     tk.lse = f32(at.lse);
     tk.grad_loss = grad_loss;
     tk.divisor = tokens;
-    tk.scalar = f32(at.scalar);
-    tk.grad_scale = ce_grad_scale(half);
+    tk.scalars = f32(at.scalars);
+    tk.z2 = 2.0f * z_coef;
+    tk.half = half;
     tk.mean = reduction == CCH_REDUCE_MEAN;
     hipLaunchKernelGGL(ce_tokens_kernel, dim3(1), dim3(CE_THREADS), 0, s, tk);
     if (const int rc = launch_status("ce_tokens_kernel")) return rc;
@@ -394,8 +413,8 @@ extern "C" int cch_linear_cross_entropy_backward(const float *grad_loss, const v
             p.v0 = (int)v0;
             p.targets = tk.target;
             p.lse = tk.lse;
-            p.z2 = 2.0f * z_coef;
-            p.grad_scale = tk.grad_scale;
+            p.z2 = tk.z2;
+            p.grad_scale = half ? tk.scalars + 1 : nullptr;
             if (const int rc = gemm16_launch(p, ROWS_NK, EPI16_GRAD, s)) return rc;
         }
         const Carve parts{ws + at.parts};
@@ -405,7 +424,7 @@ extern "C" int cch_linear_cross_entropy_backward(const float *grad_loss, const v
             q.a = d;
             q.b = rows;
             q.out = gw + v0 * h;
-            q.scale = tk.scalar;
+            q.scale = tk.scalars;
             parts.rest(q, workspace, workspace_bytes);
             if (const int rc = gemm16_launch(q, ROWS_TN, EPI16_OUT, s)) return rc;
         }
@@ -415,7 +434,7 @@ extern "C" int cch_linear_cross_entropy_backward(const float *grad_loss, const v
             q.a = d;
             q.b = pw + v0 * ldw;
             q.out = gx;
-            q.scale = tk.scalar;
+            q.scale = tk.scalars;
             q.sums_in = v0 > 0;
             q.sums_out = v0 + piece < v;
             parts.rest(q, workspace, workspace_bytes);

@@ -452,7 +452,8 @@ int cch_matmul_bias_act_backward(const void *grad_out, const void *x, const void
  * targets: int32 or int64 [t] (target_bytes 4 or 8); a token whose target lies outside 0..v-1 does not count: its nll and lse are zero, its row of grad_x too, and its
  * row of x is not looked at.  No token that counts: loss 0.  nll, lse fp32 [t], loss fp32 [1], tokens int32 [1]: how many count.
  * Backward: grad_loss fp32 [1] on the device, lse as the forward call wrote it, tokens int32 [1], what a mean divides by; grad_x [t, h], grad_w [v, h], either may be NULL.  The logits are
- * computed again, a piece of the vocabulary at a time, their gradient is rounded to dtype (half: kept times 2^11, which overflows where 1 + 2 z_coef lse passes 31).
+ * computed again, a piece of the vocabulary at a time, their gradient is rounded to dtype (half: kept times 2^11, or, where 1 + 2 z_coef lse lies outside -30..31 for some token, the largest power of
+ * two that leaves it in range).
  * t and v up to 2^30, h up to 2^22.  The same inputs give the same bits. */
 #define CCH_REDUCE_MEAN 0
 #define CCH_REDUCE_SUM 1
