@@ -833,7 +833,16 @@ def _activation(activation):
 def _check_recording(name):
     """In a node's backward: where it is being recorded into a graph and adds to a leaf that an eager graph still holds, whose gradients are accumulated on the default stream, torch would have
     that stream wait for the recording one, which ends the process."""
-    if torch.cuda.is_current_stream_capturing() and _direct.accumulates_on_default_stream() is True:
+    try:
+        if not torch.cuda.is_current_stream_capturing():
+            return
+    except RuntimeError:
+        return   # (the default stream while another thread records: not this call's matter)
+    held = _direct.accumulates_on_default_stream()
+    if held is NotImplemented:
+        raise RuntimeError("%s: its backward pass is being recorded into a graph, and without catccos_amd/_direct.so nothing says whether an eager graph of the same leaves is alive; "
+                           "record the ..._backward call instead" % name)
+    if held:
         raise RuntimeError("%s: its backward pass is being recorded into a graph while an eager graph of the same leaves is alive; drop that graph or use fresh leaves" % name)
 
 
