@@ -989,16 +989,24 @@ struct NoGradients : torch::autograd::Function<NoGradients> {
     }
 };
 
+// Whether a stream records, as tests would have it: -1 asks the stream.
+std::atomic<int64_t> g_assume_recording{-1};
+int64_t AssumeRecording(int64_t state) { return g_assume_recording.exchange(state); }
+
+bool Recording(const at::Tensor &grad)
+{
+    if (const int64_t state = g_assume_recording.load(); state >= 0) return state != 0;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(grad.device().index()).stream(), &status) == hipSuccess) return status != hipStreamCaptureStatusNone;
+    (void)hipGetLastError();   // (the default stream while another thread records: not this call's matter)
+    return false;
+}
+
 // Called in a node's backward (recorded_backward.h).
 void CheckRecording(const char *op, const at::Tensor &grad)
 {
-    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     if (!grad.is_cuda()) return;
-    if (hipStreamIsCapturing(c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(grad.device().index()).stream(), &status) != hipSuccess) {
-        (void)hipGetLastError();   // (the default stream while another thread records: not this call's matter)
-        return;
-    }
-    TORCH_CHECK(status == hipStreamCaptureStatusNone || !AccumulatesOnDefaultStream(), "catccos::", op,
+    TORCH_CHECK(!Recording(grad) || !AccumulatesOnDefaultStream(), "catccos::", op,
                 ": its backward pass is being recorded into a graph while an eager graph of the same leaves is alive; drop that graph or use fresh leaves");
 }
 
@@ -1159,6 +1167,7 @@ TORCH_LIBRARY(catccos, m)
     m.def("linear_cross_entropy(Tensor x, Tensor w, Tensor targets, str reduction, float z_coef) -> (Tensor, Tensor, Tensor, Tensor)");
     m.def("linear_cross_entropy_backward(Tensor grad_loss, Tensor x, Tensor w, Tensor targets, Tensor lse, Tensor tokens, str reduction, float z_coef, bool x_grad, "
           "bool w_grad) -> (Tensor, Tensor)");
+    m.def("_assume_recording(int state) -> int");
 }
 
 // init / finalize take no tensors: one kernel for every backend, as in the reference (torch_bindings.cpp:233-238)
@@ -1166,6 +1175,7 @@ TORCH_LIBRARY_IMPL(catccos, CompositeExplicitAutograd, m)
 {
     m.impl("init", &Init);
     m.impl("finalize", &Finalize);
+    m.impl("_assume_recording", &AssumeRecording);
 }
 
 // the GPU key (HIP devices answer to it in a ROCm build of PyTorch); CPU tensors find no kernel
