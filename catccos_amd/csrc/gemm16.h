@@ -127,7 +127,7 @@ struct Carve {
 
 // An operand's rows of `cols` elements, back to back.  `whole_operands16` makes copies in rows of pitch16(cols), zeros behind them, of those that are no whole multiples of 16 bytes
 // (space from `ws`), and points `at` there; an operand that is not there (nullptr) stays so.  With sizes (device), `group_rows` rows belong to a group each, and those of groups without
-// rows of their own are not copied (9 tokens over 128 experts x 1152 x 1007: 222 -> 62 us).
+// rows of their own are not copied (9 tokens over 128 experts x 1152 x 1007, K-major: 222 us with all of them, 39 so).
 struct Operand16 {
     const uint16_t *at;
     int64_t rows, cols;

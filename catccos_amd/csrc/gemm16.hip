@@ -58,7 +58,9 @@ Plan16 plan16(const Gemm16 &p, int layout, int epilogue)
     if (rows_kernel && asked < 0 && share <= 128) {
         // The kernel for few rows: an eighth of the steps in a row, or the weights' way from memory, again for every tile of rows (from the caches).  K-major weights come in half
         // lines.  4096 x 7168: 1 row 15.4 us (128 x 128 tiles 18.3), 32 22.4 (19.3), K-major 29 (18.7); 7168 x 2048: 1 row 8.7 (13.9), 64 17.1 (16.7), K-major 12.1 (13.8);
-        // 1024 x 1024: 1 row 4.9 (9.4), 96 5.9 (11.3), K-major 6.0 (9.5).  Its launch, prologue and epilogue take 2 us less than the others'.
+        // 1024 x 1024: 1 row 4.9 (9.4), 96 5.9 (11.3), K-major 6.0 (9.5).  Its launch, prologue and epilogue take 2 us less than the others'.  Weights from memory in all of these;
+        // where the caches hold them, 4096 x 7168: 1 row 11.5 (17.2), 32 15.6 (18.4), K-major 18.5 (17.8).  The estimate is off in two places: 17 to 32 rows of 4096 x 7168 come here, 3 to 12 %
+        // slower than tiles with weights from memory; K-major 7168 x 2048 goes to tiles up to 32 rows, 15.1 to 16.0 where this kernel takes 12.3 to 14.6.
         const int mr = rows16(p);
         const int64_t row_tiles = (share + mr - 1) / mr, workgroups = row_tiles * groups * ((p.n + 31) / 32);
         const double step = (layout == ROWS_NN ? 0.9 : 0.31) * (mr == 32 ? 1.2 : 1.0) * (double)((workgroups + CUS - 1) / CUS);
@@ -218,7 +220,8 @@ int fill_zero16(uint16_t *dst, int64_t n, hipStream_t stream)
 }
 
 // ---- dz = grad_out * act'(preact) and the bias' gradient.  A workgroup has 256 columns, 8 to a thread, and a run of rows, every eighth to a thread; its columns' sums over
-// the run go to `partial`, which a second launch adds up in the runs' order.  Sums are of the products before their rounding.  Bound by memory: two reads, one write.
+// the run go to `partial`, which a second launch adds up in the runs' order.  Sums are of the products before their rounding.  Bound by memory (two reads, one write) in wide layers:
+// 8192 x 7168 68 us.  At most 64 runs, so that the second launch stays short: narrow layers of many rows leave CUs without work (without dz, 16384 x 256 43 us, 65536 x 1024 243).
 constexpr int SUM_COLS = 256, SUM_RUNS = 64;
 static int64_t sum_runs(int64_t m) { return std::max<int64_t>(1, std::min<int64_t>((m + 7) / 8, SUM_RUNS)); }
 int64_t column_sum_bytes(int64_t m, int64_t n) { return round256(sum_runs(m) * n * 4); }

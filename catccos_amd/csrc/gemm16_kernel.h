@@ -2,7 +2,7 @@
 // filled straight from memory, DEPTH - 1 steps ahead; one barrier a step publishes what has landed and frees what was read.  A 128 x 128 step is 512 clocks of matrix
 // instructions, while memory answers in 1500 to 2500: with two stages two workgroups share a CU, so that one's waits and epilogue pass under the other's matrix instructions; where there are not
 // that many workgroups, one has four stages (256 x 4096 x 7168 on 64 tiles: 97 us with two).  Tiles too few for the chip are split along K (p.splits): each part leaves fp32 sums,
-// which gemm16_join adds up in the parts' order.
+// which join16_kernel adds up in the parts' order.
 #pragma once
 #include <atomic>
 

