@@ -38,14 +38,7 @@ def _kept_scale(most):
     return scale
 
 
-@pytest.mark.parametrize("t,h,v,z,sure,below,grad", [
-    (70, 64, 200, 0.5, 60.0, 0.0, 16.0),        # 1 + 2 z lse about 60
-    (300, 136, 1000, 2.0, 50.0, 0.0, 4.0),      # 200
-    (257, 77, 333, 1.0, 5.0, 40.0, 16.0),       # -70: all logits lie far below zero
-    (40, 64, 130, -0.5, 60.0, 0.0, 16.0),       # -60
-    (130, 72, 520, 1e3, 60.0, 0.0, 2.0 ** -6),  # 10^5, past what half holds at all
-    (1000, 64, 4100, 0.3, 70.0, 0.0, 64.0)])
-def test_gradients(t, h, v, z, sure, below, grad):
+def _verify(t, h, v, z, sure, below, grad):
     x, w, tg = _case(t, h, v, sure, below)
     loss, nll, lse, tokens = cc.linear_cross_entropy(x.cuda(), w.cuda(), tg.cuda(), z_coef=z)
     got = cc.linear_cross_entropy_backward(torch.full((), grad, device="cuda"), x.cuda(), w.cuda(), tg.cuda(), lse, tokens, z_coef=z)
@@ -77,6 +70,17 @@ def test_gradients(t, h, v, z, sure, below, grad):
     assert torch.equal(xr.grad, got[0]) and torch.equal(wr.grad, got[1])
 
 
+@pytest.mark.parametrize("t,h,v,z,sure,below,grad", [
+    (70, 64, 200, 0.5, 60.0, 0.0, 16.0),        # 1 + 2 z lse about 60
+    (300, 136, 1000, 2.0, 50.0, 0.0, 4.0),      # 200
+    (257, 77, 333, 1.0, 5.0, 40.0, 16.0),       # -70: all logits lie far below zero
+    (40, 64, 130, -0.5, 60.0, 0.0, 16.0),       # -60
+    (130, 72, 520, 1e3, 60.0, 0.0, 2.0 ** -6),  # 10^5, past what half holds at all
+    (1000, 64, 4100, 0.3, 70.0, 0.0, 64.0)])
+def test_gradients(t, h, v, z, sure, below, grad):
+    _verify(t, h, v, z, sure, below, grad)
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 def test_a_token_that_is_not_finite_leaves_the_others_alone(bad):
     """What a NaN or infinite token's lse says of the range counts for nothing: the other tokens' rows are those without it."""
@@ -90,3 +94,29 @@ def test_a_token_that_is_not_finite_leaves_the_others_alone(bad):
         _, _, lse, tokens = cc.linear_cross_entropy(xs.cuda(), w.cuda(), ts.cuda(), reduction="sum", z_coef=1.0)
         grads.append(cc.linear_cross_entropy_backward(one, xs.cuda(), w.cuda(), ts.cuda(), lse, tokens, reduction="sum", z_coef=1.0)[0])
     assert torch.equal(grads[0][keep.cuda()], grads[1]) and bool(torch.isfinite(grads[1]).all()) and bool(torch.isnan(grads[0][7]).all())
+
+
+def test_a_vocabulary_of_several_pieces():
+    """Every piece of the vocabulary, and the sums over them, take the one scale."""
+    _verify(66000, 24, 3700, 0.5, 60.0, 0.0, 1024.0)
+
+
+def test_a_recorded_step_follows_the_range():
+    """The scale is chosen on the device: a replay on values of another range equals the eager calls on them."""
+    x, w, tg = (v.cuda() for v in _case(130, 72, 520, 60.0, 0.0))
+    one = torch.full((), 0.25, device="cuda")
+
+    def step():
+        out = cc.linear_cross_entropy(x, w, tg, z_coef=2.0)
+        return out + cc.linear_cross_entropy_backward(one, x, w, tg, out[2], out[3], z_coef=2.0)
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for factor in (1.0, 0.03, 4.0, 1.0):
+        x.copy_(_case(130, 72, 520, 60.0, 0.0)[0].cuda() * factor)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, step())) and bool(torch.isfinite(held[4]).all())
